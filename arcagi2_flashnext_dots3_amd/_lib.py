@@ -65,6 +65,11 @@ SIGNATURES = {
     "spmla_mqa_logits": [P, LL, LL, P, LL, P, LL, P, I, P, P, I, I, I, P, LL, P],
     "spmla_paged_mqa_logits": [P, LL, LL, P, LL, P, LL, I, LL, P, LL, P, P, I, I, I, I, I, P, LL, P],
     "spmla_paged_mqa_logits_seq": [P, LL, LL, P, LL, P, LL, I, LL, P, LL, P, I, I, I, I, I, I, I, P, LL, P],
+    "spmla_rms_norm": [P, LL, P, LL, P, LL, P, I, F, I, I, I, P, LL, P, LL, P, LL, I, P],
+    "spmla_quant_fp8": [P, LL, I, I, I, P, LL, P, LL, I, P],
+    "spmla_linear_fp8": [P, LL, P, LL, P, LL, P, LL, I, I, I, I, P, LL, P],
+    "spmla_rope": [P, LL, LL, P, I, P, I, I, I, I, I, I, F, I, I, P, LL, LL, P],
+    "spmla_latent_write": [P, LL, P, I, F, P, I, P, I, F, P, I, P, LL, I, LL, I, F, P],
     "spmla_version": [],
     "spmla_host_e4m3_encode": [P, P, LL],
 }

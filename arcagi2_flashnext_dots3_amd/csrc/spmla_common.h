@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 namespace spmla {
 

@@ -1,0 +1,239 @@
+// RMS norm with the residual's addition and an 8-bit output, and the 8-bit quantization alone: what feeds a projection
+// on FP8 weights.
+//   z = x + residual (rounded to the type and stored),  y[d] = z[d] / sqrt(mean(z^2) + eps) * w[d]
+//   out = y rounded once to the type; codes = e4m3(y / s) with one scale s per 128 values (group_codes)
+// The sums and y stay in fp32; y is not rounded to the 16-bit type before it is quantized.
+//
+// One pass: a row's values stay in the registers of the NT threads that share it, 8 a thread in CH chunks, so x and the
+// residual are read once. A group of 128 values is 16 neighbouring lanes of a chunk. Rows of up to 512 values take one
+// wave each (no LDS), longer ones a workgroup.
+#include "spmla_quant.h"
+
+namespace spmla {
+namespace nrm {
+
+struct NormParams {
+  const void* x; long long x_st;
+  const void* res; void* res_out; long long res_st, ro_st;   // null without a residual
+  const void* w; int w_f32;                                  // null: ones
+  float eps;
+  int T, D;
+  void* out; long long o_st;                                 // null without it
+  uint8_t* codes; long long c_st;                            // null without them
+  float* scales; long long s_st;
+  int ue8m0;
+};
+
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// VEC: 16-byte loads and stores (D % 8 == 0 and aligned rows); else element by element. NORM false: y = x, a workgroup
+// per NT * 8 values of a row.
+template <int DT, bool NORM, int NT, int CH, bool VEC>
+__global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p) {
+  constexpr int RPB = NT < 256 ? 256 / NT : 1;               // rows per workgroup
+  __shared__ float part[NT / 64];
+  const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * RPB + threadIdx.x / NT;
+  const bool on = row < p.T;
+  const int base = NORM ? 0 : (int)blockIdx.y * (NT * 8);
+  float z[CH][8], w[CH][8];
+  auto at = [&](int c) { return base + (c * NT + tid) * 8; };
+  auto get = [&](const void* q, long long st, int d, float (&v)[8]) {
+    if (VEC) {
+      if (on && d < p.D) load8<DT>(q, row * st + d, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = on && d + e < p.D ? load1<DT>(q, row * st + d + e) : 0.f;
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[c][e] = 0.f;
+    get(p.x, p.x_st, at(c), z[c]);
+  }
+  float r = 1.0f;
+  if constexpr (NORM) {
+    if (p.w) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[c][e] = 0.f;
+        if (VEC) {
+          if (at(c) < p.D) {
+            if (p.w_f32) load8<DT_F32>(p.w, at(c), w[c]);
+            else load8<DT>(p.w, at(c), w[c]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (at(c) + e < p.D) w[c][e] = p.w_f32 ? ((const float*)p.w)[at(c) + e] : load1<DT>(p.w, at(c) + e);
+        }
+      }
+    }
+    if (p.res) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        float a[8] = {};
+        get(p.res, p.res_st, at(c), a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e] = round_to<DT>(z[c][e] + a[e]);
+        if (VEC) {
+          if (on && at(c) < p.D) store8<DT>(p.res_out, row * p.ro_st + at(c), z[c]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (on && at(c) + e < p.D) store1<DT>(p.res_out, row * p.ro_st + at(c) + e, z[c][e]);
+        }
+      }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float q = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q = __builtin_fmaf(z[c][e], z[c][e], q);
+      ss += q;
+    }
+    ss = wave_sum(ss);
+    if constexpr (NT > 64) {
+      if (lane == 0) part[tid >> 6] = ss;
+      __syncthreads();
+      ss = part[0];
+#pragma unroll
+      for (int i = 1; i < NT / 64; ++i) ss += part[i];
+    }
+    r = 1.0f / sqrtf(ss / (float)p.D + p.eps);
+    if (p.w) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e] *= w[c][e];
+    }
+  }
+  if (p.out) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = z[c][e] * r;
+      if (VEC) {
+        if (on && at(c) < p.D) store8<DT>(p.out, row * p.o_st + at(c), y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (on && at(c) + e < p.D) store1<DT>(p.out, row * p.o_st + at(c) + e, y[e]);
+      }
+    }
+  }
+  if (p.codes) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      uint32_t lo, hi;
+      const float s = group_codes(z[c], r, p.ue8m0 != 0, lo, hi);
+      const int d = at(c);
+      if (on && d < p.D) {
+        uint8_t* q = p.codes + row * p.c_st + d;
+        if (VEC) {
+          *(uint2*)q = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (d + e < p.D) q[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+        }
+        if ((lane & 15) == 0) p.scales[row * p.s_st + d / QGROUP] = s;
+      }
+    }
+  }
+}
+
+template <int DT, bool NORM, int NT, int CH, bool VEC>
+static void launch(const NormParams& p, hipStream_t s) {
+  constexpr int RPB = NT < 256 ? 256 / NT : 1;
+  const unsigned gy = NORM ? 1u : (unsigned)((p.D + NT * 8 - 1) / (NT * 8));
+  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, VEC>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
+                     dim3(NT < 256 ? 256 : NT), 0, s, p);
+}
+
+constexpr int MAX_D = 65536;
+
+template <int DT, bool VEC>
+static void norm_go(const NormParams& p, hipStream_t s) {
+  if (p.D <= 512) launch<DT, true, 64, 1, VEC>(p, s);
+  else if (p.D <= 2048) launch<DT, true, 256, 1, VEC>(p, s);
+  else if (p.D <= 4096) launch<DT, true, 256, 2, VEC>(p, s);
+  else if (p.D <= 16384) launch<DT, true, 1024, 2, VEC>(p, s);
+  else launch<DT, true, 1024, 8, VEC>(p, s);
+}
+
+static bool rows_aligned(const void* p, long long st, int bytes) {
+  return ((uintptr_t)p & 15) == 0 && (st * bytes & 15) == 0;
+}
+
+static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
+  const int eb = dtype == DT_F32 ? 4 : 2;
+  bool vec = p.D % 8 == 0 && rows_aligned(p.x, p.x_st, eb);
+  if (p.res) vec = vec && rows_aligned(p.res, p.res_st, eb) && rows_aligned(p.res_out, p.ro_st, eb);
+  if (p.w) vec = vec && ((uintptr_t)p.w & 15) == 0;
+  if (p.out) vec = vec && rows_aligned(p.out, p.o_st, eb);
+  if (p.codes) vec = vec && ((uintptr_t)p.codes & 7) == 0 && (p.c_st & 7) == 0;
+  auto by_type = [&](auto tag) {
+    constexpr bool V = decltype(tag)::value;
+    if (norm) {
+      if (dtype == DT_F32) norm_go<DT_F32, V>(p, s);
+      else if (dtype == DT_F16) norm_go<DT_F16, V>(p, s);
+      else norm_go<DT_BF16, V>(p, s);
+    } else {
+      if (dtype == DT_F32) launch<DT_F32, false, 256, 1, V>(p, s);
+      else if (dtype == DT_F16) launch<DT_F16, false, 256, 1, V>(p, s);
+      else launch<DT_BF16, false, 256, 1, V>(p, s);
+    }
+  };
+  if (vec) by_type(std::true_type{});
+  else by_type(std::false_type{});
+  return (int)hipGetLastError();
+}
+
+}  // namespace nrm
+}  // namespace spmla
+
+using namespace spmla;
+
+extern "C" {
+
+int spmla_rms_norm(const void* x, long long x_st, const void* residual, long long r_st, void* residual_out,
+                   long long ro_st, const void* weight, int weight_f32, float eps, int T, int D, int dtype, void* out,
+                   long long o_st, unsigned char* codes, long long c_st, float* scales, long long s_st, int ue8m0,
+                   void* stream) {
+  if (T < 0 || D <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.f)) return SPMLA_EARG;
+  if (D > nrm::MAX_D) return SPMLA_ELIMIT;
+  if (T == 0) return SPMLA_OK;
+  if (!x || (residual != nullptr) != (residual_out != nullptr) || (!out && !codes) ||
+      (codes != nullptr) != (scales != nullptr))
+    return SPMLA_EARG;
+  const int eb = dtype == DT_F32 ? 4 : 2;
+  if ((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)residual_out | (uintptr_t)out) & (eb - 1)) ||
+      ((uintptr_t)weight & (weight_f32 ? 3 : eb - 1)) || ((uintptr_t)scales & 3))
+    return SPMLA_EALIGN;
+  nrm::NormParams p{x, x_st, residual, residual_out, r_st, ro_st, weight, weight_f32, eps, T, D,
+                    out, o_st, codes, c_st, scales, s_st, ue8m0};
+  return nrm::go(p, true, dtype, (hipStream_t)stream);
+}
+
+int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsigned char* codes, long long c_st,
+                    float* scales, long long s_st, int ue8m0, void* stream) {
+  if (T < 0 || D <= 0 || dtype < 0 || dtype > 2) return SPMLA_EARG;
+  if (D > 65535 * 2048) return SPMLA_ELIMIT;
+  if (T == 0) return SPMLA_OK;
+  if (!x || !codes || !scales) return SPMLA_EARG;
+  if (((uintptr_t)x & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)scales & 3)) return SPMLA_EALIGN;
+  nrm::NormParams p{x, x_st, nullptr, nullptr, 0, 0, nullptr, 0, 0.f, T, D,
+                    nullptr, 0, codes, c_st, scales, s_st, ue8m0};
+  return nrm::go(p, false, dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

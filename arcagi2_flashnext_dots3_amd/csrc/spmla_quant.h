@@ -1,0 +1,174 @@
+// Shared device helpers of the kernels that encode values: e4m3 and e2m2 codes, quotients, 16-lane reductions, rows of
+// three element types, and the place of a cache slot.
+#pragma once
+#include "spmla_common.h"
+
+namespace spmla {
+
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+
+__device__ inline float wave_max16(float v) {   // max over aligned groups of 16 lanes
+  v = fmaxf(v, __shfl_xor(v, 1, 64));
+  v = fmaxf(v, __shfl_xor(v, 2, 64));
+  v = fmaxf(v, __shfl_xor(v, 4, 64));
+  v = fmaxf(v, __shfl_xor(v, 8, 64));
+  return v;
+}
+
+// e2m2 magnitude index of y = |x| 2^-k >= 0 (offload_rowfmt.py:93-101 with M = 2). The products are exact
+// (powers of two), so the one rounding is the fp32 add of 0.5, as in the reference.
+__device__ inline uint32_t e2m2_mag(float y) {
+  if (y < 1.0f) return (uint32_t)floorf(y * 4.0f + 0.5f);       // 0 .. 4
+  const int e2 = (y >= 2.0f) + (y >= 4.0f);
+  const float inv_stp = u2f((uint32_t)(127 + 2 - e2) << 23);     // 2^(2 - e2)
+  const uint32_t nrm = ((uint32_t)(e2 + 1) << 2) + (uint32_t)floorf(y * inv_stp + 0.5f) - 4u;
+  return nrm < 15u ? nrm : 15u;
+}
+
+__device__ inline uint32_t e4m3x4(float a, float b, float c, float d) {    // no NaN
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// x / s correctly rounded, r = 1 / s correctly rounded, x and s finite (Markstein's division step: the remainder is exact
+// unless x is below 2^-78, where the quotient by s >= 1e-12 encodes to zero either way); the sign is x's
+__device__ inline float quotient(float x, float s, float r) {
+  const float q = x * r;
+  return copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), r, q), x);
+}
+// (slot / n, slot % n) for 0 <= slot: sh = log2 n for a power of two, else -1
+__device__ inline void div_slot(long long slot, int n, int sh, long long& blk, int& off) {
+  if (sh >= 0) { blk = slot >> sh; off = (int)(slot & (n - 1)); }
+  else if ((slot >> 31) == 0) { blk = (uint32_t)slot / (uint32_t)n; off = (int)((uint32_t)slot % (uint32_t)n); }
+  else { blk = slot / n; off = (int)(slot % n); }
+}
+inline int log2_or(int n) { return n > 0 && (n & (n - 1)) == 0 ? __builtin_ctz((unsigned)n) : -1; }
+
+// Row400's latent part from the wave's 512 scaled and clamped values, 8 a lane (the 4 lanes 4b .. 4b + 3 form block b)
+__device__ inline void row400_latent(uint8_t* row, int lane, const float (&x)[8]) {
+  float am = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(x[e]));
+  am = fmaxf(am, __shfl_xor(am, 1, 64));
+  am = fmaxf(am, __shfl_xor(am, 2, 64));
+  const uint32_t rb = f2u(am / 7.0f);
+  const int ex = (int)((rb >> 23) & 255u) - 127;
+  int k = ex + ((rb & 0x7fffffu) != 0u);
+  k = ex < -126 ? -126 : (k < 127 ? k : 127);
+  const float inv = u2f((uint32_t)(127 - k) << 23);                // 2^-k
+  uint32_t nib = 0, sgn = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t mag = e2m2_mag(fabsf(x[e]) * inv);
+    nib |= mag << (4 * e);
+    sgn |= (x[e] < 0.f && mag > 0u ? 1u : 0u) << e;
+  }
+  *(uint32_t*)(row + 4 * lane) = nib;
+  row[R4_SIGN + lane] = (uint8_t)sgn;
+  if ((lane & 3) == 0) row[R4_K + (lane >> 2)] = (uint8_t)(int8_t)k;
+}
+
+// ---- element types of the norm, rotary and linear entry points: their dtype argument
+enum : int { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
+template <int DT> constexpr int elem_bytes = DT == DT_F32 ? 4 : 2;
+
+template <int DT> __device__ inline float load1(const void* p, long long i) {
+  if constexpr (DT == DT_F32) return ((const float*)p)[i];
+  else if constexpr (DT == DT_F16) return (float)((const _Float16*)p)[i];
+  else return bf2f(((const uint16_t*)p)[i]);
+}
+template <int DT> __device__ inline void store1(void* p, long long i, float v) {
+  if constexpr (DT == DT_F32) ((float*)p)[i] = v;
+  else if constexpr (DT == DT_F16) ((_Float16*)p)[i] = (_Float16)v;
+  else ((uint16_t*)p)[i] = f2bf_rne(v);
+}
+template <int DT> __device__ inline float round_to(float v) {      // v rounded to the type
+  if constexpr (DT == DT_F32) return v;
+  else if constexpr (DT == DT_F16) return (float)(_Float16)v;
+  else return bf2f(f2bf_rne(v));
+}
+template <int DT> __device__ inline uint32_t pack2(float a, float b) {   // two values of a 16-bit type
+  if constexpr (DT == DT_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2v));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2v));
+}
+template <int DT> __device__ inline void unpack8(u32x4 a, float (&v)[8]) {   // eight values of a 16-bit type
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == DT_F16) {
+      const f16x2v h = __builtin_bit_cast(f16x2v, (uint32_t)a[e]);
+      v[2 * e] = (float)h[0]; v[2 * e + 1] = (float)h[1];
+    } else {
+      v[2 * e] = u2f(a[e] << 16); v[2 * e + 1] = u2f(a[e] & 0xffff0000u);
+    }
+  }
+}
+// eight values from element i on (16-byte aligned)
+template <int DT> __device__ inline void load8(const void* p, long long i, float (&v)[8]) {
+  if constexpr (DT == DT_F32) {
+    const f32x4 a = *(const f32x4*)((const float*)p + i), b = *(const f32x4*)((const float*)p + i + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+  } else {
+    unpack8<DT>(*(const u32x4*)((const uint16_t*)p + i), v);
+  }
+}
+template <int DT> __device__ inline void store8(void* p, long long i, const float (&v)[8]) {
+  if constexpr (DT == DT_F32) {
+    *(f32x4*)((float*)p + i) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)((float*)p + i + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    *(u32x4*)((uint16_t*)p + i) = u32x4{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
+                                        pack2<DT>(v[6], v[7])};
+  }
+}
+
+// ---- e4m3 codes of eight values of a group of 128 (16 lanes of 8): y = t r, r >= 0 one factor of the group's row
+constexpr float Q_MAX = 448.0f, Q_MIN = 1e-12f;      // largest e4m3 value, smallest scale
+
+// The group's scale: s = max(amax |y| / 448, 1e-12) (ue8m0: rounded up to a power of two); codes of y over s before its
+// rounding to 32 bits. The largest value becomes 448 whatever r is, so without ue8m0 the quotient is 448 t / amax |t|,
+// correctly rounded: t is exact where it is a product of two 16-bit floats, and then so many quotients lie halfway
+// between two codes (one in some thousand) that a quotient by the rounded s would round those by s's rounding error.
+// t and amax are brought to the range in which the remainder of the division is exact by a power of two. A group of
+// infinities or NaNs (or a row factor that is one) is divided element by element: NaN codes for NaNs and inf / inf.
+__device__ inline float group_codes(const float (&t)[8], float r, bool ue8m0, uint32_t& lo, uint32_t& hi) {
+  float am = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(t[e]));
+  am = wave_max16(am);
+  float s = fmaxf(am * r / Q_MAX, Q_MIN);
+  const bool low = !(am * r > Q_MAX * Q_MIN);
+  if (ue8m0) {
+    uint32_t u = f2u(s);
+    if (u & 0x7fffffu) u = (u & 0xff800000u) + 0x800000u;      // the next power of two (or infinity)
+    s = u2f(u);
+  }
+  uint32_t mag = f2u(r) & 0x7fffffffu;       // largest magnitude as an integer: infinities and NaNs above finite ones
+#pragma unroll
+  for (int e = 0; e < 8; ++e) mag = max(mag, f2u(t[e]) & 0x7fffffffu);
+  if (__builtin_expect(__ballot(mag >= 0x7f800000u || f2u(s) >= 0x7f800000u) == 0ull, 1)) {
+    float y[8];
+    if (ue8m0 || low) {
+      const float f = 1.0f / s;              // exact for a power of two
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = ue8m0 ? t[e] * r * f : quotient(t[e] * r, s, f);
+    } else {
+      const float k = am < 0x1p-60f ? 0x1p64f : am > 0x1p100f ? 0x1p-64f : 1.0f;
+      const float a = am * k, f = 1.0f / a, up = Q_MAX * k;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = quotient(t[e] * up, a, f);
+    }
+    lo = e4m3x4(y[0], y[1], y[2], y[3]);
+    hi = e4m3x4(y[4], y[5], y[6], y[7]);
+  } else {
+    lo = hi = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo |= (uint32_t)e4m3_rne(t[e] * r / s) << (8 * e);
+      hi |= (uint32_t)e4m3_rne(t[4 + e] * r / s) << (8 * e);
+    }
+  }
+  return s;
+}
+
+}  // namespace spmla

@@ -19,46 +19,10 @@
 // these kernels (a branchy software encoder and one division per value): finite groups now use the hardware's conversion,
 // which equals e4m3_rne on every fp32 value except the sign of NaNs (all 2^32 compared), and one reciprocal per group.
 // 8192 tokens: rows 8.2 -> 4.9 us, index keys 5.0 -> 3.8; 8 tokens: 4.1 -> 2.6 and 2.9 -> 2.7.
-#include "spmla_common.h"
+#include "spmla_quant.h"
 
 namespace spmla {
 namespace wr {
-
-__device__ inline float wave_max16(float v) {   // max over aligned groups of 16 lanes
-  v = fmaxf(v, __shfl_xor(v, 1, 64));
-  v = fmaxf(v, __shfl_xor(v, 2, 64));
-  v = fmaxf(v, __shfl_xor(v, 4, 64));
-  v = fmaxf(v, __shfl_xor(v, 8, 64));
-  return v;
-}
-
-// e2m2 magnitude index of y = |x| 2^-k >= 0 (offload_rowfmt.py:93-101 with M = 2). The products are exact
-// (powers of two), so the one rounding is the fp32 add of 0.5, as in the reference.
-__device__ inline uint32_t e2m2_mag(float y) {
-  if (y < 1.0f) return (uint32_t)floorf(y * 4.0f + 0.5f);       // 0 .. 4
-  const int e2 = (y >= 2.0f) + (y >= 4.0f);
-  const float inv_stp = u2f((uint32_t)(127 + 2 - e2) << 23);     // 2^(2 - e2)
-  const uint32_t nrm = ((uint32_t)(e2 + 1) << 2) + (uint32_t)floorf(y * inv_stp + 0.5f) - 4u;
-  return nrm < 15u ? nrm : 15u;
-}
-
-__device__ inline uint32_t e4m3x4(float a, float b, float c, float d) {    // no NaN
-  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
-// x / s correctly rounded, r = 1 / s correctly rounded, x and s finite (Markstein's division step: the remainder is exact
-// unless x is below 2^-78, where the quotient by s >= 1e-12 encodes to zero either way); the sign is x's
-__device__ inline float quotient(float x, float s, float r) {
-  const float q = x * r;
-  return copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), r, q), x);
-}
-// (slot / n, slot % n) for 0 <= slot: sh = log2 n for a power of two, else -1
-__device__ inline void div_slot(long long slot, int n, int sh, long long& blk, int& off) {
-  if (sh >= 0) { blk = slot >> sh; off = (int)(slot & (n - 1)); }
-  else if ((slot >> 31) == 0) { blk = (uint32_t)slot / (uint32_t)n; off = (int)((uint32_t)slot % (uint32_t)n); }
-  else { blk = slot / n; off = (int)(slot % n); }
-}
-inline int log2_or(int n) { return n > 0 && (n & (n - 1)) == 0 ? __builtin_ctz((unsigned)n) : -1; }
 
 struct WriteParams {
   const uint16_t* kv; long long kv_st;      // kv_c_normed[n][512] bf16
@@ -114,30 +78,10 @@ __global__ void __launch_bounds__(256) cache_write_kernel(WriteParams p) {
     if ((lane & 15) == 0) *(float*)(row + SC_OFF + (lane >> 4) * 4) = s;
     if (lane < 16) *(uint2*)(row + ROPE_OFF + lane * 8) = rope;   // 64 bf16 = 16 x 8 bytes
   } else if (p.fmt == 2) {
-    // Row400: lane l holds values 8l .. 8l + 7; the 4 lanes 4b .. 4b + 3 form exponent block b
-    float am = 0.f;
+    // Row400: lane l holds values 8l .. 8l + 7
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = fminf(fmaxf(x[e] * p.inv_scale, -448.f), 448.f);
-      am = fmaxf(am, fabsf(x[e]));
-    }
-    am = fmaxf(am, __shfl_xor(am, 1, 64));
-    am = fmaxf(am, __shfl_xor(am, 2, 64));
-    const uint32_t rb = f2u(am / 7.0f);
-    const int ex = (int)((rb >> 23) & 255u) - 127;
-    int k = ex + ((rb & 0x7fffffu) != 0u);
-    k = ex < -126 ? -126 : (k < 127 ? k : 127);
-    const float inv = u2f((uint32_t)(127 - k) << 23);                // 2^-k
-    uint32_t nib = 0, sgn = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t mag = e2m2_mag(fabsf(x[e]) * inv);
-      nib |= mag << (4 * e);
-      sgn |= (x[e] < 0.f && mag > 0u ? 1u : 0u) << e;
-    }
-    *(uint32_t*)(row + 4 * lane) = nib;
-    row[R4_SIGN + lane] = (uint8_t)sgn;
-    if ((lane & 3) == 0) row[R4_K + (lane >> 2)] = (uint8_t)(int8_t)k;
+    for (int e = 0; e < 8; ++e) x[e] = clamped(x[e]);
+    row400_latent(row, lane, x);
     if (lane < 16) {   // rope: 64 values -> 64 e4m3 codes, 4 per lane
       const uint32_t c = e4m3x4(clamped(u2f(rope.x << 16)), clamped(u2f(rope.x & 0xffff0000u)), clamped(u2f(rope.y << 16)),
                                 clamped(u2f(rope.y & 0xffff0000u)));
@@ -224,7 +168,7 @@ int spmla_cache_write(const void* kv_c, long long kv_st, const void* k_pe, long 
   if (fmt != 0 && !(kv_scale > 0.f)) return SPMLA_EARG;
   wr::WriteParams p;
   p.kv = (const uint16_t*)kv_c; p.kv_st = kv_st; p.pe = (const uint16_t*)k_pe; p.pe_st = pe_st;
-  p.slots = slots; p.n = n; p.cache = (uint8_t*)cache; p.R = R; p.bs = block_size; p.sh = wr::log2_or(block_size); p.blk_stride = block_stride;
+  p.slots = slots; p.n = n; p.cache = (uint8_t*)cache; p.R = R; p.bs = block_size; p.sh = log2_or(block_size); p.blk_stride = block_stride;
   p.fmt = fmt; p.inv_scale = fmt != 0 ? 1.0f / kv_scale : 1.0f;
   hipLaunchKernelGGL(wr::cache_write_kernel, dim3((n + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
   return (int)hipGetLastError();
@@ -241,7 +185,7 @@ int spmla_index_key_write(const void* k, long long k_st, const long long* slots,
     return SPMLA_EALIGN;
   wr::KeyParams p;
   p.k = (const uint16_t*)k; p.k_st = k_st; p.slots = slots; p.n = n; p.store = (uint8_t*)store;
-  p.R_local = R_local; p.P = P; p.rank = rank; p.rpb = rows_per_block; p.sh = wr::log2_or(rows_per_block); p.blk_stride = block_stride; p.ue8m0 = ue8m0;
+  p.R_local = R_local; p.P = P; p.rank = rank; p.rpb = rows_per_block; p.sh = log2_or(rows_per_block); p.blk_stride = block_stride; p.ue8m0 = ue8m0;
   p.shuf = 0;
   hipLaunchKernelGGL(wr::key_write_kernel, dim3((n + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
   return (int)hipGetLastError();
@@ -258,7 +202,7 @@ int spmla_index_key_write_shuffle(const void* k, long long k_st, const long long
     return SPMLA_EALIGN;
   wr::KeyParams p;
   p.k = (const uint16_t*)k; p.k_st = k_st; p.slots = slots; p.n = n; p.store = (uint8_t*)cache;
-  p.R_local = num_blocks * block_size; p.P = 1; p.rank = 0; p.rpb = block_size; p.sh = wr::log2_or(block_size); p.blk_stride = block_stride;
+  p.R_local = num_blocks * block_size; p.P = 1; p.rank = 0; p.rpb = block_size; p.sh = log2_or(block_size); p.blk_stride = block_stride;
   p.ue8m0 = ue8m0; p.shuf = 1;
   hipLaunchKernelGGL(wr::key_write_kernel, dim3((n + 3) / 4), dim3(256), 0, (hipStream_t)stream, p);
   return (int)hipGetLastError();

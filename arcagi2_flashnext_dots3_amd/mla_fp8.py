@@ -4,6 +4,9 @@ mla_fp8.py) and the in-place decode query build of qcat.py, on libspmla_gfx950.s
 kv_b_proj is block-FP8 in the checkpoint (128 x 128 blocks, weight_scale_inv); vLLM's bf16 W_UK_T / W_UV are
 round_bf16(code * scale). convert() recovers the codes exactly (checked bit for bit after the round trip, mla_fp8.py:
 89-94) so the kernels read half the weight bytes and dequantize to the same bf16 values in registers.
+
+linear_fp8() is the layer's plain projections (down, up, output) on the checkpoint's codes and block scales, with the
+activations in 8 bits too.
 """
 import torch
 
@@ -48,6 +51,20 @@ def bmm_fp8(a, f, out=None):
     if out is None:
         out = torch.empty((a.shape[0], a.shape[1], codes.shape[1]), dtype=a.dtype, device=a.device)
     return kernels.bmm_fp8(a, codes, scales, scale_k, out)
+
+
+def linear_fp8(x, f, out=None, ue8m0=False):
+    """x [T, K] bf16 / fp16, quantized here per 128 values (kernels.quant_fp8), or (codes, scales) from
+    kernels.rms_norm_fp8 / quant_fp8; f = (weight codes [N, K] e4m3, weight_scale_inv [ceil(N / 128), ceil(K / 128)])
+    -> out [T, N] in x's type (bf16 for codes)."""
+    codes, scales = f
+    if isinstance(x, torch.Tensor):
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("linear_fp8: x bf16 / fp16, or (codes, scales)")
+        a, sa = kernels.quant_fp8(x, ue8m0=ue8m0)
+        return kernels.linear_fp8(a, sa, codes, scales, out=out, dtype=x.dtype)
+    a, sa = x
+    return kernels.linear_fp8(a, sa, codes, scales, out=out)
 
 
 def build_query(q_nope, q_pe, f_uk, out=None):
