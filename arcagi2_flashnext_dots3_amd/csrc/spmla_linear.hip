@@ -9,10 +9,13 @@
 // (4.5e-5 with 1 of 64 values 50 times the others), a hundredth of the 16-bit output's rounding; fp32 outputs are not
 // offered. Blocks are summed in fp32.
 //
-// Operands reach LDS by direct copies, 128-byte rows with their 16-byte chunks permuted by (row & 7), so that the
-// fragment reads of 16 rows fall on distinct banks. In the last block of a k that is no multiple of 128 the chunks
+// Operands reach LDS by direct copies, 128-byte rows with their 16-byte chunks permuted by (row / 2) % 8. A lane reads
+// chunks g and g + 4 of its row (g = l / 16): the 16 lanes that LDS serves at once (0-3, 12-15, 20-23, 24-27 and so on)
+// then fall on distinct banks, 256 bytes a clock (with chunks 2 g and 2 g + 1 two of them meet in every bank: 128). Which
+// 32 values of k a lane holds does not matter, since both operands hold the same ones. In the last block of a k that is no multiple of 128 the chunks
 // behind k are read from the row's last chunk and the weights' are overwritten with zeros in LDS.
 #include "spmla_quant.h"
+#include "spmla_rules.h"
 
 namespace spmla {
 namespace lin {
@@ -38,16 +41,32 @@ __device__ inline void dma4s(const void* base, uint32_t off, SPMLA_LDS void* l) 
   const uint32_t d = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)l);
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(d) : "memory", "m0");
 }
+// the same of 4 or 16 bytes a lane for the lanes of a mask below 2^32 of a full wave
+template <int BYTES>
+__device__ inline void dma_lo(const void* base, uint32_t off, SPMLA_LDS void* l, uint32_t lanes) {
+  static_assert(BYTES == 4 || BYTES == 16, "copies of 4 or 16 bytes a lane");
+  const uint32_t d = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)l), m = __builtin_amdgcn_readfirstlane(lanes);
+  if (BYTES == 4)
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_hi, 0\n\ts_mov_b32 exec_lo, %3\n\t"
+                 "global_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1"
+                 ::"v"(off), "s"(base), "s"(d), "s"(m) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_hi, 0\n\ts_mov_b32 exec_lo, %3\n\t"
+                 "global_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
+                 ::"v"(off), "s"(base), "s"(d), "s"(m) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
-__device__ inline i32x8 frag(const uint8_t* rows, int r, int g) {   // row r's bytes 32 g .. + 31 of a staged block
-  const i32x4 lo = *(const i32x4*)(rows + r * 128 + (((2 * g) ^ (r & 7)) << 4));
-  const i32x4 hi = *(const i32x4*)(rows + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4));
+__device__ inline i32x8 frag(const uint8_t* rows, int r, int g) {   // row r's chunks g and g + 4 of a staged block
+  const i32x4 lo = *(const i32x4*)(rows + r * 128 + ((g ^ ((r >> 1) & 7)) << 4));
+  const i32x4 hi = *(const i32x4*)(rows + r * 128 + (((g + 4) ^ ((r >> 1) & 7)) << 4));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 __device__ inline f32x4 block_sum(i32x8 w, i32x8 a) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
+typedef const __attribute__((address_space(4))) float* scalar_floats;   // read with scalar loads: uniform, not written here
+
 template <int DT>
 __device__ inline void store4(const LinearParams& p, int t, int n, f32x4 v) {   // outputs n .. n + 3 of token t
   if (t >= p.T) return;
@@ -61,97 +80,157 @@ __device__ inline void store4(const LinearParams& p, int t, int n, f32x4 v) {   
   }
 }
 
-// ---- tiles of BM tokens x BN outputs, a wave WM x WN of them; two stages of one block in LDS -----------------------
-template <int BM, int BN, int WM, int WN>
-struct Tile {
-  static constexpr int NWM = BM / WM, NW = NWM * (BN / WN);
+// ---- tiles of BM tokens x BN outputs, 8 waves of WM x WN, a ring of ST blocks in LDS ----------------------------------
+// While the sums of block b form from registers, block b + 1 is read from LDS and blocks b + 2 .. b + ST are on their way:
+// one barrier a block, behind which block b's place is free and block b + 1 has arrived.
+template <int BM, int BN, int WM, int WN, int ST>
+struct Ring {
+  static constexpr int NW = 8, NWM = BM / WM, PA = BM / 64, PW = BN / 64, NI = PA + PW + 1;   // copies of a wave and block
   static constexpr int AS = 0, WS = BM * 128, SS = WS + BN * 128, STAGE = SS + BM * 4;
-  static constexpr int LDS = 2 * STAGE;
-  static_assert(BM % 64 == 0 && BN % 64 == 0 && 128 % WN == 0 && LDS <= 160 * 1024, "tile");
+  static constexpr int LDS = ST * STAGE;
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && NWM * (BN / WN) == NW && 128 % WN == 0 && BM / NW <= 32 && ST >= 3 &&
+                ST * NI < 64 && LDS <= 160 * 1024, "ring");
 };
 
-template <int DT, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) tile_kernel(LinearParams p, int TN) {
-  using C = Tile<BM, BN, WM, WN>;
+template <int DT, int BM, int BN, int WM, int WN, int ST>
+__global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
+  using C = Ring<BM, BN, WM, WN, ST>;
+  constexpr int MT = WM / 16, NT = WN / 16;
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
-  const int L = remap_xcd((int)blockIdx.x, TN * ((p.T + BM - 1) / BM));
+  const int TM = (p.T + BM - 1) / BM, L = remap_xcd((int)blockIdx.x, TN * TM);
   if (L < 0) return;
-  const int t0 = (L / TN) * BM, n0 = (L % TN) * BN;
+  // four rows of tiles at a time, column by column: the tiles that an XCD works on share rows and columns
+  const int grp = L / (4 * TN), rem = L - grp * 4 * TN, gm = min(4, TM - grp * 4);
+  const int t0 = (grp * 4 + rem % gm) * BM, n0 = rem / gm * BN;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = (wv % C::NWM) * WM, wn = (wv / C::NWM) * WN;
   const int r = lane & 15, g = lane >> 4;
   const int kb = (p.K + 127) / 128, kt = p.K - (kb - 1) * 128;       // blocks, values of the last one
-  // copies: rows of 128 bytes, 8 a copy, dealt over the waves; a lane's chunk is (lane % 8) ^ (row % 8)
-  constexpr int PA = (BM / 8 + C::NW - 1) / C::NW, PW = (BN / 8 + C::NW - 1) / C::NW;
-  const int ch = (lane & 7) ^ (lane >> 3);
+  // copies: rows of 128 bytes, 8 a copy, dealt over the waves; a lane's chunk is (lane % 8) ^ (row / 2 % 8), the same in
+  // all of a wave's copies
+  const int ch = (lane & 7) ^ ((lane >> 4) + (wv & 1) * 4);
   const uint32_t over = ch * 16 < kt ? 0u : (uint32_t)(ch * 16 - kt + 16);     // back to the last chunk below k
   const uint8_t* ab = p.a + (long long)t0 * p.a_st;
   const uint8_t* wb = p.w + (long long)n0 * p.w_st;
   const float* sb = p.sa + (long long)t0 * p.sa_st;
-  uint32_t va[PA], vw[PW], vs;
+  uint32_t va[C::PA], vw[C::PW];
 #pragma unroll
-  for (int j = 0; j < PA; ++j) {
-    const int row = min((j * C::NW + wv) * 8 + (lane >> 3), p.T - 1 - t0);
+  for (int j = 0; j < C::PA; ++j) {
+    const int row = min((j * 8 + wv) * 8 + (lane >> 3), p.T - 1 - t0);
     va[j] = (uint32_t)(row * p.a_st) + ch * 16;
   }
 #pragma unroll
-  for (int j = 0; j < PW; ++j) {
-    const int row = min((j * C::NW + wv) * 8 + (lane >> 3), p.N - 1 - n0);
+  for (int j = 0; j < C::PW; ++j) {
+    const int row = min((j * 8 + wv) * 8 + (lane >> 3), p.N - 1 - n0);
     vw[j] = (uint32_t)(row * p.w_st) + ch * 16;
   }
-  vs = (uint32_t)(min(wv * 64 + lane, p.T - 1 - t0) * p.sa_st * 4);
-  auto issue = [&](int b) {
-    SPMLA_LDS uint8_t* st = (SPMLA_LDS uint8_t*)sm + (b & 1) * C::STAGE;
+  const uint32_t vs = (uint32_t)(min(wv * (BM / 8) + (lane & 31), p.T - 1 - t0) * p.sa_st * 4);
+  SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)sm;
+  auto copy = [&](int b, int slot, int c) {                          // number c of a block's NI copies
+    SPMLA_LDS uint8_t* st = lds + slot * C::STAGE;
     const uint32_t back = b == kb - 1 ? over : 0u;
-#pragma unroll
-    for (int j = 0; j < PA; ++j)
-      if ((j * C::NW + wv) * 8 < BM) dma16s(ab + b * 128, va[j] - back, st + C::AS + (j * C::NW + wv) * 1024);
-#pragma unroll
-    for (int j = 0; j < PW; ++j)
-      if ((j * C::NW + wv) * 8 < BN) dma16s(wb + b * 128, vw[j] - back, st + C::WS + (j * C::NW + wv) * 1024);
-    if (wv * 64 < BM) dma4s(sb + b, vs, st + C::SS + wv * 256);
+    if (c < C::PA) dma16s(ab + b * 128, va[c < C::PA ? c : 0] - back, st + C::AS + (c * 8 + wv) * 1024);
+    else if (c < C::PA + C::PW)
+      dma16s(wb + b * 128, vw[c >= C::PA && c < C::PA + C::PW ? c - C::PA : 0] - back, st + C::WS + ((c - C::PA) * 8 + wv) * 1024);
+    else dma_lo<4>(sb + b, vs, st + C::SS + wv * (BM / 8) * 4, BM / 8 == 32 ? ~0u : (1u << (BM / 8)) - 1u);
   };
-  const float* swr = p.sw + (long long)(min(n0 + wn, p.N - 1) / 128) * p.sw_st;
-  float swv = swr[min(lane, kb - 1)];
-  constexpr int MT = WM / 16, NT = WN / 16;
+  const scalar_floats swr = (scalar_floats)(p.sw + (long long)(min(n0 + wn, p.N - 1) / 128) * p.sw_st);
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  issue(0);
-  for (int b = 0; b < kb; ++b) {
-    wait_vm<0>();
-    lds_barrier();                       // block b has arrived; everyone is done with block b - 1
-    uint8_t* st = sm + (b & 1) * C::STAGE;
-    if (b == kb - 1 && kt < 128) {       // zeros behind k, one operand is enough
-      for (int i = threadIdx.x; i < BN * 8; i += 64 * C::NW) {
-        const int row = i >> 3, c = (i & 7) ^ (row & 7);
-        if (c * 16 >= kt) *(u32x4*)(st + C::WS + i * 16) = u32x4{0, 0, 0, 0};
-      }
-      lds_barrier();
+  struct Frags {
+    i32x8 a[MT], w[NT];
+    float s[MT], sw;
+  };
+  const bool z0 = g * 16 >= kt, z1 = (g + 4) * 16 >= kt;             // chunks behind k in the last block
+  constexpr int NR = NT + MT + 1;
+  auto read = [&](int b, int slot, Frags& f, int c) {                 // part c of NR: a fragment, last the scales
+    const uint8_t* st = sm + slot * C::STAGE;
+    if (c < NT) f.w[c < NT ? c : 0] = frag(st + C::WS, wn + c * 16 + r, g);
+    else if (c < NT + MT) f.a[c >= NT && c < NT + MT ? c - NT : 0] = frag(st + C::AS, wm + (c - NT) * 16 + r, g);
+    else {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) f.s[j] = *(const float*)(st + C::SS + (wm + j * 16 + r) * 4);
+      f.sw = swr[min(b, kb - 1)];
     }
-    if (b + 1 < kb) issue(b + 1);
-    if (b && (b & 63) == 0) swv = swr[min(b + lane, kb - 1)];
-    const float sw = u2f(__builtin_amdgcn_readlane(f2u(swv), b & 63));
-    i32x8 av[MT];
+  };
+  auto clip = [&](int b, Frags& f) {                                  // zeros behind k, one operand is enough
+    const bool y0 = z0 && b == kb - 1, y1 = z1 && b == kb - 1;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f.w[i][e] = y0 ? 0 : f.w[i][e];
+        f.w[i][4 + e] = y1 ? 0 : f.w[i][4 + e];
+      }
+  };
+  // the sums of row tile i run while those of i - 1 are added; between(m) behind matrix instruction m
+  auto sums = [&](const Frags& f, auto between) {
+    f32x4 d[2][MT];
     float sc[MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      av[j] = frag(st + C::AS, wm + j * 16 + r, g);
-      sc[j] = *(const float*)(st + C::SS + (wm + j * 16 + r) * 4) * sw;
-    }
+    for (int j = 0; j < MT; ++j) sc[j] = f.s[j] * f.sw;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const i32x8 wf = frag(st + C::WS, wn + i * 16 + r, g);
+    for (int i = 0; i <= NT; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const f32x4 d = block_sum(wf, av[j]);
+        if (i < NT) {
+          d[i & 1][j] = block_sum(f.w[i], f.a[j]);
+          between(i * MT + j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i > 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(d[e], sc[j], acc[i][j][e]);
+          for (int e = 0; e < 4; ++e) acc[i - 1][j][e] = __builtin_fmaf(d[(i - 1) & 1][j][e], sc[j], acc[i - 1][j][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
+  };
+  int in = 0, out = 0;                                                // slots of the next block to copy and to read
+  auto next = [](int& s) { s = s + 1 == ST ? 0 : s + 1; };
+  // (behind the last block it is copied again, so that the waits count the same copies everywhere)
+  for (int b = 0; b < ST; ++b) {
+#pragma unroll
+    for (int c = 0; c < C::NI; ++c) copy(min(b, kb - 1), b, c);
   }
+  wait_vm<(ST - 1) * C::NI>();
+  lds_barrier();
+  Frags f[2];
+#pragma unroll
+  for (int c = 0; c < NR; ++c) read(0, 0, f[0], c);
+  next(out);
+  // one block: f its fragments, n the next one's
+  auto block = [&](int b, auto tail, const Frags& f, Frags& n) {
+    wait_vm<(ST - 2) * C::NI>();
+    lds_barrier();
+    // the reads and copies lie between the matrix instructions: issued together they hold up the wave behind them, since
+    // all waves would issue theirs at once
+    sums(f, [&](int m) {
+#pragma unroll
+      for (int c = 0; c < NR; ++c)
+        if (c * NT * MT / NR == m) read(b + 1, out, n, c);
+#pragma unroll
+      for (int c = 0; c < C::NI; ++c)
+        if (c * NT * MT / C::NI == m) copy(min(b + ST, kb - 1), in, c);
+    });
+    next(out);
+    next(in);
+    if constexpr (decltype(tail)::value) clip(b + 1, n);
+  };
+  auto blocks = [&](auto tail) {                                      // tail: the last block is a part of one
+    if constexpr (decltype(tail)::value) clip(0, f[0]);
+    int b = 0;
+    for (; b + 1 < kb; b += 2) {
+      block(b, tail, f[0], f[1]);
+      block(b + 1, tail, f[1], f[0]);
+    }
+    if (b < kb) block(b, tail, f[0], f[1]);
+  };
+  if (kt == 128) blocks(std::false_type{});
+  else blocks(std::true_type{});
+  wait_vm<0>();                                                       // no copy outlives the workgroup
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -159,22 +238,376 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) tile_kernel(Linear
       if (n0 + wn + i * 16 + 4 * g < p.N) store4<DT>(p, t0 + wm + j * 16 + r, n0 + wn + i * 16 + 4 * g, acc[i][j]);
 }
 
-template <int DT, int BM, int BN, int WM, int WN>
-static int tile_go(const LinearParams& p, hipStream_t s) {
-  using C = Tile<BM, BN, WM, WN>;
+template <int DT, int BM, int BN, int WM, int WN, int ST>
+static int ring_go(const LinearParams& p, hipStream_t s) {
+  using C = Ring<BM, BN, WM, WN, ST>;
   static DynLds lds;
-  if (int rc = lds.ensure((const void*)tile_kernel<DT, BM, BN, WM, WN>, C::LDS)) return rc;
+  if (int rc = lds.ensure((const void*)ring_kernel<DT, BM, BN, WM, WN, ST>, C::LDS)) return rc;
   const int TN = (p.N + BN - 1) / BN;
   const long long n = (long long)TN * ((p.T + BM - 1) / BM);
   if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
-  hipLaunchKernelGGL((tile_kernel<DT, BM, BN, WM, WN>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * C::NW), C::LDS, s, p,
-                     TN);
+  hipLaunchKernelGGL((ring_kernel<DT, BM, BN, WM, WN, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), C::LDS, s, p, TN);
   return (int)hipGetLastError();
 }
 
+// ---- few tokens: the weights stream past 16 MT tokens --------------------------------------------------------------
+// A workgroup takes 16 NT outputs and 16 MT tokens; its NW waves take the blocks of k in turn, each with a ring of ST
+// stages of its own in LDS, so that no wave waits for another until their sums meet in LDS at the end, in wave order.
+template <int NT, int MT, int NW, int ST>
+struct Stream {
+  static constexpr int WS = 0, AS = NT * 2048, SS = AS + MT * 2048, STAGE = SS + 256;
+  static constexpr int NI = 2 * NT + 2 * MT + 1;                     // copies of a stage
+  static constexpr int RING = NW * ST * STAGE, RED = NW * NT * MT * 1024;
+  static constexpr int LDS = RING > RED ? RING : RED;
+  static_assert(MT <= 4 && (ST - 1) * NI < 64 && LDS <= 160 * 1024, "stream");
+};
+
+template <int DT, int NT, int MT, int NW, int ST>
+__global__ void __launch_bounds__(64 * NW, 2) stream_kernel(LinearParams p, int TM) {
+  using C = Stream<NT, MT, NW, ST>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
+  const int L = remap_xcd((int)blockIdx.x, TM * ((p.N + 16 * NT - 1) / (16 * NT)));
+  if (L < 0) return;
+  const int t0 = (L % TM) * 16 * MT, n0 = (L / TM) * 16 * NT;        // the token tiles of a row of weights: one XCD
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int r = lane & 15, g = lane >> 4;
+  const int kb = (p.K + 127) / 128, kt = p.K - (kb - 1) * 128;
+  const int cnt = wv < kb ? (kb - wv + NW - 1) / NW : 0;             // blocks wv, wv + NW, ..
+  const int ce = (lane & 7) ^ (lane >> 4), co = ce ^ 4;              // a lane's chunk in even and odd copies of 8 rows
+  auto over = [&](int j) { const int c = j & 1 ? co : ce; return c * 16 < kt ? 0u : (uint32_t)(c * 16 - kt + 16); };
+  const uint8_t* ab = p.a + (long long)t0 * p.a_st;
+  const uint8_t* wb = p.w + (long long)n0 * p.w_st;
+  const float* sb = p.sa + (long long)t0 * p.sa_st;
+  uint32_t va[2 * MT], vw[2 * NT];
+#pragma unroll
+  for (int j = 0; j < 2 * MT; ++j) va[j] = (uint32_t)(min(j * 8 + (lane >> 3), p.T - 1 - t0) * p.a_st) + (j & 1 ? co : ce) * 16;
+#pragma unroll
+  for (int j = 0; j < 2 * NT; ++j) vw[j] = (uint32_t)(min(j * 8 + (lane >> 3), p.N - 1 - n0) * p.w_st) + (j & 1 ? co : ce) * 16;
+  const uint32_t vs = (uint32_t)(min(lane, p.T - 1 - t0) * p.sa_st * 4);
+  uint8_t* ring = sm + wv * ST * C::STAGE;
+  const scalar_floats swr = (scalar_floats)(p.sw + (long long)(n0 / 128) * p.sw_st);   // 16 NT outputs: one block of 128
+  auto issue = [&](int i) {
+    SPMLA_LDS uint8_t* st = (SPMLA_LDS uint8_t*)ring + (i % ST) * C::STAGE;
+    const int b = wv + NW * i;
+    const bool last = b == kb - 1;
+#pragma unroll
+    for (int j = 0; j < 2 * NT; ++j) dma16s(wb + b * 128, vw[j] - (last ? over(j) : 0u), st + C::WS + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j) dma16s(ab + b * 128, va[j] - (last ? over(j) : 0u), st + C::AS + j * 1024);
+    dma4s(sb + b, vs, st + C::SS);
+  };
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < ST; ++i)
+    if (i < cnt) issue(i);
+  for (int i = 0; i < cnt; ++i) {
+    if (i + ST <= cnt) wait_vm<(ST - 1) * C::NI>();
+    else wait_vm<0>();
+    uint8_t* st = ring + (i % ST) * C::STAGE;
+    const int b = wv + NW * i;
+    if (b == kb - 1 && kt < 128) {       // zeros behind k, one operand is enough
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j)
+        if ((j & 1 ? co : ce) * 16 >= kt) *(u32x4*)(st + C::WS + j * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+    }
+    const float sw = swr[b];
+    i32x8 av[MT], wf[NT];
+    float sc[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wf[j] = frag(st + C::WS, j * 16 + r, g);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      av[j] = frag(st + C::AS, j * 16 + r, g);
+      sc[j] = *(const float*)(st + C::SS + (j * 16 + r) * 4) * sw;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the stage has been read: its ring place is free
+    if (i + ST < cnt) issue(i + ST);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const f32x4 d = block_sum(wf[n], av[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][j][e] = __builtin_fmaf(d[e], sc[j], acc[n][j][e]);
+      }
+  }
+  lds_barrier();                         // every ring is done with
+  f32x4* red = (f32x4*)sm;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[(wv * NT * MT + n * MT + j) * 64 + lane] = acc[n][j];
+  lds_barrier();
+#pragma unroll
+  for (int k = 0; k < (NT * MT + NW - 1) / NW; ++k) {
+    const int e = wv + k * NW;
+    if (e < NT * MT) {
+      f32x4 v = red[e * 64 + lane];
+#pragma unroll
+      for (int u = 1; u < NW; ++u) v += red[(u * NT * MT + e) * 64 + lane];
+      const int n = n0 + (e / MT) * 16 + 4 * g;
+      if (n < p.N) store4<DT>(p, t0 + (e % MT) * 16 + r, n, v);
+    }
+  }
+}
+
+template <int DT, int NT, int MT, int NW, int ST>
+static int stream_go(const LinearParams& p, hipStream_t s) {
+  using C = Stream<NT, MT, NW, ST>;
+  static DynLds lds;
+  if (int rc = lds.ensure((const void*)stream_kernel<DT, NT, MT, NW, ST>, C::LDS)) return rc;
+  const int TM = (p.T + 16 * MT - 1) / (16 * MT);
+  const long long n = (long long)TM * ((p.N + 16 * NT - 1) / (16 * NT));
+  if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
+  hipLaunchKernelGGL((stream_kernel<DT, NT, MT, NW, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * NW), C::LDS, s, p,
+                     TM);
+  return (int)hipGetLastError();
+}
+
+
+// ---- long chunks: tiles of 256 tokens x 256 outputs, 8 waves, the operands' halves in rings of their own --------------
+// The tile's tokens and outputs are two halves of 128 each (A0, A1, W0, W1); wave (wm, wn) takes tokens 64 wm .. + 63 of
+// both token halves and outputs 32 wn .. + 31 of both output halves: four quadrants of 8 matrix instructions each,
+//   phase 0: A0 W0   1: A0 W1   2: A1 W0   3: A1 W1.
+// A half is read into registers one phase before it is used (W1 in phase 0, A1 in 1, W0 and A0 of the next block in 3, each
+// token fragment over the one that had its last use), so its place in LDS is free again long before the block is done: the
+// copies of block b + 2 start in block b and have 1.75 blocks to arrive. A workgroup barrier stands before the phases that
+// read, behind a wait for the wave's own copies of what they read. A sum is scaled and added three matrix instructions
+// after its own. A wave's copies: 5 for A0, W0 and the scales of 32 tokens, 2 for W1, 2 for A1.
+struct Big {
+  static constexpr int HALF = 128 * 128, A = 0, W = 4 * HALF, S = 8 * HALF;   // A [stage][half], W the same, then scales
+  static constexpr int LDS = S + 8 * 1024;         // of the 256 tokens: [block % 4], or 4 blocks at once [block / 4 % 2]
+};
+
+template <int DT, bool V4>
+__global__ void __launch_bounds__(512, 2) big_kernel(LinearParams p, int TN) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
+  const int TM = (p.T + 255) / 256, L = remap_xcd((int)blockIdx.x, TN * TM);
+  if (L < 0) return;
+  // four rows of tiles at a time, column by column: the 32 tiles that an XCD works on share 4 rows and 8 columns
+  const int grp = L / (4 * TN), rem = L - grp * 4 * TN, gm = min(4, TM - grp * 4);
+  const int t0 = (grp * 4 + rem % gm) * 256, n0 = rem / gm * 256;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wv & 1, wn = wv >> 1, r = lane & 15, g = lane >> 4;
+  const int kb = (p.K + 127) / 128, kt = p.K - (kb - 1) * 128;
+  // copies: wave wv takes rows 16 wv .. + 15 of a half, 8 a copy; a lane's chunk is (lane % 8) ^ (row / 2 % 8)
+  const int ce = (lane & 7) ^ (lane >> 4), co = ce ^ 4;
+  const uint32_t oe = ce * 16 < kt ? 0u : (uint32_t)(ce * 16 - kt + 16), oo = co * 16 < kt ? 0u : (uint32_t)(co * 16 - kt + 16);
+  const uint8_t* ab = p.a + (long long)t0 * p.a_st;
+  const uint8_t* wb = p.w + (long long)n0 * p.w_st;
+  const float* sb = p.sa + (long long)t0 * p.sa_st;
+  uint32_t va[2][2], vw[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = h * 128 + wv * 16 + j * 8 + (lane >> 3);
+      va[h][j] = (uint32_t)(min(row, p.T - 1 - t0) * p.a_st) + (j ? co : ce) * 16;
+      vw[h][j] = (uint32_t)(min(row, p.N - 1 - n0) * p.w_st) + (j ? co : ce) * 16;
+    }
+  }
+  const uint32_t vs = (uint32_t)(min(wv * 32 + (lane & 31), p.T - 1 - t0) * p.sa_st * 4);
+  SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)sm;
+  auto copy_a = [&](int b, int h, int c) {
+    SPMLA_LDS uint8_t* d = lds + Big::A + ((b & 1) * 2 + h) * Big::HALF + wv * 2048;
+    dma16s(ab + b * 128, va[h][c] - (b == kb - 1 ? (c ? oo : oe) : 0u), d + c * 1024);
+  };
+  auto copy_s = [&](int b) {
+    if (V4) dma_lo<16>(sb + b, vs, lds + Big::S + (b & 4) * 1024 + wv * 512, b & 3 ? 0u : ~0u);
+    else dma_lo<4>(sb + b, vs, lds + Big::S + (b & 3) * 1024 + wv * 128, ~0u);
+  };
+  auto copy_w = [&](int b, int h, int c) {
+    SPMLA_LDS uint8_t* d = lds + Big::W + ((b & 1) * 2 + h) * Big::HALF + wv * 2048;
+    dma16s(wb + b * 128, vw[h][c] - (b == kb - 1 ? (c ? oo : oe) : 0u), d + c * 1024);
+  };
+  auto first = [&](int b) {                                           // a whole block, in the order of the loop's copies
+    copy_a(b, 0, 0);
+    copy_a(b, 0, 1);
+    copy_s(b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) copy_w(b, c >> 1, c & 1);
+    copy_a(b, 1, 0);
+    copy_a(b, 1, 1);
+  };
+  // fragment places of this lane: row r of a 16-row tile, chunks g and g + 4
+  const int f0 = r * 128 + ((g ^ (r >> 1)) << 4), f1 = f0 ^ 64;
+  auto get = [&](const uint8_t* base) {
+    const i32x4 lo = *(const i32x4*)(base + f0), hi = *(const i32x4*)(base + f1);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto a_at = [&](int b, int h, int j) { return sm + Big::A + ((b & 1) * 2 + h) * Big::HALF + (wm * 64 + j * 16) * 128; };
+  auto w_at = [&](int b, int h, int i) { return sm + Big::W + ((b & 1) * 2 + h) * Big::HALF + (wn * 32 + i * 16) * 128; };
+  auto scale_at = [&](int b, int h, int j) {
+    const int t = h * 128 + wm * 64 + j * 16 + r;
+    return *(const float*)(sm + Big::S + (V4 ? (b & 4) * 1024 + t * 16 + (b & 3) * 4 : (b & 3) * 1024 + t * 4));
+  };
+  const bool z0 = g * 16 >= kt, z1 = (g + 4) * 16 >= kt;      // chunks behind k in the last block
+  auto clip = [&](int b, i32x8& w) {                                  // zeros behind k, one operand is enough
+    const bool y0 = z0 && b == kb - 1, y1 = z1 && b == kb - 1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = y0 ? 0 : w[e];
+      w[4 + e] = y1 ? 0 : w[4 + e];
+    }
+  };
+  constexpr int NS = V4 ? 0 : 1;      // scale copies of a block that are there for certain (those of no lane may not count)
+  const int nb1 = min(n0 / 128 + 1, (p.N - 1) / 128);
+  const scalar_floats sw0 = (scalar_floats)(p.sw + (long long)(n0 / 128) * p.sw_st);
+  const scalar_floats sw1 = (scalar_floats)(p.sw + (long long)nb1 * p.sw_st);
+  f32x4 acc[4][2][4];                                                 // quadrant, output tile, token tile
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[q][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 d[4] = {};                                                    // sums not added yet
+  float s[2][4] = {}, sr[4];                  // scale products of this quadrant and the one before; the tokens' scales
+  i32x8 a[4], w0[2], w1[2];
+  first(0);
+  if (kb > 1) {
+    first(1);
+    wait_vm<12 + NS>();
+  } else {
+    wait_vm<4>();
+  }
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w0[i] = get(w_at(0, 0, i));
+    clip(0, w0[i]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    a[j] = get(a_at(0, 0, j));
+    sr[j] = scale_at(0, 0, j);
+  }
+  float sn0 = sw0[0], sn1 = sw1[0];
+  // matrix instruction 8 q + 2 j + i of a block; the sum three before it is added
+  auto step = [&](int m, const i32x8& wf, const i32x8& af) {
+    if (m < 32) d[m & 3] = block_sum(wf, af);
+    __builtin_amdgcn_sched_barrier(0);
+    const int o = m < 32 ? (m + 29) & 31 : m - 3;
+    f32x4& x = acc[o >> 3][o & 1][(o >> 1) & 3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(d[o & 3][e], s[(o >> 3) & 1][(o >> 1) & 3], x[e]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto block = [&](int b, auto more_) {                               // more_: there is a block b + 2
+    constexpr bool more = decltype(more_)::value;
+    const float sc0 = sn0, sc1 = sn1;
+    // phase 0: A0 W0; W1 is read
+    wait_vm<more ? 10 + NS : 0>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w1[i] = get(w_at(b, 1, i));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[0][j] = sr[j] * sc0;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      step(m, w0[m & 1], a[m >> 1]);
+      if (more && m < 2) copy_a(b + 2, 0, m);
+      if (more && m == 2) copy_s(b + 2);
+      if (more && m >= 3 && m < 5) copy_w(b + 2, 0, m - 3);
+    }
+    if (!more) {
+      clip(b, w1[0]);
+      clip(b, w1[1]);
+    }
+    // phase 1: A0 W1; A1 is read over A0
+    wait_vm<more ? 12 + 2 * NS : 0>();
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[1][j] = sr[j] * sc1;
+      sr[j] = scale_at(b, 1, j);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 8; m < 16; ++m) {
+      step(m, w1[m & 1], a[(m >> 1) & 3]);
+      if (m & 1) a[(m >> 1) & 3] = get(a_at(b, 1, (m >> 1) & 3));
+      else if (more && m < 12) copy_w(b + 2, 1, (m - 8) >> 1);
+    }
+    // phase 2: A1 W0
+    sn0 = sw0[min(b + 1, kb - 1)];
+    sn1 = sw1[min(b + 1, kb - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[0][j] = sr[j] * sc0;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 16; m < 24; ++m) step(m, w0[m & 1], a[(m >> 1) & 3]);
+    // phase 3: A1 W1; A0 (over A1) and W0 of the next block are read (behind the last one: values that nothing uses)
+    wait_vm<more ? 10 + NS : 0>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w0[i] = get(w_at(b + 1, 0, i));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[1][j] = sr[j] * sc1;
+      sr[j] = scale_at(b + 1, 0, j);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 24; m < 32; ++m) {
+      step(m, w1[m & 1], a[(m >> 1) & 3]);
+      if (m & 1) a[(m >> 1) & 3] = get(a_at(b + 1, 0, (m >> 1) & 3));
+      else if (more && m < 28) copy_a(b + 2, 1, (m - 24) >> 1);
+    }
+    if (!more) {
+      clip(b + 1, w0[0]);
+      clip(b + 1, w0[1]);
+    }
+  };
+  int b = 0;
+  for (; b + 2 < kb; ++b) block(b, std::true_type{});
+  for (; b < kb; ++b) block(b, std::false_type{});
+#pragma unroll
+  for (int m = 32; m < 35; ++m) step(m, w1[0], a[0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = n0 + (q & 1) * 128 + wn * 32 + i * 16 + 4 * g;
+      if (n >= p.N) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store4<DT>(p, t0 + (q >> 1) * 128 + wm * 64 + j * 16 + r, n, acc[q][i][j]);
+    }
+}
+
+template <int DT, bool V4>
+static int big_go(const LinearParams& p, hipStream_t s) {
+  static DynLds lds;
+  if (int rc = lds.ensure((const void*)big_kernel<DT, V4>, Big::LDS)) return rc;
+  const int TN = (p.N + 255) / 256;
+  const long long n = (long long)TN * ((p.T + 255) / 256);
+  if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
+  hipLaunchKernelGGL((big_kernel<DT, V4>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), Big::LDS, s, p, TN);
+  return (int)hipGetLastError();
+}
+
+// the rule's kernels in its order (rules::LINEAR)
 template <int DT>
 static int linear_go(const LinearParams& p, hipStream_t s) {
-  return tile_go<DT, 128, 128, 64, 64>(p, s);
+  // the scales of four blocks at once: rows of whole 16-byte pieces
+  const bool v4 = ((p.K + 127) / 128) % 4 == 0 && ((uintptr_t)p.sa & 15) == 0 && (p.sa_st & 3) == 0;
+  switch (rules::linear_kernel(p.T, p.N, p.K)) {
+    case 0: return stream_go<DT, 1, 1, 8, 4>(p, s);
+    case 1: return stream_go<DT, 2, 1, 4, 3>(p, s);
+    case 2: return stream_go<DT, 1, 2, 8, 3>(p, s);
+    case 3: return stream_go<DT, 2, 2, 4, 2>(p, s);
+    case 4: return stream_go<DT, 1, 4, 4, 3>(p, s);
+    case 5: return stream_go<DT, 2, 4, 4, 2>(p, s);
+    case 6: return stream_go<DT, 4, 4, 4, 2>(p, s);
+    case 7: return ring_go<DT, 64, 128, 32, 32, 3>(p, s);
+    case 8: return ring_go<DT, 128, 128, 64, 32, 3>(p, s);
+    default: return v4 ? big_go<DT, true>(p, s) : big_go<DT, false>(p, s);
+  }
 }
 
 }  // namespace lin
