@@ -124,5 +124,39 @@ def call(name, *args):
     return rc
 
 
+_TENSOR_FN = None
+
+
+def tensor_calls():
+    """{name: callable} of the extension module _tensors (csrc/py_tensors.cpp); raises if it is missing."""
+    global _TENSOR_FN
+    if _TENSOR_FN is None:
+        import torch
+        lib()
+        try:
+            from . import _tensors
+        except ImportError as e:
+            raise RuntimeError("the extension module _tensors is not built (python -m arcagi2_flashnext_dots3_amd.build, "
+                               "with Python's and torch's headers)") from e
+        dev = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+        _TENSOR_FN = _tensors.load(LIB_PATH, raw, dev)
+    return _TENSOR_FN
+
+
+def tensor_call(name, x, *args):
+    """Call `name` of tensor_calls on the tensors' GPU (x: one of them)."""
+    f = (_TENSOR_FN or tensor_calls())[name]
+    rc = f(*args)
+    if rc:
+        if rc == -1000:              # on another GPU than the current one
+            import torch
+            with torch.cuda.device(x.device):
+                rc = f(*args)
+        if rc:
+            raise RuntimeError(f"spmla_{name} failed: {rc} ({ERRORS.get(rc, 'hip error')})")
+
+
 def exported_symbols():
     return [n for n in SIGNATURES if hasattr(lib(), n)]

@@ -3,7 +3,8 @@
 Every .hip file under csrc/ is compiled to an object (in parallel) and linked into one shared library next to
 this file; the Python loader (_lib.py) and the tests load that file. Objects go to _build/ (git-ignored).
 csrc/py_call.cpp becomes the extension module _native (the loader's callables; without Python's headers or a C++
-compiler it is left out and the loader calls through ctypes).
+compiler it is left out and the loader calls through ctypes), csrc/py_tensors.cpp the extension module _tensors (the
+calls around the cache and the query on tensors, against torch's headers).
 All HIP code is compiled with packed fp32 instructions disabled (-packed-fp32-ops), see the feature flag below.
 """
 import concurrent.futures
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 REPO = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libspmla_gfx950.so")
 NATIVE = os.path.join(HERE, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
+TENSORS = os.path.join(HERE, "_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
 CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -33,17 +35,31 @@ def _run(cmd):
     return err
 
 
-def build_native():
+def _build_module(src, out, flags=(), libs=()):
     inc = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(inc, "Python.h")) or shutil.which(CXX.split()[0]) is None:
-        if os.path.exists(NATIVE):
-            os.remove(NATIVE)
+        if os.path.exists(out):
+            os.remove(out)
         return None
-    tmp = NATIVE + ".tmp"
-    _run([*CXX.split(), "-O2", "-std=c++17", "-shared", "-fPIC", "-I", inc, "-I", os.path.join(REPO, "include"),
-          os.path.join(CSRC, "py_call.cpp"), "-o", tmp, "-ldl"])
-    os.replace(tmp, NATIVE)
-    return NATIVE
+    tmp = out + ".tmp"
+    _run([*CXX.split(), "-O2", "-std=c++17", "-shared", "-fPIC", "-I", inc, "-I", os.path.join(REPO, "include"), *flags,
+          os.path.join(CSRC, src), "-o", tmp, *libs, "-ldl"])
+    os.replace(tmp, out)
+    return out
+
+
+def build_native():
+    return _build_module("py_call.cpp", NATIVE)
+
+
+def build_tensors():
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
+    return _build_module("py_tensors.cpp", TENSORS,
+                         [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc, "-I",
+                          os.path.join(inc, "torch", "csrc", "api", "include")],
+                         ["-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"])
 
 
 def build(verbose=False):
@@ -53,11 +69,13 @@ def build(verbose=False):
     objs = [os.path.join(bdir, f[:-4] + ".o") for f in srcs]
     jobs = min(len(srcs), int(os.environ.get("MAX_JOBS", "8")))
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
+        tensors = ex.submit(build_tensors)
         futs = [ex.submit(_run, [HIPCC, *FLAGS, "-c", os.path.join(CSRC, s), "-o", o]) for s, o in zip(srcs, objs)]
         for s, f in zip(srcs, futs):
             msg = f.result()
             if verbose and msg:
                 print(f"[build] {s}: {msg}", flush=True)
+        tensors.result()
     tmp = LIB + ".tmp"
     _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", tmp, *objs])
     os.replace(tmp, LIB)

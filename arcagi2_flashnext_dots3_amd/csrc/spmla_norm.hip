@@ -2,7 +2,7 @@
 // on FP8 weights.
 //   z = x + residual (rounded to the type and stored),  y[d] = z[d] / sqrt(mean(z^2) + eps) * w[d]
 //   out = y rounded once to the type; codes = e4m3(y / s) with one scale s per 128 values (group_codes)
-// The sums and y stay in fp32; y is not rounded to the 16-bit type before it is quantized.
+// Sums, root and y are held in 32 bits or more (a thread's squares in fp32, with ue8m0 in 64 bits; then 64); y is not rounded to the 16-bit type before it is quantized.
 //
 // One pass: a row's values stay in the registers of the NT threads that share it, 8 a thread in CH chunks, so x and the
 // residual are read once. A group of 128 values is 16 neighbouring lanes of a chunk. Rows of up to 512 values take one
@@ -17,6 +17,7 @@ struct NormParams {
   const void* res; void* res_out; long long res_st, ro_st;   // null without a residual
   const void* w; int w_f32;                                  // null: ones
   float eps;
+  double inv_d;                                              // 1 / D
   int T, D;
   void* out; long long o_st;                                 // null without it
   uint8_t* codes; long long c_st;                            // null without them
@@ -24,18 +25,12 @@ struct NormParams {
   int ue8m0;
 };
 
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
 // VEC: 16-byte loads and stores (D % 8 == 0 and aligned rows); else element by element. NORM false: y = x, a workgroup
 // per NT * 8 values of a row.
 template <int DT, bool NORM, int NT, int CH, bool VEC>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;               // rows per workgroup
-  __shared__ float part[NT / 64];
+  __shared__ double part[NT / 64];
   const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / NT;
   const bool on = row < p.T;
@@ -56,7 +51,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     for (int e = 0; e < 8; ++e) z[c][e] = 0.f;
     get(p.x, p.x_st, at(c), z[c]);
   }
-  float r = 1.0f;
+  Factor r{1.0f, 0.0f};
   if constexpr (NORM) {
     if (p.w) {
 #pragma unroll
@@ -91,13 +86,19 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
         }
       }
     }
-    float ss = 0.f;
+    double ss = 0.0;
+    if (p.ue8m0) {                     // in 64 bits: here an error of r moves every code of the row the same way
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)z[c][e], (double)z[c][e], ss);
+    } else {
       float q = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q = __builtin_fmaf(z[c][e], z[c][e], q);
-      ss += q;
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q = __builtin_fmaf(z[c][e], z[c][e], q);
+      ss = (double)q;
     }
     ss = wave_sum(ss);
     if constexpr (NT > 64) {
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
 #pragma unroll
       for (int i = 1; i < NT / 64; ++i) ss += part[i];
     }
-    r = 1.0f / sqrtf(ss / (float)p.D + p.eps);
+    r = factor_of(inverse_root(ss * p.inv_d + (double)p.eps));
     if (p.w) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     for (int c = 0; c < CH; ++c) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = z[c][e] * r;
+      for (int e = 0; e < 8; ++e) y[e] = z[c][e] * r.hi;
       if (VEC) {
         if (on && at(c) < p.D) store8<DT>(p.out, row * p.o_st + at(c), y);
       } else {
@@ -219,7 +220,7 @@ int spmla_rms_norm(const void* x, long long x_st, const void* residual, long lon
   if ((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)residual_out | (uintptr_t)out) & (eb - 1)) ||
       ((uintptr_t)weight & (weight_f32 ? 3 : eb - 1)) || ((uintptr_t)scales & 3))
     return SPMLA_EALIGN;
-  nrm::NormParams p{x, x_st, residual, residual_out, r_st, ro_st, weight, weight_f32, eps, T, D,
+  nrm::NormParams p{x, x_st, residual, residual_out, r_st, ro_st, weight, weight_f32, eps, 1.0 / D, T, D,
                     out, o_st, codes, c_st, scales, s_st, ue8m0};
   return nrm::go(p, true, dtype, (hipStream_t)stream);
 }
@@ -231,7 +232,7 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
   if (T == 0) return SPMLA_OK;
   if (!x || !codes || !scales) return SPMLA_EARG;
   if (((uintptr_t)x & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)scales & 3)) return SPMLA_EALIGN;
-  nrm::NormParams p{x, x_st, nullptr, nullptr, 0, 0, nullptr, 0, 0.f, T, D,
+  nrm::NormParams p{x, x_st, nullptr, nullptr, 0, 0, nullptr, 0, 0.f, 0.0, T, D,
                     nullptr, 0, codes, c_st, scales, s_st, ue8m0};
   return nrm::go(p, false, dtype, (hipStream_t)stream);
 }

@@ -8,12 +8,33 @@ namespace spmla {
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
 
+// Lane exchanges inside rows of 16 lanes (DPP: no LDS round trip): lane ^ 1, lane ^ 2 and, for values that are the same in
+// 4 or 8 neighbours, the mirrored half row and row.
+template <int CTRL> __device__ inline float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xb1, DPP_XOR2 = 0x4e, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
 __device__ inline float wave_max16(float v) {   // max over aligned groups of 16 lanes
-  v = fmaxf(v, __shfl_xor(v, 1, 64));
-  v = fmaxf(v, __shfl_xor(v, 2, 64));
-  v = fmaxf(v, __shfl_xor(v, 4, 64));
-  v = fmaxf(v, __shfl_xor(v, 8, 64));
+  v = fmaxf(v, dpp<DPP_XOR1>(v));
+  v = fmaxf(v, dpp<DPP_XOR2>(v));
+  v = fmaxf(v, dpp<DPP_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp<DPP_MIRROR>(v));
   return v;
+}
+template <int CTRL> __device__ inline double dpp(double v) {
+  const uint2 u = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, make_uint2(f2u(dpp<CTRL>(u2f(u.x))), f2u(dpp<CTRL>(u2f(u.y)))));
+}
+__device__ inline double lane_of(double v, int l) {
+  const uint2 u = __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(u.x, l), __builtin_amdgcn_readlane(u.y, l)));
+}
+__device__ inline double wave_sum(double v) {   // over the wave, in one order
+  v += dpp<DPP_XOR1>(v);
+  v += dpp<DPP_XOR2>(v);
+  v += dpp<DPP_HALF_MIRROR>(v);
+  v += dpp<DPP_MIRROR>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
 // e2m2 magnitude index of y = |x| 2^-k >= 0 (offload_rowfmt.py:93-101 with M = 2). The products are exact
@@ -122,50 +143,108 @@ template <int DT> __device__ inline void store8(void* p, long long i, const floa
   }
 }
 
-// ---- e4m3 codes of eight values of a group of 128 (16 lanes of 8): y = t r, r >= 0 one factor of the group's row
-constexpr float Q_MAX = 448.0f, Q_MIN = 1e-12f;      // largest e4m3 value, smallest scale
-
-// The group's scale: s = max(amax |y| / 448, 1e-12) (ue8m0: rounded up to a power of two); codes of y over s before its
-// rounding to 32 bits. The largest value becomes 448 whatever r is, so without ue8m0 the quotient is 448 t / amax |t|,
-// correctly rounded: t is exact where it is a product of two 16-bit floats, and then so many quotients lie halfway
-// between two codes (one in some thousand) that a quotient by the rounded s would round those by s's rounding error.
-// t and amax are brought to the range in which the remainder of the division is exact by a power of two. A group of
-// infinities or NaNs (or a row factor that is one) is divided element by element: NaN codes for NaNs and inf / inf.
-__device__ inline float group_codes(const float (&t)[8], float r, bool ue8m0, uint32_t& lo, uint32_t& hi) {
-  float am = 0.f;
+// ---- e4m3 codes of values that a row's factor r scales: r = hi + lo, to 2^-40 ----------------------------------------
+struct Factor {
+  float hi, lo;
+};
+__device__ inline Factor factor_of(double r) {
+  const float hi = (float)r;
+  return {hi, (float)(r - (double)hi)};
+}
+// 1 / sqrt(m): one Newton step in 64 bits from the fp32 root where that is in range
+__device__ inline double inverse_root(double m) {
+  if (!(m > 1e-30 && m < 1e30)) return 1.0 / sqrt(m);
+  const double r = (double)(1.0f / sqrtf((float)m));
+  return r * (1.5 - 0.5 * m * r * r);
+}
+// p + e rounded to odd, e the rest of p's rounding: the next rounding, to fewer bits, is then that of the exact value
+__device__ inline float to_odd(float p, float e) {
+  const uint32_t b = f2u(p);
+  return e == 0.f || (b & 1u) ? p : u2f(((f2u(e) ^ b) >> 31) ? b - 1u : b + 1u);
+}
+// Whether one of y[8], each within ULPS of its exact value, may lie on the other side of a middle of two e4m3 codes than
+// that (a middle has at most four bits behind its leading one), in any lane: rare, then the exact quotients are formed
+template <int ULPS> __device__ inline bool near_middle(const float (&y)[8]) {
+  uint32_t u = 0x7ffffu;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(t[e]));
-  am = wave_max16(am);
-  float s = fmaxf(am * r / Q_MAX, Q_MIN);
-  const bool low = !(am * r > Q_MAX * Q_MIN);
-  if (ue8m0) {
-    uint32_t u = f2u(s);
-    if (u & 0x7fffffu) u = (u & 0xff800000u) + 0x800000u;      // the next power of two (or infinity)
-    s = u2f(u);
+  for (int e = 0; e < 8; ++e) u = min(u, (f2u(y[e]) + ULPS) & 0x7ffffu);
+  return __ballot(u <= 2 * ULPS) != 0ull;
+}
+// y = t c, or rounded to odd where that matters for the e4m3 code
+__device__ inline void scaled(const float (&t)[8], Factor c, float (&y)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = t[e] * c.hi;                // within one unit of its last place
+  if (__builtin_expect(near_middle<1>(y), 0)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = t[e] * c.hi;
+      y[e] = to_odd(p, __builtin_fmaf(t[e], c.lo, __builtin_fmaf(t[e], c.hi, -p)));
+    }
   }
-  uint32_t mag = f2u(r) & 0x7fffffffu;       // largest magnitude as an integer: infinities and NaNs above finite ones
+}
+
+// Codes of eight values y = t r of a group of 128 (16 lanes of 8), r >= 0 one factor of the group's row, and its scale
+// s = max(amax |y| / 448, 1e-12) (ue8m0: rounded up to a power of two); the codes are those of y over s before its
+// rounding to 32 bits. The largest value becomes 448 whatever r is, so without ue8m0 the quotient is 448 t / amax |t|: t
+// is exact where it is a product of two 16-bit floats, and then many quotients lie halfway between two codes (one in some
+// thousand): a quotient by the rounded s would round those by s's rounding error. The product with 448 / amax decides
+// every code but those; where one is near, the wave divides, with t and amax brought to the range in which the remainder
+// is exact by a power of two. A group of infinities or NaNs (or a row factor that is one) is divided element by element:
+// NaN codes for NaNs and inf / inf.
+constexpr float Q_MAX = 448.0f, Q_MIN = 1e-12f;      // largest e4m3 value, smallest scale
+__device__ inline float group_codes(const float (&t)[8], Factor r, bool ue8m0, uint32_t& lo, uint32_t& hi) {
+  uint32_t top = 0;                   // largest magnitude as an integer: infinities and NaNs lie above the finite ones
 #pragma unroll
-  for (int e = 0; e < 8; ++e) mag = max(mag, f2u(t[e]) & 0x7fffffffu);
-  if (__builtin_expect(__ballot(mag >= 0x7f800000u || f2u(s) >= 0x7f800000u) == 0ull, 1)) {
+  for (int e = 0; e < 8; ++e) top = max(top, f2u(t[e]) & 0x7fffffffu);
+  top = max(top, f2u(dpp<DPP_XOR1>(u2f(top))));
+  top = max(top, f2u(dpp<DPP_XOR2>(u2f(top))));
+  top = max(top, f2u(dpp<DPP_HALF_MIRROR>(u2f(top))));
+  top = max(top, f2u(dpp<DPP_MIRROR>(u2f(top))));
+  float am = u2f(top);
+  float s = fmaxf(am * r.hi / Q_MAX, Q_MIN);
+  const bool odd = top >= 0x7f800000u || (f2u(r.hi) & 0x7fffffffu) >= 0x7f800000u || f2u(s) >= 0x7f800000u;
+  const bool low = !(am * r.hi > Q_MAX * Q_MIN);
+  auto power = [&](float v) {         // the next power of two (or infinity)
+    uint32_t u = f2u(v);
+    if (u & 0x7fffffu) u = (u & 0xff800000u) + 0x800000u;
+    return u2f(u);
+  };
+  if (ue8m0) s = power(s);
+  if (__builtin_expect(__ballot(odd) == 0ull, 1)) {
     float y[8];
-    if (ue8m0 || low) {
-      const float f = 1.0f / s;              // exact for a power of two
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = ue8m0 ? t[e] * r * f : quotient(t[e] * r, s, f);
+    if (ue8m0) {
+      const float f = 1.0f / s;                                  // exact
+      scaled(t, Factor{r.hi * f, r.lo * f}, y);
     } else {
-      const float k = am < 0x1p-60f ? 0x1p64f : am > 0x1p100f ? 0x1p-64f : 1.0f;
-      const float a = am * k, f = 1.0f / a, up = Q_MAX * k;
+      // outside these sizes of amax the product may lose bits: straight to the division
+      const bool plain = am > 0x1p-60f && am < 0x1p100f && !low;
+      const float c = Q_MAX / am;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = quotient(t[e] * up, a, f);
+      for (int e = 0; e < 8; ++e) y[e] = t[e] * c;               // within two units
+      if (__builtin_expect(near_middle<2>(y) || __ballot(!plain) != 0ull, 0)) {
+        const float k = am < 0x1p-60f ? 0x1p64f : am > 0x1p100f ? 0x1p-64f : 1.0f;
+        const float a = low ? s : am * k, up = low ? r.hi : Q_MAX * k, f = 1.0f / a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = t[e] * up, q = quotient(x, a, f);
+          y[e] = to_odd(q, __builtin_fmaf(-q, a, x));
+        }
+      }
     }
     lo = e4m3x4(y[0], y[1], y[2], y[3]);
     hi = e4m3x4(y[4], y[5], y[6], y[7]);
   } else {
+    am = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(t[e]));     // (NaNs aside)
+    am = wave_max16(am);
+    s = fmaxf(am * r.hi / Q_MAX, Q_MIN);
+    if (ue8m0) s = power(s);
     lo = hi = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      lo |= (uint32_t)e4m3_rne(t[e] * r / s) << (8 * e);
-      hi |= (uint32_t)e4m3_rne(t[4 + e] * r / s) << (8 * e);
+      lo |= (uint32_t)e4m3_rne(t[e] * r.hi / s) << (8 * e);
+      hi |= (uint32_t)e4m3_rne(t[4 + e] * r.hi / s) << (8 * e);
     }
   }
   return s;

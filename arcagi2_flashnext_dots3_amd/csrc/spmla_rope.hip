@@ -150,9 +150,16 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
   const int lane = threadIdx.x & 63, i = lane & 31;
   if (tok >= p.n) return;
   const long long slot = p.slots[tok];
+  float x[8], w[8], a, b;                   // what all tokens share is on its way before the slot decides
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+  if (p.w) {
+    if (p.w_f32) load8<DT_F32>(p.w, lane * 8, w);
+    else load8<DT_BF16>(p.w, lane * 8, w);
+  }
+  const double freq = p.freqs[i];
   if (slot < 0 || slot >= p.R) return;      // padding: its values are not read
   const uint16_t* kv = p.kv + (long long)tok * p.kv_st;
-  float x[8], w[8], a, b;
   load8<DT_BF16>(kv, lane * 8, x);
   if (INTER) {
     const uint32_t v = *(const uint32_t*)(kv + D_LAT + 2 * i);
@@ -160,25 +167,23 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
   } else {
     a = bf2f(kv[D_LAT + i]); b = bf2f(kv[D_LAT + 32 + i]);
   }
-  const double freq = p.freqs[i];
   const double pos = p.pos32 ? (double)((const int*)p.pos)[tok] : (double)((const long long*)p.pos)[tok];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = 1.0f;
-  if (p.w) {
-    if (p.w_f32) load8<DT_F32>(p.w, lane * 8, w);
-    else load8<DT_BF16>(p.w, lane * 8, w);
-  }
   const int rowb = p.fmt == 0 ? ROW656 : (p.fmt == 1 ? ROW576 : ROW400);
   long long blk;
   int off;
   div_slot(slot, p.bs, p.sh, blk, off);
   uint8_t* row = p.cache + blk * p.blk_stride + (long long)off * rowb;
-  float ss = 0.f;
+  double ss = 0.0;
+  if (p.fmt == 0) {                         // r scales codes and scale alike
+    float q = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
+    for (int e = 0; e < 8; ++e) q = __builtin_fmaf(x[e], x[e], q);
+    ss = (double)q;
+  } else {
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) ss += __shfl_xor(ss, m, 64);
-  const float r = 1.0f / sqrtf(ss / (float)D_LAT + p.eps);
+    for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)x[e], (double)x[e], ss);
+  }
+  const double r = inverse_root(wave_sum(ss) * (1.0 / D_LAT) + (double)p.eps);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] *= w[e];
   float c, s;
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
   const float ra = a * c - b * s, rb = b * c + a * s;
   uint32_t lo, hi;
   if (p.fmt == 0) {
-    const float sc = group_codes(x, r, false, lo, hi);
+    const float sc = group_codes(x, factor_of(r), false, lo, hi);
     *(uint2*)(row + lane * 8) = make_uint2(lo, hi);
     if ((lane & 15) == 0) *(float*)(row + SC_OFF + (lane >> 4) * 4) = sc;
     if (lane < 32) {
@@ -199,9 +204,11 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
     }
     return;
   }
-  auto clamped = [&](float v) -> float { return fminf(fmaxf(v * p.inv_scale, -448.f), 448.f); };   // (a NaN becomes -448)
+  auto cut = [](float v) -> float { return fminf(fmaxf(v, -448.f), 448.f); };                      // (a NaN becomes -448)
+  const Factor f = factor_of(r * (double)p.inv_scale);
+  scaled(x, f, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = clamped(x[e] * r);
+  for (int e = 0; e < 8; ++e) x[e] = cut(w[e]);
   uint8_t* rp = row + D_LAT;
   if (p.fmt == 1) {
     *(uint2*)(row + lane * 8) = make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
     row400_latent(row, lane, x);
     rp = row + R4_ROPE;
   }
-  const uint32_t rc = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped(ra), clamped(rb), 0, false);
+  const uint32_t rc = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cut(ra * p.inv_scale), cut(rb * p.inv_scale), 0, false);
   if (lane < 32) {
     if (INTER) {
       *(uint16_t*)(rp + 2 * i) = (uint16_t)rc;

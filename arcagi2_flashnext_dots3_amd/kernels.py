@@ -1012,65 +1012,10 @@ def attend_packed(q, pool, idx, sm_scale, kv_scale=1.0, ql=None, cu=None, out=No
 
 
 # ------------------------------------------------------------------------------- around the cache and the query
-# element types of the norm, projection and rotary entry points: the C-ABI's dtype argument
-_EL_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_CODE_DT = (torch.float8_e4m3fn, torch.uint8)
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def _launch(name, x, others, *args):
-    """Entry point `name` on x's device and its current stream; every tensor has to be there."""
-    d = x.get_device()
-    _need(d >= 0 and all(t is None or t.get_device() == d for t in others), f"{name}: tensors on one GPU")
-    if d == _current_device():
-        _lib.call(name, *args, _stream(x))
-    else:
-        with torch.cuda.device(d):
-            _lib.call(name, *args, _stream(x))
-
-
-def _rows(t, T, D, dtypes, what):
-    _need(t.dim() == 2 and t.shape[0] == T and t.shape[1] == D and t.dtype in dtypes and (D <= 1 or t.stride(1) == 1),
-          what)
-
-
-def _out_rows(t, T, D, dtypes, what):
-    _rows(t, T, D, dtypes, what)
-    _need(T <= 1 or t.stride(0) >= D, f"{what}: rows that do not overlap")
-
-
-def _norm_call(x, weight, eps, residual, residual_out, out, codes, scales, ue8m0):
-    _need(x.dim() == 2 and x.dtype in _EL_DT and x.shape[1] > 0, "x [T, D] fp32 / fp16 / bf16, D > 0")
-    T, D = x.shape
-    same = (x.dtype,)
-    _rows(x, T, D, same, "x [T, D] with contiguous rows")
-    if residual is not None:
-        _rows(residual, T, D, same, "residual [T, D] of x's type with contiguous rows")
-        residual_out = residual if residual_out is None else residual_out
-        _out_rows(residual_out, T, D, same, "residual_out [T, D] of x's type with contiguous rows")
-    else:
-        _need(residual_out is None, "residual_out without a residual")
-    if weight is not None:
-        _need(weight.shape == (D,) and weight.dtype in (x.dtype, torch.float32) and weight.is_contiguous(),
-              "weight [D] of x's type or fp32")
-    if out is not None:
-        _out_rows(out, T, D, same, "out [T, D] of x's type with contiguous rows")
-    if codes is not None:
-        _quant_outputs(codes, scales, T, D)
-    r, ro = residual, residual_out
-    _launch("spmla_rms_norm", x, (weight, r, ro, out, codes, scales), x.data_ptr(), x.stride(0), _ptr(r),
-            0 if r is None else r.stride(0), _ptr(ro), 0 if ro is None else ro.stride(0), _ptr(weight),
-            int(weight is not None and weight.dtype == torch.float32), float(eps), T, D, _EL_DT[x.dtype], _ptr(out),
-            0 if out is None else out.stride(0), _ptr(codes), 0 if codes is None else codes.stride(0), _ptr(scales),
-            0 if scales is None else scales.stride(0), int(bool(ue8m0)))
-
-
-def _quant_outputs(codes, scales, T, D):
-    _out_rows(codes, T, D, _CODE_DT, "codes [T, D] e4m3 / uint8 with contiguous rows")
-    _out_rows(scales, T, (D + 127) // 128, (torch.float32,), "scales [T, ceil(D / 128)] fp32 with contiguous rows")
-
-
+# These calls are a few us on the GPU; their arguments are checked in csrc/py_tensors.cpp (ValueError).
 def _new_codes(x, codes, scales):
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError("x [T, D] fp32 / fp16 / bf16, D > 0")
     T, D = x.shape
     if codes is None:
         codes = torch.empty(T, D, dtype=torch.float8_e4m3fn, device=x.device)
@@ -1085,7 +1030,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out=None, residual_out=None):
     in the residual itself). out may be x."""
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _norm_call(x, weight, eps, residual, residual_out, out, None, None, False)
+    _lib.tensor_call("rms_norm", x, x, weight, eps, residual, residual_out, out, None, None, False)
     return out
 
 
@@ -1094,21 +1039,17 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None, codes=None, scales=None, ue
     """rms_norm with an 8-bit output for linear_fp8: e4m3 codes [T, D] and one fp32 scale per 128 values, scales
     [T, ceil(D / 128)] (largest magnitude / 448; ue8m0: rounded up to a power of two). The norm's fp32 values are
     quantized; out, where given, gets them rounded to x's type as well. Returns (codes, scales)."""
-    _need(x.dim() == 2, "x [T, D]")
-    codes, scales = _new_codes(x, codes, scales)
-    _norm_call(x, weight, eps, residual, residual_out, out, codes, scales, ue8m0)
+    if codes is None or scales is None:
+        codes, scales = _new_codes(x, codes, scales)
+    _lib.tensor_call("rms_norm", x, x, weight, eps, residual, residual_out, out, codes, scales, ue8m0)
     return codes, scales
 
 
 def quant_fp8(x, codes=None, scales=None, ue8m0=False):
     """x [T, D] fp32 / fp16 / bf16 -> (e4m3 codes [T, D], scales [T, ceil(D / 128)] fp32), as rms_norm_fp8 quantizes."""
-    _need(x.dim() == 2 and x.dtype in _EL_DT and x.shape[1] > 0, "x [T, D] fp32 / fp16 / bf16, D > 0")
-    T, D = x.shape
-    _rows(x, T, D, (x.dtype,), "x [T, D] with contiguous rows")
-    codes, scales = _new_codes(x, codes, scales)
-    _quant_outputs(codes, scales, T, D)
-    _launch("spmla_quant_fp8", x, (codes, scales), x.data_ptr(), x.stride(0), T, D, _EL_DT[x.dtype], codes.data_ptr(),
-            codes.stride(0), scales.data_ptr(), scales.stride(0), int(bool(ue8m0)))
+    if codes is None or scales is None:
+        codes, scales = _new_codes(x, codes, scales)
+    _lib.tensor_call("quant_fp8", x, x, codes, scales, ue8m0)
     return codes, scales
 
 
@@ -1116,27 +1057,10 @@ def linear_fp8(a, a_scales, w, w_scales, out=None, dtype=torch.bfloat16):
     """out[t, n] = sum over blocks b of 128 k: a_scales[t, b] * w_scales[n // 128, b] * (a[t, block] . w[n, block]).
     a [T, K], w [N, K] e4m3 codes (rows 16-byte aligned, K % 16 == 0), a_scales [T, ceil(K / 128)], w_scales
     [ceil(N / 128), ceil(K / 128)] fp32; out [T, N] bf16 or fp16."""
-    _need(a.dim() == 2 and w.dim() == 2 and a.shape[1] == w.shape[1], "a [T, K], w [N, K]")
-    (T, K), N = a.shape, w.shape[0]
-    kb = (K + 127) // 128
-    _need(K > 0 and K % 16 == 0, "K a positive multiple of 16")
-    _rows(a, T, K, _CODE_DT, "a [T, K] e4m3 with contiguous rows")
-    _rows(w, N, K, _CODE_DT, "w [N, K] e4m3 with contiguous rows")
-    _rows(a_scales, T, kb, (torch.float32,), "a_scales [T, ceil(K / 128)] fp32 with contiguous rows")
-    _rows(w_scales, (N + 127) // 128, kb, (torch.float32,), "w_scales [ceil(N / 128), ceil(K / 128)] fp32")
     if out is None:
-        out = torch.empty(T, N, dtype=dtype, device=a.device)
-    _out_rows(out, T, N, (torch.bfloat16, torch.float16), "out [T, N] bf16 / fp16 with contiguous rows")
-    _launch("spmla_linear_fp8", a, (a_scales, w, w_scales, out), a.data_ptr(), a.stride(0), a_scales.data_ptr(),
-            a_scales.stride(0), w.data_ptr(), w.stride(0), w_scales.data_ptr(), w_scales.stride(0), T, N, K,
-            _EL_DT[out.dtype], out.data_ptr(), out.stride(0))
+        out = torch.empty(a.shape[0], w.shape[0], dtype=dtype, device=a.device)
+    _lib.tensor_call("linear_fp8", a, a, a_scales, w, w_scales, out)
     return out
-
-
-def _freqs_ok(positions, freqs, n):
-    _need(positions.dim() == 1 and positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous() and
-          positions.shape[0] >= n, "positions [T] int32 / int64")
-    _need(freqs.dim() == 1 and freqs.dtype == torch.float64 and freqs.is_contiguous(), "freqs [pairs] float64")
 
 
 def rope(x, positions, freqs, out=None, start=0, interleaved=True, factor=1.0, inverse=False):
@@ -1144,21 +1068,9 @@ def rope(x, positions, freqs, out=None, start=0, interleaved=True, factor=1.0, i
     positions[t] * freqs[i] radians, times factor; interleaved pairs (2i, 2i + 1), else (i, i + len(freqs)). inverse:
     by the negative angle (the gradient of the rotation). The other columns are copied. out: x itself (in place), or a
     tensor that does not overlap it (None: a new one). See rotary.Rotary for the frequencies."""
-    _need(x.dim() in (2, 3) and x.dtype in _EL_DT, "x [T, H, W] or [T, W] fp32 / fp16 / bf16")
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _need(out.shape == x.shape and out.dtype == x.dtype, "out of x's shape and type")
-    T, W = x.shape[0], x.shape[-1]
-    H = x.shape[1] if x.dim() == 3 else 1
-    _need(W <= 1 or (x.stride(-1) == 1 and out.stride(-1) == 1), "contiguous head columns")
-    _freqs_ok(positions, freqs, T)
-    n = freqs.shape[0]
-    _need(0 <= start and start + 2 * n <= W, "start + 2 len(freqs) columns inside the head")
-    x_sh, o_sh = (x.stride(1), out.stride(1)) if x.dim() == 3 else (0, 0)
-    _need((T <= 1 or out.stride(0) >= W) and (H <= 1 or o_sh >= W), "out: heads that do not overlap")
-    _launch("spmla_rope", x, (positions, freqs, out), x.data_ptr(), x.stride(0), x_sh, positions.data_ptr(),
-            int(positions.dtype == torch.int32), freqs.data_ptr(), T, H, W, int(start), n, int(bool(interleaved)),
-            float(factor), int(bool(inverse)), _EL_DT[x.dtype], out.data_ptr(), out.stride(0), o_sh)
+    _lib.tensor_call("rope", x, x, positions, freqs, out, start, interleaved, factor, inverse)
     return out
 
 
@@ -1168,28 +1080,5 @@ def latent_write(kv, weight, eps, positions, freqs, slots, cache, fmt=0, kv_scal
     (weight [512] bf16 / fp32 or None), rotary of columns 512 .. 575 (freqs [32] float64, as rope), then the rows of
     cache_write's formats (fmt, kv_scale, cache, block_size, block_stride as there) at slots [n] int64; a slot < 0 or
     beyond the cache is skipped. Both stay in fp32 until they are encoded."""
-    _need(kv.dim() == 2 and kv.dtype == torch.bfloat16 and kv.shape[1] == D_QK and kv.stride(1) == 1,
-          "kv [n, 576] bf16 with contiguous rows")
-    n = min(kv.shape[0], slots.shape[0])
-    _need(fmt in _ROWB, f"fmt must be one of {sorted(_ROWB)}")
-    rowb = _ROWB[fmt]
-    _need(cache.dtype == torch.uint8 and cache.shape[-1] == rowb and cache.stride(-1) == 1, "cache rows of uint8")
-    _need(slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous(), "slots [n] int64")
-    if weight is not None:
-        _need(weight.shape == (D_LAT,) and weight.dtype in (torch.bfloat16, torch.float32) and weight.is_contiguous(),
-              "weight [512] bf16 / fp32")
-    _freqs_ok(positions, freqs, n)
-    _need(freqs.shape[0] == D_ROPE // 2, "freqs [32] float64")
-    if cache.dim() == 3:
-        bs, bstride, R = cache.shape[1], cache.stride(0), cache.shape[0] * cache.shape[1]
-        _need(cache.stride(1) == rowb, "rows inside a block must be contiguous")
-    else:
-        _need(cache.dim() == 2 and (cache.shape[0] <= 1 or block_stride is not None or cache.stride(0) == rowb),
-              "cache [R, row] with contiguous rows, or [blocks, block_size, row]")
-        R = cache.shape[0]
-        bs = block_size or max(1, R)
-        bstride = block_stride or bs * rowb
-    _launch("spmla_latent_write", kv, (weight, positions, freqs, slots, cache), kv.data_ptr(), kv.stride(0),
-            _ptr(weight), int(weight is not None and weight.dtype == torch.float32), float(eps), positions.data_ptr(),
-            int(positions.dtype == torch.int32), freqs.data_ptr(), int(bool(interleaved)), float(factor),
-            slots.data_ptr(), n, cache.data_ptr(), R, bs, bstride, int(fmt), float(kv_scale))
+    _lib.tensor_call("latent_write", kv, kv, weight, eps, positions, freqs, slots, cache, fmt, kv_scale, interleaved,
+                     factor, block_size, block_stride)
