@@ -190,6 +190,9 @@ long quant_fp8(PyObject* const* a) {
   });
 }
 
+constexpr const char *WEIGHT = "w [N, K] e4m3", *WEIGHT_SCALES = "w_scales [ceil(N / 128), ceil(K / 128)] fp32";
+constexpr const char* PRODUCT = "out [T, N] bf16 / fp16";
+
 // linear_fp8(a, a_scales, w, w_scales, out)
 long linear_fp8(PyObject* const* v) {
   const at::Tensor *a = tensor(v[0], "a"), *as = tensor(v[1], "a_scales"), *w = tensor(v[2], "w");
@@ -197,16 +200,38 @@ long linear_fp8(PyObject* const* v) {
   if (a->dim() != 2 || w->dim() != 2 || a->size(1) != w->size(1)) refuse("a [T, K], w [N, K]: got " + shown(*a) + ", " + shown(*w));
   const int64_t T = a->size(0), K = a->size(1), N = w->size(0), kb = (K + 127) / 128;
   if (K == 0 || K % 16) refuse("K a positive multiple of 16: got " + std::to_string(K));
-  const int64_t a_st = rows(*a, T, K, E4M3 | U8, "a [T, K] e4m3"), w_st = rows(*w, N, K, E4M3 | U8, "w [N, K] e4m3");
+  const int64_t a_st = rows(*a, T, K, E4M3 | U8, "a [T, K] e4m3"), w_st = rows(*w, N, K, E4M3 | U8, WEIGHT);
   const int64_t as_st = rows(*as, T, kb, F32, "a_scales [T, ceil(K / 128)] fp32");
-  const int64_t ws_st = rows(*ws, (N + 127) / 128, kb, F32, "w_scales [ceil(N / 128), ceil(K / 128)] fp32");
-  const int64_t o_st = rows(*out, T, N, BF16 | F16, "out [T, N] bf16 / fp16", true);
+  const int64_t ws_st = rows(*ws, (N + 127) / 128, kb, F32, WEIGHT_SCALES);
+  const int64_t o_st = rows(*out, T, N, BF16 | F16, PRODUCT, true);
   const int dev = gpu_of(*a);
   for (const at::Tensor* t : {a, as, w, ws, out}) same_gpu(*t, dev, "linear_fp8");
   const int Ti = as_int(T, "T"), Ni = as_int(N, "N"), Ki = as_int(K, "K");
   return launch(dev, [&](void* s) {
     return f_linear_fp8(address(a), a_st, (const float*)address(as), as_st, address(w), w_st, (const float*)address(ws), ws_st,
                         Ti, Ni, Ki, dtype_code(type_of(*out)), address(out), o_st, s);
+  });
+}
+
+// linear_quant(x, w, w_scales, out, work, ue8m0): quant_fp8 into work (T K bytes of codes, then the scales), then linear_fp8
+long linear_quant(PyObject* const* v) {
+  const Norm n = norm_input(v[0]);
+  const at::Tensor *w = tensor(v[1], "w"), *ws = tensor(v[2], "w_scales"), *out = tensor(v[3], "out"), *work = tensor(v[4], "work");
+  const bool ue8m0 = truth(v[5]);
+  if (w->dim() != 2 || n.D != w->size(1)) refuse("x [T, K], w [N, K]: got " + shown(*n.x) + ", " + shown(*w));
+  const int64_t N = w->size(0), kb = (n.D + 127) / 128;
+  if (n.D % 16) refuse("K a positive multiple of 16: got " + std::to_string(n.D));
+  const int64_t w_st = rows(*w, N, n.D, E4M3 | U8, WEIGHT), ws_st = rows(*ws, (N + 127) / 128, kb, F32, WEIGHT_SCALES);
+  const int64_t o_st = rows(*out, n.T, N, BF16 | F16, PRODUCT, true);
+  line(*work, n.T * (n.D + 4 * kb), ANY, U8, "work [T (K + 4 ceil(K / 128))] uint8");
+  for (const at::Tensor* t : {n.x, w, ws, out, work}) same_gpu(*t, n.dev, "linear_fp8");
+  const int T = as_int(n.T, "T"), Ni = as_int(N, "N"), K = as_int(n.D, "K");
+  unsigned char* codes = (unsigned char*)address(work);
+  float* scales = (float*)(codes + n.T * n.D);
+  return launch(n.dev, [&](void* s) {
+    const int rc = f_quant_fp8(address(n.x), n.st, T, K, dtype_code(n.type), codes, n.D, scales, kb, ue8m0, s);
+    return rc ? rc : f_linear_fp8(codes, n.D, scales, kb, address(w), w_st, (const float*)address(ws), ws_st, T, Ni, K,
+                                  dtype_code(type_of(*out)), address(out), o_st, s);
   });
 }
 
@@ -294,8 +319,8 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define CALLABLE(name, n) {#name, (PyCFunction)(void (*)())entry<name, n>, METH_FASTCALL, nullptr}
-PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(rope, 8),
-                       CALLABLE(latent_write, 13)};
+PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(linear_quant, 6),
+                       CALLABLE(rope, 8), CALLABLE(latent_write, 13)};
 
 PyObject* load(PyObject*, PyObject* args) {
   const char* path;

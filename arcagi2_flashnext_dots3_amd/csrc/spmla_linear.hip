@@ -245,7 +245,6 @@ static int ring_go(const LinearParams& p, hipStream_t s) {
   if (int rc = lds.ensure((const void*)ring_kernel<DT, BM, BN, WM, WN, ST>, C::LDS)) return rc;
   const int TN = (p.N + BN - 1) / BN;
   const long long n = (long long)TN * ((p.T + BM - 1) / BM);
-  if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
   hipLaunchKernelGGL((ring_kernel<DT, BM, BN, WM, WN, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), C::LDS, s, p, TN);
   return (int)hipGetLastError();
 }
@@ -362,7 +361,6 @@ static int stream_go(const LinearParams& p, hipStream_t s) {
   if (int rc = lds.ensure((const void*)stream_kernel<DT, NT, MT, NW, ST>, C::LDS)) return rc;
   const int TM = (p.T + 16 * MT - 1) / (16 * MT);
   const long long n = (long long)TM * ((p.N + 16 * NT - 1) / (16 * NT));
-  if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
   hipLaunchKernelGGL((stream_kernel<DT, NT, MT, NW, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * NW), C::LDS, s, p,
                      TM);
   return (int)hipGetLastError();
@@ -586,7 +584,6 @@ static int big_go(const LinearParams& p, hipStream_t s) {
   if (int rc = lds.ensure((const void*)big_kernel<DT, V4>, Big::LDS)) return rc;
   const int TN = (p.N + 255) / 256;
   const long long n = (long long)TN * ((p.T + 255) / 256);
-  if (n > 0x7ffffff0LL) return SPMLA_ELIMIT;
   hipLaunchKernelGGL((big_kernel<DT, V4>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), Big::LDS, s, p, TN);
   return (int)hipGetLastError();
 }
@@ -601,12 +598,12 @@ static int linear_go(const LinearParams& p, hipStream_t s) {
     case 1: return stream_go<DT, 2, 1, 4, 3>(p, s);
     case 2: return stream_go<DT, 1, 2, 8, 3>(p, s);
     case 3: return stream_go<DT, 2, 2, 4, 2>(p, s);
-    case 4: return stream_go<DT, 1, 4, 4, 3>(p, s);
-    case 5: return stream_go<DT, 2, 4, 4, 2>(p, s);
-    case 6: return stream_go<DT, 4, 4, 4, 2>(p, s);
-    case 7: return ring_go<DT, 64, 128, 32, 32, 3>(p, s);
-    case 8: return ring_go<DT, 128, 128, 64, 32, 3>(p, s);
-    default: return v4 ? big_go<DT, true>(p, s) : big_go<DT, false>(p, s);
+    case 4: return stream_go<DT, 2, 4, 4, 2>(p, s);
+    case 5: return stream_go<DT, 4, 4, 4, 2>(p, s);
+    case 6: return ring_go<DT, 64, 128, 32, 32, 3>(p, s);
+    case 7: return ring_go<DT, 128, 128, 64, 32, 3>(p, s);
+    case 8: return v4 ? big_go<DT, true>(p, s) : big_go<DT, false>(p, s);
+    default: return SPMLA_ELIMIT;
   }
 }
 
@@ -628,6 +625,7 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
   if (((uintptr_t)a & 15) || (a_st & 15) || ((uintptr_t)w & 15) || (w_st & 15) || ((uintptr_t)a_scales & 3) ||
       ((uintptr_t)w_scales & 3) || ((uintptr_t)out & 1))
     return SPMLA_EALIGN;
+  if (T > MAX_TOKENS || N > MAX_TOKENS) return SPMLA_ELIMIT;
   if (a_st > (1 << 22) || w_st > (1 << 22) || as_st > (1 << 20)) return SPMLA_ELIMIT;   // 32-bit offsets inside a tile
   lin::LinearParams p{(const uint8_t*)a, a_st, a_scales, as_st, (const uint8_t*)w, w_st, w_scales, ws_st, out, o_st,
                       T, N, K, ((uintptr_t)out & 7) == 0 && (o_st & 3) == 0};

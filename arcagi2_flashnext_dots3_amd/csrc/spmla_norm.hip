@@ -25,9 +25,11 @@ struct NormParams {
   int ue8m0;
 };
 
-// VEC: 16-byte loads and stores (D % 8 == 0 and aligned rows); else element by element. NORM false: y = x, a workgroup
+// Loads and stores are 16 bytes of a lane at any alignment of the type (gfx950 takes them; a misaligned row costs one more
+// line a wave). WHOLE: D % 8 == 0; else the lane at a row's end goes element by element (13 x 3268 fp32 4.4 us a call, 221 x
+// 6578 fp32 5.7, 753 x 1500 bf16 4.9; with whole rows element by element 9.9, 10.1, 7.8). NORM false: y = x, a workgroup
 // per NT * 8 values of a row.
-template <int DT, bool NORM, int NT, int CH, bool VEC>
+template <int DT, bool NORM, int NT, int CH, bool WHOLE>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;               // rows per workgroup
   __shared__ double part[NT / 64];
@@ -35,55 +37,32 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / NT;
   const bool on = row < p.T;
   const int base = NORM ? 0 : (int)blockIdx.y * (NT * 8);
-  float z[CH][8], w[CH][8];
+  constexpr bool EARLY = CH <= 2;                            // weights on their way before the sum (128 registers a thread)
+  float z[CH][8], w[EARLY ? CH : 1][8];
   auto at = [&](int c) { return base + (c * NT + tid) * 8; };
-  auto get = [&](const void* q, long long st, int d, float (&v)[8]) {
-    if (VEC) {
-      if (on && d < p.D) load8<DT>(q, row * st + d, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = on && d + e < p.D ? load1<DT>(q, row * st + d + e) : 0.f;
-    }
-  };
+  auto left = [&](int c) { return on ? p.D - at(c) : 0; };   // values of the row from there on
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[c][e] = 0.f;
-    get(p.x, p.x_st, at(c), z[c]);
+    load_upto8<DT, WHOLE>(p.x, row * p.x_st + at(c), left(c), z[c]);
   }
   Factor r{1.0f, 0.0f};
   if constexpr (NORM) {
-    if (p.w) {
+    auto weights = [&](int c, float (&v)[8]) {
+      if (p.w_f32) load_upto8<DT_F32, WHOLE>(p.w, at(c), left(c), v);
+      else load_upto8<DT, WHOLE>(p.w, at(c), left(c), v);
+    };
+    if (EARLY && p.w) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[c][e] = 0.f;
-        if (VEC) {
-          if (at(c) < p.D) {
-            if (p.w_f32) load8<DT_F32>(p.w, at(c), w[c]);
-            else load8<DT>(p.w, at(c), w[c]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (at(c) + e < p.D) w[c][e] = p.w_f32 ? ((const float*)p.w)[at(c) + e] : load1<DT>(p.w, at(c) + e);
-        }
-      }
+      for (int c = 0; c < CH; ++c) weights(c, w[c]);
     }
     if (p.res) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float a[8] = {};
-        get(p.res, p.res_st, at(c), a);
+        float a[8];
+        load_upto8<DT, WHOLE>(p.res, row * p.res_st + at(c), left(c), a);
 #pragma unroll
         for (int e = 0; e < 8; ++e) z[c][e] = round_to<DT>(z[c][e] + a[e]);
-        if (VEC) {
-          if (on && at(c) < p.D) store8<DT>(p.res_out, row * p.ro_st + at(c), z[c]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (on && at(c) + e < p.D) store1<DT>(p.res_out, row * p.ro_st + at(c) + e, z[c][e]);
-        }
+        store_upto8<DT, WHOLE>(p.res_out, row * p.ro_st + at(c), left(c), z[c]);
       }
     }
     double ss = 0.0;
@@ -111,9 +90,12 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     r = factor_of(inverse_root(ss * p.inv_d + (double)p.eps));
     if (p.w) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c) {
+        float (&v)[8] = w[EARLY ? c : 0];
+        if (!EARLY) weights(c, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[c][e] *= w[c][e];
+        for (int e = 0; e < 8; ++e) z[c][e] *= v[e];
+      }
     }
   }
   if (p.out) {
@@ -122,13 +104,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = z[c][e] * r.hi;
-      if (VEC) {
-        if (on && at(c) < p.D) store8<DT>(p.out, row * p.o_st + at(c), y);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (on && at(c) + e < p.D) store1<DT>(p.out, row * p.o_st + at(c) + e, y[e]);
-      }
+      store_upto8<DT, WHOLE>(p.out, row * p.o_st + at(c), left(c), y);
     }
   }
   if (p.codes) {
@@ -136,15 +112,15 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     for (int c = 0; c < CH; ++c) {
       uint32_t lo, hi;
       const float s = group_codes(z[c], r, p.ue8m0 != 0, lo, hi);
-      const int d = at(c);
-      if (on && d < p.D) {
+      const int d = at(c), n = left(c);
+      if (n > 0) {
         uint8_t* q = p.codes + row * p.c_st + d;
-        if (VEC) {
-          *(uint2*)q = make_uint2(lo, hi);
-        } else {
+        if (n >= 8) {
+          *(codes8*)q = codes8{lo, hi};
+        } else if constexpr (!WHOLE) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (d + e < p.D) q[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+          for (int e = 0; e < 7; ++e)
+            if (e < n) q[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
         }
         if ((lane & 15) == 0) p.scales[row * p.s_st + d / QGROUP] = s;
       }
@@ -152,36 +128,26 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
   }
 }
 
-template <int DT, bool NORM, int NT, int CH, bool VEC>
+template <int DT, bool NORM, int NT, int CH, bool WHOLE>
 static void launch(const NormParams& p, hipStream_t s) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
   const unsigned gy = NORM ? 1u : (unsigned)((p.D + NT * 8 - 1) / (NT * 8));
-  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, VEC>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
+  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, WHOLE>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
                      dim3(NT < 256 ? 256 : NT), 0, s, p);
 }
 
 constexpr int MAX_D = 65536;
 
-template <int DT, bool VEC>
+template <int DT, bool WHOLE>
 static void norm_go(const NormParams& p, hipStream_t s) {
-  if (p.D <= 512) launch<DT, true, 64, 1, VEC>(p, s);
-  else if (p.D <= 2048) launch<DT, true, 256, 1, VEC>(p, s);
-  else if (p.D <= 4096) launch<DT, true, 256, 2, VEC>(p, s);
-  else if (p.D <= 16384) launch<DT, true, 1024, 2, VEC>(p, s);
-  else launch<DT, true, 1024, 8, VEC>(p, s);
-}
-
-static bool rows_aligned(const void* p, long long st, int bytes) {
-  return ((uintptr_t)p & 15) == 0 && (st * bytes & 15) == 0;
+  if (p.D <= 512) launch<DT, true, 64, 1, WHOLE>(p, s);
+  else if (p.D <= 2048) launch<DT, true, 256, 1, WHOLE>(p, s);
+  else if (p.D <= 4096) launch<DT, true, 256, 2, WHOLE>(p, s);
+  else if (p.D <= 16384) launch<DT, true, 1024, 2, WHOLE>(p, s);
+  else launch<DT, true, 1024, 8, WHOLE>(p, s);
 }
 
 static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
-  const int eb = dtype == DT_F32 ? 4 : 2;
-  bool vec = p.D % 8 == 0 && rows_aligned(p.x, p.x_st, eb);
-  if (p.res) vec = vec && rows_aligned(p.res, p.res_st, eb) && rows_aligned(p.res_out, p.ro_st, eb);
-  if (p.w) vec = vec && ((uintptr_t)p.w & 15) == 0;
-  if (p.out) vec = vec && rows_aligned(p.out, p.o_st, eb);
-  if (p.codes) vec = vec && ((uintptr_t)p.codes & 7) == 0 && (p.c_st & 7) == 0;
   auto by_type = [&](auto tag) {
     constexpr bool V = decltype(tag)::value;
     if (norm) {
@@ -194,7 +160,7 @@ static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
       else launch<DT_BF16, false, 256, 1, V>(p, s);
     }
   };
-  if (vec) by_type(std::true_type{});
+  if (p.D % 8 == 0) by_type(std::true_type{});
   else by_type(std::false_type{});
   return (int)hipGetLastError();
 }
@@ -211,7 +177,7 @@ int spmla_rms_norm(const void* x, long long x_st, const void* residual, long lon
                    long long o_st, unsigned char* codes, long long c_st, float* scales, long long s_st, int ue8m0,
                    void* stream) {
   if (T < 0 || D <= 0 || dtype < 0 || dtype > 2 || !(eps >= 0.f)) return SPMLA_EARG;
-  if (D > nrm::MAX_D) return SPMLA_ELIMIT;
+  if (D > nrm::MAX_D || T > MAX_TOKENS) return SPMLA_ELIMIT;
   if (T == 0) return SPMLA_OK;
   if (!x || (residual != nullptr) != (residual_out != nullptr) || (!out && !codes) ||
       (codes != nullptr) != (scales != nullptr))
@@ -228,7 +194,7 @@ int spmla_rms_norm(const void* x, long long x_st, const void* residual, long lon
 int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsigned char* codes, long long c_st,
                     float* scales, long long s_st, int ue8m0, void* stream) {
   if (T < 0 || D <= 0 || dtype < 0 || dtype > 2) return SPMLA_EARG;
-  if (D > 65535 * 2048) return SPMLA_ELIMIT;
+  if (D > 65535 * 2048 || T > MAX_TOKENS) return SPMLA_ELIMIT;
   if (T == 0) return SPMLA_OK;
   if (!x || !codes || !scales) return SPMLA_EARG;
   if (((uintptr_t)x & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)scales & 3)) return SPMLA_EALIGN;

@@ -123,25 +123,67 @@ template <int DT> __device__ inline void unpack8(u32x4 a, float (&v)[8]) {   // 
     }
   }
 }
-// eight values from element i on (16-byte aligned)
-template <int DT> __device__ inline void load8(const void* p, long long i, float (&v)[8]) {
+// eight values from element i on: 16-byte aligned, or _any at any alignment of the type
+template <int DT, class Q = u32x4> __device__ inline void load8(const void* p, long long i, float (&v)[8]) {
   if constexpr (DT == DT_F32) {
-    const f32x4 a = *(const f32x4*)((const float*)p + i), b = *(const f32x4*)((const float*)p + i + 4);
+    const u32x4 a = *(const Q*)((const float*)p + i), b = *(const Q*)((const float*)p + i + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    for (int e = 0; e < 4; ++e) { v[e] = u2f(a[e]); v[4 + e] = u2f(b[e]); }
   } else {
-    unpack8<DT>(*(const u32x4*)((const uint16_t*)p + i), v);
+    unpack8<DT>(*(const Q*)((const uint16_t*)p + i), v);
   }
 }
-template <int DT> __device__ inline void store8(void* p, long long i, const float (&v)[8]) {
+template <int DT, class Q = u32x4> __device__ inline void store8(void* p, long long i, const float (&v)[8]) {
   if constexpr (DT == DT_F32) {
-    *(f32x4*)((float*)p + i) = f32x4{v[0], v[1], v[2], v[3]};
-    *(f32x4*)((float*)p + i + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    *(Q*)((float*)p + i) = u32x4{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+    *(Q*)((float*)p + i + 4) = u32x4{f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])};
   } else {
-    *(u32x4*)((uint16_t*)p + i) = u32x4{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
-                                        pack2<DT>(v[6], v[7])};
+    *(Q*)((uint16_t*)p + i) = u32x4{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
+                                    pack2<DT>(v[6], v[7])};
   }
 }
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef uint32_t codes8 __attribute__((ext_vector_type(2), aligned(1)));       // eight codes at any address
+// the same of a row that ends after n values (WHOLE: after 8 or more, or none of them); zeros behind it
+template <int DT, bool WHOLE> __device__ inline void load_upto8(const void* p, long long i, int n, float (&v)[8]) {
+  if (n >= 8) {
+    load8<DT, u32x4_any>(p, i, v);
+    return;
+  }
+  u32x4 a{0, 0, 0, 0}, b{0, 0, 0, 0};
+  if constexpr (!WHOLE) {
+#pragma unroll
+    for (int e = 0; e < 7; ++e) {
+      if constexpr (DT == DT_F32) {
+        const uint32_t w = e < n ? ((const uint32_t*)p)[i + e] : 0;
+        if (e < 4) a[e] = w;
+        else b[e - 4] = w;
+      } else {
+        a[e >> 1] |= (uint32_t)(e < n ? ((const uint16_t*)p)[i + e] : 0) << (16 * (e & 1));
+      }
+    }
+  }
+  if constexpr (DT == DT_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = u2f(a[e]); v[4 + e] = u2f(b[e]); }
+  } else {
+    unpack8<DT>(a, v);
+  }
+}
+template <int DT, bool WHOLE> __device__ inline void store_upto8(void* p, long long i, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    store8<DT, u32x4_any>(p, i, v);
+  } else if constexpr (!WHOLE) {
+#pragma unroll
+    for (int e = 0; e < 7; ++e) {
+      if (e >= n) continue;
+      if constexpr (DT == DT_F32) ((float*)p)[i + e] = v[e];
+      else ((uint16_t*)p)[i + e] = (uint16_t)(pack2<DT>(v[e & 6], v[(e & 6) + 1]) >> (16 * (e & 1)));
+    }
+  }
+}
+
+constexpr int MAX_TOKENS = 1 << 23;                // rows of a call: grids stay below 2^32 threads
 
 // ---- e4m3 codes of values that a row's factor r scales: r = hi + lo, to 2^-40 ----------------------------------------
 struct Factor {

@@ -64,24 +64,24 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeParams p) {
           store1<DT>(p.out, oi + cb, b * c[0] + a * s[0]);
         } else if constexpr (INTER) {
           float v[8], y[8];
-          load8<DT>(p.x, xi + ca, v);
+          load8<DT, u32x4_any>(p.x, xi + ca, v);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             y[2 * i] = v[2 * i] * c[i] - v[2 * i + 1] * s[i];
             y[2 * i + 1] = v[2 * i + 1] * c[i] + v[2 * i] * s[i];
           }
-          store8<DT>(p.out, oi + ca, y);
+          store8<DT, u32x4_any>(p.out, oi + ca, y);
         } else {
           float a[8], b[8], y[8], z[8];
-          load8<DT>(p.x, xi + ca, a);
-          load8<DT>(p.x, xi + cb, b);
+          load8<DT, u32x4_any>(p.x, xi + ca, a);
+          load8<DT, u32x4_any>(p.x, xi + cb, b);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             y[i] = a[i] * c[i] - b[i] * s[i];
             z[i] = b[i] * c[i] + a[i] * s[i];
           }
-          store8<DT>(p.out, oi + ca, y);
-          store8<DT>(p.out, oi + cb, z);
+          store8<DT, u32x4_any>(p.out, oi + ca, y);
+          store8<DT, u32x4_any>(p.out, oi + cb, z);
         }
       }
     } else {                                                 // columns outside the turned part: copied
@@ -93,11 +93,11 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeParams p) {
           if constexpr (DT == DT_F32) ((uint32_t*)p.out)[oi] = ((const uint32_t*)p.x)[xi];
           else ((uint16_t*)p.out)[oi] = ((const uint16_t*)p.x)[xi];
         } else if constexpr (DT == DT_F32) {
-          const u32x4 a = *(const u32x4*)((const float*)p.x + xi), b = *(const u32x4*)((const float*)p.x + xi + 4);
-          *(u32x4*)((float*)p.out + oi) = a;
-          *(u32x4*)((float*)p.out + oi + 4) = b;
+          const u32x4_any a = *(const u32x4_any*)((const float*)p.x + xi), b = *(const u32x4_any*)((const float*)p.x + xi + 4);
+          *(u32x4_any*)((float*)p.out + oi) = a;
+          *(u32x4_any*)((float*)p.out + oi + 4) = b;
         } else {
-          *(u32x4*)((uint16_t*)p.out + oi) = *(const u32x4*)((const uint16_t*)p.x + xi);
+          *(u32x4_any*)((uint16_t*)p.out + oi) = *(const u32x4_any*)((const uint16_t*)p.x + xi);
         }
       }
     }
@@ -239,6 +239,7 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
                long long o_st, long long o_sh, void* stream) {
   if (T < 0 || H < 0 || W < 0 || n < 0 || start < 0 || n > W / 2 || start > W - 2 * n || dtype < 0 || dtype > 2)
     return SPMLA_EARG;
+  if (T > MAX_TOKENS) return SPMLA_ELIMIT;
   const bool inplace = out == x;
   if (inplace && (x_st != o_st || x_sh != o_sh)) return SPMLA_EARG;
   if (T == 0 || H == 0 || W == 0 || (inplace && n == 0)) return SPMLA_OK;
@@ -249,9 +250,7 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
     return SPMLA_EALIGN;
   rope::RopeParams p{x, x_st, x_sh, out, o_st, o_sh, positions, pos32, freqs, T, H, W, start, n, inplace,
                      factor, inverse ? -1.0f : 1.0f, 0, 0, 0};
-  const bool vec = ((((uintptr_t)x | (uintptr_t)out) & 15) == 0) &&
-                   (((x_st | x_sh | o_st | o_sh) * eb) & 15) == 0 && (W & 7) == 0 && (start & 7) == 0 &&
-                   (n & (interleaved ? 3 : 7)) == 0;
+  const bool vec = (W & 7) == 0 && (start & 7) == 0 && (n & (interleaved ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == DT_F32) rope::go<DT_F32>(p, vec, interleaved != 0, s);
   else if (dtype == DT_F16) rope::go<DT_F16>(p, vec, interleaved != 0, s);
@@ -265,6 +264,7 @@ int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int 
                        int fmt, float kv_scale, void* stream) {
   if (n < 0 || R < 0 || fmt < 0 || fmt > 2 || block_size <= 0 || !(eps >= 0.f)) return SPMLA_EARG;
   if (n == 0) return SPMLA_OK;
+  if (n > MAX_TOKENS) return SPMLA_ELIMIT;
   if (!kv || !positions || !freqs || !slots || !cache) return SPMLA_EARG;
   if (((uintptr_t)kv & 15) || (kv_st & 7) || ((uintptr_t)weight & 15) || ((uintptr_t)freqs & 7) ||
       ((uintptr_t)positions & (pos32 ? 3 : 7)) || ((uintptr_t)slots & 7))

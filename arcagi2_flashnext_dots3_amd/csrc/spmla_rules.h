@@ -46,33 +46,35 @@ inline int merged_splits(int T, int H, int K, int S, bool r576) {
   return best;
 }
 
-// The projection kernels (spmla_linear.hip): tile of tokens x outputs, the tokens they are considered for, and a model of a
-// launch's us, c0 + c1 rounds + c2 rounds kb + c3 wgs kb / 256 + c4 wgs / 256 with kb blocks of 128 k and rounds of 256
-// workgroups; fitted to graphed launches of 126 shapes (T 1 to 4096, N 576 to 24576, K 1536 to 16384; operands of three
-// launches ago in the caches). The largest miss of a chosen kernel against the fastest is 6 %, the mean 0.6 %.
-struct LinearKernel { int bm, bn, least, most; float c[5]; };
+// The projection kernels (spmla_linear.hip): tile of tokens x outputs and a model of a launch's us,
+// c0 + c1 rounds + c2 rounds kb + c3 wgs kb / 256 + c4 wgs / 256 with kb blocks of 128 k and rounds of 256 workgroups; fitted
+// to graphed launches of 444 shapes (T 1 to 4096, N 64 to 24576, K 512 to 16384; operands of three launches ago in the
+// caches). The chosen kernel is the fastest or within 5 % of it on 430 of them, 0.4 % slower on average, 26 % at most. Every
+// kernel is wanted: without it the chosen ones are 1 to 6 % slower on average and up to 25 to 79 % on a shape. Few tokens
+// need not mean few workgroups, nor many tokens large tiles (us, chosen / the kernel by tokens alone): 825 x 80 x 7776
+// tiles of 16 x 32 11 / 64 x 128 22; 64 x 152 x 4560 16 x 16 4.6 / 64 x 16 6.3.
+struct LinearKernel { int bm, bn; float c[5]; };
 constexpr LinearKernel LINEAR[] = {
-    {16, 16, 1, 16, {1.352f, 0.539f, 0.043f, 0.035f, 0.732f}},   // stream_kernel NT1 MT1 NW8 ST4
-    {16, 32, 1, 16, {2.014f, 0.197f, 0.069f, 0.035f, 0.801f}},   // stream_kernel NT2 MT1 NW4 ST3
-    {32, 16, 17, 32, {1.388f, 0.755f, 0.063f, 0.028f, 0.628f}},   // stream_kernel NT1 MT2 NW8 ST3
-    {32, 32, 17, 32, {2.311f, 0.253f, 0.082f, 0.045f, 0.585f}},   // stream_kernel NT2 MT2 NW4 ST2
-    {64, 16, 33, 512, {1.677f, 0.565f, 0.123f, 0.009f, 0.869f}},   // stream_kernel NT1 MT4 NW4 ST3
-    {64, 32, 33, 512, {1.589f, 1.212f, 0.153f, 0.000f, 0.729f}},   // stream_kernel NT2 MT4 NW4 ST2
-    {64, 64, 33, 2048, {1.389f, 2.314f, 0.205f, 0.035f, 0.423f}},   // stream_kernel NT4 MT4 NW4 ST2
-    {64, 128, 33, 0x7fffffff, {2.375f, 1.019f, 0.353f, 0.045f, 1.150f}},   // ring_kernel 64x128 w32x32
-    {128, 128, 33, 0x7fffffff, {0.471f, 3.850f, 0.426f, 0.161f, 0.535f}},   // ring_kernel 128x128 w64x32
-    {256, 256, 257, 0x7fffffff, {0.528f, 10.517f, 1.351f, 0.338f, 1.650f}},   // big_kernel
+    {16, 16, {1.240f, 1.142f, 0.039f, 0.044f, 0.000f}},   // stream_kernel NT1 MT1 NW8 ST4
+    {16, 32, {2.375f, 0.000f, 0.075f, 0.050f, 0.000f}},   // stream_kernel NT2 MT1 NW4 ST3
+    {32, 16, {1.154f, 1.331f, 0.060f, 0.038f, 0.000f}},   // stream_kernel NT1 MT2 NW8 ST3
+    {32, 32, {2.580f, 0.000f, 0.098f, 0.055f, 0.000f}},   // stream_kernel NT2 MT2 NW4 ST2
+    {64, 32, {1.933f, 0.600f, 0.200f, 0.000f, 0.863f}},   // stream_kernel NT2 MT4 NW4 ST2
+    {64, 64, {2.058f, 1.347f, 0.274f, 0.000f, 1.208f}},   // stream_kernel NT4 MT4 NW4 ST2
+    {64, 128, {2.012f, 0.763f, 0.437f, 0.013f, 1.913f}},   // ring_kernel 64x128 w32x32
+    {128, 128, {1.382f, 2.853f, 0.443f, 0.248f, 1.136f}},   // ring_kernel 128x128 w64x32
+    {256, 256, {5.039f, 8.372f, 1.190f, 0.886f, 0.566f}},   // big_kernel
 };
 
-// The cheapest kernel by the model.
+// The cheapest kernel by the model; -1: none takes so many workgroups.
 inline int linear_kernel(int T, int N, int K) {
   const double kb = (K + 127) / 128;
   int best = -1;
   double least = 0.0;
   for (int i = 0; i < (int)(sizeof(LINEAR) / sizeof(LINEAR[0])); ++i) {
     const LinearKernel& k = LINEAR[i];
-    if (T < k.least || T > k.most) continue;
     const long long wgs = (long long)((T - 1) / k.bm + 1) * ((N - 1) / k.bn + 1);
+    if (wgs >= 1 << 23) continue;                      // a grid of 2^32 threads or more is not launched
     const double r = (double)((wgs + 255) / 256), w = wgs / 256.0;
     const double t = k.c[0] + k.c[1] * r + k.c[2] * r * kb + k.c[3] * w * kb + k.c[4] * w;
     if (best < 0 || t < least) { best = i; least = t; }

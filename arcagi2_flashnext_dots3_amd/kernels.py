@@ -1063,6 +1063,16 @@ def linear_fp8(a, a_scales, w, w_scales, out=None, dtype=torch.bfloat16):
     return out
 
 
+def linear_quant(x, w, w_scales, out=None, ue8m0=False):
+    """linear_fp8 of x [T, K] bf16 / fp16, quantized by quant_fp8 into a workspace; out [T, N] (None: of x's type)."""
+    T, K = x.shape
+    if out is None:
+        out = torch.empty(T, w.shape[0], dtype=x.dtype, device=x.device)
+    work = torch.empty(T * (K + 4 * -(-K // 128)), dtype=torch.uint8, device=x.device)
+    _lib.tensor_call("linear_quant", x, x, w, w_scales, out, work, ue8m0)
+    return out
+
+
 def rope(x, positions, freqs, out=None, start=0, interleaved=True, factor=1.0, inverse=False):
     """Rotary positions: columns start .. start + 2 len(freqs) of x [T, H, W] or [T, W] (fp32, fp16, bf16) turn by
     positions[t] * freqs[i] radians, times factor; interleaved pairs (2i, 2i + 1), else (i, i + len(freqs)). inverse:

@@ -61,8 +61,7 @@ def linear_fp8(x, f, out=None, ue8m0=False):
     if isinstance(x, torch.Tensor):
         if x.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("linear_fp8: x bf16 / fp16, or (codes, scales)")
-        a, sa = kernels.quant_fp8(x, ue8m0=ue8m0)
-        return kernels.linear_fp8(a, sa, codes, scales, out=out, dtype=x.dtype)
+        return kernels.linear_quant(x, codes, scales, out=out, ue8m0=ue8m0)
     a, sa = x
     return kernels.linear_fp8(a, sa, codes, scales, out=out)
 

@@ -56,6 +56,21 @@ def test_linear():
     _refused("bf16 / fp16", mla_fp8.linear_fp8, _t(4, 256, dtype=torch.float32), (w, sw))
 
 
+def test_linear_quant():
+    x, w, sw = _t(4, 256), _t(300, 256, dtype=F8), _t(3, 2, dtype=torch.float32)
+    _refused("one GPU", kernels.linear_quant, x, w, sw)
+    _refused("x \\[T, K\\], w", kernels.linear_quant, x, w[:, :128], sw)
+    _refused("multiple of 16", kernels.linear_quant, x[:, :120], w[:, :120], sw)
+    _refused("D > 0", kernels.linear_quant, x[:, :0], w[:, :0], sw)
+    _refused("x \\[T, D\\]", kernels.linear_quant, x.to(F8), w, sw)
+    _refused("w \\[N, K\\] e4m3", kernels.linear_quant, x, _t(300, 256), sw)
+    _refused("w_scales", kernels.linear_quant, x, w, sw[:, :1])
+    _refused("out", kernels.linear_quant, x, w, sw, out=_t(4, 299))
+    _refused("out", kernels.linear_quant, x, w, sw, out=_t(4, 300, dtype=torch.float32))
+    _refused("overlap", kernels.linear_quant, x, w, sw, out=_t(1, 300).expand(4, 300))
+    _refused("unpack", kernels.linear_quant, x[0], w, sw)
+
+
 def test_rope():
     x, pos, f = _t(4, 2, 64), torch.zeros(4, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
     _refused("one GPU", kernels.rope, x, pos, f)
@@ -110,6 +125,12 @@ def test_latent_write():
     ("spmla_rope", (256, 64, 64, 256, 0, 256, 1, 1, 64, 0, 32, 1, 1.0, 0, 2, 256, 128, 64, None), -2),  # in place, strides
     ("spmla_rope", (256, 64, 64, None, 0, 256, 1, 1, 64, 0, 32, 1, 1.0, 0, 2, 512, 64, 64, None), -2),
     ("spmla_rope", (257, 64, 64, 256, 0, 256, 1, 1, 64, 0, 32, 1, 1.0, 0, 2, 512, 64, 64, None), -3),
+    ("spmla_rms_norm", (256, 8, None, 0, None, 0, None, 0, 1e-6, (1 << 23) + 1, 8, 2, 256, 8, None, 0, None, 0, 0, None), -5),
+    ("spmla_quant_fp8", (256, 8, (1 << 23) + 1, 8, 2, 256, 8, 256, 1, 0, None), -5),
+    ("spmla_linear_fp8", (256, 32, 256, 1, 256, 32, 256, 1, (1 << 23) + 1, 8, 32, 2, 256, 8, None), -5),
+    ("spmla_linear_fp8", (256, 32, 256, 1, 256, 32, 256, 1, 1 << 23, 1 << 23, 32, 2, 256, 1 << 23, None), -5),   # too many tiles
+    ("spmla_rope", (256, 64, 64, 256, 0, 256, (1 << 23) + 1, 1, 64, 0, 32, 1, 1.0, 0, 2, 512, 64, 64, None), -5),
+    ("spmla_latent_write", (256, 576, None, 0, 1e-6, 256, 0, 256, 1, 1.0, 256, (1 << 23) + 1, 256, 8, 8, 8 * 656, 0, 1.0, None), -5),
     ("spmla_latent_write", (256, 576, None, 0, 1e-6, 256, 0, 256, 1, 1.0, 256, 1, 256, 8, 8, 8 * 656, 3, 1.0, None), -2),
     ("spmla_latent_write", (256, 576, None, 0, 1e-6, 256, 0, 256, 1, 1.0, 256, 1, 256, 8, 8, 8 * 576, 1, 0.0, None), -2),
     ("spmla_latent_write", (258, 576, None, 0, 1e-6, 256, 0, 256, 1, 1.0, 256, 1, 256, 8, 8, 8 * 656, 0, 1.0, None), -3),
