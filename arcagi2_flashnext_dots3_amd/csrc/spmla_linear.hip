@@ -27,7 +27,7 @@ struct LinearParams {
   const float* sw; long long sw_st;
   void* out; long long o_st;
   int T, N, K;
-  int o_vec;                     // 8-byte stores of four outputs
+  int o_vec, o_seg;              // 8-byte stores of four outputs; rows of whole, aligned 64-byte segments
 };
 
 #pragma clang diagnostic push
@@ -41,26 +41,23 @@ __device__ inline void dma4s(const void* base, uint32_t off, SPMLA_LDS void* l) 
   const uint32_t d = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)l);
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(d) : "memory", "m0");
 }
-// the same of 4 or 16 bytes a lane for the lanes of a mask below 2^32 of a full wave
-template <int BYTES>
-__device__ inline void dma_lo(const void* base, uint32_t off, SPMLA_LDS void* l, uint32_t lanes) {
-  static_assert(BYTES == 4 || BYTES == 16, "copies of 4 or 16 bytes a lane");
-  const uint32_t d = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)l), m = __builtin_amdgcn_readfirstlane(lanes);
-  if (BYTES == 4)
-    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_hi, 0\n\ts_mov_b32 exec_lo, %3\n\t"
-                 "global_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1"
-                 ::"v"(off), "s"(base), "s"(d), "s"(m) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_hi, 0\n\ts_mov_b32 exec_lo, %3\n\t"
-                 "global_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
-                 ::"v"(off), "s"(base), "s"(d), "s"(m) : "memory", "m0");
+// 4 bytes from each address of a full wave's first LANES lanes
+template <int LANES>
+__device__ inline void dma4_first(const float* v, SPMLA_LDS void* l) {
+  static_assert(LANES > 0 && LANES < 64, "lanes");
+  constexpr uint64_t M = (1ull << LANES) - 1;
+  const uint32_t d = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)l);
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b32 exec_lo, %2\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %0, off\n\t"
+               "s_mov_b64 exec, -1" ::"v"(v), "s"(d), "i"((uint32_t)M), "i"((uint32_t)(M >> 32)) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
-__device__ inline i32x8 frag(const uint8_t* rows, int r, int g) {   // row r's chunks g and g + 4 of a staged block
-  const i32x4 lo = *(const i32x4*)(rows + r * 128 + ((g ^ ((r >> 1) & 7)) << 4));
-  const i32x4 hi = *(const i32x4*)(rows + r * 128 + (((g + 4) ^ ((r >> 1) & 7)) << 4));
+__device__ inline i32x8 frag_at(const uint8_t* rows, int at) {      // the chunk at `at` and the one four chunks from it
+  const i32x4 lo = *(const i32x4*)(rows + at), hi = *(const i32x4*)(rows + (at ^ 64));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ inline i32x8 frag(const uint8_t* rows, int r, int g) {   // row r's chunks g and g + 4 of a staged block
+  return frag_at(rows, r * 128 + ((g ^ ((r >> 1) & 7)) << 4));
 }
 __device__ inline f32x4 block_sum(i32x8 w, i32x8 a) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
@@ -83,12 +80,16 @@ __device__ inline void store4(const LinearParams& p, int t, int n, f32x4 v) {   
 // ---- tiles of BM tokens x BN outputs, 8 waves of WM x WN, a ring of ST blocks in LDS ----------------------------------
 // While the sums of block b form from registers, block b + 1 is read from LDS and blocks b + 2 .. b + ST are on their way:
 // one barrier a block, behind which block b's place is free and block b + 1 has arrived.
+// Bound by LDS: the copies of a block of 128 x 128 (33 KB, 64 bytes a clock) and its reads (100 KB, 256 a clock) take 900
+// clocks, the matrix instructions 512; a block takes 1000. 1455 x 2112 x 4096 21 us (1.2 PFLOP/s, 204 workgroups), 6 of them
+// before and behind the blocks; 64 x 24576 x 1536 in tiles of 64 x 128 9.4 us (4.3 TB/s of weights and outputs). 16 waves,
+// wave tiles of 64 x 64 and a ring of 4 blocks were no faster, two workgroups a unit (128 registers) 10 % slower.
 template <int BM, int BN, int WM, int WN, int ST>
 struct Ring {
   static constexpr int NW = 8, NWM = BM / WM, PA = BM / 64, PW = BN / 64, NI = PA + PW + 1;   // copies of a wave and block
-  static constexpr int AS = 0, WS = BM * 128, SS = WS + BN * 128, STAGE = SS + BM * 4;
+  static constexpr int AS = 0, WS = BM * 128, SS = WS + BN * 128, STAGE = SS + 1024;   // scales [wave][32]
   static constexpr int LDS = ST * STAGE;
-  static_assert(BM % 64 == 0 && BN % 64 == 0 && NWM * (BN / WN) == NW && 128 % WN == 0 && BM / NW <= 32 && ST >= 3 &&
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && NWM * (BN / WN) == NW && BN == 128 && WN == 32 && BM / NW < 32 && ST >= 3 &&
                 ST * NI < 64 && LDS <= 160 * 1024, "ring");
 };
 
@@ -106,13 +107,13 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
   const int wm = (wv % C::NWM) * WM, wn = (wv / C::NWM) * WN;
   const int r = lane & 15, g = lane >> 4;
   const int kb = (p.K + 127) / 128, kt = p.K - (kb - 1) * 128;       // blocks, values of the last one
-  // copies: rows of 128 bytes, 8 a copy, dealt over the waves; a lane's chunk is (lane % 8) ^ (row / 2 % 8), the same in
-  // all of a wave's copies
-  const int ch = (lane & 7) ^ ((lane >> 4) + (wv & 1) * 4);
+  // copies: rows of 128 bytes, 8 a copy, dealt over the waves; a lane's chunk is (lane % 8) ^ (row / 2 % 8) of tokens,
+  // (lane % 8) ^ (row / 2 % 2 + 2 (row / 8 % 4)) of outputs, the same in all of a wave's copies
+  const int ch = (lane & 7) ^ ((lane >> 4) + (wv & 1) * 4), cw = (lane & 7) ^ ((lane >> 4) & 1) ^ (wv & 3) * 2;
   const uint32_t over = ch * 16 < kt ? 0u : (uint32_t)(ch * 16 - kt + 16);     // back to the last chunk below k
+  const uint32_t overw = cw * 16 < kt ? 0u : (uint32_t)(cw * 16 - kt + 16);
   const uint8_t* ab = p.a + (long long)t0 * p.a_st;
   const uint8_t* wb = p.w + (long long)n0 * p.w_st;
-  const float* sb = p.sa + (long long)t0 * p.sa_st;
   uint32_t va[C::PA], vw[C::PW];
 #pragma unroll
   for (int j = 0; j < C::PA; ++j) {
@@ -122,19 +123,22 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
 #pragma unroll
   for (int j = 0; j < C::PW; ++j) {
     const int row = min((j * 8 + wv) * 8 + (lane >> 3), p.N - 1 - n0);
-    vw[j] = (uint32_t)(row * p.w_st) + ch * 16;
+    vw[j] = (uint32_t)(row * p.w_st) + cw * 16;
   }
-  const uint32_t vs = (uint32_t)(min(wv * (BM / 8) + (lane & 31), p.T - 1 - t0) * p.sa_st * 4);
+  // the scales of BM / 8 tokens and, in the lane behind them, of the tile's block of outputs
+  const float* tokens = p.sa + (long long)min(t0 + wv * (BM / 8) + (lane & 31), p.T - 1) * p.sa_st;
+  const float* outputs = p.sw + (long long)(n0 / 128) * p.sw_st;
+  asm volatile("" : "+v"(tokens), "+v"(outputs));                    // two values, not one load of a selected argument
+  const float* sp = lane < BM / 8 ? tokens : outputs;
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)sm;
   auto copy = [&](int b, int slot, int c) {                          // number c of a block's NI copies
     SPMLA_LDS uint8_t* st = lds + slot * C::STAGE;
-    const uint32_t back = b == kb - 1 ? over : 0u;
+    const uint32_t back = b != kb - 1 ? 0u : c < C::PA ? over : overw;
     if (c < C::PA) dma16s(ab + b * 128, va[c < C::PA ? c : 0] - back, st + C::AS + (c * 8 + wv) * 1024);
     else if (c < C::PA + C::PW)
       dma16s(wb + b * 128, vw[c >= C::PA && c < C::PA + C::PW ? c - C::PA : 0] - back, st + C::WS + ((c - C::PA) * 8 + wv) * 1024);
-    else dma_lo<4>(sb + b, vs, st + C::SS + wv * (BM / 8) * 4, BM / 8 == 32 ? ~0u : (1u << (BM / 8)) - 1u);
+    else dma4_first<BM / 8 + 1>(sp + b, st + C::SS + wv * 128);
   };
-  const scalar_floats swr = (scalar_floats)(p.sw + (long long)(min(n0 + wn, p.N - 1) / 128) * p.sw_st);
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -146,14 +150,19 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
   };
   const bool z0 = g * 16 >= kt, z1 = (g + 4) * 16 >= kt;             // chunks behind k in the last block
   constexpr int NR = NT + MT + 1;
-  auto read = [&](int b, int slot, Frags& f, int c) {                 // part c of NR: a fragment, last the scales
+  // row 8 (r / 4) + 4 i + r % 4 of a wave's 32 outputs: the sums of i = 0 and 1 are eight outputs in turn, from 8 g on
+  const int fw = C::WS + (wn + 8 * (r >> 2) + (r & 3)) * 128 + ((g ^ (r >> 1)) << 4);
+  auto read = [&](int slot, Frags& f, int c) {                        // part c of NR: a fragment, last the scales
     const uint8_t* st = sm + slot * C::STAGE;
-    if (c < NT) f.w[c < NT ? c : 0] = frag(st + C::WS, wn + c * 16 + r, g);
+    if (c < NT) f.w[c < NT ? c : 0] = frag_at(st + c * 512, fw);
     else if (c < NT + MT) f.a[c >= NT && c < NT + MT ? c - NT : 0] = frag(st + C::AS, wm + (c - NT) * 16 + r, g);
     else {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) f.s[j] = *(const float*)(st + C::SS + (wm + j * 16 + r) * 4);
-      f.sw = swr[min(b, kb - 1)];
+      for (int j = 0; j < MT; ++j) {
+        const int t = wm + j * 16 + r;
+        f.s[j] = *(const float*)(st + C::SS + t / (BM / 8) * 128 + t % (BM / 8) * 4);
+      }
+      f.sw = *(const float*)(st + C::SS + wv * 128 + BM / 8 * 4);
     }
   };
   auto clip = [&](int b, Frags& f) {                                  // zeros behind k, one operand is enough
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
   lds_barrier();
   Frags f[2];
 #pragma unroll
-  for (int c = 0; c < NR; ++c) read(0, 0, f[0], c);
+  for (int c = 0; c < NR; ++c) read(0, f[0], c);
   next(out);
   // one block: f its fragments, n the next one's
   auto block = [&](int b, auto tail, const Frags& f, Frags& n) {
@@ -210,7 +219,7 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
     sums(f, [&](int m) {
 #pragma unroll
       for (int c = 0; c < NR; ++c)
-        if (c * NT * MT / NR == m) read(b + 1, out, n, c);
+        if (c * NT * MT / NR == m) read(out, n, c);
 #pragma unroll
       for (int c = 0; c < C::NI; ++c)
         if (c * NT * MT / C::NI == m) copy(min(b + ST, kb - 1), in, c);
@@ -232,10 +241,12 @@ __global__ void __launch_bounds__(512, 2) ring_kernel(LinearParams p, int TN) {
   else blocks(std::true_type{});
   wait_vm<0>();                                                       // no copy outlives the workgroup
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-      if (n0 + wn + i * 16 + 4 * g < p.N) store4<DT>(p, t0 + wm + j * 16 + r, n0 + wn + i * 16 + 4 * g, acc[i][j]);
+  for (int j = 0; j < MT; ++j) {
+    const f32x4 &x = acc[0][j], &y = acc[1][j];
+    const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    const int t = t0 + wm + j * 16 + r, n = n0 + wn + 8 * g;
+    if (t < p.T) store_upto8<DT, false>(p.out, t * p.o_st + n, p.N - n, v);
+  }
 }
 
 template <int DT, int BM, int BN, int WM, int WN, int ST>
@@ -369,122 +380,184 @@ static int stream_go(const LinearParams& p, hipStream_t s) {
 
 // ---- long chunks: tiles of 256 tokens x 256 outputs, 8 waves, the operands' halves in rings of their own --------------
 // The tile's tokens and outputs are two halves of 128 each (A0, A1, W0, W1); wave (wm, wn) takes tokens 64 wm .. + 63 of
-// both token halves and outputs 32 wn .. + 31 of both output halves: four quadrants of 8 matrix instructions each,
+// both token halves and 64 outputs from 64 wn on, 32 in each output half: four quadrants of 8 matrix instructions each,
 //   phase 0: A0 W0   1: A0 W1   2: A1 W0   3: A1 W1.
-// A half is read into registers one phase before it is used (W1 in phase 0, A1 in 1, W0 and A0 of the next block in 3, each
-// token fragment over the one that had its last use), so its place in LDS is free again long before the block is done: the
-// copies of block b + 2 start in block b and have 1.75 blocks to arrive. A workgroup barrier stands before the phases that
-// read, behind a wait for the wave's own copies of what they read. A sum is scaled and added three matrix instructions
-// after its own. A wave's copies: 5 for A0, W0 and the scales of 32 tokens, 2 for W1, 2 for A1.
+// Registers are filled one phase before they are used (W1 in phase 0, A1 in 1, W0 and A0 of the next block in 3, each token
+// fragment over the one that had its last use). A half's place in LDS is filled again as soon as a barrier stands between:
+// A0, W0 and the scales of block b + 2 in phases 1 and 2 of block b, W1 and A1 in 3, so that every copy has 1 to 1 1/2
+// blocks to arrive. The two barriers of a block stand where no read is on its way, behind a wait for the wave's
+// own copies of what is read after them. A sum is scaled and added three matrix instructions after its own.
+// A wave copies the scales of 32 tokens and, in lane 32, of its own 64 outputs in one instruction.
+//
+// Several tiles a workgroup (k a multiple of 128, more tiles than compute units): the copies run on into the next tile, so
+// that it begins at once and while the finished one's stores are under way.
+//
+// Bound by the matrix cores at the clock that the power limit leaves them: 4096 x 4096 x 16384 224 us (2.45 PFLOP/s, a
+// product with one scale a tensor at full rate 183), 188 with operands of zeros. What the steps to here gave, at that size
+// and at 4096 x 24576 x 1536 (us): one barrier a phase, scalar loads of the outputs' scales 252, 200; two barriers a block,
+// all scales by the copies 238, 195; several tiles a workgroup 236, 184; stores of 16 bytes a lane in 64-byte segments in
+// place of 8 and 32 236, 173; past the caches where the rows are whole segments 236, 161 (1.9 PFLOP/s; without stores 130).
+// 32 x 32 matrix instructions took 265, since their sums left no registers free.
 struct Big {
-  static constexpr int HALF = 128 * 128, A = 0, W = 4 * HALF, S = 8 * HALF;   // A [stage][half], W the same, then scales
-  static constexpr int LDS = S + 8 * 1024;         // of the 256 tokens: [block % 4], or 4 blocks at once [block / 4 % 2]
+  static constexpr int HALF = 128 * 128, A = 0, W = 4 * HALF, S = 8 * HALF;   // A [block % 2][half], W the same, then the
+  static constexpr int LDS = S + 4 * 2048;                                     // scales [block % 4][wave][64]
 };
 
-template <int DT, bool V4>
+// waits until at most N of the wave's memory operations are on their way, or MORE more of them where more != 0
+template <int N, int MORE>
+__device__ inline void wait_vm_or(int more) {
+  static_assert(N + MORE < 64, "vmcnt range");
+  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 .Lmore%=\n\ts_waitcnt vmcnt(%1)\n\ts_branch .Ldone%=\n.Lmore%=:\n\t"
+               "s_waitcnt vmcnt(%2)\n.Ldone%=:"
+               ::"s"(__builtin_amdgcn_readfirstlane(more)), "i"(N), "i"(N + MORE) : "memory", "scc");
+}
+
+template <int DT>
 __global__ void __launch_bounds__(512, 2) big_kernel(LinearParams p, int TN) {
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
-  const int TM = (p.T + 255) / 256, L = remap_xcd((int)blockIdx.x, TN * TM);
-  if (L < 0) return;
-  // four rows of tiles at a time, column by column: the 32 tiles that an XCD works on share 4 rows and 8 columns
-  const int grp = L / (4 * TN), rem = L - grp * 4 * TN, gm = min(4, TM - grp * 4);
-  const int t0 = (grp * 4 + rem % gm) * 256, n0 = rem / gm * 256;
+  constexpr int STORES = 16;             // of a wave and a tile that has all its tokens and outputs, 16 bytes a lane
+  const int TM = (p.T + 255) / 256, tiles = TN * TM, per = (tiles + 7) >> 3;
+  int at = (int)blockIdx.x, t0, n0;
+  // tile number at, XCD by XCD: four rows of tiles at a time, column by column, so that the 32 tiles that an XCD works on
+  // share 4 rows and 8 columns
+  auto tile = [&](int i, int& t, int& n) {
+    const int L = (i >> 3) < per ? remap_xcd(i, tiles) : -1;
+    if (L < 0) return false;
+    const int grp = L / (4 * TN), rem = L - grp * 4 * TN, gm = min(4, TM - grp * 4);
+    t = (grp * 4 + rem % gm) * 256;
+    n = rem / gm * 256;
+    return true;
+  };
+  if (!tile(at, t0, n0)) return;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = wv & 1, wn = wv >> 1, r = lane & 15, g = lane >> 4;
   const int kb = (p.K + 127) / 128, kt = p.K - (kb - 1) * 128;
-  // copies: wave wv takes rows 16 wv .. + 15 of a half, 8 a copy; a lane's chunk is (lane % 8) ^ (row / 2 % 8)
-  const int ce = (lane & 7) ^ (lane >> 4), co = ce ^ 4;
-  const uint32_t oe = ce * 16 < kt ? 0u : (uint32_t)(ce * 16 - kt + 16), oo = co * 16 < kt ? 0u : (uint32_t)(co * 16 - kt + 16);
-  const uint8_t* ab = p.a + (long long)t0 * p.a_st;
-  const uint8_t* wb = p.w + (long long)n0 * p.w_st;
-  const float* sb = p.sa + (long long)t0 * p.sa_st;
+  // copies: wave wv takes rows 16 wv .. + 15 of a half, 8 a copy
+  const uint8_t *ap, *wp;                // the next block to copy
+  const float* sp;                       // of this lane's scale
   uint32_t va[2][2], vw[2][2];
+  auto here = [&] {                      // the lane, for what is formed once a tile and not kept in registers between
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+  };
+  // a lane's chunk: (lane % 8) ^ (row / 2 % 8) of tokens, (lane % 8) ^ (row / 2 % 2 + 2 (row / 8 % 4)) of outputs
+  auto chunk = [](int l, int j) { return (l & 7) ^ (l >> 4) ^ (j * 4); };
+  auto chunk_w = [&](int l, int j) { return (l & 7) ^ ((l >> 4) & 1) ^ (((wv & 1) * 2 + j) * 2); };
+  auto row_of = [&](int l, int h, int j) { return h * 128 + wv * 16 + j * 8 + (l >> 3); };
+  auto out_of = [&](int l, int h, int j) { return (wv >> 1) * 64 + h * 32 + (wv & 1) * 16 + j * 8 + (l >> 3); };
+  auto begin = [&](int t, int n) {
+    const int l = here();
+    ap = p.a + (long long)t * p.a_st;
+    wp = p.w + (long long)n * p.w_st;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = h * 128 + wv * 16 + j * 8 + (lane >> 3);
-      va[h][j] = (uint32_t)(min(row, p.T - 1 - t0) * p.a_st) + (j ? co : ce) * 16;
-      vw[h][j] = (uint32_t)(min(row, p.N - 1 - n0) * p.w_st) + (j ? co : ce) * 16;
-    }
-  }
-  const uint32_t vs = (uint32_t)(min(wv * 32 + (lane & 31), p.T - 1 - t0) * p.sa_st * 4);
+      for (int j = 0; j < 2; ++j) {
+        va[h][j] = (uint32_t)(min(row_of(l, h, j), p.T - 1 - t) * p.a_st) + chunk(l, j) * 16;
+        vw[h][j] = (uint32_t)(min(out_of(l, h, j), p.N - 1 - n) * p.w_st) + chunk_w(l, j) * 16;
+      }
+    const float* tokens = p.sa + (long long)min(t + wv * 32 + (l & 31), p.T - 1) * p.sa_st;
+    const float* outputs = p.sw + (long long)min(n / 128 + (wn >> 1), (p.N - 1) / 128) * p.sw_st;
+    asm volatile("" : "+v"(tokens), "+v"(outputs));        // two values, not one load of a selected argument
+    sp = l < 32 ? tokens : outputs;
+  };
+  // the chunks behind k in the last block are read from the row's last one: before its copies
+  auto over = [&](int chunk) { const int e = chunk * 16 + 16 - kt; return (uint32_t)(e > 0 ? e : 0); };
+  auto end = [&] {
+    const int l = here();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        va[h][j] -= over(chunk(l, j));
+        vw[h][j] -= over(chunk_w(l, j));
+      }
+  };
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)sm;
-  auto copy_a = [&](int b, int h, int c) {
-    SPMLA_LDS uint8_t* d = lds + Big::A + ((b & 1) * 2 + h) * Big::HALF + wv * 2048;
-    dma16s(ab + b * 128, va[h][c] - (b == kb - 1 ? (c ? oo : oe) : 0u), d + c * 1024);
+  auto place = [&](int base, int c, int h, int j) {                    // of block number c of the workgroup
+    return lds + base + ((c & 1) * 2 + h) * Big::HALF + wv * 2048 + j * 1024;
   };
-  auto copy_s = [&](int b) {
-    if (V4) dma_lo<16>(sb + b, vs, lds + Big::S + (b & 4) * 1024 + wv * 512, b & 3 ? 0u : ~0u);
-    else dma_lo<4>(sb + b, vs, lds + Big::S + (b & 3) * 1024 + wv * 128, ~0u);
+  auto copy_a = [&](int c, int h, int j) { dma16s(ap, va[h][j], place(Big::A, c, h, j)); };
+  auto copy_w = [&](int c, int h, int j) { dma16s(wp, vw[h][j], place(Big::W, c, h, j)); };
+  auto copy_s = [&](int c) { dma4_first<33>(sp, lds + Big::S + (c & 3) * 2048 + wv * 256); };
+  // fragment places of this lane, chunks g and g + 4 of a row: row r of 16 tokens; row 8 (r / 4) + 4 i + r % 4 of 32 outputs,
+  // so that the sums of i = 0 and 1 are eight outputs in turn, from 8 g on: 16-byte stores, 64 bytes of a token a wave
+  const int fa = r * 128 + ((g ^ (r >> 1)) << 4), fw = (8 * (r >> 2) + (r & 3)) * 128 + ((g ^ (r >> 1)) << 4);
+  auto a_of = [&](int c, int h, int j) {
+    return frag_at(sm + Big::A + ((c & 1) * 2 + h) * Big::HALF + (wm * 64 + j * 16) * 128, fa);
   };
-  auto copy_w = [&](int b, int h, int c) {
-    SPMLA_LDS uint8_t* d = lds + Big::W + ((b & 1) * 2 + h) * Big::HALF + wv * 2048;
-    dma16s(wb + b * 128, vw[h][c] - (b == kb - 1 ? (c ? oo : oe) : 0u), d + c * 1024);
+  auto w_of = [&](int c, int h, int i) {
+    return frag_at(sm + Big::W + ((c & 1) * 2 + h) * Big::HALF + wn * 32 * 128 + i * 512, fw);
   };
-  auto first = [&](int b) {                                           // a whole block, in the order of the loop's copies
-    copy_a(b, 0, 0);
-    copy_a(b, 0, 1);
-    copy_s(b);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) copy_w(b, c >> 1, c & 1);
-    copy_a(b, 1, 0);
-    copy_a(b, 1, 1);
+  auto scale_at = [&](int c, int h, int j) {                           // token h 128 + wm 64 + j 16 + r
+    return *(const float*)(sm + Big::S + (c & 3) * 2048 + (h * 4 + wm * 2 + (j >> 1)) * 256 + ((j & 1) * 16 + r) * 4);
   };
-  // fragment places of this lane: row r of a 16-row tile, chunks g and g + 4
-  const int f0 = r * 128 + ((g ^ (r >> 1)) << 4), f1 = f0 ^ 64;
-  auto get = [&](const uint8_t* base) {
-    const i32x4 lo = *(const i32x4*)(base + f0), hi = *(const i32x4*)(base + f1);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  auto a_at = [&](int b, int h, int j) { return sm + Big::A + ((b & 1) * 2 + h) * Big::HALF + (wm * 64 + j * 16) * 128; };
-  auto w_at = [&](int b, int h, int i) { return sm + Big::W + ((b & 1) * 2 + h) * Big::HALF + (wn * 32 + i * 16) * 128; };
-  auto scale_at = [&](int b, int h, int j) {
-    const int t = h * 128 + wm * 64 + j * 16 + r;
-    return *(const float*)(sm + Big::S + (V4 ? (b & 4) * 1024 + t * 16 + (b & 3) * 4 : (b & 3) * 1024 + t * 4));
-  };
-  const bool z0 = g * 16 >= kt, z1 = (g + 4) * 16 >= kt;      // chunks behind k in the last block
-  auto clip = [&](int b, i32x8& w) {                                  // zeros behind k, one operand is enough
-    const bool y0 = z0 && b == kb - 1, y1 = z1 && b == kb - 1;
+  auto w_scale_at = [&](int c) { return *(const float*)(sm + Big::S + (c & 3) * 2048 + wv * 256 + 128); };
+  const bool z0 = g * 16 >= kt, z1 = (g + 4) * 16 >= kt;               // chunks behind k in the last block
+  auto clip = [&](i32x8& w) {                                          // zeros there, one operand is enough
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      w[e] = y0 ? 0 : w[e];
-      w[4 + e] = y1 ? 0 : w[4 + e];
+      w[e] = z0 ? 0 : w[e];
+      w[4 + e] = z1 ? 0 : w[4 + e];
     }
   };
-  constexpr int NS = V4 ? 0 : 1;      // scale copies of a block that are there for certain (those of no lane may not count)
-  const int nb1 = min(n0 / 128 + 1, (p.N - 1) / 128);
-  const scalar_floats sw0 = (scalar_floats)(p.sw + (long long)(n0 / 128) * p.sw_st);
-  const scalar_floats sw1 = (scalar_floats)(p.sw + (long long)nb1 * p.sw_st);
-  f32x4 acc[4][2][4];                                                 // quadrant, output tile, token tile
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[q][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  f32x4 d[4] = {};                                                    // sums not added yet
-  float s[2][4] = {}, sr[4];                  // scale products of this quadrant and the one before; the tokens' scales
+  f32x4 acc[4][2][4];                                                  // quadrant, output tile, token tile
+  f32x4 d[4];                                                          // sums not added yet
+  float s[2][4], sr[4], sc;       // scale products of this block's token halves; the tokens' and the outputs' scales
   i32x8 a[4], w0[2], w1[2];
-  first(0);
+  auto clear = [&] {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      d[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[1][q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[q][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  clear();
+  auto early = [&](int c) {              // the copies of a block, in the order of the loop's
+    copy_a(c, 0, 0);
+    copy_a(c, 0, 1);
+    copy_s(c);
+    copy_w(c, 0, 0);
+    copy_w(c, 0, 1);
+  };
+  auto late = [&](int c) {
+    copy_w(c, 1, 0);
+    copy_w(c, 1, 1);
+    copy_a(c, 1, 0);
+    copy_a(c, 1, 1);
+    ap += 128;
+    wp += 128;
+    sp += 1;
+  };
+  begin(t0, n0);
+  if (kb == 1) end();
+  early(0);
+  late(0);
   if (kb > 1) {
-    first(1);
-    wait_vm<12 + NS>();
+    if (kb == 2) end();
+    early(1);
+    wait_vm<7>();
   } else {
-    wait_vm<4>();
+    wait_vm<2>();
   }
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    w0[i] = get(w_at(0, 0, i));
-    clip(0, w0[i]);
+    w0[i] = w_of(0, 0, i);
+    if (kb == 1) clip(w0[i]);
   }
+  sc = w_scale_at(0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    a[j] = get(a_at(0, 0, j));
+    a[j] = a_of(0, 0, j);
     sr[j] = scale_at(0, 0, j);
   }
-  float sn0 = sw0[0], sn1 = sw1[0];
+  if (kb > 1) late(1);
   // matrix instruction 8 q + 2 j + i of a block; the sum three before it is added
   auto step = [&](int m, const i32x8& wf, const i32x8& af) {
     if (m < 32) d[m & 3] = block_sum(wf, af);
@@ -492,117 +565,150 @@ __global__ void __launch_bounds__(512, 2) big_kernel(LinearParams p, int TN) {
     const int o = m < 32 ? (m + 29) & 31 : m - 3;
     f32x4& x = acc[o >> 3][o & 1][(o >> 1) & 3];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(d[o & 3][e], s[(o >> 3) & 1][(o >> 1) & 3], x[e]);
+    for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(d[o & 3][e], s[o >> 4][(o >> 1) & 3], x[e]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto block = [&](int b, auto more_) {                               // more_: there is a block b + 2
-    constexpr bool more = decltype(more_)::value;
-    const float sc0 = sn0, sc1 = sn1;
+  // block number c of the workgroup; more_: the tiles' blocks behind it that are copied, up to 2; near, far: STORES stores
+  // were issued between what the first, the second wait is for and its wait
+  auto block = [&](int c, int near, int far, auto more_) {
+    constexpr int more = decltype(more_)::value;
     // phase 0: A0 W0; W1 is read
-    wait_vm<more ? 10 + NS : 0>();
-    lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w1[i] = get(w_at(b, 1, i));
+    for (int i = 0; i < 2; ++i) w1[i] = w_of(c, 1, i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[0][j] = sr[j] * sc0;
+    for (int j = 0; j < 4; ++j) s[0][j] = sr[j] * sc;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
       step(m, w0[m & 1], a[m >> 1]);
-      if (more && m < 2) copy_a(b + 2, 0, m);
-      if (more && m == 2) copy_s(b + 2);
-      if (more && m >= 3 && m < 5) copy_w(b + 2, 0, m - 3);
     }
-    if (!more) {
-      clip(b, w1[0]);
-      clip(b, w1[1]);
+    if (more == 0) {
+      clip(w1[0]);
+      clip(w1[1]);
     }
     // phase 1: A0 W1; A1 is read over A0
-    wait_vm<more ? 12 + 2 * NS : 0>();
+    if (more) wait_vm_or<9, STORES>(near);
+    else wait_vm<0>();
     lds_barrier();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[1][j] = sr[j] * sc1;
-      sr[j] = scale_at(b, 1, j);
-    }
+    for (int j = 0; j < 4; ++j) sr[j] = scale_at(c, 1, j);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 8; m < 16; ++m) {
       step(m, w1[m & 1], a[(m >> 1) & 3]);
-      if (m & 1) a[(m >> 1) & 3] = get(a_at(b, 1, (m >> 1) & 3));
-      else if (more && m < 12) copy_w(b + 2, 1, (m - 8) >> 1);
+      if (m & 1) a[(m >> 1) & 3] = a_of(c, 1, (m >> 1) & 3);
+      else if (more > 1 && m < 12) copy_a(c + 2, 0, (m - 8) >> 1);
     }
     // phase 2: A1 W0
-    sn0 = sw0[min(b + 1, kb - 1)];
-    sn1 = sw1[min(b + 1, kb - 1)];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[0][j] = sr[j] * sc0;
+    for (int j = 0; j < 4; ++j) s[1][j] = sr[j] * sc;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int m = 16; m < 24; ++m) step(m, w0[m & 1], a[(m >> 1) & 3]);
-    // phase 3: A1 W1; A0 (over A1) and W0 of the next block are read (behind the last one: values that nothing uses)
-    wait_vm<more ? 10 + NS : 0>();
-    lds_barrier();
+    for (int m = 16; m < 24; ++m) {
+      step(m, w0[m & 1], a[(m >> 1) & 3]);
+      if (more > 1 && m == 16) copy_s(c + 2);
+      if (more > 1 && m >= 17 && m < 19) copy_w(c + 2, 0, m - 17);
+    }
+    // phase 3: A1 W1; A0 (over A1) and W0 of the next block are read
+    if (more > 0) {
+      if (more == 2) wait_vm_or<7, STORES>(far);
+      else wait_vm<2>();
+      lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w0[i] = get(w_at(b + 1, 0, i));
+      for (int i = 0; i < 2; ++i) w0[i] = w_of(c + 1, 0, i);
+    }
+    if (more > 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[1][j] = sr[j] * sc1;
-      sr[j] = scale_at(b + 1, 0, j);
+      for (int j = 0; j < 4; ++j) sr[j] = scale_at(c + 1, 0, j);
+      sc = w_scale_at(c + 1);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 24; m < 32; ++m) {
       step(m, w1[m & 1], a[(m >> 1) & 3]);
-      if (m & 1) a[(m >> 1) & 3] = get(a_at(b + 1, 0, (m >> 1) & 3));
-      else if (more && m < 28) copy_a(b + 2, 1, (m - 24) >> 1);
+      if (more > 0 && (m & 1)) a[(m >> 1) & 3] = a_of(c + 1, 0, (m >> 1) & 3);
+      else if (more > 1 && !(m & 1) && m < 28) copy_w(c + 2, 1, (m - 24) >> 1);
+      else if (more > 1 && !(m & 1)) copy_a(c + 2, 1, (m - 28) >> 1);
     }
-    if (!more) {
-      clip(b + 1, w0[0]);
-      clip(b + 1, w0[1]);
+    if (more == 1) {
+      clip(w0[0]);
+      clip(w0[1]);
     }
+    ap += 128;
+    wp += 128;
+    sp += 1;
   };
-  int b = 0;
-  for (; b + 2 < kb; ++b) block(b, std::true_type{});
-  for (; b < kb; ++b) block(b, std::false_type{});
-#pragma unroll
-  for (int m = 32; m < 35; ++m) step(m, w1[0], a[0]);
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = n0 + (q & 1) * 128 + wn * 32 + i * 16 + 4 * g;
-      if (n >= p.N) continue;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) store4<DT>(p, t0 + (q >> 1) * 128 + wm * 64 + j * 16 + r, n, acc[q][i][j]);
+  int c = 0, stores = 0;                 // c: the workgroup's blocks before this tile
+  for (;;) {
+    int t1 = 0, n1 = 0;
+    at += (int)gridDim.x;
+    const bool go_on = tile(at, t1, n1);
+    const int most = go_on ? kb : kb - 2;
+    int b = 0;
+    for (; b < most; ++b) {
+      if (b == kb - 3) end();            // the copies are two blocks ahead
+      if (b == kb - 2) begin(t1, n1);
+      block(c + b, b < 2 ? stores : 0, b ? 0 : stores, std::integral_constant<int, 2>{});
     }
+    if (!go_on) {
+      if (kb > 1) block(c + b, b < 2 ? stores : 0, 0, std::integral_constant<int, 1>{});
+      block(c + kb - 1, 0, 0, std::integral_constant<int, 0>{});
+    }
+#pragma unroll
+    for (int m = 32; m < 35; ++m) step(m, w1[0], a[0]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)          // the sums are formed here, not each in the branch that stores it
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(acc[q][i][j]));
+    const int l = here(), lr = l & 15, lg = l >> 4;
+    const bool whole = t0 + 256 <= p.T && n0 + 256 <= p.N;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 &x = acc[q][0][j], &y = acc[q][1][j];
+        const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        const int t = t0 + (q >> 1) * 128 + wm * 64 + j * 16 + lr, n = n0 + wn * 64 + (q & 1) * 32 + 8 * lg;
+        const u32x4_any w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
+        u32x4_any* o = (u32x4_any*)((uint16_t*)p.out + t * p.o_st + n);
+        if (whole && p.o_seg) __builtin_nontemporal_store(w, o);
+        else if (whole) *o = w;
+        else if (t < p.T) store_upto8<DT, false>(p.out, t * p.o_st + n, p.N - n, v);
+      }
+    if (!go_on) return;
+    stores = __builtin_amdgcn_readfirstlane((int)whole);
+    t0 = t1;
+    n0 = n1;
+    c += kb;
+    clear();
+  }
 }
 
-template <int DT, bool V4>
+template <int DT>
 static int big_go(const LinearParams& p, hipStream_t s) {
   static DynLds lds;
-  if (int rc = lds.ensure((const void*)big_kernel<DT, V4>, Big::LDS)) return rc;
+  if (int rc = lds.ensure((const void*)big_kernel<DT>, Big::LDS)) return rc;
   const int TN = (p.N + 255) / 256;
-  const long long n = (long long)TN * ((p.T + 255) / 256);
-  hipLaunchKernelGGL((big_kernel<DT, V4>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), Big::LDS, s, p, TN);
+  long long n = ((long long)TN * ((p.T + 255) / 256) + 7) / 8 * 8;
+  if (p.K % 128 == 0 && p.K > 128 && n > 256) n = 256;                 // several tiles a workgroup, one workgroup a unit
+  hipLaunchKernelGGL((big_kernel<DT>), dim3((unsigned)n), dim3(512), Big::LDS, s, p, TN);
   return (int)hipGetLastError();
 }
 
 // the rule's kernels in its order (rules::LINEAR)
 template <int DT>
 static int linear_go(const LinearParams& p, hipStream_t s) {
-  // the scales of four blocks at once: rows of whole 16-byte pieces
-  const bool v4 = ((p.K + 127) / 128) % 4 == 0 && ((uintptr_t)p.sa & 15) == 0 && (p.sa_st & 3) == 0;
   switch (rules::linear_kernel(p.T, p.N, p.K)) {
     case 0: return stream_go<DT, 1, 1, 8, 4>(p, s);
     case 1: return stream_go<DT, 2, 1, 4, 3>(p, s);
-    case 2: return stream_go<DT, 1, 2, 8, 3>(p, s);
-    case 3: return stream_go<DT, 2, 2, 4, 2>(p, s);
-    case 4: return stream_go<DT, 2, 4, 4, 2>(p, s);
-    case 5: return stream_go<DT, 4, 4, 4, 2>(p, s);
-    case 6: return ring_go<DT, 64, 128, 32, 32, 3>(p, s);
-    case 7: return ring_go<DT, 128, 128, 64, 32, 3>(p, s);
-    case 8: return v4 ? big_go<DT, true>(p, s) : big_go<DT, false>(p, s);
+    case 2: return stream_go<DT, 2, 2, 4, 2>(p, s);
+    case 3: return stream_go<DT, 2, 4, 4, 2>(p, s);
+    case 4: return stream_go<DT, 4, 4, 4, 2>(p, s);
+    case 5: return ring_go<DT, 64, 128, 32, 32, 3>(p, s);
+    case 6: return ring_go<DT, 128, 128, 64, 32, 3>(p, s);
+    case 7: return big_go<DT>(p, s);
     default: return SPMLA_ELIMIT;
   }
 }
@@ -628,7 +734,7 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
   if (T > MAX_TOKENS || N > MAX_TOKENS) return SPMLA_ELIMIT;
   if (a_st > (1 << 22) || w_st > (1 << 22) || as_st > (1 << 20)) return SPMLA_ELIMIT;   // 32-bit offsets inside a tile
   lin::LinearParams p{(const uint8_t*)a, a_st, a_scales, as_st, (const uint8_t*)w, w_st, w_scales, ws_st, out, o_st,
-                      T, N, K, ((uintptr_t)out & 7) == 0 && (o_st & 3) == 0};
+                      T, N, K, ((uintptr_t)out & 7) == 0 && (o_st & 3) == 0, ((uintptr_t)out & 63) == 0 && (o_st & 31) == 0};
   if (dtype == DT_F16) return lin::linear_go<DT_F16>(p, (hipStream_t)stream);
   return lin::linear_go<DT_BF16>(p, (hipStream_t)stream);
 }

@@ -48,22 +48,21 @@ inline int merged_splits(int T, int H, int K, int S, bool r576) {
 
 // The projection kernels (spmla_linear.hip): tile of tokens x outputs and a model of a launch's us,
 // c0 + c1 rounds + c2 rounds kb + c3 wgs kb / 256 + c4 wgs / 256 with kb blocks of 128 k and rounds of 256 workgroups; fitted
-// to graphed launches of 444 shapes (T 1 to 4096, N 64 to 24576, K 512 to 16384; operands of three launches ago in the
-// caches). The chosen kernel is the fastest or within 5 % of it on 430 of them, 0.4 % slower on average, 26 % at most. Every
-// kernel is wanted: without it the chosen ones are 1 to 6 % slower on average and up to 25 to 79 % on a shape. Few tokens
-// need not mean few workgroups, nor many tokens large tiles (us, chosen / the kernel by tokens alone): 825 x 80 x 7776
-// tiles of 16 x 32 11 / 64 x 128 22; 64 x 152 x 4560 16 x 16 4.6 / 64 x 16 6.3.
+// to graphed launches of 486 shapes (T 1 to 8192, N 64 to 24576, K 512 to 16384; operands of three launches ago in the
+// caches). The chosen kernel is the fastest or within 5 % of it on 477 of them, 0.2 % slower on average, 11 % at most. Every
+// kernel is wanted: without it the chosen ones are 1 to 7 % slower on average and up to 24 to 88 % on a shape. Few tokens
+// need not mean few workgroups, nor many tokens large tiles (us): 825 x 80 x 7776 tiles of 16 x 32 11 / 64 x 128 22; 64 x
+// 152 x 4560 16 x 16 4.3 / 64 x 16 6.3.
 struct LinearKernel { int bm, bn; float c[5]; };
 constexpr LinearKernel LINEAR[] = {
-    {16, 16, {1.240f, 1.142f, 0.039f, 0.044f, 0.000f}},   // stream_kernel NT1 MT1 NW8 ST4
-    {16, 32, {2.375f, 0.000f, 0.075f, 0.050f, 0.000f}},   // stream_kernel NT2 MT1 NW4 ST3
-    {32, 16, {1.154f, 1.331f, 0.060f, 0.038f, 0.000f}},   // stream_kernel NT1 MT2 NW8 ST3
-    {32, 32, {2.580f, 0.000f, 0.098f, 0.055f, 0.000f}},   // stream_kernel NT2 MT2 NW4 ST2
-    {64, 32, {1.933f, 0.600f, 0.200f, 0.000f, 0.863f}},   // stream_kernel NT2 MT4 NW4 ST2
-    {64, 64, {2.058f, 1.347f, 0.274f, 0.000f, 1.208f}},   // stream_kernel NT4 MT4 NW4 ST2
-    {64, 128, {2.012f, 0.763f, 0.437f, 0.013f, 1.913f}},   // ring_kernel 64x128 w32x32
-    {128, 128, {1.382f, 2.853f, 0.443f, 0.248f, 1.136f}},   // ring_kernel 128x128 w64x32
-    {256, 256, {5.039f, 8.372f, 1.190f, 0.886f, 0.566f}},   // big_kernel
+    {16, 16, {1.358f, 0.989f, 0.041f, 0.045f, 0.000f}},   // stream_kernel NT1 MT1 NW8 ST4
+    {16, 32, {2.377f, 0.000f, 0.079f, 0.040f, 0.053f}},   // stream_kernel NT2 MT1 NW4 ST3
+    {32, 32, {2.577f, 0.000f, 0.096f, 0.047f, 0.140f}},   // stream_kernel NT2 MT2 NW4 ST2
+    {64, 32, {1.664f, 1.121f, 0.180f, 0.021f, 0.454f}},   // stream_kernel NT2 MT4 NW4 ST2
+    {64, 64, {1.921f, 1.572f, 0.269f, 0.000f, 0.937f}},   // stream_kernel NT4 MT4 NW4 ST2
+    {64, 128, {2.623f, 0.000f, 0.401f, 0.014f, 1.643f}},   // ring_kernel 64x128 w32x32
+    {128, 128, {1.861f, 1.342f, 0.522f, 0.096f, 1.174f}},   // ring_kernel 128x128 w64x32
+    {256, 256, {0.795f, 6.197f, 0.986f, 0.780f, 0.502f}},   // big_kernel
 };
 
 // The cheapest kernel by the model; -1: none takes so many workgroups.

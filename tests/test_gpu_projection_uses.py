@@ -20,9 +20,12 @@ def test_every_projection_kernel(dev, kernel, T, N, K, dt):
     want = ref.linear(a, sa, w, sw)[0].float().to(DT[dt])
     out = torch.full((T, N + 3), 5.0, dtype=DT[dt], device=dev)
     print(f"[linear] kernel {kernel} T={T} N={N} K={K}", flush=True)
-    kernels.linear_fp8(_wide(a, 16, dev), sa.to(dev), _wide(w, 16, dev), sw.to(dev), out=out[:, :N])
+    args = _wide(a, 16, dev), sa.to(dev), _wide(w, 16, dev), sw.to(dev)
+    kernels.linear_fp8(*args, out=out[:, :N])
+    whole = kernels.linear_fp8(*args, dtype=DT[dt])           # rows that begin on 64 bytes where N allows it
     torch.cuda.synchronize()
     assert torch.equal(out[:, :N].cpu(), want) and bool((out[:, N:] == 5.0).all())
+    assert torch.equal(whole.cpu(), want)
 
 
 @pytest.mark.parametrize("T,D", [(3, 256), (2, 1536), (5, 1500), (2, 4096), (3, 3268), (2, 6578), (70, 15), (2, 16385)])
