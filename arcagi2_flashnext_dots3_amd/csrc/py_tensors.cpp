@@ -252,7 +252,10 @@ long rope(PyObject* const* a) {
   line(*freqs, 0, ANY, F64, "freqs [pairs] float64");
   const int64_t n = freqs->size(0);
   if (start < 0 || n > W / 2 || start > W - 2 * n) refuse("start + 2 len(freqs) columns inside the head");
-  if ((T > 1 && o_st < W) || (H > 1 && o_sh < W)) refuse("out: heads that do not overlap");
+  // heads of a token or tokens of a head lie behind one another: no element is written twice
+  if (T > 0 && H > 0 && ((T > 1 && o_st < W) || (H > 1 && o_sh < W) ||
+                         (T > 1 && H > 1 && o_st < (H - 1) * o_sh + W && o_sh < (T - 1) * o_st + W)))
+    refuse("out: heads that do not overlap");
   const int dev = gpu_of(*x);
   for (const at::Tensor* t : {x, pos, freqs, out}) same_gpu(*t, dev, "rope");
   const int Ti = as_int(T, "T"), Hi = as_int(H, "H"), Wi = as_int(W, "W");

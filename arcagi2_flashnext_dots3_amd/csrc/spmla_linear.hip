@@ -80,8 +80,8 @@ __device__ inline void store4(const LinearParams& p, int t, int n, f32x4 v) {   
 // ---- tiles of BM tokens x BN outputs, 8 waves of WM x WN, a ring of ST blocks in LDS ----------------------------------
 // While the sums of block b form from registers, block b + 1 is read from LDS and blocks b + 2 .. b + ST are on their way:
 // one barrier a block, behind which block b's place is free and block b + 1 has arrived.
-// Bound by LDS: the copies of a block of 128 x 128 (33 KB, 64 bytes a clock) and its reads (100 KB, 256 a clock) take 900
-// clocks, the matrix instructions 512; a block takes 1000. 1455 x 2112 x 4096 21 us (1.2 PFLOP/s, 204 workgroups), 6 of them
+// Bound by LDS: the copies of a block of 128 x 128 (33 KB at 64 bytes a clock) take 510 clocks and its reads 470, the matrix
+// instructions 510; a block takes 1000 to 1200. 1455 x 2112 x 4096 21 us (1.2 PFLOP/s, 204 workgroups), 6 of them
 // before and behind the blocks; 64 x 24576 x 1536 in tiles of 64 x 128 9.4 us (4.3 TB/s of weights and outputs). 16 waves,
 // wave tiles of 64 x 64 and a ring of 4 blocks were no faster, two workgroups a unit (128 registers) 10 % slower.
 template <int BM, int BN, int WM, int WN, int ST>
@@ -263,6 +263,10 @@ static int ring_go(const LinearParams& p, hipStream_t s) {
 // ---- few tokens: the weights stream past 16 MT tokens --------------------------------------------------------------
 // A workgroup takes 16 NT outputs and 16 MT tokens; its NW waves take the blocks of k in turn, each with a ring of ST
 // stages of its own in LDS, so that no wave waits for another until their sums meet in LDS at the end, in wave order.
+// Bound by HBM once the weights are many: 1 x 4096 x 16384 12.1 us (5.5 TB/s), 32 x 4096 x 16384 14.0 (4.8), 16 x 24576 x
+// 1536 8.8 (4.4); before that by the launch and the first loads' way: 1 x 2112 x 4096 3.8 us in a graph, of 1.7 at the copy's
+// rate. Tiles of 16 x 16 with 8 waves give the most workgroups and the shortest part of k a wave; 4 waves of two output tiles
+// read the tokens half as often.
 template <int NT, int MT, int NW, int ST>
 struct Stream {
   static constexpr int WS = 0, AS = NT * 2048, SS = AS + MT * 2048, STAGE = SS + 256;
@@ -314,6 +318,7 @@ __global__ void __launch_bounds__(64 * NW, 2) stream_kernel(LinearParams p, int 
 #pragma unroll
   for (int i = 0; i < ST; ++i)
     if (i < cnt) issue(i);
+  float sw = swr[min(wv, kb - 1)];
   for (int i = 0; i < cnt; ++i) {
     if (i + ST <= cnt) wait_vm<(ST - 1) * C::NI>();
     else wait_vm<0>();
@@ -324,7 +329,6 @@ __global__ void __launch_bounds__(64 * NW, 2) stream_kernel(LinearParams p, int 
       for (int j = 0; j < 2 * NT; ++j)
         if ((j & 1 ? co : ce) * 16 >= kt) *(u32x4*)(st + C::WS + j * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
     }
-    const float sw = swr[b];
     i32x8 av[MT], wf[NT];
     float sc[MT];
 #pragma unroll
@@ -336,6 +340,9 @@ __global__ void __launch_bounds__(64 * NW, 2) stream_kernel(LinearParams p, int 
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the stage has been read: its ring place is free
     if (i + ST < cnt) issue(i + ST);
+    __builtin_amdgcn_sched_barrier(0);
+    sw = swr[min(b + NW, kb - 1)];                                    // on its way while this block's sums form
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -460,8 +460,7 @@ int spmla_topk_overlap(const int* sets, long long s_l, long long s_r, int L, int
  * of y with one fp32 scale per 128 values, s = max(amax / 448, 1e-12) (ue8m0: rounded up to a power of two), the code of
  * y over s before s's own rounding; the last group of a row may be shorter. x, residual, residual_out, out [T][D] rows of
  * dtype 0 fp32, 1 fp16, 2 bf16 (row strides in elements; out may be x); weight [D] of the same type, or fp32 with
- * weight_f32; codes [T][D] bytes, scales [T][ceil(D / 128)]. D <= 65536. Rows aligned to 16 bytes with D % 8 == 0 (codes
- * to 8) take 16-byte accesses, others are read by elements.
+ * weight_f32; codes [T][D] bytes, scales [T][ceil(D / 128)]. D <= 65536, T <= 2^23 (here and in the four calls below).
  * No counterpart in the reference's tree: vLLM's fused norms run in its place there. */
 int spmla_rms_norm(const void* x, long long x_st, const void* residual, long long r_st, void* residual_out,
                    long long ro_st, const void* weight, int weight_f32, float eps, int T, int D, int dtype, void* out,
@@ -476,7 +475,8 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
 /* Projection of 8-bit activations on FP8 block-scaled weights:
  * out[t][n] = sum_b a_scales[t][b] * w_scales[n / 128][b] * sum_{k in block b} a[t][k] * w[n][k], blocks of 128 k.
  * a [T][K], w [N][K] e4m3 codes (row strides a multiple of 16 bytes, at most 2^22), a_scales [T][ceil(K / 128)], w_scales
- * [ceil(N / 128)][ceil(K / 128)] fp32 (the checkpoint's weight_scale_inv), out [T][N] dtype 1 fp16 or 2 bf16. K % 16 == 0.
+ * [ceil(N / 128)][ceil(K / 128)] fp32 (the checkpoint's weight_scale_inv), out [T][N] dtype 1 fp16 or 2 bf16. K % 16 == 0,
+ * N <= 2^23.
  * The 128 products of a block are added by the matrix core (1.4e-5 of the sum's size on normally distributed codes), the
  * blocks in fp32. No counterpart in the reference's tree: vLLM's block-FP8 linear layers run in its place there. */
 int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long long as_st, const void* w,
@@ -495,7 +495,8 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
 
 /* A token's cache row from its down-projected latent: kv [n][512 latent | 64 rope] bf16 (row stride kv_st) -> RMS norm of
  * the latent (weight [512] bf16 or fp32, null: 1), rotary of the rope values (freqs [32], as spmla_rope), then the row of
- * spmla_cache_write's formats 0, 1 and 2 at slots[i] (slot < 0 or >= R: skipped, its values not read). The norm and the
+ * spmla_cache_write's formats 0, 1 and 2 at slots[i] (slot < 0 or >= R: skipped, its values not read; of tokens with the same slot any may be
+ * the one kept, or parts of several). The norm and the
  * rotation stay in fp32 until they are encoded: Row656's codes are those of spmla_rms_norm, its rope is rounded once to
  * bf16. Replaces the norm, rotary and do_kv_cache_update calls around dsa_sm89.py:281-290. */
 int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int weight_f32, float eps,

@@ -83,6 +83,9 @@ def test_rope():
     _refused("out of x's", kernels.rope, x, pos, f, out=x.float())
     _refused("contiguous head", kernels.rope, _t(4, 2, 128)[..., ::2], pos, f)
     _refused("overlap", kernels.rope, x, pos, f, out=_t(4, 1, 64).expand(4, 2, 64))
+    _refused("overlap", kernels.rope, x, pos, f, out=_t(5 * 64).as_strided((4, 2, 64), (64, 64, 1)))
+    _refused("overlap", kernels.rope, x, pos, f, out=_t(1024).as_strided((4, 2, 64), (65, 64, 1)))
+    _refused("one GPU", kernels.rope, x, pos, f, out=_t(2, 4, 64).transpose(0, 1))       # heads outermost: taken
 
 
 def test_latent_write():
