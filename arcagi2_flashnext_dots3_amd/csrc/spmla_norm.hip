@@ -5,12 +5,12 @@
 // Sums, root and y are held in 32 bits or more (a thread's squares in fp32, with ue8m0 in 64 bits; then 64); y is not
 // rounded to the 16-bit type before it is quantized.
 //
-// One pass: a row's values stay in the registers of the NT threads that share it, 8 a thread in CH chunks, so x and the
-// residual are read once. A group of 128 values is 16 neighbouring lanes of a chunk. Rows of up to 512 values take one
-// wave each (no LDS), longer ones a workgroup.
-// Bound by HBM for long chunks: 8192 x 4096 bf16 with residual and codes 48 us (236 MB, 4.9 TB/s; a device copy moves 5.1).
-// Few rows: the chain of a row's loads, sum, root and codes, 3.4 us (64 x 1536) to 4.1 us (1 x 4096) of GPU time; alone, the
-// quantization of 32 x 16384 takes 2.4.
+// One pass: a row's values stay in the registers of the threads that share it, 8 a thread in CH chunks, so x and the
+// residual are read once; x, residual and weights are all on their way before the first is needed. A group of 128 values is
+// 16 neighbouring lanes of a chunk. Rows of up to 512 values take one wave each (no LDS), longer ones several.
+// Bound by HBM for long chunks: 8192 x 4096 bf16 with residual and codes 44 us (236 MB, 5.3 TB/s with part of it in the last
+// cache; a device copy moves 5.1). Few rows: the chain of a row's loads, sum, root and codes, 3.3 us (64 x 1536) to 3.5 us
+// (1 x 4096) a launch in a graph; the quantization of 32 x 16384 alone takes 2.3.
 #include "spmla_quant.h"
 
 namespace spmla {
@@ -27,46 +27,60 @@ struct NormParams {
   uint8_t* codes; long long c_st;                            // null without them
   float* scales; long long s_st;
   int ue8m0;
+  int nt;                                                    // threads that share a row, where a workgroup has one
 };
 
 // Loads and stores are 16 bytes of a lane at any alignment of the type (gfx950 takes them; a misaligned row costs one more
-// line a wave). WHOLE: D % 8 == 0; else the lane at a row's end goes element by element (13 x 3268 fp32 4.4 us a call, 221 x
-// 6578 fp32 5.7, 753 x 1500 bf16 4.9; with whole rows element by element 9.9, 10.1, 7.8). NORM false: y = x, a workgroup
-// per NT * 8 values of a row.
-template <int DT, bool NORM, int NT, int CH, bool WHOLE>
+// line a wave). ROW: how rows end (load_raw); ends that are no whole eights are stored element by element. In a graph 13 x
+// 3268 fp32 3.8 us, 8192 x 3268 bf16 42; element by element the calls took two to three times as long. NORM false: y = x, a
+// workgroup per NT * 8 values of a row.
+template <int DT, bool NORM, int NT, int CH, int ROW>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;               // rows per workgroup
-  __shared__ double part[NT / 64];
-  const int tid = threadIdx.x % NT, lane = threadIdx.x & 63;
+  __shared__ double part[RPB][NT / 64];
+  const int tid = threadIdx.x % NT, lane = threadIdx.x & 63, nt = NORM && RPB == 1 ? p.nt : NT;   // threads of a row
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / NT;
   const bool on = row < p.T;
+  const long long from = on ? row : p.T - 1;                 // (a row without a thread's own is read, not written)
   const int base = NORM ? 0 : (int)blockIdx.y * (NT * 8);
-  constexpr bool EARLY = CH <= 2;                            // weights on their way before the sum (128 registers a thread)
-  float z[CH][8], w[EARLY ? CH : 1][8];
-  auto at = [&](int c) { return base + (c * NT + tid) * 8; };
-  auto left = [&](int c) { return on ? p.D - at(c) : 0; };   // values of the row from there on
+  constexpr bool AHEAD = CH <= 2;                            // all that is read on its way at once (128 registers a thread)
+  float z[CH][8];
+  auto at = [&](int c) { return base + (c * nt + tid) * 8; };
+  auto left = [&](int c) { return p.D - at(c); };            // values of the row from there on
+  auto mine = [&](int c) { return on ? left(c) : 0; };
+  Raw8<DT> x[CH], a[AHEAD ? CH : 1];
+  Raw8<DT_F32> wf[AHEAD ? CH : 1];
+  Raw8<DT> wd[AHEAD ? CH : 1];
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    load_upto8<DT, WHOLE>(p.x, row * p.x_st + at(c), left(c), z[c]);
+  for (int c = 0; c < CH; ++c) load_raw<DT, ROW>(p.x, from * p.x_st + at(c), left(c), x[c]);
+  auto load_residual = [&](int c) { load_raw<DT, ROW>(p.res, from * p.res_st + at(c), left(c), a[AHEAD ? c : 0]); };
+  auto load_weights = [&](int c) {
+    if (DT == DT_F32 || p.w_f32) load_raw<DT_F32, ROW>(p.w, at(c), left(c), wf[AHEAD ? c : 0]);
+    else load_raw<DT, ROW>(p.w, at(c), left(c), wd[AHEAD ? c : 0]);
+  };
+  if constexpr (NORM && AHEAD) {
+    if (p.res) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) load_residual(c);
+    }
+    if (p.w) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) load_weights(c);
+    }
   }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) values_of<DT, ROW>(x[c], left(c), z[c]);
   Factor r{1.0f, 0.0f};
   if constexpr (NORM) {
-    auto weights = [&](int c, float (&v)[8]) {
-      if (p.w_f32) load_upto8<DT_F32, WHOLE>(p.w, at(c), left(c), v);
-      else load_upto8<DT, WHOLE>(p.w, at(c), left(c), v);
-    };
-    if (EARLY && p.w) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c) weights(c, w[c]);
-    }
     if (p.res) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float a[8];
-        load_upto8<DT, WHOLE>(p.res, row * p.res_st + at(c), left(c), a);
+        if (!AHEAD) load_residual(c);
+        float b[8];
+        values_of<DT, ROW>(a[AHEAD ? c : 0], left(c), b);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[c][e] = round_to<DT>(z[c][e] + a[e]);
-        store_upto8<DT, WHOLE>(p.res_out, row * p.ro_st + at(c), left(c), z[c]);
+        for (int e = 0; e < 8; ++e) z[c][e] = round_to<DT>(z[c][e] + b[e]);
+        store_upto8<DT, ROW == WHOLE>(p.res_out, row * p.ro_st + at(c), mine(c), z[c]);
       }
     }
     double ss = 0.0;
@@ -85,18 +99,24 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     }
     ss = wave_sum(ss);
     if constexpr (NT > 64) {
-      if (lane == 0) part[tid >> 6] = ss;
+      double* of = part[threadIdx.x / NT];
+      if (lane == 0) of[tid >> 6] = ss;
       __syncthreads();
-      ss = part[0];
-#pragma unroll
-      for (int i = 1; i < NT / 64; ++i) ss += part[i];
+      const int i = lane & (NT / 64 - 1);                    // the waves' sums, one a lane, added in one order
+      ss = i * 64 < nt ? of[i] : 0.0;
+      ss += dpp<DPP_XOR1>(ss);
+      if (NT > 128) ss += dpp<DPP_XOR2>(ss);
+      if (NT > 256) ss += dpp<DPP_HALF_MIRROR>(ss);
+      if (NT > 512) ss += dpp<DPP_MIRROR>(ss);
     }
     r = factor_of(inverse_root(ss * p.inv_d + (double)p.eps));
     if (p.w) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float (&v)[8] = w[EARLY ? c : 0];
-        if (!EARLY) weights(c, v);
+        if (!AHEAD) load_weights(c);
+        float v[8];
+        if (DT == DT_F32 || p.w_f32) values_of<DT_F32, ROW>(wf[AHEAD ? c : 0], left(c), v);
+        else values_of<DT, ROW>(wd[AHEAD ? c : 0], left(c), v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) z[c][e] *= v[e];
       }
@@ -108,7 +128,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = z[c][e] * r.hi;
-      store_upto8<DT, WHOLE>(p.out, row * p.o_st + at(c), left(c), y);
+      store_upto8<DT, ROW == WHOLE>(p.out, row * p.o_st + at(c), mine(c), y);
     }
   }
   if (p.codes) {
@@ -116,12 +136,12 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
     for (int c = 0; c < CH; ++c) {
       uint32_t lo, hi;
       const float s = group_codes(z[c], r, p.ue8m0 != 0, lo, hi);
-      const int d = at(c), n = left(c);
+      const int d = at(c), n = mine(c);
       if (n > 0) {
         uint8_t* q = p.codes + row * p.c_st + d;
         if (n >= 8) {
           *(codes8*)q = codes8{lo, hi};
-        } else if constexpr (!WHOLE) {
+        } else if constexpr (ROW != WHOLE) {
 #pragma unroll
           for (int e = 0; e < 7; ++e)
             if (e < n) q[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
@@ -132,40 +152,54 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
   }
 }
 
-template <int DT, bool NORM, int NT, int CH, bool WHOLE>
-static void launch(const NormParams& p, hipStream_t s) {
+template <int DT, bool NORM, int NT, int CH, int ROW>
+static void launch(NormParams p, hipStream_t s) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
+  p.nt = NORM && RPB == 1 ? (p.D + 512 * CH - 1) / (512 * CH) * 64 : NT;   // no wave without a value
   const unsigned gy = NORM ? 1u : (unsigned)((p.D + NT * 8 - 1) / (NT * 8));
-  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, WHOLE>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
-                     dim3(NT < 256 ? 256 : NT), 0, s, p);
+  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, ROW>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
+                     dim3((unsigned)(p.nt * RPB)), 0, s, p);
 }
 
 constexpr int MAX_D = 65536;
 
-template <int DT, bool WHOLE>
+template <int DT, int ROW>
 static void norm_go(const NormParams& p, hipStream_t s) {
-  if (p.D <= 512) launch<DT, true, 64, 1, WHOLE>(p, s);
-  else if (p.D <= 2048) launch<DT, true, 256, 1, WHOLE>(p, s);
-  else if (p.D <= 4096) launch<DT, true, 256, 2, WHOLE>(p, s);
-  else if (p.D <= 16384) launch<DT, true, 1024, 2, WHOLE>(p, s);
-  else launch<DT, true, 1024, 8, WHOLE>(p, s);
+  // as few threads and chunks as hold the row: idle ones cost as much as busy ones (8192 x 576 64 x 1 to 256 x 1: 13.7 to
+  // 21.5 us). Of equal ones many threads for few rows (4096 values, 1 row: 512 x 1 3.6, 256 x 2 4.6; 7168: 1024 x 1 4.6, 512 x
+  // 2 5.1), fewer that each have more on their way for many (8192 rows: 45 / 42, 104 / 88).
+  if constexpr (ROW == TINY) {
+    launch<DT, true, 64, 1, ROW>(p, s);
+    return;
+  } else {
+  if (p.D <= 512) launch<DT, true, 64, 1, ROW>(p, s);
+  else if (p.D <= 1024) launch<DT, true, 128, 1, ROW>(p, s);
+  else if (p.D <= 2048) launch<DT, true, 256, 1, ROW>(p, s);
+  else if (p.D <= 4096 && p.T <= 4096) launch<DT, true, 512, 1, ROW>(p, s);
+  else if (p.D <= 4096) launch<DT, true, 256, 2, ROW>(p, s);
+  else if (p.D <= 8192 && p.T <= 1024) launch<DT, true, 1024, 1, ROW>(p, s);
+  else if (p.D <= 8192) launch<DT, true, 512, 2, ROW>(p, s);
+  else if (p.D <= 16384) launch<DT, true, 1024, 2, ROW>(p, s);
+  else launch<DT, true, 1024, 8, ROW>(p, s);
+  }
 }
 
 static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
   auto by_type = [&](auto tag) {
-    constexpr bool V = decltype(tag)::value;
+    constexpr int R = decltype(tag)::value;
     if (norm) {
-      if (dtype == DT_F32) norm_go<DT_F32, V>(p, s);
-      else if (dtype == DT_F16) norm_go<DT_F16, V>(p, s);
-      else norm_go<DT_BF16, V>(p, s);
+      if (dtype == DT_F32) norm_go<DT_F32, R>(p, s);
+      else if (dtype == DT_F16) norm_go<DT_F16, R>(p, s);
+      else norm_go<DT_BF16, R>(p, s);
     } else {
-      if (dtype == DT_F32) launch<DT_F32, false, 256, 1, V>(p, s);
-      else if (dtype == DT_F16) launch<DT_F16, false, 256, 1, V>(p, s);
-      else launch<DT_BF16, false, 256, 1, V>(p, s);
+      if (dtype == DT_F32) launch<DT_F32, false, 256, 1, R>(p, s);
+      else if (dtype == DT_F16) launch<DT_F16, false, 256, 1, R>(p, s);
+      else launch<DT_BF16, false, 256, 1, R>(p, s);
     }
   };
-  if (p.D % 8 == 0) by_type(std::true_type{});
-  else by_type(std::false_type{});
+  if (p.D % 8 == 0) by_type(std::integral_constant<int, WHOLE>{});
+  else if (p.D > 8) by_type(std::integral_constant<int, ENDS>{});
+  else by_type(std::integral_constant<int, TINY>{});
   return (int)hipGetLastError();
 }
 
@@ -191,7 +225,7 @@ int spmla_rms_norm(const void* x, long long x_st, const void* residual, long lon
       ((uintptr_t)weight & (weight_f32 ? 3 : eb - 1)) || ((uintptr_t)scales & 3))
     return SPMLA_EALIGN;
   nrm::NormParams p{x, x_st, residual, residual_out, r_st, ro_st, weight, weight_f32, eps, 1.0 / D, T, D,
-                    out, o_st, codes, c_st, scales, s_st, ue8m0};
+                    out, o_st, codes, c_st, scales, s_st, ue8m0, 0};
   return nrm::go(p, true, dtype, (hipStream_t)stream);
 }
 
@@ -203,7 +237,7 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
   if (!x || !codes || !scales) return SPMLA_EARG;
   if (((uintptr_t)x & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)scales & 3)) return SPMLA_EALIGN;
   nrm::NormParams p{x, x_st, nullptr, nullptr, 0, 0, nullptr, 0, 0.f, 0.0, T, D,
-                    nullptr, 0, codes, c_st, scales, s_st, ue8m0};
+                    nullptr, 0, codes, c_st, scales, s_st, ue8m0, 0};
   return nrm::go(p, false, dtype, (hipStream_t)stream);
 }
 

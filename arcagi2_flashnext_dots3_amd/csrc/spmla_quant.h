@@ -144,36 +144,69 @@ template <int DT, class Q = u32x4> __device__ inline void store8(void* p, long l
 }
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef uint32_t codes8 __attribute__((ext_vector_type(2), aligned(1)));       // eight codes at any address
-// the same of a row that ends after n values (WHOLE: after 8 or more, or none of them); zeros behind it
-template <int DT, bool WHOLE> __device__ inline void load_upto8(const void* p, long long i, int n, float (&v)[8]) {
-  if (n >= 8) {
-    load8<DT, u32x4_any>(p, i, v);
-    return;
-  }
-  u32x4 a{0, 0, 0, 0}, b{0, 0, 0, 0};
-  if constexpr (!WHOLE) {
+// Eight values of a row from element i on, the row's last n values from there (n <= 0: behind it), as the words in memory and
+// then as numbers with zeros behind the row: no branch stands between several loads. WHOLE rows are whole eights, ENDS
+// rows have 8 values or more (their last eight are loaded where they end earlier, and moved down), TINY ones fewer.
+enum : int { WHOLE = 0, ENDS = 1, TINY = 2 };
+template <int DT> struct Raw8 {
+  static constexpr int NW = DT == DT_F32 ? 8 : 4;
+  uint32_t w[NW];
+};
+template <int DT, int ROW> __device__ inline void load_raw(const void* p, long long i, int n, Raw8<DT>& r) {
+  if constexpr (ROW == TINY) {
+#pragma unroll
+    for (int e = 0; e < Raw8<DT>::NW; ++e) r.w[e] = 0;
 #pragma unroll
     for (int e = 0; e < 7; ++e) {
-      if constexpr (DT == DT_F32) {
-        const uint32_t w = e < n ? ((const uint32_t*)p)[i + e] : 0;
-        if (e < 4) a[e] = w;
-        else b[e - 4] = w;
-      } else {
-        a[e >> 1] |= (uint32_t)(e < n ? ((const uint16_t*)p)[i + e] : 0) << (16 * (e & 1));
+      if (e >= n) continue;
+      if constexpr (DT == DT_F32) r.w[e] = ((const uint32_t*)p)[i + e];
+      else r.w[e >> 1] |= (uint32_t)((const uint16_t*)p)[i + e] << (16 * (e & 1));
+    }
+  } else {
+    const char* q = (const char*)p + (i + min(n - 8, 0)) * (DT == DT_F32 ? 4 : 2);
+#pragma unroll
+    for (int h = 0; h < Raw8<DT>::NW / 4; ++h) {
+      const u32x4 a = *(const u32x4_any*)(q + 16 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.w[4 * h + e] = a[e];
+    }
+  }
+}
+template <int DT, int ROW> __device__ inline void values_of(Raw8<DT> r, int n, float (&v)[8]) {
+  constexpr int NW = Raw8<DT>::NW;
+  if constexpr (ROW == ENDS) {
+    if (n < 8) {
+      const int by = 8 - n;
+      auto down = [&](int words) {
+#pragma unroll
+        for (int e = 0; e < NW; ++e) r.w[e] = e + words < NW ? r.w[e + words < NW ? e + words : 0] : 0;
+      };
+      if (by & 4) down(NW / 2);
+      if (by & 2) down(NW / 4);
+      if (by & 1) {
+        if constexpr (DT == DT_F32) {
+          down(1);
+        } else {
+#pragma unroll
+          for (int e = 0; e < NW; ++e) r.w[e] = r.w[e] >> 16 | (e + 1 < NW ? r.w[e + 1 < NW ? e + 1 : 0] << 16 : 0);
+        }
       }
     }
   }
+#pragma unroll
+  for (int e = 0; e < NW; ++e) r.w[e] = n > 0 ? r.w[e] : 0;
   if constexpr (DT == DT_F32) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = u2f(a[e]); v[4 + e] = u2f(b[e]); }
+    for (int e = 0; e < 8; ++e) v[e] = u2f(r.w[e]);
   } else {
-    unpack8<DT>(a, v);
+    unpack8<DT>(u32x4{r.w[0], r.w[1], r.w[2], r.w[3]}, v);
   }
 }
-template <int DT, bool WHOLE> __device__ inline void store_upto8(void* p, long long i, int n, const float (&v)[8]) {
+// the first n of eight values (n <= 0: none) from element i on; EIGHTS: n >= 8 or n <= 0
+template <int DT, bool EIGHTS> __device__ inline void store_upto8(void* p, long long i, int n, const float (&v)[8]) {
   if (n >= 8) {
     store8<DT, u32x4_any>(p, i, v);
-  } else if constexpr (!WHOLE) {
+  } else if constexpr (!EIGHTS) {
 #pragma unroll
     for (int e = 0; e < 7; ++e) {
       if (e >= n) continue;

@@ -157,3 +157,20 @@ def test_quantized_product_in_pieces(dev):
             assert got.dtype == torch.float16 and torch.equal(got, want)
             assert mla_fp8.linear_fp8(x, f, out=out, ue8m0=ue8m0) is out
             assert torch.equal(out, kernels.linear_fp8(*kernels.quant_fp8(x, ue8m0=ue8m0), *f))
+
+
+@pytest.mark.parametrize("T,D", [(4100, 2056), (4097, 4001), (1030, 4104), (1025, 7001), (600, 1000), (2, 5), (1, 9)])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_norm_of_many_rows_and_of_few_values(dev, T, D, dt):
+    """Sizes on the other side of the norm's choices by rows, and rows around eight values, against 64 bits; the sums in place."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    g = torch.Generator().manual_seed(T)
+    x, r = (torch.randn(T, D, generator=g).to(DT[dt]) for _ in range(2))
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    y, z = ref.normed(x, w, 1e-6, r)
+    xd, rd = x.to(dev), r.to(dev)
+    codes, scales = kernels.rms_norm_fp8(xd, w.to(dev), residual=rd, out=xd)
+    torch.cuda.synchronize()
+    assert torch.equal(rd.cpu(), z)
+    assert ((xd.cpu().double() - y).abs() <= y.abs() * (ref.HALF[x.dtype] + ref.NORM_REL) + ref.TINY[x.dtype]).all()
+    ref.check_codes(codes.cpu(), scales.cpu(), y)
