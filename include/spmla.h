@@ -461,7 +461,7 @@ int spmla_topk_overlap(const int* sets, long long s_l, long long s_r, int L, int
  * y over s before s's own rounding; the last group of a row may be shorter. x, residual, residual_out, out [T][D] rows of
  * dtype 0 fp32, 1 fp16, 2 bf16 (row strides in elements; out may be x); weight [D] of the same type, or fp32 with
  * weight_f32; codes [T][D] bytes, scales [T][ceil(D / 128)]. D <= 65536, T <= 2^23 (here and in the four calls below).
- * No counterpart in the reference's tree: vLLM's fused norms run in its place there. */
+ * No counterpart in the reference's tree: the serving engine's own layers run in its place. */
 int spmla_rms_norm(const void* x, long long x_st, const void* residual, long long r_st, void* residual_out,
                    long long ro_st, const void* weight, int weight_f32, float eps, int T, int D, int dtype, void* out,
                    long long o_st, unsigned char* codes, long long c_st, float* scales, long long s_st, int ue8m0,
@@ -478,7 +478,7 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
  * [ceil(N / 128)][ceil(K / 128)] fp32 (the checkpoint's weight_scale_inv), out [T][N] dtype 1 fp16 or 2 bf16. K % 16 == 0,
  * N <= 2^23.
  * The 128 products of a block are added by the matrix core (1.4e-5 of the sum's size on normally distributed codes), the
- * blocks in fp32. No counterpart in the reference's tree: vLLM's block-FP8 linear layers run in its place there. */
+ * blocks in fp32. No counterpart in the reference's tree: the serving engine's own layers run in its place. */
 int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long long as_st, const void* w,
                      long long w_st, const float* w_scales, long long ws_st, int T, int N, int K, int dtype, void* out,
                      long long o_st, void* stream);
@@ -487,8 +487,8 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
  * (pairs (start + 2i, start + 2i + 1) with interleaved, else (start + i, start + n + i)): (a, b) -> factor * (a cos -
  * b sin, b cos + a sin), inverse: by the negative angle. The other columns are copied (out == x: left). Angles in 64
  * bits: positions (int64, or int32 with pos32) up to 2^31 keep theirs to 2^-22. freqs [n] float64 on the device. dtype as
- * spmla_rms_norm. out is x itself (same strides) or does not overlap it. No counterpart in the reference's tree (vLLM's
- * rotary embedding). */
+ * spmla_rms_norm. out is x itself (same strides) or does not overlap it. No counterpart in the reference's tree (the
+ * serving engine's own layer). */
 int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positions, int pos32, const double* freqs,
                int T, int H, int W, int start, int n, int interleaved, float factor, int inverse, int dtype, void* out,
                long long o_st, long long o_sh, void* stream);
