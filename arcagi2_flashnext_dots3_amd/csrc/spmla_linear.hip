@@ -256,8 +256,8 @@ static int ring_go(const LinearParams& p, hipStream_t s) {
   if (int rc = lds.ensure((const void*)ring_kernel<DT, BM, BN, WM, WN, ST>, C::LDS)) return rc;
   const int TN = (p.N + BN - 1) / BN;
   const long long n = (long long)TN * ((p.T + BM - 1) / BM);
-  hipLaunchKernelGGL((ring_kernel<DT, BM, BN, WM, WN, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(512), C::LDS, s, p, TN);
-  return (int)hipGetLastError();
+  static Launcher start;
+  return start((const void*)ring_kernel<DT, BM, BN, WM, WN, ST>, dim3((unsigned)((n + 7) / 8 * 8)), 512, C::LDS, s, p, TN);
 }
 
 // ---- few tokens: the weights stream past 16 MT tokens --------------------------------------------------------------
@@ -379,9 +379,8 @@ static int stream_go(const LinearParams& p, hipStream_t s) {
   if (int rc = lds.ensure((const void*)stream_kernel<DT, NT, MT, NW, ST>, C::LDS)) return rc;
   const int TM = (p.T + 16 * MT - 1) / (16 * MT);
   const long long n = (long long)TM * ((p.N + 16 * NT - 1) / (16 * NT));
-  hipLaunchKernelGGL((stream_kernel<DT, NT, MT, NW, ST>), dim3((unsigned)((n + 7) / 8 * 8)), dim3(64 * NW), C::LDS, s, p,
-                     TM);
-  return (int)hipGetLastError();
+  static Launcher start;
+  return start((const void*)stream_kernel<DT, NT, MT, NW, ST>, dim3((unsigned)((n + 7) / 8 * 8)), 64 * NW, C::LDS, s, p, TM);
 }
 
 
@@ -700,8 +699,8 @@ static int big_go(const LinearParams& p, hipStream_t s) {
   const int TN = (p.N + 255) / 256;
   long long n = ((long long)TN * ((p.T + 255) / 256) + 7) / 8 * 8;
   if (p.K % 128 == 0 && p.K > 128 && n > 256) n = 256;                 // several tiles a workgroup, one workgroup a unit
-  hipLaunchKernelGGL((big_kernel<DT>), dim3((unsigned)n), dim3(512), Big::LDS, s, p, TN);
-  return (int)hipGetLastError();
+  static Launcher start;
+  return start((const void*)big_kernel<DT>, dim3((unsigned)n), 512, Big::LDS, s, p, TN);
 }
 
 // the rule's kernels in its order (rules::LINEAR)

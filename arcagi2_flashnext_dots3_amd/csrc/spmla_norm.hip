@@ -153,54 +153,47 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
 }
 
 template <int DT, bool NORM, int NT, int CH, int ROW>
-static void launch(NormParams p, hipStream_t s) {
+static int launch(NormParams p, hipStream_t s) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
   p.nt = NORM && RPB == 1 ? (p.D + 512 * CH - 1) / (512 * CH) * 64 : NT;   // no wave without a value
   const unsigned gy = NORM ? 1u : (unsigned)((p.D + NT * 8 - 1) / (NT * 8));
-  hipLaunchKernelGGL((norm_kernel<DT, NORM, NT, CH, ROW>), dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
-                     dim3((unsigned)(p.nt * RPB)), 0, s, p);
+  static Launcher start;
+  return start((const void*)norm_kernel<DT, NORM, NT, CH, ROW>, dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
+               p.nt * RPB, 0, s, p);
 }
 
 constexpr int MAX_D = 65536;
 
 template <int DT, int ROW>
-static void norm_go(const NormParams& p, hipStream_t s) {
+static int norm_go(const NormParams& p, hipStream_t s) {
   // as few threads and chunks as hold the row: idle ones cost as much as busy ones (8192 x 576 64 x 1 to 256 x 1: 13.7 to
   // 21.5 us). Of equal ones many threads for few rows (4096 values, 1 row: 512 x 1 3.6, 256 x 2 4.6; 7168: 1024 x 1 4.6, 512 x
   // 2 5.1), fewer that each have more on their way for many (8192 rows: 45 / 42, 104 / 88).
   if constexpr (ROW == TINY) {
-    launch<DT, true, 64, 1, ROW>(p, s);
-    return;
+    return launch<DT, true, 64, 1, ROW>(p, s);
   } else {
-  if (p.D <= 512) launch<DT, true, 64, 1, ROW>(p, s);
-  else if (p.D <= 1024) launch<DT, true, 128, 1, ROW>(p, s);
-  else if (p.D <= 2048) launch<DT, true, 256, 1, ROW>(p, s);
-  else if (p.D <= 4096 && p.T <= 4096) launch<DT, true, 512, 1, ROW>(p, s);
-  else if (p.D <= 4096) launch<DT, true, 256, 2, ROW>(p, s);
-  else if (p.D <= 8192 && p.T <= 1024) launch<DT, true, 1024, 1, ROW>(p, s);
-  else if (p.D <= 8192) launch<DT, true, 512, 2, ROW>(p, s);
-  else if (p.D <= 16384) launch<DT, true, 1024, 2, ROW>(p, s);
-  else launch<DT, true, 1024, 8, ROW>(p, s);
+    if (p.D <= 512) return launch<DT, true, 64, 1, ROW>(p, s);
+    if (p.D <= 1024) return launch<DT, true, 128, 1, ROW>(p, s);
+    if (p.D <= 2048) return launch<DT, true, 256, 1, ROW>(p, s);
+    if (p.D <= 4096 && p.T <= 4096) return launch<DT, true, 512, 1, ROW>(p, s);
+    if (p.D <= 4096) return launch<DT, true, 256, 2, ROW>(p, s);
+    if (p.D <= 8192 && p.T <= 1024) return launch<DT, true, 1024, 1, ROW>(p, s);
+    if (p.D <= 8192) return launch<DT, true, 512, 2, ROW>(p, s);
+    if (p.D <= 16384) return launch<DT, true, 1024, 2, ROW>(p, s);
+    return launch<DT, true, 1024, 8, ROW>(p, s);
   }
 }
 
 static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
   auto by_type = [&](auto tag) {
     constexpr int R = decltype(tag)::value;
-    if (norm) {
-      if (dtype == DT_F32) norm_go<DT_F32, R>(p, s);
-      else if (dtype == DT_F16) norm_go<DT_F16, R>(p, s);
-      else norm_go<DT_BF16, R>(p, s);
-    } else {
-      if (dtype == DT_F32) launch<DT_F32, false, 256, 1, R>(p, s);
-      else if (dtype == DT_F16) launch<DT_F16, false, 256, 1, R>(p, s);
-      else launch<DT_BF16, false, 256, 1, R>(p, s);
-    }
+    if (norm) return dtype == DT_F32 ? norm_go<DT_F32, R>(p, s) : dtype == DT_F16 ? norm_go<DT_F16, R>(p, s) : norm_go<DT_BF16, R>(p, s);
+    return dtype == DT_F32 ? launch<DT_F32, false, 256, 1, R>(p, s) : dtype == DT_F16 ? launch<DT_F16, false, 256, 1, R>(p, s)
+                                                                                       : launch<DT_BF16, false, 256, 1, R>(p, s);
   };
-  if (p.D % 8 == 0) by_type(std::integral_constant<int, WHOLE>{});
-  else if (p.D > 8) by_type(std::integral_constant<int, ENDS>{});
-  else by_type(std::integral_constant<int, TINY>{});
-  return (int)hipGetLastError();
+    if (p.D % 8 == 0) return by_type(std::integral_constant<int, WHOLE>{});
+    if (p.D > 8) return by_type(std::integral_constant<int, ENDS>{});
+    return by_type(std::integral_constant<int, TINY>{});
 }
 
 }  // namespace nrm

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeParams p) {
 }
 
 template <int DT, int V, bool INTER>
-static void launch(RopeParams& p, hipStream_t s) {
+static int launch(RopeParams& p, hipStream_t s) {
   constexpr int NP = V == 1 ? 1 : INTER ? 4 : 8;
   const int NU = p.n / NP + (p.inplace ? 0 : (p.W - 2 * p.n) / V);
   p.us = NU < 256 ? NU : 256;
@@ -119,18 +119,14 @@ static void launch(RopeParams& p, hipStream_t s) {
   // small batches: a token's heads over several workgroups until each compute unit has a few
   const long long most = (p.H + p.hp - 1) / p.hp, want = (1024 + gx - 1) / gx;
   const unsigned gy = (unsigned)(want < most ? want : most);
-  hipLaunchKernelGGL((rope_kernel<DT, V, INTER>), dim3((unsigned)gx, gy), dim3(256), 0, s, p);
+  static Launcher start;
+  return start((const void*)rope_kernel<DT, V, INTER>, dim3((unsigned)gx, gy), 256, 0, s, p);
 }
 
 template <int DT>
-static void go(RopeParams& p, bool vec, bool inter, hipStream_t s) {
-  if (vec) {
-    if (inter) launch<DT, 8, true>(p, s);
-    else launch<DT, 8, false>(p, s);
-  } else {
-    if (inter) launch<DT, 1, true>(p, s);
-    else launch<DT, 1, false>(p, s);
-  }
+static int go(RopeParams& p, bool vec, bool inter, hipStream_t s) {
+  if (vec) return inter ? launch<DT, 8, true>(p, s) : launch<DT, 8, false>(p, s);
+  return inter ? launch<DT, 1, true>(p, s) : launch<DT, 1, false>(p, s);
 }
 
 // ---- a token's cache row ------------------------------------------------------------------------------------
@@ -255,10 +251,9 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
                      factor, inverse ? -1.0f : 1.0f, 0, 0, 0};
   const bool vec = (W & 7) == 0 && (start & 7) == 0 && (n & (interleaved ? 3 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DT_F32) rope::go<DT_F32>(p, vec, interleaved != 0, s);
-  else if (dtype == DT_F16) rope::go<DT_F16>(p, vec, interleaved != 0, s);
-  else rope::go<DT_BF16>(p, vec, interleaved != 0, s);
-  return (int)hipGetLastError();
+  if (dtype == DT_F32) return rope::go<DT_F32>(p, vec, interleaved != 0, s);
+  if (dtype == DT_F16) return rope::go<DT_F16>(p, vec, interleaved != 0, s);
+  return rope::go<DT_BF16>(p, vec, interleaved != 0, s);
 }
 
 int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int weight_f32, float eps,
@@ -278,11 +273,9 @@ int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int 
   rope::LatentParams p{(const uint16_t*)kv, kv_st, weight, weight_f32, eps, positions, pos32, freqs, factor, slots, n,
                        (uint8_t*)cache, R, block_size, log2_or(block_size), block_stride, fmt,
                        fmt != 0 ? 1.0f / kv_scale : 1.0f};
-  if (interleaved)
-    hipLaunchKernelGGL((rope::latent_write_kernel<true>), dim3((n - 1) / 4 + 1), dim3(256), 0, (hipStream_t)stream, p);
-  else
-    hipLaunchKernelGGL((rope::latent_write_kernel<false>), dim3((n - 1) / 4 + 1), dim3(256), 0, (hipStream_t)stream, p);
-  return (int)hipGetLastError();
+  static Launcher start[2];
+  const void* kernel = interleaved ? (const void*)rope::latent_write_kernel<true> : (const void*)rope::latent_write_kernel<false>;
+  return start[interleaved != 0](kernel, dim3((n - 1) / 4 + 1), 256, 0, (hipStream_t)stream, p);
 }
 
 }  // extern "C"
