@@ -9,11 +9,12 @@
 // (4.5e-5 with 1 of 64 values 50 times the others), a hundredth of the 16-bit output's rounding; fp32 outputs are not
 // offered. Blocks are summed in fp32.
 //
-// Operands reach LDS by direct copies, 128-byte rows with their 16-byte chunks permuted by (row / 2) % 8. A lane reads
-// chunks g and g + 4 of its row (g = l / 16): the 16 lanes that LDS serves at once (0-3, 12-15, 20-23, 24-27 and so on)
-// then fall on distinct banks, 256 bytes a clock (with chunks 2 g and 2 g + 1 two of them meet in every bank: 128). Which
-// 32 values of k a lane holds does not matter, since both operands hold the same ones. In the last block of a k that is no multiple of 128 the chunks
-// behind k are read from the row's last chunk and the weights' are overwritten with zeros in LDS.
+// Operands reach LDS by direct copies, 128-byte rows with their 16-byte chunks permuted by (row / 2) % 8 (the outputs of the
+// tile kernels, whose lanes take other rows, by what is the same number for the lane). A lane reads chunks g and g + 4 of its
+// row (g = l / 16): the 16 lanes that LDS serves at once (0-3, 12-15, 20-23, 24-27 and so on) then fall on distinct banks, 256
+// bytes a clock (with chunks 2 g and 2 g + 1 two of them meet in every bank: 128). Which 32 values of k a lane holds does not
+// matter, since both operands hold the same ones. In the last block of a k that is no multiple of 128 the chunks behind k are
+// read from the row's last chunk and the weights' are replaced by zeros.
 #include "spmla_quant.h"
 #include "spmla_rules.h"
 

@@ -187,7 +187,8 @@ static int norm_go(const NormParams& p, hipStream_t s) {
 static int go(const NormParams& p, bool norm, int dtype, hipStream_t s) {
   auto by_type = [&](auto tag) {
     constexpr int R = decltype(tag)::value;
-    if (norm) return dtype == DT_F32 ? norm_go<DT_F32, R>(p, s) : dtype == DT_F16 ? norm_go<DT_F16, R>(p, s) : norm_go<DT_BF16, R>(p, s);
+    if (norm) return dtype == DT_F32 ? norm_go<DT_F32, R>(p, s) : dtype == DT_F16 ? norm_go<DT_F16, R>(p, s)
+                                                                                  : norm_go<DT_BF16, R>(p, s);
     return dtype == DT_F32 ? launch<DT_F32, false, 256, 1, R>(p, s) : dtype == DT_F16 ? launch<DT_F16, false, 256, 1, R>(p, s)
                                                                                        : launch<DT_BF16, false, 256, 1, R>(p, s);
   };
