@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeParams p) {
   }
 }
 
+constexpr int MAX_HEAD = 1 << 30;   // heads of a token, columns of a head: the strides of the loops stay inside 32 bits
+
 template <int DT, int V, bool INTER>
 static int launch(RopeParams& p, hipStream_t s) {
   constexpr int NP = V == 1 ? 1 : INTER ? 4 : 8;
@@ -238,7 +240,7 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
                long long o_st, long long o_sh, void* stream) {
   if (T < 0 || H < 0 || W < 0 || n < 0 || start < 0 || n > W / 2 || start > W - 2 * n || dtype < 0 || dtype > 2)
     return SPMLA_EARG;
-  if (T > MAX_TOKENS) return SPMLA_ELIMIT;
+  if (T > MAX_TOKENS || H > rope::MAX_HEAD || W > rope::MAX_HEAD) return SPMLA_ELIMIT;
   const bool inplace = out == x;
   if (inplace && (x_st != o_st || x_sh != o_sh)) return SPMLA_EARG;
   if (T == 0 || H == 0 || W == 0 || (inplace && n == 0)) return SPMLA_OK;

@@ -487,8 +487,8 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
  * (pairs (start + 2i, start + 2i + 1) with interleaved, else (start + i, start + n + i)): (a, b) -> factor * (a cos -
  * b sin, b cos + a sin), inverse: by the negative angle. The other columns are copied (out == x: left). Angles in 64
  * bits: positions (int64, or int32 with pos32) up to 2^31 keep theirs to 2^-22. freqs [n] float64 on the device. dtype as
- * spmla_rms_norm. out is x itself (same strides) or does not overlap it. No counterpart in the reference's tree (the
- * serving engine's own layer). */
+ * spmla_rms_norm. out is x itself (same strides) or does not overlap it. H, W <= 2^30. No counterpart in the
+ * reference's tree (the serving engine's own layer). */
 int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positions, int pos32, const double* freqs,
                int T, int H, int W, int start, int n, int interleaved, float factor, int inverse, int dtype, void* out,
                long long o_st, long long o_sh, void* stream);

@@ -1,0 +1,14 @@
+"""Sizes at which the norm, projection and rotary calls would leave their index arithmetic or their grids, on the CPU: refused
+before a launch."""
+import pytest
+
+from arcagi2_flashnext_dots3_amd import _lib
+
+ELIMIT = -5
+
+
+@pytest.mark.parametrize("H,W,n,out", [((1 << 30) + 1, 2, 1, 256), ((1 << 31) - 1, 2, 1, 256), (1, (1 << 31) - 1, 1, 512),
+                                       (1, (1 << 30) + 1, 0, 512)])
+def test_rope_of_more_heads_or_columns_than_the_loops_count(H, W, n, out):
+    """A loop's variable passes the size by up to its stride: beyond 2^31 it would wrap to a negative index."""
+    assert _lib.status("spmla_rope", 256, H * W, W, 256, 0, 256, 1, H, W, 0, n, 1, 1.0, 0, 2, out, H * W, W, None) == ELIMIT
