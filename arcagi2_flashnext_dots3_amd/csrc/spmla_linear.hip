@@ -725,6 +725,8 @@ static int linear_go(const LinearParams& p, hipStream_t s) {
 
 using namespace spmla;
 
+constexpr int MAX_K = 1 << 22;         // and rows' strides in bytes: blocks are counted and places inside a tile formed in 32 bits
+
 extern "C" {
 
 int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long long as_st, const void* w,
@@ -732,6 +734,7 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
                      long long o_st, void* stream) {
   if (T < 0 || N < 0 || K <= 0 || (K & 15) || (dtype != DT_F16 && dtype != DT_BF16)) return SPMLA_EARG;
   if (T == 0 || N == 0) return SPMLA_OK;
+  if (K > MAX_K) return SPMLA_ELIMIT;
   if (!a || !a_scales || !w || !w_scales || !out) return SPMLA_EARG;
   const int kb = (K + 127) / 128;
   if ((T > 1 && (a_st < K || as_st < kb || o_st < N)) || (N > 1 && w_st < K) || (N > 128 && ws_st < kb)) return SPMLA_EARG;
@@ -739,7 +742,7 @@ int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long 
       ((uintptr_t)w_scales & 3) || ((uintptr_t)out & 1))
     return SPMLA_EALIGN;
   if (T > MAX_TOKENS || N > MAX_TOKENS) return SPMLA_ELIMIT;
-  if (a_st > (1 << 22) || w_st > (1 << 22) || as_st > (1 << 20)) return SPMLA_ELIMIT;   // 32-bit offsets inside a tile
+  if (a_st > MAX_K || w_st > MAX_K || as_st > (1 << 20)) return SPMLA_ELIMIT;
   lin::LinearParams p{(const uint8_t*)a, a_st, a_scales, as_st, (const uint8_t*)w, w_st, w_scales, ws_st, out, o_st,
                       T, N, K, ((uintptr_t)out & 7) == 0 && (o_st & 3) == 0, ((uintptr_t)out & 63) == 0 && (o_st & 31) == 0};
   if (dtype == DT_F16) return lin::linear_go<DT_F16>(p, (hipStream_t)stream);

@@ -476,7 +476,7 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
  * out[t][n] = sum_b a_scales[t][b] * w_scales[n / 128][b] * sum_{k in block b} a[t][k] * w[n][k], blocks of 128 k.
  * a [T][K], w [N][K] e4m3 codes (row strides a multiple of 16 bytes, at most 2^22), a_scales [T][ceil(K / 128)], w_scales
  * [ceil(N / 128)][ceil(K / 128)] fp32 (the checkpoint's weight_scale_inv), out [T][N] dtype 1 fp16 or 2 bf16. K % 16 == 0,
- * N <= 2^23.
+ * K <= 2^22, N <= 2^23.
  * The 128 products of a block are added by the matrix core (1.4e-5 of the sum's size on normally distributed codes), the
  * blocks in fp32. No counterpart in the reference's tree: the serving engine's own layers run in its place. */
 int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long long as_st, const void* w,

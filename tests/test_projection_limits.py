@@ -12,3 +12,9 @@ ELIMIT = -5
 def test_rope_of_more_heads_or_columns_than_the_loops_count(H, W, n, out):
     """A loop's variable passes the size by up to its stride: beyond 2^31 it would wrap to a negative index."""
     assert _lib.status("spmla_rope", 256, H * W, W, 256, 0, 256, 1, H, W, 0, n, 1, 1.0, 0, 2, out, H * W, W, None) == ELIMIT
+
+
+@pytest.mark.parametrize("K", [(1 << 22) + 16, (1 << 31) - 16])
+def test_linear_of_more_k_than_its_blocks_count(K):
+    """One token and one output whose rows' strides say nothing of k: k + 127 passed 2^31."""
+    assert _lib.status("spmla_linear_fp8", 256, 16, 256, 1, 256, 16, 256, 1, 1, 1, K, 2, 256, 1, None) == ELIMIT
