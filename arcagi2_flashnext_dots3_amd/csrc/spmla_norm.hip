@@ -156,10 +156,11 @@ template <int DT, bool NORM, int NT, int CH, int ROW>
 static int launch(NormParams p, hipStream_t s) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
   p.nt = NORM && RPB == 1 ? (p.D + 512 * CH - 1) / (512 * CH) * 64 : NT;   // no wave without a value
+  const long long groups = ((long long)p.T + RPB - 1) / RPB;
+  if (groups * (p.nt * RPB) >= 1ll << 32) return SPMLA_ELIMIT;             // wide rows take up to 1024 threads each
   const unsigned gy = NORM ? 1u : (unsigned)((p.D + NT * 8 - 1) / (NT * 8));
   static Launcher start;
-  return start((const void*)norm_kernel<DT, NORM, NT, CH, ROW>, dim3((unsigned)(((long long)p.T + RPB - 1) / RPB), gy),
-               p.nt * RPB, 0, s, p);
+  return start((const void*)norm_kernel<DT, NORM, NT, CH, ROW>, dim3((unsigned)groups, gy), p.nt * RPB, 0, s, p);
 }
 
 constexpr int MAX_D = 65536;

@@ -460,7 +460,8 @@ int spmla_topk_overlap(const int* sets, long long s_l, long long s_r, int L, int
  * of y with one fp32 scale per 128 values, s = max(amax / 448, 1e-12) (ue8m0: rounded up to a power of two), the code of
  * y over s before s's own rounding; the last group of a row may be shorter. x, residual, residual_out, out [T][D] rows of
  * dtype 0 fp32, 1 fp16, 2 bf16 (row strides in elements; out may be x); weight [D] of the same type, or fp32 with
- * weight_f32; codes [T][D] bytes, scales [T][ceil(D / 128)]. D <= 65536, T <= 2^23 (here and in the four calls below).
+ * weight_f32; codes [T][D] bytes, scales [T][ceil(D / 128)]. D <= 65536, T <= 2^23 (here and in the four calls
+ * below; rows of this call beyond 7168 values: T < 2^22).
  * No counterpart in the reference's tree: the serving engine's own layers run in its place. */
 int spmla_rms_norm(const void* x, long long x_st, const void* residual, long long r_st, void* residual_out,
                    long long ro_st, const void* weight, int weight_f32, float eps, int T, int D, int dtype, void* out,

@@ -18,3 +18,13 @@ def test_rope_of_more_heads_or_columns_than_the_loops_count(H, W, n, out):
 def test_linear_of_more_k_than_its_blocks_count(K):
     """One token and one output whose rows' strides say nothing of k: k + 127 passed 2^31."""
     assert _lib.status("spmla_linear_fp8", 256, 16, 256, 1, 256, 16, 256, 1, 1, 1, K, 2, 256, 1, None) == ELIMIT
+
+
+@pytest.mark.parametrize("T,D", [(1 << 23, 8192), (1 << 22, 16384), (1 << 22, 15361), (1 << 22, 65536), (1 << 23, 32769)])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_norm_of_more_threads_than_a_grid_takes(T, D, dtype):
+    """Wide rows take 512 or 1024 threads each: 2^32 in all."""
+    for odd in (0, 1):
+        d = D - odd if D != 15361 and D != 32769 else D + odd
+        assert _lib.status("spmla_rms_norm", 256, d, None, 0, None, 0, None, 0, 1e-6, T, d, dtype, 256, d, None, 0, None, 0, 0,
+                           None) == ELIMIT
