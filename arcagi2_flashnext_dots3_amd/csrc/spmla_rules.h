@@ -73,7 +73,8 @@ inline int linear_kernel(int T, int N, int K) {
   for (int i = 0; i < (int)(sizeof(LINEAR) / sizeof(LINEAR[0])); ++i) {
     const LinearKernel& k = LINEAR[i];
     const long long wgs = (long long)((T - 1) / k.bm + 1) * ((N - 1) / k.bn + 1);
-    if (wgs >= 1 << 23) continue;                      // a grid of 2^32 threads or more is not launched
+    if ((wgs + 7) / 8 * 8 >= 1 << 23) continue;        // a grid (whole eights of up to 512 threads) of 2^32 threads or more is
+                                                       // not launched
     const double r = (double)((wgs + 255) / 256), w = wgs / 256.0;
     const double t = k.c[0] + k.c[1] * r + k.c[2] * r * kb + k.c[3] * w * kb + k.c[4] * w;
     if (best < 0 || t < least) { best = i; least = t; }

@@ -3,6 +3,7 @@ before a launch."""
 import pytest
 
 from arcagi2_flashnext_dots3_amd import _lib
+from tests.test_linear_choice import choose  # noqa: F401 (a fixture)
 
 ELIMIT = -5
 
@@ -28,3 +29,11 @@ def test_norm_of_more_threads_than_a_grid_takes(T, D, dtype):
         d = D - odd if D != 15361 and D != 32769 else D + odd
         assert _lib.status("spmla_rms_norm", 256, d, None, 0, None, 0, None, 0, 1e-6, T, d, dtype, 256, d, None, 0, None, 0, 0,
                            None) == ELIMIT
+
+
+def test_projection_of_more_threads_than_a_grid_takes(choose):  # noqa: F811
+    """24892 x 337 tiles of 256 x 256 lie below 2^23, but a grid has whole eights of workgroups: 2^23, of 512 threads."""
+    assert choose(24892 * 256, 337 * 256, 16) == -1
+    assert choose(24892 * 256, 336 * 256, 16) >= 0
+    assert _lib.status("spmla_linear_fp8", 256, 16, 256, 1, 256, 16, 256, 1, 24892 * 256, 337 * 256, 16, 2, 256, 337 * 256,
+                       None) == ELIMIT
