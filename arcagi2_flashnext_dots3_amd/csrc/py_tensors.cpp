@@ -85,13 +85,13 @@ std::string shown(const at::Tensor& t) {
 }
 void* address(const at::Tensor* t) { return t ? const_cast<void*>(t->const_data_ptr()) : nullptr; }
 
-// row stride of t [T, D] with contiguous rows; written: rows that do not overlap
+// row stride of t [T, D] with contiguous rows (a single row's is D, whatever its tensor says); written: rows that do not overlap
 int64_t rows(const at::Tensor& t, int64_t T, int64_t D, unsigned types, const char* what, bool written = false) {
   if (t.dim() != 2 || t.size(0) != T || t.size(1) != D || !(type_of(t) & types))
     refuse(std::string(what) + " expected, (" + std::to_string(T) + ", " + std::to_string(D) + "): got " + shown(t));
   if (D > 1 && t.stride(1) != 1) refuse(std::string(what) + ": contiguous rows");
   if (written && T > 1 && t.stride(0) < D) refuse(std::string(what) + ": rows that do not overlap");
-  return t.stride(0);
+  return T > 1 ? t.stride(0) : D;
 }
 void line(const at::Tensor& t, int64_t least, int64_t most, unsigned types, const char* what) {
   if (t.dim() != 1 || t.size(0) < least || t.size(0) > most || !(type_of(t) & types) || !t.is_contiguous())
@@ -246,7 +246,8 @@ long rope(PyObject* const* a) {
   if ((d != 2 && d != 3) || !(type & (F32 | F16 | BF16))) refuse("x [T, H, W] or [T, W] fp32 / fp16 / bf16: got " + shown(*x));
   if (out->sizes() != x->sizes() || type_of(*out) != type) refuse("out of x's shape and type: got " + shown(*out));
   const int64_t T = x->size(0), H = d == 3 ? x->size(1) : 1, W = x->size(d - 1);
-  const int64_t x_st = x->stride(0), o_st = out->stride(0), x_sh = d == 3 ? x->stride(1) : 0, o_sh = d == 3 ? out->stride(1) : 0;
+  auto stride = [](const at::Tensor& t, int64_t i) -> int64_t { return t.size(i) > 1 ? t.stride(i) : 0; };   // a single one's says nothing
+  const int64_t x_st = stride(*x, 0), o_st = stride(*out, 0), x_sh = d == 3 ? stride(*x, 1) : 0, o_sh = d == 3 ? stride(*out, 1) : 0;
   if (W > 1 && (x->stride(d - 1) != 1 || out->stride(d - 1) != 1)) refuse("contiguous head columns");
   line(*pos, T, ANY, I32 | I64, "positions [T] int32 / int64");
   line(*freqs, 0, ANY, F64, "freqs [pairs] float64");
@@ -287,7 +288,7 @@ long latent_write(PyObject* const* a) {
   if (cd == 3) {
     R = cache->size(0) * cache->size(1);
     bs = cache->size(1);
-    bstride = cache->stride(0);
+    bstride = cache->size(0) > 1 ? cache->stride(0) : bs * rowb;
     if (bs > 1 && cache->stride(1) != rowb) refuse("cache: rows inside a block must be contiguous");
   } else {
     R = cache->size(0);
@@ -300,7 +301,7 @@ long latent_write(PyObject* const* a) {
     if (t) same_gpu(*t, dev, "latent_write");
   const int ni = as_int(n, "n"), bsi = as_int(bs, "block_size"), wf = w && type_of(*w) == F32;
   return launch(dev, [&](void* s) {
-    return f_latent_write(address(kv), kv->stride(0), address(w), wf, (float)eps, address(pos), type_of(*pos) == I32,
+    return f_latent_write(address(kv), kv->size(0) > 1 ? kv->stride(0) : 576, address(w), wf, (float)eps, address(pos), type_of(*pos) == I32,
                           (const double*)address(freqs), inter, (float)factor, (const long long*)address(slots), ni, address(cache),
                           R, bsi, bstride, (int)fmt, (float)kv_scale, s);
   });
