@@ -154,6 +154,8 @@ def tensor_call(name, x, *args):
             import torch
             with torch.cuda.device(x.device):
                 rc = f(*args)
+        if rc in ERRORS:             # the entry point's own checks, also before a launch
+            raise ValueError(f"{name}: {ERRORS[rc]}")
         if rc:
             raise RuntimeError(f"spmla_{name} failed: {rc} ({ERRORS.get(rc, 'hip error')})")
 

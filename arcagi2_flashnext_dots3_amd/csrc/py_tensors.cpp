@@ -1,8 +1,8 @@
 // The norm, quantization, projection, rotary and latent-row calls on tensors: checks of shapes, types, strides and devices,
 // then the entry point (include/spmla.h) on the current stream. _tensors.load(path, raw_stream, get_device) opens the
-// library and returns {name: callable}; a callable raises ValueError for what the call does not take and returns the entry
-// point's value, or AWAY when the tensors are on another GPU than the current one. These calls are a few us on the GPU:
-// the same checks in Python took 4 us of 7, here 0.4.
+// library and returns {name: callable}; a callable raises ValueError for what the call does not take, before it launches
+// anything, and returns the entry point's value, or AWAY when the tensors are on another GPU than the current one. These
+// calls are a few us on the GPU: the same checks in Python took 4 us of 7, here 0.4.
 #include <ATen/ATen.h>
 #include <Python.h>
 #include <dlfcn.h>
@@ -12,6 +12,7 @@
 #include <string>
 
 #include "spmla.h"
+#include "spmla_rules.h"
 
 namespace {
 
@@ -98,6 +99,18 @@ void line(const at::Tensor& t, int64_t least, int64_t most, unsigned types, cons
     refuse(std::string(what) + " expected: got " + shown(t));
 }
 constexpr int64_t ANY = INT64_MAX;
+void on_bytes(const at::Tensor& t, int64_t stride_bytes, int bytes, const char* what) {   // address and rows
+  if (((uintptr_t)t.const_data_ptr() | (uint64_t)stride_bytes) & (bytes - 1))
+    refuse(std::string(what) + ": rows on " + std::to_string(bytes) + " bytes");
+}
+void at_most(int64_t v, int64_t most, const char* name) {
+  if (v > most) refuse(std::string(name) + " of " + std::to_string(v) + ": at most " + std::to_string(most));
+}
+constexpr int64_t MAX_TOKENS = 1 << 23;
+float epsilon(double eps) {
+  if (!((float)eps >= 0.f)) refuse("eps >= 0: got " + std::to_string(eps));
+  return (float)eps;
+}
 
 // the current stream of dev as an address, or AWAY's flag
 bool stream_of(int dev, void*& s) {
@@ -139,6 +152,7 @@ Norm norm_input(PyObject* o) {
   if (x->dim() != 2 || !(type & (F32 | F16 | BF16)) || x->size(1) == 0) refuse("x [T, D] fp32 / fp16 / bf16, D > 0: got " + shown(*x));
   Norm n{x, x->size(0), x->size(1), 0, type, gpu_of(*x)};
   n.st = rows(*x, n.T, n.D, type, "x [T, D]");
+  at_most(n.T, MAX_TOKENS, "T");
   return n;
 }
 constexpr const char* CODES = "codes [T, D] e4m3 / uint8";
@@ -149,8 +163,9 @@ long rms_norm(PyObject* const* a) {
   const Norm n = norm_input(a[0]);
   const at::Tensor *w = maybe(a[1], "weight"), *r = maybe(a[3], "residual"), *ro = maybe(a[4], "residual_out");
   const at::Tensor *out = maybe(a[5], "out"), *codes = maybe(a[6], "codes"), *scales = maybe(a[7], "scales");
-  const double eps = number(a[2]);
+  const float eps = epsilon(number(a[2]));
   const bool ue8m0 = truth(a[8]);
+  at_most(n.D, 65536, "D");
   int64_t rs = 0, ros = 0, os = 0, cs = 0, ss = 0;
   if (r) {
     rs = rows(*r, n.T, n.D, n.type, "residual [T, D] of x's type");
@@ -170,7 +185,7 @@ long rms_norm(PyObject* const* a) {
     if (t) same_gpu(*t, n.dev, "rms_norm");
   const int T = as_int(n.T, "T"), D = as_int(n.D, "D"), wf = w && type_of(*w) == F32;
   return launch(n.dev, [&](void* s) {
-    return f_rms_norm(address(n.x), n.st, address(r), rs, address(ro), ros, address(w), wf, (float)eps, T, D, dtype_code(n.type),
+    return f_rms_norm(address(n.x), n.st, address(r), rs, address(ro), ros, address(w), wf, eps, T, D, dtype_code(n.type),
                       address(out), os, (unsigned char*)address(codes), cs, (float*)address(scales), ss, ue8m0, s);
   });
 }
@@ -180,6 +195,7 @@ long quant_fp8(PyObject* const* a) {
   const Norm n = norm_input(a[0]);
   const at::Tensor *codes = tensor(a[1], "codes"), *scales = tensor(a[2], "scales");
   const bool ue8m0 = truth(a[3]);
+  at_most(n.D, 65535 * 2048, "D");
   const int64_t cs = rows(*codes, n.T, n.D, E4M3 | U8, CODES, true);
   const int64_t ss = rows(*scales, n.T, (n.D + 127) / 128, F32, SCALES, true);
   for (const at::Tensor* t : {n.x, codes, scales}) same_gpu(*t, n.dev, "quant_fp8");
@@ -192,23 +208,48 @@ long quant_fp8(PyObject* const* a) {
 
 constexpr const char *WEIGHT = "w [N, K] e4m3", *WEIGHT_SCALES = "w_scales [ceil(N / 128), ceil(K / 128)] fp32";
 constexpr const char* PRODUCT = "out [T, N] bf16 / fp16";
+constexpr int64_t MAX_K = 1 << 22;
+
+struct Weight {                                          // a projection's weight and scales, for T rows of K values
+  int64_t N, w_st, ws_st;
+};
+Weight weight(const at::Tensor& w, const at::Tensor& ws, int64_t T, int64_t K) {
+  const int64_t N = w.size(0), kb = (K + 127) / 128;
+  if (K == 0 || K % 16) refuse("K a positive multiple of 16: got " + std::to_string(K));
+  const Weight f{N, rows(w, N, K, E4M3 | U8, WEIGHT, true), rows(ws, (N + 127) / 128, kb, F32, WEIGHT_SCALES, true)};
+  if (T == 0 || N == 0) return f;
+  on_bytes(w, f.w_st, 16, WEIGHT);
+  at_most(T, MAX_TOKENS, "T");
+  at_most(N, MAX_TOKENS, "N");
+  at_most(K, MAX_K, "K");
+  at_most(f.w_st, MAX_K, "stride of w");
+  // tiles of 16 x 16 are the most workgroups: where these are many, the rule says
+  if ((T / 16 + 1) * (N / 16 + 1) >= 1 << 22 && spmla::rules::linear_kernel((int)T, (int)N, (int)K) < 0)
+    refuse("T, N of " + std::to_string(T) + ", " + std::to_string(N) + ": more tiles than one launch takes");
+  return f;
+}
 
 // linear_fp8(a, a_scales, w, w_scales, out)
 long linear_fp8(PyObject* const* v) {
   const at::Tensor *a = tensor(v[0], "a"), *as = tensor(v[1], "a_scales"), *w = tensor(v[2], "w");
   const at::Tensor *ws = tensor(v[3], "w_scales"), *out = tensor(v[4], "out");
   if (a->dim() != 2 || w->dim() != 2 || a->size(1) != w->size(1)) refuse("a [T, K], w [N, K]: got " + shown(*a) + ", " + shown(*w));
-  const int64_t T = a->size(0), K = a->size(1), N = w->size(0), kb = (K + 127) / 128;
-  if (K == 0 || K % 16) refuse("K a positive multiple of 16: got " + std::to_string(K));
-  const int64_t a_st = rows(*a, T, K, E4M3 | U8, "a [T, K] e4m3"), w_st = rows(*w, N, K, E4M3 | U8, WEIGHT);
-  const int64_t as_st = rows(*as, T, kb, F32, "a_scales [T, ceil(K / 128)] fp32");
-  const int64_t ws_st = rows(*ws, (N + 127) / 128, kb, F32, WEIGHT_SCALES);
+  const int64_t T = a->size(0), K = a->size(1), kb = (K + 127) / 128;
+  const Weight f = weight(*w, *ws, T, K);
+  const int64_t N = f.N;
+  const int64_t a_st = rows(*a, T, K, E4M3 | U8, "a [T, K] e4m3", true);
+  const int64_t as_st = rows(*as, T, kb, F32, "a_scales [T, ceil(K / 128)] fp32", true);
+  if (T > 0 && N > 0) {
+    on_bytes(*a, a_st, 16, "a [T, K] e4m3");
+    at_most(a_st, MAX_K, "stride of a");
+    at_most(as_st, 1 << 20, "stride of a_scales");
+  }
   const int64_t o_st = rows(*out, T, N, BF16 | F16, PRODUCT, true);
   const int dev = gpu_of(*a);
   for (const at::Tensor* t : {a, as, w, ws, out}) same_gpu(*t, dev, "linear_fp8");
   const int Ti = as_int(T, "T"), Ni = as_int(N, "N"), Ki = as_int(K, "K");
   return launch(dev, [&](void* s) {
-    return f_linear_fp8(address(a), a_st, (const float*)address(as), as_st, address(w), w_st, (const float*)address(ws), ws_st,
+    return f_linear_fp8(address(a), a_st, (const float*)address(as), as_st, address(w), f.w_st, (const float*)address(ws), f.ws_st,
                         Ti, Ni, Ki, dtype_code(type_of(*out)), address(out), o_st, s);
   });
 }
@@ -219,9 +260,8 @@ long linear_quant(PyObject* const* v) {
   const at::Tensor *w = tensor(v[1], "w"), *ws = tensor(v[2], "w_scales"), *out = tensor(v[3], "out"), *work = tensor(v[4], "work");
   const bool ue8m0 = truth(v[5]);
   if (w->dim() != 2 || n.D != w->size(1)) refuse("x [T, K], w [N, K]: got " + shown(*n.x) + ", " + shown(*w));
-  const int64_t N = w->size(0), kb = (n.D + 127) / 128;
-  if (n.D % 16) refuse("K a positive multiple of 16: got " + std::to_string(n.D));
-  const int64_t w_st = rows(*w, N, n.D, E4M3 | U8, WEIGHT), ws_st = rows(*ws, (N + 127) / 128, kb, F32, WEIGHT_SCALES);
+  const Weight f = weight(*w, *ws, n.T, n.D);
+  const int64_t N = f.N, kb = (n.D + 127) / 128;
   const int64_t o_st = rows(*out, n.T, N, BF16 | F16, PRODUCT, true);
   line(*work, n.T * (n.D + 4 * kb), ANY, U8, "work [T (K + 4 ceil(K / 128))] uint8");
   for (const at::Tensor* t : {n.x, w, ws, out, work}) same_gpu(*t, n.dev, "linear_fp8");
@@ -230,7 +270,7 @@ long linear_quant(PyObject* const* v) {
   float* scales = (float*)(codes + n.T * n.D);
   return launch(n.dev, [&](void* s) {
     const int rc = f_quant_fp8(address(n.x), n.st, T, K, dtype_code(n.type), codes, n.D, scales, kb, ue8m0, s);
-    return rc ? rc : f_linear_fp8(codes, n.D, scales, kb, address(w), w_st, (const float*)address(ws), ws_st, T, Ni, K,
+    return rc ? rc : f_linear_fp8(codes, n.D, scales, kb, address(w), f.w_st, (const float*)address(ws), f.ws_st, T, Ni, K,
                                   dtype_code(type_of(*out)), address(out), o_st, s);
   });
 }
@@ -257,6 +297,10 @@ long rope(PyObject* const* a) {
   if (T > 0 && H > 0 && ((T > 1 && o_st < W) || (H > 1 && o_sh < W) ||
                          (T > 1 && H > 1 && o_st < (H - 1) * o_sh + W && o_sh < (T - 1) * o_st + W)))
     refuse("out: heads that do not overlap");
+  if (T > 0 && H > 0 && W > 0 && address(out) == address(x) && (x_st != o_st || x_sh != o_sh)) refuse("out: x's strides where it is x itself");
+  at_most(T, MAX_TOKENS, "T");
+  at_most(H, 1 << 30, "H");
+  at_most(W, 1 << 30, "W");
   const int dev = gpu_of(*x);
   for (const at::Tensor* t : {x, pos, freqs, out}) same_gpu(*t, dev, "rope");
   const int Ti = as_int(T, "T"), Hi = as_int(H, "H"), Wi = as_int(W, "W");
@@ -270,7 +314,8 @@ long rope(PyObject* const* a) {
 long latent_write(PyObject* const* a) {
   const at::Tensor *kv = tensor(a[0], "kv"), *w = maybe(a[1], "weight"), *pos = tensor(a[3], "positions"), *freqs = tensor(a[4], "freqs");
   const at::Tensor *slots = tensor(a[5], "slots"), *cache = tensor(a[6], "cache");
-  const double eps = number(a[2]), kv_scale = number(a[8]), factor = number(a[10]);
+  const float eps = epsilon(number(a[2])), kv_scale = (float)number(a[8]);
+  const double factor = number(a[10]);
   const long long fmt = integer(a[7]);
   const bool inter = truth(a[9]);
   if (kv->dim() != 2 || kv->size(1) != 576 || type_of(*kv) != BF16 || kv->stride(1) != 1)
@@ -279,8 +324,12 @@ long latent_write(PyObject* const* a) {
   const int64_t rowb = fmt == 0 ? 656 : fmt == 1 ? 576 : 400, cd = cache->dim();
   if (cd < 2 || cd > 3 || type_of(*cache) != U8 || cache->size(cd - 1) != rowb || cache->stride(cd - 1) != 1)
     refuse("cache rows of uint8, " + std::to_string(rowb) + " bytes, [R, row] or [blocks, block_size, row]: got " + shown(*cache));
+  if (fmt != 0 && !(kv_scale > 0.f)) refuse("kv_scale > 0: got " + std::to_string(kv_scale));
   line(*slots, 0, ANY, I64, "slots [n] int64");
-  const int64_t n = std::min(kv->size(0), slots->size(0));
+  const int64_t n = std::min(kv->size(0), slots->size(0)), kv_st = kv->size(0) > 1 ? kv->stride(0) : 576;
+  at_most(n, MAX_TOKENS, "n");
+  if (n > 0) on_bytes(*kv, 2 * kv_st, 16, "kv [n, 576] bf16");
+  if (n > 0 && w) on_bytes(*w, 0, 16, "weight [512]");
   if (w) line(*w, 512, 512, BF16 | F32, "weight [512] bf16 / fp32");
   line(*pos, n, ANY, I32 | I64, "positions [T] int32 / int64");
   line(*freqs, 32, 32, F64, "freqs [32] float64");
@@ -296,14 +345,19 @@ long latent_write(PyObject* const* a) {
     bs = a[11] == Py_None ? std::max<int64_t>(1, R) : integer(a[11]);
     bstride = a[12] == Py_None ? bs * rowb : integer(a[12]);
   }
+  const int ni = as_int(n, "n"), bsi = as_int(bs, "block_size"), wf = w && type_of(*w) == F32;
+  if (n > 0 && R > 0) {
+    if (bs <= 0) refuse("block_size > 0: got " + std::to_string(bs));
+    on_bytes(*cache, bstride, 8, "cache");
+    if (bstride < bs * rowb) refuse("block_stride of " + std::to_string(bstride) + ": blocks of " + std::to_string(bs) + " rows overlap");
+  }
   const int dev = gpu_of(*kv);
   for (const at::Tensor* t : {kv, w, pos, freqs, slots, cache})
     if (t) same_gpu(*t, dev, "latent_write");
-  const int ni = as_int(n, "n"), bsi = as_int(bs, "block_size"), wf = w && type_of(*w) == F32;
   return launch(dev, [&](void* s) {
-    return f_latent_write(address(kv), kv->size(0) > 1 ? kv->stride(0) : 576, address(w), wf, (float)eps, address(pos), type_of(*pos) == I32,
-                          (const double*)address(freqs), inter, (float)factor, (const long long*)address(slots), ni, address(cache),
-                          R, bsi, bstride, (int)fmt, (float)kv_scale, s);
+    return f_latent_write(address(kv), kv_st, address(w), wf, eps, address(pos), type_of(*pos) == I32, (const double*)address(freqs), inter,
+                          (float)factor, (const long long*)address(slots), ni, address(cache),
+                          R, bsi, bstride, (int)fmt, kv_scale, s);
   });
 }
 
