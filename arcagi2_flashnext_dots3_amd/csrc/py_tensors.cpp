@@ -350,6 +350,10 @@ long latent_write(PyObject* const* a) {
     if (bs <= 0) refuse("block_size > 0: got " + std::to_string(bs));
     on_bytes(*cache, bstride, 8, "cache");
     if (bstride < bs * rowb) refuse("block_stride of " + std::to_string(bstride) + ": blocks of " + std::to_string(bs) + " rows overlap");
+    // a [R, row] tensor with strides of its own says where its first row lies, its memory where the last may end
+    const __int128 last = (__int128)((R - 1) / bs) * bstride + (R - 1) % bs * rowb + rowb;
+    if (cd == 2 && last > (int64_t)cache->storage().nbytes() - cache->storage_offset())
+      refuse("cache: " + std::to_string(R) + " rows in blocks of " + std::to_string(bs) + ", " + std::to_string(bstride) + " bytes apart, end behind its memory");
   }
   const int dev = gpu_of(*kv);
   for (const at::Tensor* t : {kv, w, pos, freqs, slots, cache})

@@ -110,3 +110,23 @@ def test_codes_of_the_library_are_value_errors(monkeypatch):
     monkeypatch.setattr(_lib, "_TENSOR_FN", {"rope": lambda *a: 100})
     with pytest.raises(RuntimeError, match="hip error"):
         _lib.tensor_call("rope", None)
+
+
+@pytest.mark.parametrize("fmt,rowb", [(0, 656), (1, 576), (2, 400)])
+def test_latents_into_blocks_behind_the_caches_memory(fmt, rowb):
+    """A [R, row] cache with a block_stride: the last block has to lie inside the memory that the tensor is part of."""
+    pos, f = torch.zeros(4, dtype=torch.int64), torch.ones(32, dtype=torch.float64)
+    pool = torch.zeros(3 * (4 * rowb + 64) + rowb, dtype=torch.uint8)
+    args = torch.zeros(4, 576, dtype=BF), None, 1e-6, pos, f, torch.arange(4)
+
+    def call(R, at=0, **kw):
+        kernels.latent_write(*args, pool[at:].as_strided((R, rowb), (rowb, 1)), fmt=fmt, **kw)
+    apart = dict(block_size=4, block_stride=4 * rowb + 64)
+    _refused("one GPU", call, 12, **apart)
+    _refused("one GPU", call, 13, **apart)                    # one row in the fourth block
+    _refused("behind its memory", call, 13, at=8, **apart)
+    _refused("behind its memory", call, 12, block_size=4, block_stride=6 * rowb)
+    for stride in (1 << 40, 1 << 62):
+        _refused("behind its memory", call, 8, block_size=1, block_stride=stride)
+    _refused("one GPU", call, 12, block_size=5)
+    _refused("one GPU", call, 12)
