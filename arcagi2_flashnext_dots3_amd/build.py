@@ -4,7 +4,7 @@ Every .hip file under csrc/ is compiled to an object (in parallel) and linked in
 this file; the Python loader (_lib.py) and the tests load that file. Objects go to _build/ (git-ignored).
 csrc/py_call.cpp becomes the extension module _native (the loader's callables; without Python's headers or a C++
 compiler it is left out and the loader calls through ctypes), csrc/py_tensors.cpp the extension module _tensors (the
-calls around the cache and the query on tensors, against torch's headers).
+calls around the cache and the query on tensors; without torch's headers it is left out too, and those calls raise).
 All HIP code is compiled with packed fp32 instructions disabled (-packed-fp32-ops), see the feature flag below.
 """
 import concurrent.futures
@@ -35,9 +35,10 @@ def _run(cmd):
     return err
 
 
-def _build_module(src, out, flags=(), libs=()):
+def _build_module(src, out, flags=(), libs=(), headers=()):
     inc = sysconfig.get_paths()["include"]
-    if not os.path.exists(os.path.join(inc, "Python.h")) or shutil.which(CXX.split()[0]) is None:
+    headers = [os.path.join(inc, "Python.h"), *headers]
+    if not all(os.path.exists(h) for h in headers) or shutil.which(CXX.split()[0]) is None:
         if os.path.exists(out):
             os.remove(out)
         return None
@@ -53,13 +54,16 @@ def build_native():
 
 
 def build_tensors():
-    import torch
-    root = os.path.dirname(torch.__file__)
+    try:
+        import torch
+        root, abi = os.path.dirname(torch.__file__), int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    except ImportError:
+        root, abi = "", 1
     inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
     return _build_module("py_tensors.cpp", TENSORS,
-                         [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", inc, "-I",
-                          os.path.join(inc, "torch", "csrc", "api", "include")],
-                         ["-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"])
+                         [f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include")],
+                         ["-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"],
+                         [os.path.join(inc, "ATen", "ATen.h"), os.path.join(inc, "torch", "csrc", "autograd", "python_variable.h")])
 
 
 def build(verbose=False):
@@ -75,11 +79,11 @@ def build(verbose=False):
             msg = f.result()
             if verbose and msg:
                 print(f"[build] {s}: {msg}", flush=True)
-        tensors.result()
     tmp = LIB + ".tmp"
     _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", tmp, *objs])
     os.replace(tmp, LIB)
     build_native()
+    tensors.result()          # the library needs nothing of it: whatever this raises, the library is there
     return LIB
 
 
