@@ -2,12 +2,13 @@
 //
 // Rotary: pairs (a, b) of columns start .. start + 2n of a head turn by the token's position times the pair's frequency:
 //   (a, b) -> factor (a cos - b sin, b cos + a sin); interleaved pairs are (2i, 2i + 1), else (i, i + n).
-// The angle is formed in 64 bits, in quarter turns: its distance from the nearest whole one is exact to 2^-53 of the
-// angle, so positions far beyond 2^24 keep their angles; cosine and sine come from their Taylor series on +-45 degrees
+// The angle is formed in quarter turns, from 2 / pi and products in twice 64 bits: its distance from the nearest whole one is
+// exact to 2^-54 up to positions of 2^31 (rounded products alone: to 2^-21 there), so that only its rounding to 32 bits counts;
+// cosine and sine come from their Taylor series on +-45 degrees
 // (remainders x^11 / 11! and x^12 / 12!, below 2^-28). No table of positions is read.
 // Bound by HBM for long chunks: a head is read and written once (8192 tokens x 64 heads x 128 bf16 53 us, 268 MB, 5.0 TB/s;
 // a device copy moves 5.1); 64 tokens x 128 heads 3.3 us. A thread keeps its columns and turns them for several heads of one
-// token, so that an angle (some 50 instructions, 10 of them in 64 bits) is formed once for them. Loads and stores are 16
+// token, so that an angle (some 50 instructions, 11 of them in 64 bits) is formed once for them. Loads and stores are 16
 // bytes of a lane at any alignment of the type.
 //
 // Latent row: RMS norm of the 512 latent values and rotary of the 64 rope values, both in fp32, then the row that
@@ -19,12 +20,12 @@ namespace spmla {
 namespace rope {
 
 __device__ inline void turn(double pos, double freq, float factor, float sign, float& c, float& s) {
-  const double q = pos * (freq * 0.63661977236758134308);          // 2 / pi: quarter turns
+  constexpr double C = 0.63661977236758134308, C_LO = -3.935735335036497e-17;   // 2 / pi: quarter turns
+  const double f = freq * C, f_lo = __builtin_fma(freq, C_LO, __builtin_fma(freq, C, -f));
+  const double q = pos * f, q_lo = __builtin_fma(pos, f_lo, __builtin_fma(pos, f, -q));
   const double k = rint(q);
-  const float x = (float)(q - k) * 1.57079632679489661923f, y = x * x;
-  double m = k * 0.25;
-  m -= floor(m);                                                   // which quarter: 0, 1/4, 1/2, 3/4
-  const int n = (int)(m * 4.0);
+  const float x = (float)((q - k) + q_lo) * 1.57079632679489661923f, y = x * x;
+  const int n = (int)__builtin_bit_cast(uint64_t, k + 0x1.8p52) & 3;   // which quarter: the sum's last bit is 1
   const float sn = x * (1.0f + y * (-1.0f / 6 + y * (1.0f / 120 + y * (-1.0f / 5040 + y * (1.0f / 362880)))));
   const float cs = 1.0f + y * (-0.5f + y * (1.0f / 24 + y * (-1.0f / 720 + y * (1.0f / 40320 + y * (-1.0f / 3628800)))));
   const float a = n & 1 ? sn : cs, b = n & 1 ? cs : sn;
