@@ -356,8 +356,10 @@ long latent_write(PyObject* const* a) {
       refuse("cache: " + std::to_string(R) + " rows in blocks of " + std::to_string(bs) + ", " + std::to_string(bstride) + " bytes apart, end behind its memory");
   }
   const int dev = gpu_of(*kv);
-  for (const at::Tensor* t : {kv, w, pos, freqs, slots, cache})
+  for (const at::Tensor* t : {kv, w, pos, freqs, slots})
     if (t) same_gpu(*t, dev, "latent_write");
+  if (cache->is_cuda()) same_gpu(*cache, dev, "latent_write");
+  else if (!cache->is_pinned()) refuse("cache: on the GPU or in pinned host memory");      // an offloaded layer's rows
   return launch(dev, [&](void* s) {
     return f_latent_write(address(kv), kv_st, address(w), wf, eps, address(pos), type_of(*pos) == I32, (const double*)address(freqs), inter,
                           (float)factor, (const long long*)address(slots), ni, address(cache),

@@ -1087,8 +1087,9 @@ def rope(x, positions, freqs, out=None, start=0, interleaved=True, factor=1.0, i
 def latent_write(kv, weight, eps, positions, freqs, slots, cache, fmt=0, kv_scale=1.0, interleaved=True, factor=1.0,
                  block_size=None, block_stride=None):
     """Cache rows from the down projection's latents in one launch: kv [n, 576] bf16 (rows 16-byte aligned) -> RMS norm of
-    columns 0 .. 511 (weight [512] bf16 / fp32 or None), rotary of columns 512 .. 575 (freqs [32] float64, as rope), then the rows of
-    cache_write's formats (fmt, kv_scale, cache, block_size, block_stride as there) at slots [n] int64; a slot < 0 or
-    beyond the cache is skipped. Both stay in fp32 until they are encoded."""
+    columns 0 .. 511 (weight [512] bf16 / fp32 or None), rotary of columns 512 .. 575 (freqs [32] float64, as rope), then the
+    rows of cache_write's formats (fmt, kv_scale, cache, block_size, block_stride as there) at slots [n] int64; a slot < 0
+    or beyond the cache is skipped. Both stay in fp32 until they are encoded. cache: on the GPU, or in pinned host memory
+    (LayerOffload.store_latent keeps a layer's cached copies too)."""
     _lib.tensor_call("latent_write", kv, kv, weight, eps, positions, freqs, slots, cache, fmt, kv_scale, interleaved,
                      factor, block_size, block_stride)

@@ -164,15 +164,28 @@ class LayerOffload:
         n = min(kv_c_normed.shape[0], slots.shape[0])
         if n == 0:
             return
+        kv, kpe = kv_c_normed[:n], k_pe.reshape(k_pe.shape[0], -1)[:n]
+        self._store(n, slots, kv_scale, lambda at, rows, fmt: kernels.cache_write(kv, kpe, at, rows, fmt=fmt, kv_scale=kv_scale))
+
+    def store_latent(self, kv, weight, eps, rot, positions, slots, kv_scale=1.0):
+        """store() of the down projection's latents kv [n, 576] bf16: their norm (weight, eps), the rotation `rot` (a
+        rotary.Rotary) by positions [n] and the rows in one launch (Rotary.write_latent), for cached copies too."""
+        n = min(kv.shape[0], slots.shape[0])
+        kv, positions = kv[:n], positions[:n]
+        self._store(n, slots, kv_scale, lambda at, rows, fmt: rot.write_latent(kv, weight, eps, positions, at, rows, fmt=fmt,
+                                                                                kv_scale=kv_scale))
+
+    def _store(self, n, slots, kv_scale, write):
+        """write(slots, rows, fmt) puts the n tokens' rows at slots (none for -1) of rows: the host's, then the cached ones."""
+        if n == 0:
+            return
         compact = self.row_fmt == "e2m2"
         if not compact and float(kv_scale) != 1.0:
             raise ValueError("LayerOffload.store: Row656 rows carry their own scales; kv_scale must be 1")
-        kpe = k_pe.reshape(k_pe.shape[0], -1)
         slots = slots[:n].to(torch.int64)
         if self.trace is not None:
             self.trace.stored(slots)
-        fmt = 2 if compact else 0
-        kernels.cache_write(kv_c_normed[:n], kpe[:n], slots, self.host, fmt=fmt, kv_scale=kv_scale)
+        write(slots, self.host, 2 if compact else 0)
         if self.wc is not None:
             kernels.wcache_invalidate(self.wc, slots, self.R)      # rewritten rows: the next lookup misses
         elif self.C:
@@ -183,13 +196,13 @@ class LayerOffload:
                 # HBM scratch (the encoder is deterministic) and copy or decode them into their lines
                 tmp = self._buf("wt", (n, kernels.ROW400), torch.uint8)
                 ident = torch.arange(n, dtype=torch.int64, device=self.device)
-                kernels.cache_write(kv_c_normed[:n], kpe[:n], ident, tmp, fmt=2, kv_scale=kv_scale)
+                write(ident, tmp, 2)
                 if self.cache_fmt == "e2m2":
                     kernels.copy_rows(tmp, ident, self.cache[:self.C], lines)
                 else:
                     kernels.row400_copy(tmp, ident, self.cache[:self.C], lines)
             else:
-                kernels.cache_write(kv_c_normed[:n], kpe[:n], lines, self.cache[:self.C])
+                write(lines, self.cache[:self.C], 0)
 
     def gather(self, rows, out):
         """out[i] = host row rows[i] (int64; zero row when outside [0, R)); out [N, 656] uint8 in HBM

@@ -496,8 +496,8 @@ int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positi
 
 /* A token's cache row from its down-projected latent: kv [n][512 latent | 64 rope] bf16 (row stride kv_st) -> RMS norm of
  * the latent (weight [512] bf16 or fp32, null: 1), rotary of the rope values (freqs [32], as spmla_rope), then the row of
- * spmla_cache_write's formats 0, 1 and 2 at slots[i] (slot < 0 or >= R: skipped, its values not read; of tokens with the same slot any may be
- * the one kept, or parts of several). The norm and the
+ * spmla_cache_write's formats 0, 1 and 2 at slots[i] (slot < 0 or >= R: skipped, its values not read; of tokens with
+ * the same slot any may be the one kept, or parts of several); the cache may lie in pinned host memory. The norm and the
  * rotation stay in fp32 until they are encoded: Row656's codes are those of spmla_rms_norm, its rope is rounded once to
  * bf16. Replaces the norm, rotary and do_kv_cache_update calls around dsa_sm89.py:281-290. */
 int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int weight_f32, float eps,
