@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) norm_kernel(NormParams p)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       uint32_t lo, hi;
-      const float s = group_codes<!NORM, !NORM && DT != DT_F32>(z[c], r, p.ue8m0 != 0, lo, hi);
+      const float s = group_codes<!NORM>(z[c], r, p.ue8m0 != 0, DT != DT_F32 && (!NORM || !p.w), lo, hi);
       const int d = at(c), n = mine(c);
       if (n > 0) {
         uint8_t* q = p.codes + row * p.c_st + d;

@@ -301,13 +301,13 @@ __device__ inline void scaled(const float (&t)[8], Factor c, float (&y)[8]) {
 // thousand): a quotient by the rounded s would round those by s's rounding error. The product with 448 / amax decides
 // every code but those (codes_about); where a lane has one, the wave divides, with t and amax brought to the range in which
 // the remainder is exact by a power of two: 15 % of the waves on products of normally distributed bf16 values (norm of 8192 x
-// 4096 28 us, 36 if all divide). UNIT: r is 1. TIES: t are 16-bit floats, whose quotients are halfway in 69 % of the waves, so
+// 4096 28 us, 36 if all divide). UNIT: r is 1. ties: t are 16-bit floats, whose quotients are halfway in 69 % of the waves, so
 // that all that are not zeros divide at once (quantization of 4096 x 16384 52 us, 56 with the products first).
 // A group of infinities or NaNs (or a row factor that is one) is divided element by element: NaN codes for NaNs and
 // inf / inf.
 constexpr float Q_MAX = 448.0f, Q_MIN = 1e-12f;      // largest e4m3 value, smallest scale
-template <bool UNIT = false, bool TIES = false>
-__device__ inline float group_codes(const float (&t)[8], Factor r, bool ue8m0, uint32_t& lo, uint32_t& hi) {
+template <bool UNIT = false>
+__device__ inline float group_codes(const float (&t)[8], Factor r, bool ue8m0, bool ties, uint32_t& lo, uint32_t& hi) {
   uint32_t top = 0;                   // largest magnitude as an integer: infinities and NaNs lie above the finite ones
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, f2u(t[e]) & 0x7fffffffu);
@@ -338,7 +338,7 @@ __device__ inline float group_codes(const float (&t)[8], Factor r, bool ue8m0, u
       if (__builtin_expect(__ballot(!codes_about(t, c.hi, lo, hi)) == 0ull, 1)) return s;
       odd_products(t, c, y);
     } else {
-      if constexpr (TIES) {
+      if (ties) {
         if (__ballot(top != 0u) == 0ull) {
           lo = e4m3x4(t[0], t[1], t[2], t[3]);
           hi = e4m3x4(t[4], t[5], t[6], t[7]);

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256) latent_write_kernel(LatentParams p) {
   const float ra = a * c - b * s, rb = b * c + a * s;
   uint32_t lo, hi;
   if (p.fmt == 0) {
-    const float sc = group_codes(x, factor_of(r), false, lo, hi);
+    const float sc = group_codes(x, factor_of(r), false, !p.w, lo, hi);
     *(uint2*)(row + lane * 8) = make_uint2(lo, hi);
     if ((lane & 15) == 0) *(float*)(row + SC_OFF + (lane >> 4) * 4) = sc;
     if (lane < 32) {
