@@ -5,9 +5,10 @@
 // v_mfma_f32_16x16x128_f8f6f4 takes a whole block of k, its sum starts from zero and goes into the fp32 accumulator with
 // one FMA per value, by the product of the two scales. The weights are the row operand, so that a lane holds one token
 // (column l % 16, outputs 4 (l / 16) .. + 3) and needs one scale product for all the outputs of a 128-block. The matrix
-// core adds the 128 products with less than fp32's precision: 1.4e-5 of the sum's size on normally distributed codes
-// (4.5e-5 with 1 of 64 values 50 times the others), a hundredth of the 16-bit output's rounding; fp32 outputs are not
-// offered. Blocks are summed in fp32.
+// core adds the 128 products with less than fp32's precision. Against the sum of their magnitudes its error was at most 1.8e-5
+// on normally distributed codes and 2.0e-4 with 1 of 64 values 50 times the others (1.4e-5 and 4.4e-5 of the sums' size, root
+// mean square; other forms of the instruction reached 2.6e-4): half a step of a bf16 output is 3.9e-3 of the value, of fp16
+// 4.9e-4, so that outliers, and sums that cancel, show in fp16. fp32 outputs are not offered. Blocks are summed in fp32.
 //
 // Operands reach LDS by direct copies, 128-byte rows with their 16-byte chunks permuted by (row / 2) % 8 (the outputs of the
 // tile kernels, whose lanes take other rows, by what is the same number for the lane). A lane reads chunks g and g + 4 of its
@@ -81,10 +82,11 @@ __device__ inline void store4(const LinearParams& p, int t, int n, f32x4 v) {   
 // ---- tiles of BM tokens x BN outputs, 8 waves of WM x WN, a ring of ST blocks in LDS ----------------------------------
 // While the sums of block b form from registers, block b + 1 is read from LDS and blocks b + 2 .. b + ST are on their way:
 // one barrier a block, behind which block b's place is free and block b + 1 has arrived.
-// Bound by LDS: the copies of a block of 128 x 128 (33 KB at 64 bytes a clock) take 510 clocks and its reads 470, the matrix
-// instructions 510; a block takes 1000 to 1200. 1455 x 2112 x 4096 21 us (1.2 PFLOP/s, 204 workgroups), 6 of them
-// before and behind the blocks; 64 x 24576 x 1536 in tiles of 64 x 128 9.4 us (4.3 TB/s of weights and outputs). 16 waves,
-// wave tiles of 64 x 64 and a ring of 4 blocks were no faster, two workgroups a unit (128 registers) 10 % slower.
+// Bound by the chain of a block: its eight waves go from barrier to barrier in step, 1290 clocks a block of 128 x 128 (41,300
+// cycles over 32 blocks), in which the matrix cores are busy for 500 (39 %) and the LDS reads for 470 (36 %, no conflicts); no
+// unit is at its limit. 1455 x 2112 x 4096 20 to 22 us (1.2 PFLOP/s, 204 workgroups), 6 of them before and behind the blocks; 64
+// x 24576 x 1536 in tiles of 64 x 128 9.4 us (4.3 TB/s of weights and outputs). 16 waves, wave tiles of 64 x 64 and a ring of 4
+// blocks were no faster, two workgroups a unit (128 registers) 10 % slower.
 template <int BM, int BN, int WM, int WN, int ST>
 struct Ring {
   static constexpr int NW = 8, NWM = BM / WM, PA = BM / 64, PW = BN / 64, NI = PA + PW + 1;   // copies of a wave and block

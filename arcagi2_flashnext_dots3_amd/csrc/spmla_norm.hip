@@ -8,9 +8,12 @@
 // One pass: a row's values stay in the registers of the threads that share it, 8 a thread in CH chunks, so x and the
 // residual are read once; x, residual and weights are all on their way before the first is needed. A group of 128 values is
 // 16 neighbouring lanes of a chunk. Rows of up to 512 values take one wave each (no LDS), longer ones several.
-// Bound by HBM for long chunks: 8192 x 4096 bf16 with residual and codes 44 us (236 MB, 5.3 TB/s with part of it in the last
-// cache; a device copy moves 5.1). Few rows: the chain of a row's loads, sum, root and codes, 3.3 us (64 x 1536) to 3.5 us
-// (1 x 4096) a launch in a graph; the quantization of 32 x 16384 alone takes 2.3.
+// Bound by HBM for long chunks of wide rows: 8192 x 4096 bf16 with residual and codes 43 us (236 MB, 5.5 TB/s with part of it
+// in the last cache; a device copy moves 5.1), 8192 x 7168 83. Narrow rows by the chain of each (loads, sum, root, codes) and
+// by lanes without a value: 8192 x 576 with residual and codes 14 us of 6.5 at the copy's rate (72 of a row's 128 threads have
+// values), 8192 x 1536 20 of 17. The quantization alone: 4096 x 16384 52 us, its divisions, and 39.5 with scales of powers of
+// two (5.1 TB/s). Few rows: one row's chain, 3.3 us (1 x 4096 and 64 x 1536) a launch in a graph; the quantization of 32 x
+// 16384 2.8.
 #include "spmla_quant.h"
 
 namespace spmla {
@@ -167,8 +170,8 @@ constexpr int MAX_D = 65536;
 
 template <int DT, int ROW>
 static int norm_go(const NormParams& p, hipStream_t s) {
-  // as few threads and chunks as hold the row: idle ones cost as much as busy ones (8192 x 576 64 x 1 to 256 x 1: 13.7 to
-  // 21.5 us). Of equal ones many threads for few rows (4096 values, 1 row: 512 x 1 3.6, 256 x 2 4.6; 7168: 1024 x 1 4.6, 512 x
+  // as few threads and chunks as hold the row, idle ones cost too (8192 x 1024 with residual and codes: 128 x 1 15.7 us, 256 x
+  // 1 16.6). Of equal ones many threads for few rows (4096 values, 1 row: 512 x 1 3.6, 256 x 2 4.6; 7168: 1024 x 1 4.6, 512 x
   // 2 5.1), fewer that each have more on their way for many (8192 rows: 45 / 42, 104 / 88).
   if constexpr (ROW == TINY) {
     return launch<DT, true, 64, 1, ROW>(p, s);

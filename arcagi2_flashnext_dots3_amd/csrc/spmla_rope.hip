@@ -4,8 +4,8 @@
 //   (a, b) -> factor (a cos - b sin, b cos + a sin); interleaved pairs are (2i, 2i + 1), else (i, i + n).
 // The angle is formed in quarter turns, from 2 / pi and products in twice 64 bits: its distance from the nearest whole one is
 // exact to 2^-54 up to positions of 2^31 (rounded products alone: to 2^-21 there), so that only its rounding to 32 bits counts;
-// cosine and sine come from their Taylor series on +-45 degrees
-// (remainders x^11 / 11! and x^12 / 12!, below 2^-28). No table of positions is read.
+// cosine and sine come from their Taylor series on +-45 degrees (remainders x^11 / 11! and x^12 / 12!, below 2^-28). No table
+// of positions is read.
 // Bound by HBM for long chunks: a head is read and written once (8192 tokens x 64 heads x 128 bf16 53 us, 268 MB, 5.0 TB/s;
 // a device copy moves 5.1); 64 tokens x 128 heads 3.3 us. A thread keeps its columns and turns them for several heads of one
 // token, so that an angle (some 50 instructions, 11 of them in 64 bits) is formed once for them. Loads and stores are 16
@@ -13,7 +13,8 @@
 //
 // Latent row: RMS norm of the 512 latent values and rotary of the 64 rope values, both in fp32, then the row that
 // spmla_cache_write would write of them (Row656 codes: group_codes); nothing is rounded to bf16 between. One wave a token:
-// 64 tokens 3.5 us, the chain of slot, latent, sum and codes; 8192 tokens 5.4 us (14 MB, 2.6 TB/s: too short to reach more).
+// 64 tokens 2.9 us (Row576) to 3.6 (Row400), the chain of slot, latent, sum and codes; 8192 tokens 5.8 us into Row576 (14 MB,
+// 2.4 TB/s: too short to reach more), 6.9 into Row656, 8.2 into Row400.
 #include "spmla_quant.h"
 
 namespace spmla {
@@ -25,7 +26,7 @@ __device__ inline void turn(double pos, double freq, float factor, float sign, f
   const double q = pos * f, q_lo = __builtin_fma(pos, f_lo, __builtin_fma(pos, f, -q));
   const double k = rint(q);
   const float x = (float)((q - k) + q_lo) * 1.57079632679489661923f, y = x * x;
-  const int n = (int)__builtin_bit_cast(uint64_t, k + 0x1.8p52) & 3;   // which quarter: the sum's last bit is 1
+  const int n = (int)__builtin_bit_cast(uint64_t, k + 0x1.8p52) & 3;   // which quarter: the sum's last bit counts ones
   const float sn = x * (1.0f + y * (-1.0f / 6 + y * (1.0f / 120 + y * (-1.0f / 5040 + y * (1.0f / 362880)))));
   const float cs = 1.0f + y * (-0.5f + y * (1.0f / 24 + y * (-1.0f / 720 + y * (1.0f / 40320 + y * (-1.0f / 3628800)))));
   const float a = n & 1 ? sn : cs, b = n & 1 ? cs : sn;

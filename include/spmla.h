@@ -478,16 +478,17 @@ int spmla_quant_fp8(const void* x, long long x_st, int T, int D, int dtype, unsi
  * a [T][K], w [N][K] e4m3 codes (row strides a multiple of 16 bytes, at most 2^22), a_scales [T][ceil(K / 128)], w_scales
  * [ceil(N / 128)][ceil(K / 128)] fp32 (the checkpoint's weight_scale_inv), out [T][N] dtype 1 fp16 or 2 bf16. K % 16 == 0,
  * K <= 2^22, N <= 2^23.
- * The 128 products of a block are added by the matrix core (1.4e-5 of the sum's size on normally distributed codes), the
- * blocks in fp32. No counterpart in the reference's tree: the serving engine's own layers run in its place. */
+ * The 128 products of a block are added by the matrix core, to 1.8e-5 of the sum of their magnitudes on normally distributed
+ * codes and 2.0e-4 with outliers (the largest errors found; 1.4e-5 and 4.4e-5 root mean square), the blocks in fp32.
+ * No counterpart in the reference's tree: the serving engine's own layers run in its place. */
 int spmla_linear_fp8(const void* a, long long a_st, const float* a_scales, long long as_st, const void* w,
                      long long w_st, const float* w_scales, long long ws_st, int T, int N, int K, int dtype, void* out,
                      long long o_st, void* stream);
 
 /* Rotary positions: columns start .. start + 2n of every head of x [T][H][W] turn by positions[t] * freqs[i] radians
  * (pairs (start + 2i, start + 2i + 1) with interleaved, else (start + i, start + n + i)): (a, b) -> factor * (a cos -
- * b sin, b cos + a sin), inverse: by the negative angle. The other columns are copied (out == x: left). Angles in 64
- * bits: positions (int64, or int32 with pos32) up to 2^31 keep theirs to 2^-22. freqs [n] float64 on the device. dtype as
+ * b sin, b cos + a sin), inverse: by the negative angle. The other columns are copied (out == x: left). Angles in twice 64
+ * bits: cosine and sine of positions (int64, or int32 with pos32) up to 2^31 are within 2^-22. freqs [n] float64 on the device. dtype as
  * spmla_rms_norm. out is x itself (same strides) or does not overlap it. H, W <= 2^30. No counterpart in the
  * reference's tree (the serving engine's own layer). */
 int spmla_rope(const void* x, long long x_st, long long x_sh, const void* positions, int pos32, const double* freqs,
