@@ -70,11 +70,16 @@ SIGNATURES = {
     "spmla_linear_fp8": [P, LL, P, LL, P, LL, P, LL, I, I, I, I, P, LL, P],
     "spmla_rope": [P, LL, LL, P, I, P, I, I, I, I, I, I, F, I, I, P, LL, LL, P],
     "spmla_latent_write": [P, LL, P, I, F, P, I, P, I, F, P, I, P, LL, I, LL, I, F, P],
+    "spmla_page_step": [P, I, P, P, P, LL, I, P, I, P, I, I, P, P, P, P, P],
+    "spmla_page_trim": [P, I, P, P, P, LL, I, P, I, P, I, P],
+    "spmla_attn_prompt": [P, LL, LL, P, LL, LL, P, LL, LL, P, I, I, I, I, I, I, F, I, I, P, LL, LL, P, LL, P],
+    "spmla_attn_chunk_ws_bytes": [I, I, I],
+    "spmla_attn_chunk": [P, LL, LL, P, LL, I, I, LL, P, LL, I, P, P, I, I, I, F, F, I, I, P, LL, LL, P, LL, P, LL, P],
     "spmla_version": [],
     "spmla_host_e4m3_encode": [P, P, LL],
 }
 _RESTYPE = {"spmla_version": ctypes.c_char_p, "spmla_host_e4m3_encode": None, "spmla_topk_ws_bytes": LL,
-            "spmla_topk_scratch_bytes": LL, "spmla_attn_ws_bytes": LL}
+            "spmla_topk_scratch_bytes": LL, "spmla_attn_ws_bytes": LL, "spmla_attn_chunk_ws_bytes": LL}
 
 ERRORS = {-2: "bad argument", -3: "misaligned pointer or stride", -5: "size beyond the kernel's limit"}
 

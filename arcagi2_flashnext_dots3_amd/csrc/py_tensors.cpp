@@ -1,4 +1,4 @@
-// The norm, quantization, projection, rotary and latent-row calls on tensors: checks of shapes, types, strides and devices,
+// The norm, quantization, projection, rotary, latent-row, page-table and dense attention calls on tensors: checks of shapes, types, strides and devices,
 // then the entry point (include/spmla.h) on the current stream. _tensors.load(path, raw_stream, get_device) opens the
 // library and returns {name: callable}; a callable raises ValueError for what the call does not take, before it launches
 // anything, and returns the entry point's value, or AWAY when the tensors are on another GPU than the current one. These
@@ -29,6 +29,10 @@ decltype(&::spmla_quant_fp8) f_quant_fp8 = nullptr;
 decltype(&::spmla_linear_fp8) f_linear_fp8 = nullptr;
 decltype(&::spmla_rope) f_rope = nullptr;
 decltype(&::spmla_latent_write) f_latent_write = nullptr;
+decltype(&::spmla_page_step) f_page_step = nullptr;
+decltype(&::spmla_page_trim) f_page_trim = nullptr;
+decltype(&::spmla_attn_prompt) f_attn_prompt = nullptr;
+decltype(&::spmla_attn_chunk) f_attn_chunk = nullptr;
 PyObject *raw_stream = nullptr, *get_device = nullptr;
 
 // ---- arguments
@@ -367,6 +371,159 @@ long latent_write(PyObject* const* a) {
   });
 }
 
+// ---- a pool of pages: table [M, W], lens [M], held [M], free [P], state [4]
+struct Pool {
+  const at::Tensor *table, *lens, *held, *free, *state;
+  int64_t M, W, st, P;
+  int bs, dev;
+};
+Pool pool_of(PyObject* const* a, PyObject* block) {
+  Pool p{tensor(a[0], "table"), tensor(a[1], "lens"), tensor(a[2], "held"), tensor(a[3], "free"), tensor(a[4], "state"), 0, 0, 0, 0, 0, 0};
+  if (p.table->dim() != 2) refuse("table [requests, pages of a request] int32: got " + shown(*p.table));
+  p.M = p.table->size(0), p.W = p.table->size(1);
+  if (p.M == 0) refuse("table: at least one request");
+  at_most(p.M, 8192, "requests");
+  p.st = rows(*p.table, p.M, p.W, I32, "table [requests, pages of a request] int32", true);
+  line(*p.lens, p.M, p.M, I32, "lens [requests] int32");
+  line(*p.held, p.M, p.M, I32, "held [requests] int32");
+  line(*p.free, 0, 0x7fffffff, I32, "free [pages] int32");
+  line(*p.state, 4, 4, I32, "state [4] int32");
+  p.P = p.free->size(0);
+  const long long bs = integer(block);
+  if (bs < 1 || bs > 1 << 20) refuse("block_size of 1 to 2^20: got " + std::to_string(bs));
+  p.bs = (int)bs;
+  p.dev = gpu_of(*p.table);
+  for (const at::Tensor* t : {p.table, p.lens, p.held, p.free, p.state}) same_gpu(*t, p.dev, "pool");
+  return p;
+}
+
+// page_step(table, lens, held, free, state, block_size, new, start, req, positions, slots)
+long page_step(PyObject* const* a) {
+  const Pool p = pool_of(a, a[5]);
+  const at::Tensor *fresh = tensor(a[6], "new"), *start = tensor(a[7], "start"), *req = tensor(a[8], "req");
+  const at::Tensor *pos = tensor(a[9], "positions"), *slots = tensor(a[10], "slots");
+  line(*fresh, p.M, p.M, I32, "new [requests] int32");
+  line(*start, p.M + 1, p.M + 1, I32, "start [requests + 1] int32");
+  line(*req, 0, MAX_TOKENS, I32, "req [n] int32");
+  const int64_t n = req->size(0);
+  line(*pos, n, n, I64, "positions [n] int64");
+  line(*slots, n, n, I64, "slots [n] int64");
+  for (const at::Tensor* t : {fresh, start, req, pos, slots}) same_gpu(*t, p.dev, "page_step");
+  return launch(p.dev, [&](void* s) {
+    return f_page_step((const int*)address(fresh), (int)p.M, (int*)address(p.lens), (int*)address(p.held), (int*)address(p.table), p.st,
+                       as_int(p.W, "W"), (int*)address(p.free), (int)p.P, (int*)address(p.state), p.bs, (int)n, (int*)address(start),
+                       (int*)address(req), (long long*)address(pos), (long long*)address(slots), s);
+  });
+}
+
+// page_trim(table, lens, held, free, state, block_size, keep)
+long page_trim(PyObject* const* a) {
+  const Pool p = pool_of(a, a[5]);
+  const at::Tensor* keep = tensor(a[6], "keep");
+  line(*keep, p.M, p.M, I32, "keep [requests] int32");
+  same_gpu(*keep, p.dev, "page_trim");
+  return launch(p.dev, [&](void* s) {
+    return f_page_trim((const int*)address(keep), (int)p.M, (int*)address(p.lens), (int*)address(p.held), (int*)address(p.table), p.st,
+                       as_int(p.W, "W"), (int*)address(p.free), (int)p.P, (int*)address(p.state), p.bs, s);
+  });
+}
+
+// token and head strides of x [T, H, D] with contiguous heads; 16-byte rows; written: heads that do not overlap
+struct Heads {
+  int64_t st, sh;
+};
+Heads heads(const at::Tensor& x, int64_t T, int64_t H, int64_t D, unsigned type, const char* what, bool written = false) {
+  if (x.dim() != 3 || x.size(0) != T || x.size(1) != H || x.size(2) != D || type_of(x) != type)
+    refuse(std::string(what) + " expected, (" + std::to_string(T) + ", " + std::to_string(H) + ", " + std::to_string(D) + "): got " + shown(x));
+  const Heads s{T > 1 ? x.stride(0) : 0, H > 1 ? x.stride(1) : 0};
+  if (T == 0 || H == 0 || D == 0) return s;
+  if (D > 1 && x.stride(2) != 1) refuse(std::string(what) + ": contiguous heads");
+  on_bytes(x, (s.st | s.sh) * 2, 16, what);
+  if (written && ((T > 1 && s.st < D) || (H > 1 && s.sh < D) || (T > 1 && H > 1 && s.st < (H - 1) * s.sh + D && s.sh < (T - 1) * s.st + D)))
+    refuse(std::string(what) + ": heads that do not overlap");
+  return s;
+}
+// lse [T, H] fp32: token stride
+int64_t sums(const at::Tensor* lse, int64_t T, int64_t H) { return lse ? rows(*lse, T, H, F32, "lse [T, H] fp32", true) : 0; }
+int64_t starts(const at::Tensor& start) {
+  line(start, 1, MAX_TOKENS, I32, "start [requests + 1] int32");
+  return start.size(0) - 1;
+}
+
+// attend_prompt(q, k, v, start, scale, causal, out, lse)
+long attend_prompt(PyObject* const* a) {
+  const at::Tensor *q = tensor(a[0], "q"), *k = tensor(a[1], "k"), *v = tensor(a[2], "v"), *start = tensor(a[3], "start");
+  const at::Tensor *out = tensor(a[6], "out"), *lse = maybe(a[7], "lse");
+  const double scale = number(a[4]);
+  const bool causal = truth(a[5]);
+  const unsigned type = type_of(*q);
+  if (q->dim() != 3 || !(type & (F16 | BF16))) refuse("q [T, H, D] fp16 / bf16: got " + shown(*q));
+  if (k->dim() != 3 || v->dim() != 3) refuse("k [T, Hk, D], v [T, Hk, Dv]: got " + shown(*k) + ", " + shown(*v));
+  const int64_t T = q->size(0), H = q->size(1), D = q->size(2), Hk = k->size(1), Dv = v->size(2);
+  if (Hk == 0 || H % Hk) refuse("heads of q a multiple of k's: got " + std::to_string(H) + ", " + std::to_string(Hk));
+  if (D == 0 || Dv == 0 || D % 8 || Dv % 8 || D > 256 || Dv > 256)
+    refuse("D, Dv multiples of 8 up to 256: got " + std::to_string(D) + ", " + std::to_string(Dv));
+  if (!((float)scale - (float)scale == 0.f)) refuse("scale: a finite number");
+  at_most(T, MAX_TOKENS, "T");
+  at_most(H, 65536, "H");
+  const Heads qs = heads(*q, T, H, D, type, "q [T, H, D]"), ks = heads(*k, T, Hk, D, type, "k [T, Hk, D] of q's type");
+  const Heads vs = heads(*v, T, Hk, Dv, type, "v [T, Hk, Dv] of q's type"), os = heads(*out, T, H, Dv, type, "out [T, H, Dv] of q's type", true);
+  const int64_t ls = sums(lse, T, H), B = starts(*start);
+  const int dev = gpu_of(*q);
+  for (const at::Tensor* t : {q, k, v, start, out, lse})
+    if (t) same_gpu(*t, dev, "attend_prompt");
+  return launch(dev, [&](void* s) {
+    return f_attn_prompt(address(q), qs.st, qs.sh, address(k), ks.st, ks.sh, address(v), vs.st, vs.sh, (const int*)address(start), (int)B,
+                         (int)T, (int)H, (int)Hk, (int)D, (int)Dv, (float)scale, causal, dtype_code(type), address(out), os.st, os.sh,
+                         (float*)address(lse), ls, s);
+  });
+}
+
+// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, split, span, out, lse, ws)
+long attend_chunk(PyObject* const* a) {
+  const at::Tensor *q = tensor(a[0], "q"), *cache = tensor(a[1], "cache"), *table = tensor(a[2], "block_table"), *seqs = tensor(a[3], "seq_lens");
+  const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[9], "out"), *lse = maybe(a[10], "lse"), *ws = maybe(a[11], "ws");
+  const double sm = number(a[5]), kvs = number(a[6]);
+  const long long split = integer(a[7]), span = integer(a[8]);
+  if (q->dim() != 3 || type_of(*q) != BF16 || q->size(2) != 576) refuse("q [T, H, 576] bf16: got " + shown(*q));
+  const int64_t T = q->size(0), H = q->size(1), B = starts(*start);
+  at_most(T, MAX_TOKENS, "T");
+  at_most(H, 65536, "H");
+  const Heads qs = heads(*q, T, H, 576, BF16, "q [T, H, 576]"), os = heads(*out, T, H, 512, BF16, "out [T, H, 512] bf16", true);
+  const int64_t ls = sums(lse, T, H);
+  if (cache->dim() != 3 || type_of(*cache) != U8 || (cache->size(2) != 656 && cache->size(2) != 576))
+    refuse("cache [blocks, block_size, 656 or 576] uint8: got " + shown(*cache));
+  const int64_t blocks = cache->size(0), bs = cache->size(1), rowb = cache->size(2);
+  if (bs == 0) refuse("cache: blocks of at least one row");
+  if (cache->stride(2) != 1 || (bs > 1 && cache->stride(1) != rowb)) refuse("cache: rows inside a block must be contiguous");
+  const int64_t bst = blocks > 1 ? cache->stride(0) : bs * rowb;
+  if (bst % rowb || bst < bs * rowb) refuse("cache: blocks a whole number of rows apart that do not overlap");
+  on_bytes(*cache, 0, 16, "cache");
+  const int64_t stride = bst / rowb, total = blocks > 0 ? (blocks - 1) * stride + bs : 0;
+  at_most(total, 0x7fffffff, "rows of the cache");
+  if (table->dim() != 2) refuse("block_table [requests, columns] int32: got " + shown(*table));
+  const int64_t W = table->size(1), tst = rows(*table, B, W, I32, "block_table [requests, columns] int32");
+  at_most(W * bs, 0x7fffff00, "positions of a block table's row");
+  line(*seqs, B, B, I32, "seq_lens [requests] int32");
+  if (!((float)(sm * kvs) - (float)(sm * kvs) == 0.f)) refuse("sm_scale, kv_scale: finite numbers");
+  if (split < 1 || split > 256) refuse("split of 1 to 256: got " + std::to_string(split));
+  if (span < 32 || span % 32 || span > 0x7fffffe0) refuse("span: a positive multiple of 32");
+  if (split > 1) {
+    if (!ws) refuse("ws: a workspace for split > 1");
+    line(*ws, T * H * split * 513 * 4, ANY, U8, "ws [T * H * split * 2052] uint8");
+    on_bytes(*ws, 0, 16, "ws");
+  }
+  const int dev = gpu_of(*q);
+  for (const at::Tensor* t : {q, cache, table, seqs, start, out, lse, ws})
+    if (t) same_gpu(*t, dev, "attend_chunk");
+  return launch(dev, [&](void* s) {
+    return f_attn_chunk(address(q), qs.st, qs.sh, address(cache), total, (int)rowb, as_int(bs, "block_size"), stride,
+                        (const int*)address(table), tst, (int)W, (const int*)address(seqs), (const int*)address(start), (int)B, (int)T,
+                        (int)H, (float)sm, (float)kvs, (int)split, (int)span, address(out), os.st, os.sh, (float*)address(lse), ls,
+                        address(ws), ws ? ws->numel() : 0, s);
+  });
+}
+
 template <long (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != N) return PyErr_Format(PyExc_TypeError, "%d arguments expected, got %zd", N, n);
@@ -384,7 +541,8 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define CALLABLE(name, n) {#name, (PyCFunction)(void (*)())entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(linear_quant, 6),
-                       CALLABLE(rope, 8), CALLABLE(latent_write, 13)};
+                       CALLABLE(rope, 8), CALLABLE(latent_write, 13), CALLABLE(page_step, 11), CALLABLE(page_trim, 7),
+                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 12)};
 
 PyObject* load(PyObject*, PyObject* args) {
   const char* path;
@@ -395,7 +553,8 @@ PyObject* load(PyObject*, PyObject* args) {
 #define BIND(name)                                                                                   \
   f_##name = (decltype(f_##name))dlsym(h, "spmla_" #name);                                           \
   if (!f_##name) return PyErr_Format(PyExc_OSError, "%s: no spmla_" #name, path);
-  BIND(rms_norm) BIND(quant_fp8) BIND(linear_fp8) BIND(rope) BIND(latent_write)
+  BIND(rms_norm) BIND(quant_fp8) BIND(linear_fp8) BIND(rope) BIND(latent_write) BIND(page_step) BIND(page_trim)
+  BIND(attn_prompt) BIND(attn_chunk)
   Py_INCREF(rs);
   Py_INCREF(gd);
   raw_stream = rs;

@@ -250,6 +250,32 @@ class PortableSparseImpl:
             return o_ref, None
         return self._forward_paged(q, kv_c_and_k_pe_cache, attn_metadata, kv_scale), None
 
+    def forward_dense(self, q, kv_c_and_k_pe_cache, attn_metadata, layer=None):
+        """forward_mqa without a selection (layers without an indexer, or contexts of at most topk rows): every token of
+        q [T, H, 576] bf16 (or the pair (q_nope, q_pe)) attends all cached rows of its request up to its own -> (out [T, H,
+        512] bf16, lse [T, H] fp32). attn_metadata: CommonAttentionMetadata (with seq_lens). The rows are in the paged cache:
+        not for an offloaded layer."""
+        if self._offload:
+            raise NotImplementedError("forward_dense: the rows of an offloaded layer are not in the paged cache")
+        if isinstance(q, tuple):
+            q = torch.cat(q, dim=-1)
+        if not kernels.query_ok(q):
+            q = q.contiguous()
+        md = attn_metadata
+        if md.seq_lens is None:
+            raise ValueError("forward_dense: attn_metadata.seq_lens")
+        c = kv_c_and_k_pe_cache
+        c = c.view(torch.uint8) if c.dtype != torch.uint8 else c
+        kv_scale = float(getattr(layer, "_k_scale_float", 1.0)) if layer is not None else 1.0
+        return kernels.attend_chunk(q, c, md.block_table_tensor, md.seq_lens, md.query_start_loc, self.softmax_scale, kv_scale,
+                                    max_seq_len=md.max_seq_len)
+
+    def forward_mha(self, q, k, v, attn_metadata):
+        """Prompts of which nothing is cached yet, on expanded heads: q, k [T, H, 192], v [T, H, 128] (any widths that
+        kernels.attend_prompt takes) -> (out [T, H, 128], lse [T, H] fp32), causal within each request of
+        attn_metadata.query_start_loc."""
+        return kernels.attend_prompt(q, k, v, attn_metadata.query_start_loc, self.softmax_scale)
+
     def _run(self, q, kvc, gidx, kv_scale=1.0):
         """Attention of q over cache rows gidx [n, K] (-1 or out of range: none) of a paged or flat cache."""
         c, num_rows, _, rb = self._rows_view(kvc)

@@ -1093,3 +1093,84 @@ def latent_write(kv, weight, eps, positions, freqs, slots, cache, fmt=0, kv_scal
     (LayerOffload.store_latent keeps a layer's cached copies too)."""
     _lib.tensor_call("latent_write", kv, kv, weight, eps, positions, freqs, slots, cache, fmt, kv_scale, interleaved,
                      factor, block_size, block_stride)
+
+
+# ---------------------------------------------------------------------------------- dense attention of a serving step
+def page_step(pool, new, n=None, start=None, req=None, positions=None, slots=None):
+    """The tables of a step, built on the GPU: new [requests] int32 new tokens of each request of pool (paging.PagePool; <= 0:
+    none) -> (start [requests + 1] int32 sums of the new tokens; req [n] int32, positions [n] int64 and slots [n] int64 of
+    each token). Pages the tokens need come from the pool's free stack and are entered in its table; where the stack is
+    empty the rest go without (slot -1; pool.state[1] counts the missing pages, and a later step fills them in). n: places
+    for tokens (None: that of req); those behind the last token hold the last request, position 0 and slot -1, tokens
+    beyond n have none."""
+    dev = pool.table.device
+    if n is None:
+        _need(req is not None, "page_step: n, or req [n]")
+        n = req.shape[0]
+    if start is None:
+        start = torch.empty(pool.table.shape[0] + 1, dtype=torch.int32, device=dev)
+    req = torch.empty(n, dtype=torch.int32, device=dev) if req is None else req
+    positions = torch.empty(n, dtype=torch.int64, device=dev) if positions is None else positions
+    slots = torch.empty(n, dtype=torch.int64, device=dev) if slots is None else slots
+    _need(req.shape == (n,), "req [n] int32")
+    _lib.tensor_call("page_step", pool.table, pool.table, pool.lens, pool.held, pool.free, pool.state, pool.block_size, new,
+                     start, req, positions, slots)
+    return start, req, positions, slots
+
+
+def page_trim(pool, keep):
+    """Request b of pool keeps its first keep[b] tokens at most (keep [requests] int32; 0: it is finished, its length or more:
+    left as it is): the pages behind them go back to the free stack, their table entries become -1."""
+    _lib.tensor_call("page_trim", pool.table, pool.table, pool.lens, pool.held, pool.free, pool.state, pool.block_size, keep)
+
+
+def attend_prompt(q, k, v, start, scale, causal=True, out=None, lse=None):
+    """Attention over whole prompts, packed: sequence b is tokens start[b] .. start[b + 1] - 1 (start [B + 1] int32, ascending;
+    tokens of no sequence are left alone). q [T, H, D], k [T, Hk, D], v [T, Hk, Dv] bf16 or fp16 (H a multiple of Hk: query
+    head h reads head h // (H // Hk); D and Dv multiples of 8 up to 256; rows on 16 bytes, any strides) -> (out [T, H,
+    Dv] of q's type, lse [T, H] fp32). causal: token i sees tokens up to i of its sequence, else all of them."""
+    _need(q.dim() == 3 and v.dim() == 3, "q [T, H, D], v [T, Hk, Dv]")
+    if out is None:
+        out = torch.empty(q.shape[0], q.shape[1], v.shape[2], dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device)
+    _lib.tensor_call("attend_prompt", q, q, k, v, start, scale, causal, out, lse)
+    return out, lse
+
+
+@functools.lru_cache(maxsize=4096)
+def chunk_split(T, H, B, longest, cus=256):
+    """(splits, positions of each) of attend_chunk for T tokens of H heads in B requests of up to `longest` cached rows."""
+    tiles = T * H // 64 + min(B, T)
+    tiles = max(1, tiles)
+    units = max(1, -(-longest // 32))                    # tiles of 32 positions
+    split = max(1, min(2 * cus // tiles, -(-units // 8), 128))
+    span = -(-units // split)
+    return -(-units // span), 32 * span
+
+
+def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0, max_seq_len=None, out=None, lse=None,
+                 split=None):
+    """Attention of new tokens over every cached row of their request: tokens start[b] .. start[b + 1] - 1 of q [T, H, 576] bf16
+    (start [B + 1] int32) are the last of the seq_lens[b] rows that request b has in cache [blocks, block_size, 656 or 576]
+    uint8 (already written; block stride any whole number of rows) through block_table [B, columns] int32; each token sees
+    its own position and those before it, but for pages that are not there (-1). Returns (out [T, H, 512] bf16, lse [T, H]
+    fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: about the
+    longest seq_lens, known on the host (None: what the table can hold), by which the positions are split; the result does
+    not depend on it. split: splits of the positions (None: chunk_split), joined through a temporary workspace."""
+    _need(q.dim() == 3 and cache.dim() == 3 and block_table.dim() == 2, "q [T, H, 576], cache [blocks, block_size, row], block_table [B, columns]")
+    T, H = q.shape[0], q.shape[1]
+    room = block_table.shape[1] * cache.shape[1]
+    longest = max(1, room if max_seq_len is None else min(int(max_seq_len), room))
+    if split is None:
+        split, span = chunk_split(T, H, block_table.shape[0], longest)
+    else:
+        _need(1 <= split <= 256, "split of 1 to 256")
+        span = -(-longest // (32 * split)) * 32
+    if out is None:
+        out = torch.empty(T, H, D_LAT, dtype=torch.bfloat16, device=q.device)
+    if lse is None:
+        lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
+    ws = torch.empty(T * H * split * (D_LAT + 1) * 4, dtype=torch.uint8, device=q.device) if split > 1 else None
+    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, split, span, out, lse, ws)
+    return out, lse

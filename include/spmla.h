@@ -506,6 +506,52 @@ int spmla_latent_write(const void* kv, long long kv_st, const void* weight, int 
                        const long long* slots, int n, void* cache, long long R, int block_size, long long block_stride,
                        int fmt, float kv_scale, void* stream);
 
+/* The tables of a serving step, built on the GPU. State of a pool of P pages for M requests (all device memory):
+ * lens [M] tokens of each request, held [M] pages it holds, table [M][W] (row stride table_st) its pages, free [P] the
+ * stack of pages nobody holds, state [4]: how many of them, pages missing in the last step, and two of the kernels' own
+ * (zero at first). Calls on one pool run in order.
+ * step: fresh [M] new tokens of each request (<= 0: none). Pages come from the top of the stack in the requests' order
+ * (where it is empty the rest go without; a later step fills them in) and are entered in the table; start [M + 1] = sums
+ * of the new tokens; for each of n places the token's request, position and slot (page * block_size + offset; -1 without a
+ * page). Places behind the last token: request M - 1, position 0, slot -1; tokens beyond n have no place. lens, held and
+ * the stack are updated.
+ * trim: request b keeps its first keep[b] tokens at most; the pages behind them go back to the stack (so that a step and a
+ * trim to the lengths before it are the identity), their table entries become -1.
+ * M <= 8192. The counterpart of what vLLM's scheduler and model runner form on the host for CommonAttentionMetadata
+ * (block_table_tensor, slot_mapping; read at dsa_sm89.py:484-499). */
+int spmla_page_step(const int* fresh, int M, int* lens, int* held, int* table, long long table_st, int W, int* free,
+                    int P, int* state, int block_size, int n, int* start, int* req, long long* positions,
+                    long long* slots, void* stream);
+int spmla_page_trim(const int* keep, int M, int* lens, int* held, int* table, long long table_st, int W, int* free,
+                    int P, int* state, int block_size, void* stream);
+
+/* Attention over whole prompts: B sequences packed into T tokens, sequence b tokens start[b] .. start[b + 1] - 1 (start
+ * [B + 1], ascending, on the device); tokens outside are neither read nor written.
+ * out[t][h] = softmax_j(scale q[t][h] . k[j][h / (H / Hk)]) v over the tokens j of t's sequence (causal: j <= t), lse[t][h]
+ * (optional) the natural log of the sum of the exponentials. q [T][H][D], k [T][Hk][D], v [T][Hk][Dv], out [T][H][Dv] of
+ * dtype 1 fp16 or 2 bf16; D and Dv multiples of 8 up to 256, rows on 16 bytes. Scores, statistics and sums in fp32, the
+ * weights rounded to dtype for their product with v. No counterpart in the reference's tree (masked_mha_available = False,
+ * dsa_sm89.py:216-230: the serving engine's prefill attention). */
+int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void* k, long long k_st, long long k_sh,
+                      const void* v, long long v_st, long long v_sh, const int* start, int B, int T, int H, int Hk,
+                      int D, int Dv, float scale, int causal, int dtype, void* out, long long o_st, long long o_sh,
+                      float* lse, long long l_st, void* stream);
+
+/* Attention of new tokens over every cached row of their request: tokens start[b] .. start[b + 1] - 1 are the last of
+ * request b's seqs[b] cached rows; token i of n sees positions x < seqs[b] - n + i + 1 whose page table[b][x / block_size]
+ * (row stride t_st, W columns) is not negative: cache row page * stride_rows + x % block_size (stride_rows: rows from a block
+ * to the next; rows beyond `rows` are not read). row_bytes 656 or 576; s = sm_scale * kv_scale * (q . row), out [T][H][512]
+ * bf16 = kv_scale * sum p latent, lse [T][H] optional, as spmla_attn_splitk over all of these rows; a token without one gets
+ * 0 and -inf, tokens of no request nothing. Positions are cut into S splits of span each (a multiple of 32; the last one
+ * takes the rest; S <= 256), joined by a second kernel through a workspace of spmla_attn_chunk_ws_bytes (S > 1).
+ * The dense counterpart of PortableSparseImpl.forward_mqa (dsa_sm89.py:379-470) for layers without an indexer. */
+long long spmla_attn_chunk_ws_bytes(int T, int H, int S);
+int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
+                     int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
+                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
+                     long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes,
+                     void* stream);
+
 /* Build identification string (static storage). */
 const char* spmla_version(void);
 

@@ -1,0 +1,221 @@
+"""Attention of new tokens over a request's paged latent rows against 64 bits."""
+import pytest
+import torch
+
+from tests import refs_dense as ref
+
+pytestmark = pytest.mark.gpu
+SM = 192 ** -0.5
+
+
+def _case(seqs, lens, H, row, bs, seed, gap=0, spare=3, spread=0.3, missing=()):
+    """(q, cache, table, seqs, start) on the CPU: pages in no order, what lies behind a sequence's end is no number."""
+    g = torch.Generator().manual_seed(seed)
+    held = [-(-n // bs) for n in seqs]
+    cache = ref.make_cache(sum(held) + spare, bs, row, g, spread, gap)
+    pages = torch.randperm(sum(held) + spare, generator=g).to(torch.int32)
+    W = max(held) + 2
+    table = torch.full((len(seqs), W), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(held):
+        table[b, :n] = pages[at:at + n]
+        at += n
+        if seqs[b] % bs:
+            cache[table[b, n - 1], seqs[b] % bs:] = 0x7F
+    for p in pages[at:]:
+        cache[p] = 0x7F
+    for b, c in missing:
+        table[b, c] = -1
+    q = torch.randn(sum(lens), H, 576, generator=g)
+    q[:, 0] *= 4.0
+    start = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32)
+    return q.to(torch.bfloat16), cache, table, torch.tensor(seqs, dtype=torch.int32), start
+
+
+def _device(x, dev):
+    """x on the device with the strides it has."""
+    y = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=dev)
+    y.copy_(x)
+    return y
+
+
+def _check(out, lse, q, cache, table, seqs, start, kv_scale, bs):
+    for b in range(len(seqs)):
+        t0, t1, L = int(start[b]), int(start[b + 1]), int(seqs[b])
+        n = t1 - t0
+        if n == 0:
+            continue
+        x = torch.arange(max(L, 0))
+        page = table[b].long()[x // bs]
+        has = page >= 0
+        rows = ref.rows64(cache[page.clamp(min=0), x % bs]) * kv_scale if L > 0 else torch.zeros(0, 576, dtype=torch.float64)
+        rows = torch.where(has[:, None], rows, 0.0)
+        seen = (x <= (L - n + torch.arange(n))[:, None]) & has
+        qs = q[t0:t1].double().transpose(0, 1)
+        r = ref.softmax_product(qs, rows[None], rows[None, :, :512], seen, SM)
+        # weights in f16, the largest of a row 2^9 at least: a subnormal one loses 2^-25; values in f16 too (Row656: half a
+        # step for the scale and half for the product), below their normal range 2^-39 of the largest magnitude
+        top = float(rows.abs().max()) if L > 0 else 0.0
+        half = ref.HALF[torch.float16] * (1 if cache.shape[2] == 576 else 3)
+        floor = L * 2.0 ** -34 * top + 2.0 ** -38 * top
+        ref.check(out[t0:t1].transpose(0, 1), lse[t0:t1].transpose(0, 1), r, 576, max(L, 1), torch.bfloat16, half, floor, f"request {b}: {n} of {L}")
+
+
+def _run(dev, case, bs, kv_scale=1.0, **kw):
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, seqs, start = case
+    out, lse = kernels.attend_chunk(q.to(dev), _device(cache, dev), table.to(dev), seqs.to(dev), start.to(dev), SM, kv_scale, **kw)
+    torch.cuda.synchronize()
+    _check(out.cpu(), lse.cpu(), q, cache, table, seqs, start, kv_scale, bs)
+    return out, lse
+
+
+CASES = [  # rows cached (with the new ones), new tokens, heads, page
+    ([1], [1], 1, 64), ([33], [1], 128, 64), ([5, 64, 700], [1, 1, 1], 16, 64), ([40], [40], 8, 16), ([100, 31, 65], [3, 1, 65], 32, 16),
+    ([300, 3], [70, 2], 5, 48), ([1100], [4], 128, 64), ([129, 200], [129, 7], 1, 7), ([90], [2], 200, 128), ([64, 32, 96], [2, 0, 33], 40, 1),
+    ([2300, 600], [1, 1], 128, 64), ([520], [130], 64, 64),
+]
+
+
+@pytest.mark.parametrize("seqs,lens,H,bs", CASES)
+@pytest.mark.parametrize("row", [656, 576])
+def test_against_64_bits(dev, seqs, lens, H, bs, row):
+    _run(dev, _case(seqs, lens, H, row, bs, H + bs), bs, 1.0 if row == 656 else 0.25)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("split", [1, 2, 3, 7, 40])
+def test_splits(dev, row, split):
+    """Splits without positions among them (40 of 1000 rows, of 31 and of none)."""
+    case = _case([1000, 31, 640, 0], [1, 2, 33, 0], 16, row, 64, split)
+    _run(dev, case, 64, 0.5, split=split, max_seq_len=1000)
+
+
+def test_result_does_not_depend_on_max_seq_len(dev):
+    """Rows beyond a max_seq_len that is too small are still seen (the last split takes the rest)."""
+    case = _case([1500, 900], [2, 1], 32, 656, 64, 3)
+    _run(dev, case, 64, split=4, max_seq_len=256)
+    _run(dev, case, 64, max_seq_len=1)
+    _run(dev, case, 64)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+def test_pages_that_are_not_there(dev, row):
+    """Negative table entries: their positions are not seen; a request without any page gets 0 and -inf."""
+    case = _case([300, 64, 200, 10], [2, 1, 150, 1], 16, row, 16, 8, missing=[(0, 0), (0, 7), (0, 18), (1, 0), (1, 1), (1, 2), (1, 3), (2, 5), (3, 0)])
+    out, lse = _run(dev, case, 16)
+    assert bool((out[2] == 0).all()) and bool((lse[2] == -torch.inf).all()) and bool((lse[-1] == -torch.inf).all())
+    _run(dev, case, 16, split=5, max_seq_len=300)
+
+
+def test_more_new_tokens_than_rows(dev):
+    """Tokens before the first cached row see nothing; lengths of zero and below too."""
+    case = _case([5, 40, 0], [9, 41, 2], 4, 656, 16, 5)
+    out, lse = _run(dev, case, 16)
+    assert bool((lse[:4] == -torch.inf).all()) and bool((out[:4] == 0).all())
+    q, cache, table, seqs, start = case
+    _run(dev, (q, cache, table, torch.tensor([5, 40, -3], dtype=torch.int32), start), 16)
+
+
+def test_padded_block_stride_and_strided_query(dev):
+    """Blocks with rows between them; queries and outputs inside wider tensors; tokens of no request stay as they were."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, seqs, start = _case([200, 77], [40, 3], 12, 656, 16, 6, gap=2)
+    T, H = q.shape[:2]
+    wide = torch.full((T + 7, H + 1, 584), float("nan"), dtype=torch.bfloat16, device=dev)
+    wide[2:2 + T, :H, 8:] = q.to(dev)
+    for split in (1, 3):
+        out = torch.full((T + 7, H, 520), 7.0, dtype=torch.bfloat16, device=dev)
+        lse = torch.full((T + 7, H), 7.0, device=dev)
+        kernels.attend_chunk(wide[:, :H, 8:], _device(cache, dev), table.to(dev), seqs.to(dev), (start + 2).to(dev), SM, out=out[..., 8:],
+                             lse=lse, split=split)
+        torch.cuda.synchronize()
+        o, z = out.cpu(), lse.cpu()
+        _check(o[2:2 + T, :, 8:], z[2:2 + T], q, cache, table, seqs, start, 1.0, 16)
+        for x in (o[:2], o[2 + T:], o[..., :8], z[:2], z[2 + T:]):
+            assert bool((x == 7.0).all())
+
+
+@pytest.mark.parametrize("spread", [3.0, 8.0])
+def test_scales_far_apart(dev, spread):
+    """Latents of very different sizes in one context (scale ratios up to e^40): bounded by the largest."""
+    _run(dev, _case([400, 90], [3, 40], 16, 656, 16, 12, spread=spread), 16)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+def test_no_numbers_in_rows_behind_a_token(dev, row):
+    """A chunk's row that is no number reaches the tokens at and behind it only."""
+    q, cache, table, seqs, start = _case([150], [100], 4, row, 16, 2)
+    at = 120                                                   # position of the chunk's token 70
+    page, off = int(table[0, at // 16]), at % 16
+    before = cache[page, off].clone()
+    cache[page, off, 300] = 0x7F                               # a NaN code, dim 300
+    from arcagi2_flashnext_dots3_amd import kernels
+    out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM)
+    torch.cuda.synchronize()
+    assert bool(out[:70].isfinite().all()) and bool(lse[:70].isfinite().all())
+    assert bool(out[70:, :, 300].isnan().all())
+    cache[page, off] = before
+    _check(out[:70].cpu(), lse[:70].cpu(), q[:70], cache, table, torch.tensor([at]), torch.tensor([0, 70]), 1.0, 16)
+    if row == 656:                                             # a scale that is infinite
+        cache[page, off, 516:520] = torch.tensor([float("inf")]).view(torch.uint8)
+        out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM)
+        torch.cuda.synchronize()
+        cache[page, off] = before
+        _check(out[:70].cpu(), lse[:70].cpu(), q[:70], cache, table, torch.tensor([at]), torch.tensor([0, 70]), 1.0, 16)
+
+
+def test_same_as_attend_over_the_list(dev):
+    """The dense result is attend's over the list of all rows, to both kernels' roundings."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, seqs, start = _case([600], [1], 128, 656, 64, 21)
+    c = cache.to(dev)
+    out, lse = kernels.attend_chunk(q.to(dev), c, table.to(dev), seqs.to(dev), start.to(dev), SM)
+    x = torch.arange(600)
+    idx = (table[0].long()[x // 64] * 64 + x % 64).to(torch.int32)[None].to(dev)
+    o2, z2 = kernels.attend(q.to(dev), c.view(-1, 656), idx, SM)
+    torch.cuda.synchronize()
+    assert float((lse - z2).abs().max()) <= 2e-5
+    assert float((out.float() - o2.float()).abs().max()) <= 2.0 ** -7 * float(o2.float().abs().max())
+
+
+def test_long_cache_passes_32_bits(dev):
+    """Rows whose byte offsets pass 2^32: a view of a large allocation, its last pages used."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, seqs, start = _case([130], [2], 16, 656, 64, 30, spare=0)
+    blocks = (1 << 33) // (64 * 656) + 8
+    big = torch.empty(blocks, 64, 656, dtype=torch.uint8, device=dev)
+    far = blocks - cache.shape[0]
+    big[far:] = cache.to(dev)
+    out, lse = kernels.attend_chunk(q.to(dev), big, torch.where(table < 0, table, table + far).to(dev), seqs.to(dev), start.to(dev), SM)
+    torch.cuda.synchronize()
+    _check(out.cpu(), lse.cpu(), q, cache, table, seqs, start, 1.0, 64)
+
+
+def test_streams_and_graphs(dev):
+    """Two captured graphs of split launches beside each other and beside eager calls: workspaces of their own."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    a, b = _case([3000, 2000], [1, 1], 128, 656, 64, 40), _case([2500], [2], 64, 576, 64, 41)
+    dev_args = [[_device(x, dev) if x.dim() == 3 else x.to(dev) for x in c] for c in (a, b)]
+    want = [kernels.attend_chunk(*x, SM, max_seq_len=3000) for x in dev_args]
+    torch.cuda.synchronize()
+    graphs = []
+    for x, (o, z) in zip(dev_args, want):
+        g, out, lse = torch.cuda.CUDAGraph(), torch.zeros_like(o), torch.zeros_like(z)
+        with torch.cuda.graph(g):
+            kernels.attend_chunk(*x, SM, max_seq_len=3000, out=out, lse=lse)
+        graphs.append((g, out, lse))
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        for g, out, lse in graphs:
+            out.zero_()
+            lse.zero_()
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(s):
+            graphs[1][0].replay()
+        e = kernels.attend_chunk(*dev_args[0], SM, max_seq_len=3000)
+        torch.cuda.synchronize()
+        for (g, out, lse), (o, z) in zip(graphs, want):
+            assert torch.equal(out, o) and torch.equal(lse, z)
+        assert torch.equal(e[0], want[0][0])
