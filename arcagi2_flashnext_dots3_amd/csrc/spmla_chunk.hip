@@ -10,7 +10,7 @@
 // number of heads, a cached row is copied once for 64 query rows, and a decode step of 16 heads fills 16 of them.
 // 4 waves, tiles of 32 positions, a ring of three in LDS filled by direct copies; two workgroups a compute unit:
 //   * QK: wave 2 i + d multiplies half d of the dims (two scale groups, half of the rope) of query rows 32 i .. 32 i + 31:
-//     S^T partials in bf16 MFMA 32x32x16, codes converted exactly, so a code is converted by two waves and the query takes
+//     S^T partials in bf16 MFMA 16x16x32, codes converted exactly, so a code is converted by two waves and the query takes
 //     72 registers. (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
 //     the summed magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32
 //     scales, then the rope. The two waves exchange half of their partials through LDS: each ends with 16 query rows;
@@ -32,7 +32,7 @@ namespace chunk {
 
 constexpr int MR = 64;                // query rows per workgroup
 constexpr int TR = 32;                // positions per tile
-constexpr int IDS = 512;              // positions whose rows are looked up at a time
+constexpr int IDS = 256;              // positions whose rows are looked up at a time
 constexpr int NRING = 3;
 constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;
 
@@ -59,13 +59,13 @@ struct Lds {
   static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
   static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
   static constexpr int TILE = CODE + RP + SC;
-  static constexpr int X = NRING * TILE;                   // exchanged partials [wave][2][64 lanes][16]
+  static constexpr int X = NRING * TILE;                   // exchanged partials [wave][16 positions][64 lanes][16]
   static constexpr int P = X + 4 * 2048;                   // [64 query rows][32 positions] f16
   static constexpr int FAC = P + MR * TR * 2;              // rescale factors [64]
   static constexpr int FLAG = FAC + MR * 4;                // a wave's factors are not all 1
   static constexpr int SCH = FLAG + 16;                    // a wave's scales in f16, [4][32]
-  static constexpr int ID = SCH + 4 * TR * 2;              // rows of two times IDS positions
-  static constexpr int OK = ID + 2 * IDS * 4;              // which of a tile's positions have rows, a bit each
+  static constexpr int ID = (SCH + 4 * TR * 2 + 7) & ~7;   // addresses of the rows of two times IDS positions
+  static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
   static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
   static_assert(2 * TOTAL <= 160 * 1024, "two workgroups a compute unit");
 };
@@ -164,72 +164,72 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   }
   const int* btrow = p.table + (long long)b * p.t_st;
 
-  // ---- rows of IDS positions: looked up (x beyond ke: none), then written with a bit per position
-  auto look = [&](int half, int (&x)[2]) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int at = half * IDS + tid + 256 * k, pos = kb + at;
-      int row = -1;
-      if (pos < ke) {
-        const int page = btrow[pos / p.bs];
-        const long long y = (long long)page * p.stride + pos % p.bs;
-        row = page >= 0 && y < p.rows ? (int)y : -1;
-      }
-      x[k] = row;
-    }
+  // ---- rows of IDS positions: looked up (x beyond ke: none), then their addresses written with a bit per position
+  auto look = [&](int half) -> int {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int pos = kb + half * IDS + tid;
+    if (pos >= ke) return -1;
+    const int page = btrow[pos / p.bs];
+    const long long y = (long long)page * p.stride + pos % p.bs;
+    return page >= 0 && y < p.rows ? (int)y : -1;
   };
-  auto note = [&](int half, const int (&x)[2]) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int at = (half & 1) * IDS + tid + 256 * k;
-      ((SPMLA_LDS int*)(lds + L::ID))[at] = x[k];
-      const uint64_t has = __ballot(x[k] >= 0);
-      if (l32 == 0) ((SPMLA_LDS uint32_t*)(lds + L::OK))[at >> 5] = (uint32_t)(has >> (lane & 32));
-    }
+  auto note = [&](int half, int row) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31;
+    const int at = (half & 1) * IDS + tid;
+    const uint64_t a = (uint64_t)(uintptr_t)p.cache + (uint64_t)(uint32_t)row * RB;
+    ((SPMLA_LDS uint64_t*)(lds + L::ID))[at] = row >= 0 ? a : (uint64_t)(uintptr_t)zero_row;
+    const uint64_t has = __ballot(row >= 0);
+    if (l32 == 0) ((SPMLA_LDS uint32_t*)(lds + L::OK))[at >> 5] = (uint32_t)(has >> (lane & 32));
   };
-  int ids[2];
-  look(0, ids);
+  int found = look(0);
 
-  // ---- query operands: rows 32 (w / 2) + l32, half dh of the dims (chunk 2 i + hh of 16 dims serves MFMAs 2 i and 2 i + 1)
+  // ---- query operands [chunk pair or rope][half chunk][query rows 16 i ..] of rows 32 (w / 2) .. and half dh of the dims: B
+  // operands of 16x16x32, lane quarter qt the dims 64 n + 16 qt + 8 e .. + 7 (one 16-byte read of codes serves both e)
   const int dh = w & 1, qb = 32 * (w >> 1);
-  bf16x8 qf[18];
-  {
-    const long long r = r0 + (qb + l32 < live ? qb + l32 : live - 1);
+  bf16x8 qf[4][2][2], qpe[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const long long r = r0 + (qb + 16 * i + l16 < live ? qb + 16 * i + l16 : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
     const uint32_t turn = p.flip ? 0x80008000u : 0u;
 #pragma unroll
-    for (int i = 0; i < 18; ++i) {
-      const int at = i < 16 ? 256 * dh + 16 * (i & ~1) + 16 * hh + 8 * (i & 1)
-                   : R5     ? D_LAT + 32 * dh + 16 * hh + 8 * (i & 1)
-                            : D_LAT + 32 * dh + 16 * (i & 1) + 8 * hh;
-      qf[i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + at) ^ turn);
-    }
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[n][e][i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + 256 * dh + 64 * n + 16 * qt + 8 * e) ^ turn);
+    qpe[i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + D_LAT + 32 * dh + 8 * qt) ^ turn);
   }
   const int qr = 16 * w + l16;                            // the query row whose softmax this lane shares
-  const int limit = limit_of(qr < live ? qr : live - 1);
-  note(0, ids);
+  note(0, found);
   if (tid < 4) ((SPMLA_LDS int*)(lds + L::FLAG))[tid] = 0;
   lds_barrier();
 
   // ---- copies of a tile: wave w the codes of scale group w (copy i: rows 8 i + lane / 8, the chunk whose place is
   // lane % 8), a share of the rope and of the scales. COPIES instructions a wave whatever the tile.
   constexpr int COPIES = R5 ? 5 : 6;
-  auto source = [&](int row, int off) -> const void* {
-    const uint8_t* a = p.cache + (uint64_t)(uint32_t)row * RB;
-    return (row >= 0 ? a : (const uint8_t*)zero_row) + off;
+  // the lane id, opaque in every step: LDS places made of it are formed again, not kept (spilled, a tile's wait for one would
+  // wait for all copies)
+  auto here = [&]() -> int {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
   };
   auto issue = [&](int j, int slot) {
-    SPMLA_LDS int* id = (SPMLA_LDS int*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
+    const int lane = here(), l32 = lane & 31, hh = lane >> 5;
+    SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
     SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
     const int r = lane >> 3, place = (lane & 7) ^ swz(r);
+    auto copy = [&](int row, uint32_t off, SPMLA_LDS uint8_t* to) { dma16((const void*)(id[row] + off), to); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dma16(source(id[8 * i + r], 128 * w + 16 * (place ^ ((i & 1) << 1))), d + w * 4096 + i * 1024);
+    for (int i = 0; i < 4; ++i) copy(8 * i + r, 128 * w + 16 * (place ^ ((i & 1) << 1)), d + w * 4096 + i * 1024);
     if constexpr (R5) {                                   // 16 rows of 64 bytes a copy; waves 2 and 3 repeat those of 0 and 1
       const int rr = 16 * (w & 1) + (lane >> 2);
-      dma16(source(id[rr], D_LAT + 16 * ((lane & 3) ^ ((rr >> 2) & 3))), d + L::CODE + (w & 1) * 1024);
+      copy(rr, D_LAT + 16 * ((lane & 3) ^ ((rr >> 2) & 3)), d + L::CODE + (w & 1) * 1024);
     } else {
-      dma16(source(id[8 * w + r], ROPE_OFF + 16 * (place ^ ((w & 1) << 1))), d + L::CODE + w * 1024);
-      dma4(source(id[l32], SC_OFF + 4 * (2 * (w & 1) + hh)), d + L::CODE + L::RP + (w & 1) * 256);
+      copy(8 * w + r, ROPE_OFF + 16 * (place ^ ((w & 1) << 1)), d + L::CODE + w * 1024);
+      dma4((const void*)(id[l32] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + hh))), d + L::CODE + L::RP + (w & 1) * 256);
     }
   };
 
@@ -243,75 +243,85 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   int ex2 = -126;                                         // Row656: V' and O carry 2^-ex2
   int odd_from = 0x7fffffff;
 
-  // partial scores of a tile over this wave's dims: the 16 query rows that the other wave joins go to LDS, the own stay
+  // partial scores of a tile over this wave's dims: S^T blocks of 16 positions x 16 query rows; those of the rows that the
+  // other wave joins go to LDS, the own stay. Reads run two or three units (a read, 8 conversions, 4 MFMAs) ahead.
   f32x4 part[2];
   auto partials = [&](int slot) {
+    const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
-    SPMLA_LDS uint8_t* at = d + (2 * dh) * 4096 + l32 * 128;
-    const int x = swz(l32);
-    f32x16 s = {};
+    SPMLA_LDS uint8_t* at = d + (2 * dh) * 4096 + l16 * 128;
+    const int x = swz(l16);
+    auto kread = [&](int n) -> i32x4 {                    // unit n: positions 16 (n / 4) .., group 2 dh + n / 2 % 2, chunks 4 (n % 2) ..
+      return *(SPMLA_LDS i32x4*)(at + (n >> 2) * 2048 + ((n >> 1) & 1) * 4096 + 16 * ((4 * (n & 1) + qt) ^ x));
+    };
+    auto rread = [&](int u) -> i32x4 {                    // rope of positions 16 u ..: Row576 8 codes, Row656 8 bf16
+      if constexpr (R5) {
+        const i32x2 y = *(SPMLA_LDS i32x2*)(d + L::CODE + u * 1024 + l16 * 64 + 16 * ((2 * dh + (qt >> 1)) ^ ((l16 >> 2) & 3)) + 8 * (qt & 1));
+        return i32x4{y[0], y[1], 0, 0};
+      } else {
+        return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + 16 * ((4 * dh + qt) ^ x));
+      }
+    };
+    constexpr int AHEAD = R5 ? 3 : 2;
+    i32x4 k[AHEAD];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      f32x16 acc = {};
+    for (int n = 0; n < AHEAD; ++n) k[n] = kread(n);
+    i32x4 kr;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const i32x4 k = *(SPMLA_LDS i32x4*)(at + g * 4096 + 16 * ((2 * i + hh) ^ x));
+    for (int u = 0; u < 2; ++u) {
+      f32x4 s[2] = {};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bf16x8 y = codes8(k[2 * e], k[2 * e + 1]);
-          if constexpr (R5) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, qf[8 * g + 2 * i + e], s, 0, 0, 0);
-          else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, qf[8 * g + 2 * i + e], acc, 0, 0, 0);
+      for (int g = 0; g < 2; ++g) {
+        f32x4 acc[2] = {}, sc = {};
+        if constexpr (!R5) sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (2 * dh + g) * 128 + u * 64 + qt * 16);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int n = 4 * u + 2 * g + c;
+          const bf16x8 y0 = codes8(k[n % AHEAD][0], k[n % AHEAD][1]), y1 = codes8(k[n % AHEAD][2], k[n % AHEAD][3]);
+          if (n + AHEAD < 8) k[n % AHEAD] = kread(n + AHEAD);
+          if (n == 4 * u + 2) kr = rread(u);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            f32x4& to = R5 ? s[i] : acc[i];
+            to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y0, qf[2 * g + c][0][i], to, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            f32x4& to = R5 ? s[i] : acc[i];
+            to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y1, qf[2 * g + c][1][i], to, 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (!R5)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[i][r] = __builtin_fmaf(acc[i][r], sc[r], s[i][r]);
       }
-      if constexpr (!R5) {
+      const bf16x8 y = R5 ? codes8(kr[0], kr[1]) : __builtin_bit_cast(bf16x8, kr);
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const f32x4 sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (2 * dh + g) * 128 + 32 * a + 16 * hh);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[4 * a + r] = g == 0 ? acc[4 * a + r] * sc[r] : __builtin_fmaf(acc[4 * a + r], sc[r], s[4 * a + r]);
-        }
-      }
-    }
-    if constexpr (R5) {
-      const i32x4 k = *(SPMLA_LDS i32x4*)(d + L::CODE + l32 * 64 + 16 * ((2 * dh + hh) ^ ((l32 >> 2) & 3)));
-#pragma unroll
-      for (int e = 0; e < 2; ++e) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes8(k[2 * e], k[2 * e + 1]), qf[16 + e], s, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bf16x8 y = __builtin_bit_cast(bf16x8, *(SPMLA_LDS u32x4*)(d + L::CODE + l32 * 128 + 16 * ((4 * dh + 2 * e + hh) ^ x)));
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y, qf[16 + e], s, 0, 0, 0);
-      }
-    }
-    // lanes 16 .. 31 and 48 .. 63 of value r change places with lanes 0 .. 15 and 32 .. 47 of value r + 8: then query rows
-    // 0 .. 15 lie in the first, 16 .. 31 in the second, 8 positions a lane
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      f32x4 send;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const auto y = __builtin_amdgcn_permlane16_swap(f2u(s[4 * a + r]), f2u(s[8 + 4 * a + r]), false, false);
-        const uint32_t lo = y[0], hi = y[1];
-        part[a][r] = u2f(dh ? hi : lo);
-        send[r] = u2f(dh ? lo : hi);
-      }
-      *(SPMLA_LDS f32x4*)(lds + L::X + w * 2048 + a * 1024 + lane * 16) = send;
+      for (int i = 0; i < 2; ++i) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, qpe[i], s[i], 0, 0, 0);
+      part[u] = dh ? s[1] : s[0];
+      *(SPMLA_LDS f32x4*)(lds + L::X + w * 2048 + u * 1024 + lane * 16) = dh ? s[0] : s[1];
     }
   };
 
-  // softmax of tile j, its P and factors: value 4 a + r of a lane is position 16 (qt % 2) + 8 a + 4 (qt / 2) + r
+  // softmax of tile j, its P and factors: value 4 u + r of a lane is position 16 u + 4 qt + r
   auto softmax = [&](int j) {
+    const int lane = here(), l16 = lane & 15, qt = lane >> 4, qr = 16 * w + l16;
     f32x4 s[2];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) s[a] = part[a] + *(SPMLA_LDS f32x4*)(lds + L::X + (w ^ 1) * 2048 + a * 1024 + lane * 16);
+    for (int u = 0; u < 2; ++u) s[u] = part[u] + *(SPMLA_LDS f32x4*)(lds + L::X + (w ^ 1) * 2048 + u * 1024 + lane * 16);
     const uint32_t has = __builtin_amdgcn_readfirstlane(((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
     const int k0 = kb + j * TR;
-    if (has != 0xffffffffu || k0 + TR > least) {
+    if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
+      asm volatile("" : "+v"(s[0]), "+v"(s[1]));           // (a branch, not 40 selects in every tile)
+      const int limit = limit_of(qr < live ? qr : live - 1);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int x = 16 * (qt & 1) + 8 * u + 4 * (qt >> 1) + r;
+          const int x = 16 * u + 4 * qt + r;
           s[u][r] = (has >> x & 1) && k0 + x < limit ? s[u][r] : -__builtin_inff();
         }
     }
@@ -347,24 +357,27 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) l += s[u][r];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {                          // half of chunk 2 (qt % 2) + u
-      const int ch = (2 * (qt & 1) + u) ^ ((qr >> 2) & 3);
-      *(SPMLA_LDS i32x2*)(lds + L::P + qr * 64 + 16 * ch + 8 * (qt >> 1)) = i32x2{(int)pk_f16(s[u][0], s[u][1]), (int)pk_f16(s[u][2], s[u][3])};
+    for (int u = 0; u < 2; ++u) {                          // half of chunk 2 u + qt / 2
+      const int ch = (2 * u + (qt >> 1)) ^ ((qr >> 2) & 3);
+      *(SPMLA_LDS i32x2*)(lds + L::P + qr * 64 + 16 * ch + 8 * (qt & 1)) = i32x2{(int)pk_f16(s[u][0], s[u][1]), (int)pk_f16(s[u][2], s[u][3])};
     }
   };
 
-  const int vrow = 8 * hh + ((lane & 15) >> 1);           // V^T: row of the transposing read, its 16-byte chunk's parity
   // O += V^T P^T of tile j
   auto values = [&](int j, int slot) {
+    const int lane = here(), l32 = lane & 31, hh = lane >> 5;
+    const int vrow = 8 * hh + ((lane & 15) >> 1);         // V^T: row of the transposing read
     SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
+    const int k0 = kb + j * TR;
     const i32x4 fl = *(SPMLA_LDS i32x4*)(lds + L::FLAG);
     const int any = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
     float sc = 0.f;
     if constexpr (!R5) {
       sc = *(SPMLA_LDS float*)(d + L::CODE + L::RP + w * 128 + l32 * 4);
       const float fin = fabsf(sc) < __builtin_inff() ? fabsf(sc) : 0.f;
-      if (__any(fin * u2f((uint32_t)(127 - ex2) << 23) > 64.f)) {           // a larger scale than any before: e follows
+      if (__builtin_expect(__any(fin * u2f((uint32_t)(127 - ex2) << 23) > 64.f), 0)) {      // a larger scale than any before: e follows
         float top = fin;
+        asm volatile("" : "+v"(top));
 #pragma unroll
         for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
         int e = (int)(f2u(top) >> 23) - 127 - 5;                            // scale * 2^-e < 64
@@ -378,7 +391,8 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) O[x][i][r] *= a;
       }
-      const _Float16 h = (_Float16)(sc * u2f((uint32_t)(127 - ex2) << 23));
+      const bool masked = k0 + TR > least && least < most && !(fabsf(sc) < __builtin_inff());
+      const _Float16 h = masked ? (_Float16)0.f : (_Float16)(sc * u2f((uint32_t)(127 - ex2) << 23));
       ((SPMLA_LDS _Float16*)(lds + L::SCH))[w * TR + l32] = h;
     }
     if (any) {
@@ -395,71 +409,81 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
           for (int r = 0; r < 16; ++r) O[x][i][r] *= a;
       }
     }
-    const int k0 = kb + j * TR;
-    const bool cut = k0 + TR > least && least < most;
-    uint32_t odd = 0;
-    f16x8 pb[2][2];
+    if (__builtin_expect(k0 + TR > least && least < most, 0)) {
+      // the mask cuts this tile: codes that are no numbers become 0 in the wave's own group, which only it reads now
+      uint32_t odd = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 4; ++i) {
+        SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(d + w * 4096 + i * 1024 + lane * 16);
+        u32x4 y = *at;
+        uint32_t bad = 0;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const int row = 32 * i + l32;
-        pb[i][ks] = __builtin_bit_cast(f16x8, *(SPMLA_LDS u32x4*)(lds + L::P + row * 64 + 16 * ((2 * ks + hh) ^ ((row >> 2) & 3))));
-      }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4 scp = {};
-      if constexpr (!R5) scp = *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 16 * ks + 8 * hh) * 2);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int ch = 2 * x + ((lane >> 4) & 1);
-        const i32x2 t = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (SPMLA_LDS i32x2*)(d + w * 4096 + (16 * ks + vrow) * 128 + 16 * (ch ^ swz(vrow)) + 8 * (lane & 1)));
-        u32x4 v = {lo_f16x2((uint32_t)t[0]), hi_f16x2((uint32_t)t[0]), lo_f16x2((uint32_t)t[1]), hi_f16x2((uint32_t)t[1])};
-        if constexpr (!R5)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = mul_f16x2(v[e], scp[e]);
-        if (cut) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t keep = ((v[e] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((v[e] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
-            odd |= ~keep;
-            v[e] &= keep;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t nan = ((y[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          bad |= nan;
+          y[e] &= ~((nan >> 7) * 255u);
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (32 * i < live) O[x][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pb[i][ks], O[x][i], 0, 0, 0);
+        odd |= bad;
+        if (bad) *at = y;
       }
+      if constexpr (!R5) odd |= fabsf(sc) < __builtin_inff() ? 0u : 1u;     // (its f16 form is 0)
+      if (__any(odd != 0)) odd_from = odd_from < k0 ? odd_from : k0;
     }
-    if (cut && __any(odd != 0)) odd_from = odd_from < k0 ? odd_from : k0;
+    const int vo = w * 4096 + vrow * 128 + 8 * (lane & 1), vs = swz(vrow) ^ ((lane >> 4) & 1);
+    auto vread = [&](int n) -> i32x2 {                    // unit n: positions 16 (n / 4) .., dims 32 (n % 4) ..
+      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((SPMLA_LDS i32x2*)(d + vo + 16 * (vs ^ (2 * (n & 3))) + (n >> 2) * 2048));
+    };
+    auto pread = [&](int ks, int i) -> f16x8 {
+      return __builtin_bit_cast(f16x8, *(SPMLA_LDS u32x4*)(lds + L::P + (32 * i + l32) * 64 + 16 * ((2 * ks + hh) ^ ((l32 >> 2) & 3))));
+    };
+    i32x2 t[4] = {vread(0), vread(1), vread(2), vread(3)};
+    f16x8 pb[2] = {pread(0, 0), pread(0, 1)};
+    u32x4 scp = {};
+    if constexpr (!R5) scp = *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 8 * hh) * 2);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const i32x2 c = t[n % 4];
+      u32x4 v = {lo_f16x2((uint32_t)c[0]), hi_f16x2((uint32_t)c[0]), lo_f16x2((uint32_t)c[1]), hi_f16x2((uint32_t)c[1])};
+      if (n + 4 < 8) t[n % 4] = vread(n + 4);
+      if constexpr (!R5)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = mul_f16x2(v[e], scp[e]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        O[n & 3][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pb[i], O[n & 3][i], 0, 0, 0);
+      if (n == 3) {
+        pb[0] = pread(1, 0);
+        pb[1] = pread(1, 1);
+        if constexpr (!R5) scp = *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 16 + 8 * hh) * 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
-  const bool mine = 16 * w < live, pair = qb < live;      // this wave has query rows, it or its partner has
   if (nt > 0) {
     issue(0, 0);
     if (nt > 1) issue(1, 1);
     if (nt > 2) issue(2, 2);
     if (nt > 2) wait_vm<2 * COPIES>(); else if (nt > 1) wait_vm<COPIES>(); else wait_vm<0>();
     lds_barrier();
-    if (pair) partials(0);
+    partials(0);
     lds_barrier();
-    if (mine) softmax(0);
+    softmax(0);
     if (nt > 2) wait_vm<COPIES>(); else wait_vm<0>();
     lds_barrier();
   }
   int slot = 0;                                           // of tile j; tiles j + 1 and j + 2 follow
   for (int j = 0; j < nt; ++j) {
     const int s1 = slot == 2 ? 0 : slot + 1;
-    // rows of the next IDS positions: looked up 8 tiles before a half ends, written 5 before
+    // rows of the next IDS positions: looked up 7 tiles before a half ends, written 4 before, copied from 3 before
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
-    if (in == IDS / TR - 8 && next * (IDS / TR) < nt) look(next, ids);
-    if (in == IDS / TR - 5 && next * (IDS / TR) < nt) note(next, ids);
+    if (in == IDS / TR - 7 && next * (IDS / TR) < nt) found = look(next);
+    if (in == IDS / TR - 4 && next * (IDS / TR) < nt) note(next, found);
+    partials(s1);                                         // (behind the last tile: of what lies there, not used)
     values(j, slot);
-    if (j + 1 < nt && pair) partials(s1);
     lds_barrier();                                        // partials are there; tile j and P are done with
     if (j + 3 < nt) issue(j + 3, slot);
-    if (j + 1 < nt && mine) softmax(j + 1);
+    if (j + 1 < nt) softmax(j + 1);
     if (j + 3 < nt) wait_vm<COPIES>(); else wait_vm<0>();
     lds_barrier();                                        // P and tile j + 2 are there
     slot = s1;
