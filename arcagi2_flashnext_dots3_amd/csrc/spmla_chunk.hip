@@ -30,10 +30,9 @@
 namespace spmla {
 namespace chunk {
 
-constexpr int MR = 64;                // query rows per workgroup
+constexpr int HR = 64;                // query rows per half (4 waves)
 constexpr int TR = 32;                // positions per tile
 constexpr int IDS = 256;              // positions whose rows are looked up at a time
-constexpr int NRING = 3;
 constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -53,21 +52,22 @@ struct Params {
   float* opart; float* lpart;                              // [S][T][H][512], [S][T][H]
 };
 
-template <bool R5>
+template <bool R5, int NH>
 struct Lds {
+  static constexpr int RING = NH == 1 ? 3 : 4;
   static constexpr int CODE = 4 * TR * 128;                // codes by scale group, [4][32 rows][128]
   static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
   static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
   static constexpr int TILE = CODE + RP + SC;
-  static constexpr int X = NRING * TILE;                   // exchanged partials [wave][16 positions][64 lanes][16]
-  static constexpr int P = X + 4 * 2048;                   // [64 query rows][32 positions] f16
-  static constexpr int FAC = P + MR * TR * 2;              // rescale factors [64]
-  static constexpr int FLAG = FAC + MR * 4;                // a wave's factors are not all 1
-  static constexpr int SCH = FLAG + 16;                    // a wave's scales in f16, [4][32]
-  static constexpr int ID = (SCH + 4 * TR * 2 + 7) & ~7;   // addresses of the rows of two times IDS positions
+  static constexpr int X = RING * TILE;                    // exchanged partials [wave][16 positions][64 lanes][16]
+  static constexpr int P = X + 4 * NH * 2048;              // [64 NH query rows][32 positions] f16
+  static constexpr int FAC = P + NH * HR * TR * 2;         // rescale factors [64 NH]
+  static constexpr int FLAG = FAC + NH * HR * 4;           // a wave's factors are not all 1
+  static constexpr int SCH = FLAG + 16 * NH;               // a wave's scales in f16, [4 NH][32]
+  static constexpr int ID = SCH + 4 * NH * TR * 2;         // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
   static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
-  static_assert(2 * TOTAL <= 160 * 1024, "two workgroups a compute unit");
+  static_assert(TOTAL <= (NH == 1 ? 80 : 160) * 1024 && ID % 8 == 0, "two workgroups of 4 waves a compute unit, or one of 8");
 };
 
 __device__ __attribute__((aligned(16))) uint8_t zero_row[ROW656];
@@ -117,13 +117,14 @@ __device__ inline bf16x8 codes8(int a, int b) {
 // place of chunk c (16 bytes) in a row of 128 bytes: c ^ swz(row); 16 rows' chunks c lie in all 64 banks
 __device__ inline int swz(int row) { return ((row & 2) << 1) | ((row & 4) >> 2) | ((row & 8) >> 2); }
 
-template <bool R5>
-__global__ void __launch_bounds__(256, 2) kernel(Params p) {
-  using L = Lds<R5>;
-  constexpr int RB = R5 ? ROW576 : ROW656;
+template <bool R5, int NH>
+__global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
+  using L = Lds<R5, NH>;
+  constexpr int RB = R5 ? ROW576 : ROW656, MR = HR * NH;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = NH == 1 ? 0 : w >> 2, wl = w & 3;      // this wave's half and its number there
   const int l16 = lane & 15, l32 = lane & 31, qt = lane >> 4, hh = lane >> 5;
 
   // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / 64 + b.
@@ -165,20 +166,21 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   const int* btrow = p.table + (long long)b * p.t_st;
 
   // ---- rows of IDS positions: looked up (x beyond ke: none), then their addresses written with a bit per position
-  auto look = [&](int half) -> int {
+  auto look = [&](int part) -> int {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
-    const int pos = kb + half * IDS + tid;
-    if (pos >= ke) return -1;
+    const int pos = kb + part * IDS + tid;
+    if (pos >= ke || (NH > 1 && tid >= IDS)) return -1;
     const int page = btrow[pos / p.bs];
     const long long y = (long long)page * p.stride + pos % p.bs;
     return page >= 0 && y < p.rows ? (int)y : -1;
   };
-  auto note = [&](int half, int row) {
+  auto note = [&](int part, int row) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, l32 = lane & 31;
-    const int at = (half & 1) * IDS + tid;
+    if (NH > 1 && tid >= IDS) return;
+    const int at = (part & 1) * IDS + tid;
     const uint64_t a = (uint64_t)(uintptr_t)p.cache + (uint64_t)(uint32_t)row * RB;
     ((SPMLA_LDS uint64_t*)(lds + L::ID))[at] = row >= 0 ? a : (uint64_t)(uintptr_t)zero_row;
     const uint64_t has = __ballot(row >= 0);
@@ -186,13 +188,14 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   };
   int found = look(0);
 
-  // ---- query operands [chunk pair or rope][half chunk][query rows 16 i ..] of rows 32 (w / 2) .. and half dh of the dims: B
+  // ---- query operands [chunk pair or rope][half chunk][own or partner's 16 query rows] of rows 32 (w / 2) .. and half dh of the dims: B
   // operands of 16x16x32, lane quarter qt the dims 64 n + 16 qt + 8 e .. + 7 (one 16-byte read of codes serves both e)
-  const int dh = w & 1, qb = 32 * (w >> 1);
+  const int dh = wl & 1, qb = HR * half + 32 * (wl >> 1);
   bf16x8 qf[4][2][2], qpe[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const long long r = r0 + (qb + 16 * i + l16 < live ? qb + 16 * i + l16 : live - 1);
+    const int row = qb + 16 * (i ^ dh) + l16;             // (i = 0: the rows that this wave joins)
+    const long long r = r0 + (row < live ? row : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
     const uint32_t turn = p.flip ? 0x80008000u : 0u;
 #pragma unroll
@@ -201,14 +204,15 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
       for (int e = 0; e < 2; ++e) qf[n][e][i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + 256 * dh + 64 * n + 16 * qt + 8 * e) ^ turn);
     qpe[i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + D_LAT + 32 * dh + 8 * qt) ^ turn);
   }
-  const int qr = 16 * w + l16;                            // the query row whose softmax this lane shares
+  const int qr = HR * half + 16 * wl + l16;               // the query row whose softmax this lane shares
   note(0, found);
-  if (tid < 4) ((SPMLA_LDS int*)(lds + L::FLAG))[tid] = 0;
+  if (tid < 4 * NH) ((SPMLA_LDS int*)(lds + L::FLAG))[tid] = 0;
   lds_barrier();
 
-  // ---- copies of a tile: wave w the codes of scale group w (copy i: rows 8 i + lane / 8, the chunk whose place is
-  // lane % 8), a share of the rope and of the scales. COPIES instructions a wave whatever the tile.
-  constexpr int COPIES = R5 ? 5 : 6;
+  // ---- copies of a tile: rows 8 i + lane / 8 of a scale group's codes, the chunk whose place is lane % 8 (4 waves: wave w
+  // all of group w, 8 waves: half of group w % 4), a share of the rope and of the scales (some twice). COPIES instructions a
+  // wave whatever the tile.
+  constexpr int COPIES = (R5 ? 1 : NH == 1 ? 2 : 1) + 4 / NH;
   // the lane id, opaque in every step: LDS places made of it are formed again, not kept (spilled, a tile's wait for one would
   // wait for all copies)
   auto here = [&]() -> int {
@@ -223,13 +227,17 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
     const int r = lane >> 3, place = (lane & 7) ^ swz(r);
     auto copy = [&](int row, uint32_t off, SPMLA_LDS uint8_t* to) { dma16((const void*)(id[row] + off), to); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) copy(8 * i + r, 128 * w + 16 * (place ^ ((i & 1) << 1)), d + w * 4096 + i * 1024);
-    if constexpr (R5) {                                   // 16 rows of 64 bytes a copy; waves 2 and 3 repeat those of 0 and 1
+    for (int n = 0; n < 4 / NH; ++n) {
+      const int i = n + 2 * half;
+      copy(8 * i + r, 128 * wl + 16 * (place ^ ((i & 1) << 1)), d + wl * 4096 + i * 1024);
+    }
+    auto scales = [&]() { dma4((const void*)(id[l32] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + hh))), d + L::CODE + L::RP + (w & 1) * 256); };
+    if constexpr (R5) {                                   // 16 rows of 64 bytes a copy
       const int rr = 16 * (w & 1) + (lane >> 2);
       copy(rr, D_LAT + 16 * ((lane & 3) ^ ((rr >> 2) & 3)), d + L::CODE + (w & 1) * 1024);
     } else {
-      copy(8 * w + r, ROPE_OFF + 16 * (place ^ ((w & 1) << 1)), d + L::CODE + w * 1024);
-      dma4((const void*)(id[l32] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + hh))), d + L::CODE + L::RP + (w & 1) * 256);
+      if (NH == 1 || half == 0) copy(8 * wl + r, ROPE_OFF + 16 * (place ^ ((wl & 1) << 1)), d + L::CODE + wl * 1024);
+      if (NH == 1 || half == 1) scales();
     }
   };
 
@@ -243,72 +251,81 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   int ex2 = -126;                                         // Row656: V' and O carry 2^-ex2
   int odd_from = 0x7fffffff;
 
-  // partial scores of a tile over this wave's dims: S^T blocks of 16 positions x 16 query rows; those of the rows that the
-  // other wave joins go to LDS, the own stay. Reads run two or three units (a read, 8 conversions, 4 MFMAs) ahead.
+  // Partial scores of a tile over this wave's dims: S^T blocks of 16 positions x 16 query rows (block 0: the rows this wave
+  // joins, kept; block 1: its partner's, to LDS). Steps of two products (20: 16 of codes, 4 a block pair of rope at the end of
+  // its positions): the conversions of the next step's operand run under the products of this one, reads two ahead.
   f32x4 part[2];
   auto partials = [&](int slot) {
     const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
     SPMLA_LDS uint8_t* at = d + (2 * dh) * 4096 + l16 * 128;
-    const int x = swz(l16);
+    const int x0 = 16 * (qt ^ swz(l16)), x1 = x0 ^ 64;
     auto kread = [&](int n) -> i32x4 {                    // unit n: positions 16 (n / 4) .., group 2 dh + n / 2 % 2, chunks 4 (n % 2) ..
-      return *(SPMLA_LDS i32x4*)(at + (n >> 2) * 2048 + ((n >> 1) & 1) * 4096 + 16 * ((4 * (n & 1) + qt) ^ x));
+      return *(SPMLA_LDS i32x4*)(at + (n >> 2) * 2048 + ((n >> 1) & 1) * 4096 + ((n & 1) ? x1 : x0));
     };
     auto rread = [&](int u) -> i32x4 {                    // rope of positions 16 u ..: Row576 8 codes, Row656 8 bf16
       if constexpr (R5) {
         const i32x2 y = *(SPMLA_LDS i32x2*)(d + L::CODE + u * 1024 + l16 * 64 + 16 * ((2 * dh + (qt >> 1)) ^ ((l16 >> 2) & 3)) + 8 * (qt & 1));
         return i32x4{y[0], y[1], 0, 0};
       } else {
-        return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + 16 * ((4 * dh + qt) ^ x));
+        return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + 16 * ((4 * dh + qt) ^ swz(l16)));
       }
     };
-    constexpr int AHEAD = R5 ? 3 : 2;
-    i32x4 k[AHEAD];
+    i32x4 k[3] = {kread(0), kread(1), kread(2)}, kr;
+    bf16x8 y[2];
+    y[0] = codes8(k[0][0], k[0][1]);
+    f32x4 s[2] = {}, acc[2] = {}, sc = {};
 #pragma unroll
-    for (int n = 0; n < AHEAD; ++n) k[n] = kread(n);
-    i32x4 kr;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x4 s[2] = {};
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        f32x4 acc[2] = {}, sc = {};
-        if constexpr (!R5) sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (2 * dh + g) * 128 + u * 64 + qt * 16);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int n = 4 * u + 2 * g + c;
-          const bf16x8 y0 = codes8(k[n % AHEAD][0], k[n % AHEAD][1]), y1 = codes8(k[n % AHEAD][2], k[n % AHEAD][3]);
-          if (n + AHEAD < 8) k[n % AHEAD] = kread(n + AHEAD);
-          if (n == 4 * u + 2) kr = rread(u);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            f32x4& to = R5 ? s[i] : acc[i];
-            to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y0, qf[2 * g + c][0][i], to, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            f32x4& to = R5 ? s[i] : acc[i];
-            to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y1, qf[2 * g + c][1][i], to, 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < 18; ++t) {                        // t % 9 < 8: half e of unit 4 u + t % 9 / 2; 8: rope
+      const int u = t / 9, i9 = t % 9, n = 4 * u + i9 / 2;
+      // the next step's operand
+      if (i9 < 8) {
+        if (i9 & 1) {
+          if (n + 3 < 8) k[n % 3] = kread(n + 3);         // (its codes are converted)
+          if (i9 == 7) y[(t + 1) & 1] = R5 ? codes8(kr[0], kr[1]) : __builtin_bit_cast(bf16x8, kr);
+          else y[(t + 1) & 1] = codes8(k[(n + 1) % 3][0], k[(n + 1) % 3][1]);
+        } else {
+          y[(t + 1) & 1] = codes8(k[n % 3][2], k[n % 3][3]);
+          if (i9 == 4) kr = rread(u);
         }
-        if constexpr (!R5)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[i][r] = __builtin_fmaf(acc[i][r], sc[r], s[i][r]);
+      } else if (u == 0) {
+        y[(t + 1) & 1] = codes8(k[4 % 3][0], k[4 % 3][1]);
       }
-      const bf16x8 y = R5 ? codes8(kr[0], kr[1]) : __builtin_bit_cast(bf16x8, kr);
+      if constexpr (!R5)
+        if (i9 == 1 || i9 == 5) sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (2 * dh + i9 / 4) * 128 + u * 64 + qt * 16);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, qpe[i], s[i], 0, 0, 0);
-      part[u] = dh ? s[1] : s[0];
-      *(SPMLA_LDS f32x4*)(lds + L::X + w * 2048 + u * 1024 + lane * 16) = dh ? s[0] : s[1];
+      for (int i = 0; i < 2; ++i) {
+        const bf16x8 q = i9 == 8 ? qpe[i] : qf[(i9 / 2) & 3][i9 & 1][i];
+        f32x4& to = R5 || i9 == 8 ? s[i] : acc[i];
+        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[t & 1], q, to, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {                       // a product, two conversions, ...
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!R5) {
+        if (i9 == 3 || i9 == 7) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[i][r] = i9 == 3 ? acc[i][r] * sc[r] : __builtin_fmaf(acc[i][r], sc[r], s[i][r]);
+            acc[i] = f32x4{};
+          }
+        }
+      }
+      if (i9 == 8) {
+        part[u] = s[0];
+        *(SPMLA_LDS f32x4*)(lds + L::X + w * 2048 + u * 1024 + lane * 16) = s[1];
+        s[0] = s[1] = f32x4{};
+      }
     }
   };
 
   // softmax of tile j, its P and factors: value 4 u + r of a lane is position 16 u + 4 qt + r
   auto softmax = [&](int j) {
-    const int lane = here(), l16 = lane & 15, qt = lane >> 4, qr = 16 * w + l16;
+    const int lane = here(), l16 = lane & 15, qt = lane >> 4, qr = HR * half + 16 * wl + l16;
     f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) s[u] = part[u] + *(SPMLA_LDS f32x4*)(lds + L::X + (w ^ 1) * 2048 + u * 1024 + lane * 16);
@@ -331,14 +348,16 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
     mx = quad_max(mx);
+    float fac = 1.f;
     const bool move = __any(mx * p.c > m * p.c + TAU);
     if (move) {
       const float mn = fmaxf(m, mx), a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.c);
       m = mn;
       l *= a;
       far = __any(fabsf(mn * p.c) > FAR && mn > -__builtin_inff());
-      if (qt == 0) ((SPMLA_LDS float*)(lds + L::FAC))[qr] = a;
+      fac = a;
     }
+    if (qt == 0) ((SPMLA_LDS float*)(lds + L::FAC))[qr] = fac;
     if (lane == 0) ((SPMLA_LDS int*)(lds + L::FLAG))[w] = move;
     const float base = m == -__builtin_inff() ? 0.f : m, ref = UP - base * p.c;
     if (__builtin_expect(far, 0)) {                        // the rounding of m c would count: differences first
@@ -369,11 +388,11 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
     const int vrow = 8 * hh + ((lane & 15) >> 1);         // V^T: row of the transposing read
     SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
     const int k0 = kb + j * TR;
-    const i32x4 fl = *(SPMLA_LDS i32x4*)(lds + L::FLAG);
+    const i32x4 fl = *(SPMLA_LDS i32x4*)(lds + L::FLAG + 16 * half);
     const int any = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
     float sc = 0.f;
     if constexpr (!R5) {
-      sc = *(SPMLA_LDS float*)(d + L::CODE + L::RP + w * 128 + l32 * 4);
+      sc = *(SPMLA_LDS float*)(d + L::CODE + L::RP + wl * 128 + l32 * 4);
       const float fin = fabsf(sc) < __builtin_inff() ? fabsf(sc) : 0.f;
       if (__builtin_expect(__any(fin * u2f((uint32_t)(127 - ex2) << 23) > 64.f), 0)) {      // a larger scale than any before: e follows
         float top = fin;
@@ -395,14 +414,10 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
       const _Float16 h = masked ? (_Float16)0.f : (_Float16)(sc * u2f((uint32_t)(127 - ex2) << 23));
       ((SPMLA_LDS _Float16*)(lds + L::SCH))[w * TR + l32] = h;
     }
-    if (any) {
+    if (__builtin_expect(any, 0)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float a = 1.f;
-        if (fl[2 * i] | fl[2 * i + 1]) {
-          a = ((SPMLA_LDS float*)(lds + L::FAC))[32 * i + l32];
-          a = fl[2 * i + (l32 >> 4)] ? a : 1.f;
-        }
+        const float a = ((SPMLA_LDS float*)(lds + L::FAC))[HR * half + 32 * i + l32];
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -410,11 +425,12 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
       }
     }
     if (__builtin_expect(k0 + TR > least && least < most, 0)) {
-      // the mask cuts this tile: codes that are no numbers become 0 in the wave's own group, which only it reads now
+      // the mask cuts this tile: codes that are no numbers become 0 in the wave's group, whose values alone are read from now on
+      // (8 waves: by the other half's wave of the group as well, whose turn comes later)
       uint32_t odd = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(d + w * 4096 + i * 1024 + lane * 16);
+        SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(d + wl * 4096 + i * 1024 + lane * 16);
         u32x4 y = *at;
         uint32_t bad = 0;
 #pragma unroll
@@ -429,64 +445,86 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
       if constexpr (!R5) odd |= fabsf(sc) < __builtin_inff() ? 0u : 1u;     // (its f16 form is 0)
       if (__any(odd != 0)) odd_from = odd_from < k0 ? odd_from : k0;
     }
-    const int vo = w * 4096 + vrow * 128 + 8 * (lane & 1), vs = swz(vrow) ^ ((lane >> 4) & 1);
+    const int vo = wl * 4096 + vrow * 128 + 8 * (lane & 1), vs = swz(vrow) ^ ((lane >> 4) & 1);
     auto vread = [&](int n) -> i32x2 {                    // unit n: positions 16 (n / 4) .., dims 32 (n % 4) ..
       return __builtin_amdgcn_ds_read_tr8_b64_v2i32((SPMLA_LDS i32x2*)(d + vo + 16 * (vs ^ (2 * (n & 3))) + (n >> 2) * 2048));
     };
     auto pread = [&](int ks, int i) -> f16x8 {
-      return __builtin_bit_cast(f16x8, *(SPMLA_LDS u32x4*)(lds + L::P + (32 * i + l32) * 64 + 16 * ((2 * ks + hh) ^ ((l32 >> 2) & 3))));
+      return __builtin_bit_cast(f16x8, *(SPMLA_LDS u32x4*)(lds + L::P + (HR * half + 32 * i + l32) * 64 + 16 * ((2 * ks + hh) ^ ((l32 >> 2) & 3))));
     };
-    i32x2 t[4] = {vread(0), vread(1), vread(2), vread(3)};
-    f16x8 pb[2] = {pread(0, 0), pread(0, 1)};
-    u32x4 scp = {};
-    if constexpr (!R5) scp = *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 8 * hh) * 2);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const i32x2 c = t[n % 4];
+    auto vconv = [&](i32x2 c, u32x4 f) -> u32x4 {
       u32x4 v = {lo_f16x2((uint32_t)c[0]), hi_f16x2((uint32_t)c[0]), lo_f16x2((uint32_t)c[1]), hi_f16x2((uint32_t)c[1])};
-      if (n + 4 < 8) t[n % 4] = vread(n + 4);
       if constexpr (!R5)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = mul_f16x2(v[e], scp[e]);
+        for (int e = 0; e < 4; ++e) v[e] = mul_f16x2(v[e], f[e]);
+      return v;
+    };
+    auto sread = [&](int ks) -> u32x4 {
+      if constexpr (R5) return u32x4{};
+      else return *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 16 * ks + 8 * hh) * 2);
+    };
+    u32x4 f[2] = {sread(0)};
+    i32x2 t[3] = {vread(0), vread(1), vread(2)};
+    f16x8 pb[2] = {pread(0, 0), pread(0, 1)};
+    u32x4 v[2];
+    v[0] = vconv(t[0], f[0]);
+    t[0] = vread(3);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        O[n & 3][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pb[i], O[n & 3][i], 0, 0, 0);
-      if (n == 3) {
-        pb[0] = pread(1, 0);
-        pb[1] = pread(1, 1);
-        if constexpr (!R5) scp = *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 16 + 8 * hh) * 2);
+    for (int n = 0; n < 8; ++n) {                         // the next unit's conversions under this one's products
+      if (n == 1) f[1] = sread(1);
+      if (n < 7) v[(n + 1) & 1] = vconv(t[(n + 1) % 3], f[n >= 3]);
+      if (n < 4) t[(n + 1) % 3] = vread(n + 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        O[n & 3][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[n & 1]), pb[i], O[n & 3][i], 0, 0, 0);
+        if (n == 3) pb[i] = pread(1, i);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, R5 ? 2 : 4, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
+  // ---- steps: half 0 takes the products of tile s / 2 in even steps and a softmax in odd ones, half 1 the other way round, so
+  // that one half's products run beside the other's softmax
+  const bool works = HR * half < live;
   if (nt > 0) {
-    issue(0, 0);
-    if (nt > 1) issue(1, 1);
-    if (nt > 2) issue(2, 2);
+    for (int j = 0; j < 3 && j < nt; ++j) issue(j, j);
     if (nt > 2) wait_vm<2 * COPIES>(); else if (nt > 1) wait_vm<COPIES>(); else wait_vm<0>();
     lds_barrier();
-    partials(0);
+    if (works) partials(0);
     lds_barrier();
-    softmax(0);
+    if (half == 0) softmax(0);
     if (nt > 2) wait_vm<COPIES>(); else wait_vm<0>();
     lds_barrier();
   }
-  int slot = 0;                                           // of tile j; tiles j + 1 and j + 2 follow
-  for (int j = 0; j < nt; ++j) {
-    const int s1 = slot == 2 ? 0 : slot + 1;
-    // rows of the next IDS positions: looked up 7 tiles before a half ends, written 4 before, copied from 3 before
-    const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
-    if (in == IDS / TR - 7 && next * (IDS / TR) < nt) found = look(next);
-    if (in == IDS / TR - 4 && next * (IDS / TR) < nt) note(next, found);
-    partials(s1);                                         // (behind the last tile: of what lies there, not used)
-    values(j, slot);
-    lds_barrier();                                        // partials are there; tile j and P are done with
-    if (j + 3 < nt) issue(j + 3, slot);
-    if (j + 1 < nt) softmax(j + 1);
-    if (j + 3 < nt) wait_vm<COPIES>(); else wait_vm<0>();
-    lds_barrier();                                        // P and tile j + 2 are there
-    slot = s1;
+  int slot = 0;                                           // of tile s / 2; the next ones follow
+  for (int s = 0; s < 2 * nt; ++s) {
+    const int j = s >> 1;
+    if (!(s & 1)) {
+      // rows of the next IDS positions: looked up 7 tiles before a part ends, written 4 before, copied from 3 before
+      const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
+      if (in == IDS / TR - 7 && next * (IDS / TR) < nt) found = look(next);
+      if (in == IDS / TR - 4 && next * (IDS / TR) < nt) note(next, found);
+    }
+    if ((s & 1) == half) {
+      if (works) {
+        partials(slot + 1 == L::RING ? 0 : slot + 1);     // (behind the last tile: of what lies there, not used)
+        values(j, slot);
+      }
+    } else {
+      // tile j + 3 into the slot of tile j, whose values are taken (4 waves), or of tile j - 1
+      if (j + 3 < nt) issue(j + 3, NH == 1 ? slot : (slot + 3) & 3);
+      if (works && (s + 1) / 2 < nt) softmax((s + 1) / 2);
+    }
+    if (s & 1) {                                          // tile j + 2 is there
+      if (j + 3 < nt) wait_vm<COPIES>(); else wait_vm<0>();
+      slot = slot + 1 == L::RING ? 0 : slot + 1;
+    }
+    lds_barrier();
   }
 
   // ---- join of a row's four lanes, 1 / l for the waves that hold its dims
@@ -503,11 +541,16 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
       p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
     }
   }
+  if (lane == 0) ((SPMLA_LDS int*)(lds + L::FLAG))[w] = odd_from;
   lds_barrier();
+  if constexpr (NH > 1) {                                 // (the wave of the same group that came first took them out for both)
+    const int other = __builtin_amdgcn_readfirstlane(((SPMLA_LDS int*)(lds + L::FLAG))[w ^ 4]);
+    odd_from = odd_from < other ? odd_from : other;
+  }
   const float back = p.kv_scale;
   float a[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) a[i] = inv[32 * i + l32] * back;
+  for (int i = 0; i < 2; ++i) a[i] = inv[HR * half + 32 * i + l32] * back;
   const float e2 = R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23);
 #pragma unroll
   for (int x = 0; x < 4; ++x)
@@ -518,18 +561,21 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   if (__builtin_expect(odd_from < ke, 0)) {               // V that is no number, for the rows that see it
     int lim[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) lim[i] = limit_of(32 * i + l32 < live ? 32 * i + l32 : live - 1);
+    for (int i = 0; i < 2; ++i) {
+      const int row = HR * half + 32 * i + l32;
+      lim[i] = limit_of(row < live ? row : live - 1);
+    }
     for (int pos = odd_from; pos < ke; ++pos) {
       const int page = btrow[pos / p.bs];
       const long long y = (long long)page * p.stride + pos % p.bs;
       if (page < 0 || y >= p.rows) continue;
       const uint8_t* row = p.cache + y * RB;
-      const float sc = R5 ? 1.f : *(const float*)(row + SC_OFF + 4 * w);
+      const float sc = R5 ? 1.f : *(const float*)(row + SC_OFF + 4 * wl);
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float v = e4m3_to_f32(row[128 * w + 32 * x + 8 * (r >> 2) + 4 * hh + (r & 3)]) * sc * p.kv_scale;
+          const float v = e4m3_to_f32(row[128 * wl + 32 * x + 8 * (r >> 2) + 4 * hh + (r & 3)]) * sc * p.kv_scale;
           const float add = fabsf(v) < __builtin_inff() ? 0.f : v;
 #pragma unroll
           for (int i = 0; i < 2; ++i) O[x][i][r] += pos < lim[i] ? add : 0.f;
@@ -539,8 +585,9 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   if (!whole) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (32 * i + l32 >= live) continue;
-      float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r0 + 32 * i + l32) * D_LAT + 128 * w + 4 * hh;
+      const int row = HR * half + 32 * i + l32;
+      if (row >= live) continue;
+      float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r0 + row) * D_LAT + 128 * wl + 4 * hh;
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -551,7 +598,7 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
   }
   // bf16 rows through LDS, 32 at a time: the wave's 128 dims, 16-byte chunks permuted by the row
   SPMLA_LDS uint8_t* ob = lds + w * (32 * 256);
-  static_assert(4 * 32 * 256 <= L::FAC, "the output's rows fit below the factors");
+  static_assert(4 * NH * 32 * 256 <= L::FAC, "the output's rows fit below the factors");
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -564,9 +611,9 @@ __global__ void __launch_bounds__(256, 2) kernel(Params p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int row = 4 * k + qt;
-      if (32 * i + row < live) {
-        const long long r = r0 + 32 * i + row;
-        *(u32x4*)(p.out + (t0 + r / p.H) * p.o_st + (r % p.H) * p.o_sh + 128 * w + 8 * l16) =
+      if (HR * half + 32 * i + row < live) {
+        const long long r = r0 + HR * half + 32 * i + row;
+        *(u32x4*)(p.out + (t0 + r / p.H) * p.o_st + (r % p.H) * p.o_sh + 128 * wl + 8 * l16) =
             *(SPMLA_LDS u32x4*)(ob + row * 256 + 16 * (l16 ^ (row & 15)));
       }
     }
@@ -627,7 +674,7 @@ extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int S) {
 
 extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                                 int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
+                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, int wide, void* out,
                                 long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream) {
   if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || S < 1 || span < 1 ||
       span % chunk::TR || (row_bytes != ROW656 && row_bytes != ROW576))
@@ -640,7 +687,8 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
     return SPMLA_EALIGN;
   if (S > 1 && (!ws || ((uintptr_t)ws & 15))) return ws ? SPMLA_EALIGN : SPMLA_EARG;
   if (S > 1 && ws_bytes < spmla_attn_chunk_ws_bytes(T, H, S)) return SPMLA_EARG;
-  const long long tiles = (long long)T * H / chunk::MR + B;
+  const int r5 = row_bytes == ROW576, nh = wide ? 2 : 1;
+  const long long tiles = (long long)T * H / (chunk::HR * nh) + B;
   if (tiles * S > (1ll << 30)) return SPMLA_ELIMIT;
   float* opart = (float*)ws;
   float* lpart = opart ? opart + (long long)T * H * S * D_LAT : nullptr;
@@ -648,14 +696,15 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
                   H, S, span, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)tiles, (uint16_t*)out, o_st, o_sh, lse,
                   l_st, opart, lpart};
-  static DynLds attr[2];
-  static Launcher go[2];
-  const int r5 = row_bytes == ROW576;
-  const void* fn = r5 ? (const void*)chunk::kernel<true> : (const void*)chunk::kernel<false>;
-  const int lds = r5 ? chunk::Lds<true>::TOTAL : chunk::Lds<false>::TOTAL;
-  if (const int rc = attr[r5].ensure(fn, lds)) return rc;
+  static DynLds attr[4];
+  static Launcher go[4];
+  const int at = 2 * (nh - 1) + r5;
+  const void* fn[4] = {(const void*)chunk::kernel<false, 1>, (const void*)chunk::kernel<true, 1>, (const void*)chunk::kernel<false, 2>,
+                       (const void*)chunk::kernel<true, 2>};
+  const int lds[4] = {chunk::Lds<false, 1>::TOTAL, chunk::Lds<true, 1>::TOTAL, chunk::Lds<false, 2>::TOTAL, chunk::Lds<true, 2>::TOTAL};
+  if (const int rc = attr[at].ensure(fn[at], lds[at])) return rc;
   hipStream_t s = (hipStream_t)stream;
-  if (const int rc = go[r5](fn, dim3((unsigned)((tiles * S + 7) / 8 * 8)), 256, lds, s, p)) return rc;
+  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), 256 * nh, lds[at], s, p)) return rc;
   if (S == 1) return SPMLA_OK;
   static Launcher join;
   const chunk::MergeParams mp{opart, lpart, start, B, T, H, S, (uint16_t*)out, o_st, o_sh, lse, l_st};
