@@ -479,13 +479,12 @@ long attend_prompt(PyObject* const* a) {
   });
 }
 
-// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, split, span, out, lse, ws, wide)
+// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, split, span, out, lse, ws)
 long attend_chunk(PyObject* const* a) {
   const at::Tensor *q = tensor(a[0], "q"), *cache = tensor(a[1], "cache"), *table = tensor(a[2], "block_table"), *seqs = tensor(a[3], "seq_lens");
   const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[9], "out"), *lse = maybe(a[10], "lse"), *ws = maybe(a[11], "ws");
   const double sm = number(a[5]), kvs = number(a[6]);
   const long long split = integer(a[7]), span = integer(a[8]);
-  const bool wide = truth(a[12]);
   if (q->dim() != 3 || type_of(*q) != BF16 || q->size(2) != 576) refuse("q [T, H, 576] bf16: got " + shown(*q));
   const int64_t T = q->size(0), H = q->size(1), B = starts(*start);
   at_most(T, MAX_TOKENS, "T");
@@ -520,7 +519,7 @@ long attend_chunk(PyObject* const* a) {
   return launch(dev, [&](void* s) {
     return f_attn_chunk(address(q), qs.st, qs.sh, address(cache), total, (int)rowb, as_int(bs, "block_size"), stride,
                         (const int*)address(table), tst, (int)W, (const int*)address(seqs), (const int*)address(start), (int)B, (int)T,
-                        (int)H, (float)sm, (float)kvs, (int)split, (int)span, wide, address(out), os.st, os.sh, (float*)address(lse), ls,
+                        (int)H, (float)sm, (float)kvs, (int)split, (int)span, address(out), os.st, os.sh, (float*)address(lse), ls,
                         address(ws), ws ? ws->numel() : 0, s);
   });
 }
@@ -543,7 +542,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define CALLABLE(name, n) {#name, (PyCFunction)(void (*)())entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(linear_quant, 6),
                        CALLABLE(rope, 8), CALLABLE(latent_write, 13), CALLABLE(page_step, 11), CALLABLE(page_trim, 7),
-                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 13)};
+                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 12)};
 
 PyObject* load(PyObject*, PyObject* args) {
   const char* path;

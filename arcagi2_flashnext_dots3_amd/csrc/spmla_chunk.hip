@@ -6,23 +6,20 @@
 //   s = sm_scale kv_scale (q[:512] . latent + q[512:] . rope),  p = exp(s - m),  o = kv_scale sum p latent / sum p,
 //   lse = ln sum exp(s)
 //
-// One workgroup = 64 rows of (token, head) of one request, token by token, over one split of the positions: whatever the
-// number of heads, a cached row is copied once for 64 query rows, and a decode step of 16 heads fills 16 of them.
-// 4 waves, tiles of 32 positions, a ring of three in LDS filled by direct copies; two workgroups a compute unit:
-//   * QK: wave 2 i + d multiplies half d of the dims (two scale groups, half of the rope) of query rows 32 i .. 32 i + 31:
-//     S^T partials in bf16 MFMA 16x16x32, codes converted exactly, so a code is converted by two waves and the query takes
-//     72 registers. (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
-//     the summed magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32
-//     scales, then the rope. The two waves exchange half of their partials through LDS: each ends with 16 query rows;
-//   * softmax: one query row per lane (and three others); base 2, 32 bits; the reference maximum moves only past TAU.
-//     P goes to LDS in f16, times 2^UP so that few weights are f16 subnormals;
-//   * PV: wave g owns dims 128 g .. of all 64 rows: O^T = V^T P^T (f16 MFMA 32x32x16), V^T by the 8-bit transposing read,
-//     converted to f16 exactly and (Row656) multiplied by scale * 2^-e in f16; e (per wave) keeps that in range: it follows
-//     the largest scale so far (a value is off by half an f16 step, or 2^-39 of the largest magnitude so far).
-// Two barriers a tile: partials of tile j + 1 and PV of tile j; then the softmax of tile j + 1, while the other
-// workgroup's products run.
-// Masked positions take no part: scores of -inf, and where the mask cuts a tile V's values that are no numbers are taken
-// out of the product and given to the rows that see them at the end.
+// One workgroup = up to 128 rows of (token, head) of one request, token by token, over one split of the positions: whatever
+// the number of heads, a cached row is copied once for them. 8 waves of 16 rows each; where a request has 64 rows or fewer
+// (PS = 2) 4 of them take every other tile, and both join at the end. Tiles of 32 positions in a ring in LDS, filled by
+// direct copies, one barrier a tile; otherwise a wave is on its own, from the scores to its output:
+//   * QK: S^T = K Q^T in bf16 MFMA 16x16x32, codes converted exactly, the query in 72 registers. (8-bit MFMA would take the
+//     codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of the summed magnitudes, 1.3e-5 at most,
+//     against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales;
+//   * softmax: one query row per lane (and three others); base 2, 32 bits; the reference maximum moves only past TAU. A lane's
+//     weights are the operand it needs: the k slots of V^T follow the rows of the accumulator, P never leaves its registers;
+//   * PV: O^T = V^T P^T in f16 MFMA 16x16x32, V^T by the 8-bit transposing read, converted exactly; P in f16 times 2^UP so
+//     that few weights are f16 subnormals. Row656: P times the scales of the four groups times 2^-e, e following the largest
+//     scale so far (a product p * scale is off by half an f16 step, or 2^-34 of the largest scale).
+// Masked positions take no part: scores of -inf, and where the mask cuts a tile codes and scales that are no numbers become 0
+// after the scores (a row that sees one has a score that is none).
 // Splits leave normalized fp32 partials and their lse in a workspace; a second kernel joins them.
 #include "spmla_common.h"
 #include "spmla_quant.h"
@@ -30,7 +27,6 @@
 namespace spmla {
 namespace chunk {
 
-constexpr int HR = 64;                // query rows per half (4 waves)
 constexpr int TR = 32;                // positions per tile
 constexpr int IDS = 256;              // positions whose rows are looked up at a time
 constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;
@@ -52,22 +48,20 @@ struct Params {
   float* opart; float* lpart;                              // [S][T][H][512], [S][T][H]
 };
 
-template <bool R5, int NH>
+template <bool R5, int PS>
 struct Lds {
-  static constexpr int RING = NH == 1 ? 3 : 4;
+  static constexpr int MR = 128 / PS;                      // query rows
+  static constexpr int RING = 6;
   static constexpr int CODE = 4 * TR * 128;                // codes by scale group, [4][32 rows][128]
   static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
   static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
   static constexpr int TILE = CODE + RP + SC;
-  static constexpr int X = RING * TILE;                    // exchanged partials [wave][16 positions][64 lanes][16]
-  static constexpr int P = X + 4 * NH * 2048;              // [64 NH query rows][32 positions] f16
-  static constexpr int FAC = P + NH * HR * TR * 2;         // rescale factors [64 NH]
-  static constexpr int FLAG = FAC + NH * HR * 4;           // a wave's factors are not all 1
-  static constexpr int SCH = FLAG + 16 * NH;               // a wave's scales in f16, [4 NH][32]
-  static constexpr int ID = SCH + 4 * NH * TR * 2;         // addresses of the rows of two times IDS positions
+  static constexpr int ID = RING * TILE;                   // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
   static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
-  static_assert(TOTAL <= (NH == 1 ? 80 : 160) * 1024 && ID % 8 == 0, "two workgroups of 4 waves a compute unit, or one of 8");
+  static constexpr int JOIN = 4 * 32768;                   // at the end, PS = 2: O of 4 waves; then maxima and sums
+  static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0, "one workgroup a compute unit");
+  static constexpr int BYTES = PS == 2 && TOTAL < JOIN + 2048 ? JOIN + 2048 : TOTAL < 131072 ? 131072 : TOTAL;
 };
 
 __device__ __attribute__((aligned(16))) uint8_t zero_row[ROW656];
@@ -101,33 +95,33 @@ __device__ inline float quad_sum(float x) { return swap16_sum(swap32_sum(x)); }
 
 __device__ inline uint32_t pk_f16(float a, float b) { return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b}); }
 __device__ inline uint32_t pk_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }
-__device__ inline uint32_t lo_f16x2(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)); }
-__device__ inline uint32_t hi_f16x2(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)); }
-__device__ inline uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) * __builtin_bit_cast(f16x2, b));
-}
-
-// 8 e4m3 codes -> 8 bf16, exact
-__device__ inline bf16x8 codes8(int a, int b) {
+// 8 e4m3 codes -> 8 bf16 / f16, exact
+__device__ inline bf16x8 codes8_bf16(int a, int b) {
   return __builtin_bit_cast(bf16x8, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false)),
                                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true)),
                                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false)),
                                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true))});
 }
+__device__ inline f16x8 codes8_f16(int a, int b) {
+  return __builtin_bit_cast(f16x8, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false)),
+                                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true)),
+                                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false)),
+                                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true))});
+}
 // place of chunk c (16 bytes) in a row of 128 bytes: c ^ swz(row); 16 rows' chunks c lie in all 64 banks
 __device__ inline int swz(int row) { return ((row & 2) << 1) | ((row & 4) >> 2) | ((row & 8) >> 2); }
 
-template <bool R5, int NH>
-__global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
-  using L = Lds<R5, NH>;
-  constexpr int RB = R5 ? ROW576 : ROW656, MR = HR * NH;
+template <bool R5, int PS>
+__global__ void __launch_bounds__(512, 2) kernel(Params p) {
+  using L = Lds<R5, PS>;
+  constexpr int RB = R5 ? ROW576 : ROW656, MR = L::MR;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int half = NH == 1 ? 0 : w >> 2, wl = w & 3;      // this wave's half and its number there
-  const int l16 = lane & 15, l32 = lane & 31, qt = lane >> 4, hh = lane >> 5;
+  const int wr = PS == 1 ? w : w & 3, wp = PS == 1 ? 0 : w >> 2;          // the wave's 16 rows; which of PS tiles it takes
+  const int l16 = lane & 15, l32 = lane & 31, qt = lane >> 4;
 
-  // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / 64 + b.
+  // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / MR + b.
   const int f = remap_xcd(blockIdx.x, p.tiles * p.S);
   if (f < 0) return;
   const int sp = f / p.tiles, ti = p.tiles - 1 - f % p.tiles;
@@ -157,29 +151,21 @@ __global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
   const int ke = sp + 1 < p.S && first + p.span < most ? (int)(first + p.span) : most;       // (the last split takes the rest)
   const int nt = (ke - kb + TR - 1) / TR;
   if (nt <= 0 && sp > 0) {                                                 // nothing of this split: no weight in the join
-    if (tid < live) {
-      const long long r = r0 + tid;
-      p.lpart[((long long)sp * p.T + t0) * p.H + r] = -__builtin_inff();
-    }
+    if (tid < live) p.lpart[((long long)sp * p.T + t0) * p.H + r0 + tid] = -__builtin_inff();
     return;
   }
   const int* btrow = p.table + (long long)b * p.t_st;
 
   // ---- rows of IDS positions: looked up (x beyond ke: none), then their addresses written with a bit per position
   auto look = [&](int part) -> int {
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
     const int pos = kb + part * IDS + tid;
-    if (pos >= ke || (NH > 1 && tid >= IDS)) return -1;
+    if (pos >= ke || tid >= IDS) return -1;
     const int page = btrow[pos / p.bs];
     const long long y = (long long)page * p.stride + pos % p.bs;
     return page >= 0 && y < p.rows ? (int)y : -1;
   };
   auto note = [&](int part, int row) {
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, l32 = lane & 31;
-    if (NH > 1 && tid >= IDS) return;
+    if (tid >= IDS) return;
     const int at = (part & 1) * IDS + tid;
     const uint64_t a = (uint64_t)(uintptr_t)p.cache + (uint64_t)(uint32_t)row * RB;
     ((SPMLA_LDS uint64_t*)(lds + L::ID))[at] = row >= 0 ? a : (uint64_t)(uintptr_t)zero_row;
@@ -188,147 +174,99 @@ __global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
   };
   int found = look(0);
 
-  // ---- query operands [chunk pair or rope][half chunk][own or partner's 16 query rows] of rows 32 (w / 2) .. and half dh of the dims: B
-  // operands of 16x16x32, lane quarter qt the dims 64 n + 16 qt + 8 e .. + 7 (one 16-byte read of codes serves both e)
-  const int dh = wl & 1, qb = HR * half + 32 * (wl >> 1);
-  bf16x8 qf[4][2][2], qpe[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = qb + 16 * (i ^ dh) + l16;             // (i = 0: the rows that this wave joins)
-    const long long r = r0 + (row < live ? row : live - 1);
+  // ---- query operands of rows 16 wr ..: B operands of 16x16x32, lane quarter qt the dims 64 n + 16 qt + 8 e .. + 7 (one
+  // 16-byte read of codes serves both e); rope (n = 8): Row576 as the codes, Row656 dims 32 e + 8 qt ..
+  const int qr = 16 * wr + l16;                           // the query row of this lane
+  bf16x8 qf[9][2];
+  {
+    const long long r = r0 + (qr < live ? qr : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
     const uint32_t turn = p.flip ? 0x80008000u : 0u;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 9; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) qf[n][e][i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + 256 * dh + 64 * n + 16 * qt + 8 * e) ^ turn);
-    qpe[i] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + D_LAT + 32 * dh + 8 * qt) ^ turn);
+      for (int e = 0; e < 2; ++e) {
+        const int at = n == 8 && !R5 ? D_LAT + 32 * e + 8 * qt : 64 * n + 16 * qt + 8 * e;
+        qf[n][e] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + at) ^ turn);
+      }
   }
-  const int qr = HR * half + 16 * wl + l16;               // the query row whose softmax this lane shares
   note(0, found);
-  if (tid < 4 * NH) ((SPMLA_LDS int*)(lds + L::FLAG))[tid] = 0;
   lds_barrier();
 
-  // ---- copies of a tile: rows 8 i + lane / 8 of a scale group's codes, the chunk whose place is lane % 8 (4 waves: wave w
-  // all of group w, 8 waves: half of group w % 4), a share of the rope and of the scales (some twice). COPIES instructions a
-  // wave whatever the tile.
-  constexpr int COPIES = (R5 ? 1 : NH == 1 ? 2 : 1) + 4 / NH;
-  // the lane id, opaque in every step: LDS places made of it are formed again, not kept (spilled, a tile's wait for one would
-  // wait for all copies)
-  auto here = [&]() -> int {
-    int x = lane;
-    asm volatile("" : "+v"(x));
-    return x;
-  };
-  auto issue = [&](int j, int slot) {
-    const int lane = here(), l32 = lane & 31, hh = lane >> 5;
+  // ---- copies of a tile: rows 8 i + lane / 8 of a scale group's codes, the chunk whose place is lane % 8 (a wave half of
+  // group w % 4), a share of the rope and of the scales (some twice). COPIES instructions a wave whatever the tile.
+  constexpr int COPIES = 3;
+  auto issue = [&](int j) {
     SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
-    SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
-    const int r = lane >> 3, place = (lane & 7) ^ swz(r);
+    SPMLA_LDS uint8_t* d = lds + (j % L::RING) * L::TILE;
+    const int r = lane >> 3, place = (lane & 7) ^ swz(r), wl = w & 3, half = w >> 2;
     auto copy = [&](int row, uint32_t off, SPMLA_LDS uint8_t* to) { dma16((const void*)(id[row] + off), to); };
 #pragma unroll
-    for (int n = 0; n < 4 / NH; ++n) {
-      const int i = n + 2 * half;
-      copy(8 * i + r, 128 * wl + 16 * (place ^ ((i & 1) << 1)), d + wl * 4096 + i * 1024);
-    }
-    auto scales = [&]() { dma4((const void*)(id[l32] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + hh))), d + L::CODE + L::RP + (w & 1) * 256); };
+    for (int n = 0; n < 2; ++n) copy(8 * (n + 2 * half) + r, 128 * wl + 16 * (place ^ (n << 1)), d + wl * 4096 + (n + 2 * half) * 1024);
     if constexpr (R5) {                                   // 16 rows of 64 bytes a copy
       const int rr = 16 * (w & 1) + (lane >> 2);
       copy(rr, D_LAT + 16 * ((lane & 3) ^ ((rr >> 2) & 3)), d + L::CODE + (w & 1) * 1024);
+    } else if (half == 0) {
+      copy(8 * wl + r, ROPE_OFF + 16 * (place ^ ((wl & 1) << 1)), d + L::CODE + wl * 1024);
     } else {
-      if (NH == 1 || half == 0) copy(8 * wl + r, ROPE_OFF + 16 * (place ^ ((wl & 1) << 1)), d + L::CODE + wl * 1024);
-      if (NH == 1 || half == 1) scales();
+      dma4((const void*)(id[lane & 31] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + (lane >> 5)))), d + L::CODE + L::RP + (w & 1) * 256);
     }
   };
 
-  f32x16 O[4][2];                                         // [32 dims of group w][32 query rows]
+  f32x4 O[32];                                            // O^T: dims 16 n + 4 qt .., query row qr; times 2^-ex2 (Row656)
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) O[d][i] = f32x16{};
+  for (int n = 0; n < 32; ++n) O[n] = f32x4{};
   float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, shared by its four lanes; l: this lane's)
   bool far = false;                                       // a reference is beyond FAR
-  int ex2 = -126;                                         // Row656: V' and O carry 2^-ex2
-  int odd_from = 0x7fffffff;
+  int ex2 = -126;
+  f32x4 s[2];                                             // scores, then weights: value 4 u + r is position 16 u + 4 qt + r
 
-  // Partial scores of a tile over this wave's dims: S^T blocks of 16 positions x 16 query rows (block 0: the rows this wave
-  // joins, kept; block 1: its partner's, to LDS). Steps of two products (20: 16 of codes, 4 a block pair of rope at the end of
-  // its positions): the conversions of the next step's operand run under the products of this one, reads two ahead.
-  f32x4 part[2];
-  auto partials = [&](int slot) {
-    const int lane = here(), l16 = lane & 15, qt = lane >> 4;
-    SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
-    SPMLA_LDS uint8_t* at = d + (2 * dh) * 4096 + l16 * 128;
+  auto scores = [&](SPMLA_LDS uint8_t* d) {
+    SPMLA_LDS uint8_t* at = d + l16 * 128;
     const int x0 = 16 * (qt ^ swz(l16)), x1 = x0 ^ 64;
-    auto kread = [&](int n) -> i32x4 {                    // unit n: positions 16 (n / 4) .., group 2 dh + n / 2 % 2, chunks 4 (n % 2) ..
-      return *(SPMLA_LDS i32x4*)(at + (n >> 2) * 2048 + ((n >> 1) & 1) * 4096 + ((n & 1) ? x1 : x0));
+    // unit n = 9 u + i: positions 16 u .., dims 64 i .. (i = 8: rope)
+    auto kread = [&](int n) -> i32x4 {
+      const int u = n / 9, i = n % 9;
+      if (i < 8) return *(SPMLA_LDS i32x4*)(at + (i >> 1) * 4096 + u * 2048 + ((i & 1) ? x1 : x0));
+      if constexpr (R5) return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 1024 + l16 * 64 + 16 * (qt ^ ((l16 >> 2) & 3)));
+      else return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + x0);
     };
-    auto rread = [&](int u) -> i32x4 {                    // rope of positions 16 u ..: Row576 8 codes, Row656 8 bf16
-      if constexpr (R5) {
-        const i32x2 y = *(SPMLA_LDS i32x2*)(d + L::CODE + u * 1024 + l16 * 64 + 16 * ((2 * dh + (qt >> 1)) ^ ((l16 >> 2) & 3)) + 8 * (qt & 1));
-        return i32x4{y[0], y[1], 0, 0};
+    i32x4 k[3] = {kread(0), kread(1), kread(2)};
+    f32x4 acc = {};
+#pragma unroll
+    for (int n = 0; n < 18; ++n) {
+      const int u = n / 9, i = n % 9;
+      bf16x8 y[2];
+      if (i == 8 && !R5) {
+        y[0] = __builtin_bit_cast(bf16x8, k[n % 3]);
+        y[1] = __builtin_bit_cast(bf16x8, *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + x1));
       } else {
-        return *(SPMLA_LDS i32x4*)(d + L::CODE + u * 2048 + l16 * 128 + 16 * ((4 * dh + qt) ^ swz(l16)));
+        y[0] = codes8_bf16(k[n % 3][0], k[n % 3][1]);
+        y[1] = codes8_bf16(k[n % 3][2], k[n % 3][3]);
       }
-    };
-    i32x4 k[3] = {kread(0), kread(1), kread(2)}, kr;
-    bf16x8 y[2];
-    y[0] = codes8(k[0][0], k[0][1]);
-    f32x4 s[2] = {}, acc[2] = {}, sc = {};
+      if (n + 3 < 18) k[n % 3] = kread(n + 3);
+      if (i == 0) s[u] = f32x4{};
+      if constexpr (R5) {
 #pragma unroll
-    for (int t = 0; t < 18; ++t) {                        // t % 9 < 8: half e of unit 4 u + t % 9 / 2; 8: rope
-      const int u = t / 9, i9 = t % 9, n = 4 * u + i9 / 2;
-      // the next step's operand
-      if (i9 < 8) {
-        if (i9 & 1) {
-          if (n + 3 < 8) k[n % 3] = kread(n + 3);         // (its codes are converted)
-          if (i9 == 7) y[(t + 1) & 1] = R5 ? codes8(kr[0], kr[1]) : __builtin_bit_cast(bf16x8, kr);
-          else y[(t + 1) & 1] = codes8(k[(n + 1) % 3][0], k[(n + 1) % 3][1]);
-        } else {
-          y[(t + 1) & 1] = codes8(k[n % 3][2], k[n % 3][3]);
-          if (i9 == 4) kr = rread(u);
+        for (int e = 0; e < 2; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[e], qf[i][e], s[u], 0, 0, 0);
+      } else if (i < 8) {
+        if (!(i & 1)) acc = f32x4{};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[e], qf[i][e], acc, 0, 0, 0);
+        if (i & 1) {
+          const f32x4 sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (i >> 1) * 128 + u * 64 + qt * 16);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[u][r] = __builtin_fmaf(acc[r], sc[r], s[u][r]);
         }
-      } else if (u == 0) {
-        y[(t + 1) & 1] = codes8(k[4 % 3][0], k[4 % 3][1]);
-      }
-      if constexpr (!R5)
-        if (i9 == 1 || i9 == 5) sc = *(SPMLA_LDS f32x4*)(d + L::CODE + L::RP + (2 * dh + i9 / 4) * 128 + u * 64 + qt * 16);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bf16x8 q = i9 == 8 ? qpe[i] : qf[(i9 / 2) & 3][i9 & 1][i];
-        f32x4& to = R5 || i9 == 8 ? s[i] : acc[i];
-        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[t & 1], q, to, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {                       // a product, two conversions, ...
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (!R5) {
-        if (i9 == 3 || i9 == 7) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[i][r] = i9 == 3 ? acc[i][r] * sc[r] : __builtin_fmaf(acc[i][r], sc[r], s[i][r]);
-            acc[i] = f32x4{};
-          }
-        }
-      }
-      if (i9 == 8) {
-        part[u] = s[0];
-        *(SPMLA_LDS f32x4*)(lds + L::X + w * 2048 + u * 1024 + lane * 16) = s[1];
-        s[0] = s[1] = f32x4{};
+        for (int e = 0; e < 2; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[e], qf[8][e], s[u], 0, 0, 0);
       }
     }
   };
 
-  // softmax of tile j, its P and factors: value 4 u + r of a lane is position 16 u + 4 qt + r
+  // softmax of tile j: s becomes the weights, O and l follow a moved maximum
   auto softmax = [&](int j) {
-    const int lane = here(), l16 = lane & 15, qt = lane >> 4, qr = HR * half + 16 * wl + l16;
-    f32x4 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) s[u] = part[u] + *(SPMLA_LDS f32x4*)(lds + L::X + (w ^ 1) * 2048 + u * 1024 + lane * 16);
     const uint32_t has = __builtin_amdgcn_readfirstlane(((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
     const int k0 = kb + j * TR;
     if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
@@ -348,17 +286,14 @@ __global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
     mx = quad_max(mx);
-    float fac = 1.f;
-    const bool move = __any(mx * p.c > m * p.c + TAU);
-    if (move) {
+    if (__any(mx * p.c > m * p.c + TAU)) {
       const float mn = fmaxf(m, mx), a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.c);
       m = mn;
       l *= a;
+#pragma unroll
+      for (int n = 0; n < 32; ++n) O[n] *= a;
       far = __any(fabsf(mn * p.c) > FAR && mn > -__builtin_inff());
-      fac = a;
     }
-    if (qt == 0) ((SPMLA_LDS float*)(lds + L::FAC))[qr] = fac;
-    if (lane == 0) ((SPMLA_LDS int*)(lds + L::FLAG))[w] = move;
     const float base = m == -__builtin_inff() ? 0.f : m, ref = UP - base * p.c;
     if (__builtin_expect(far, 0)) {                        // the rounding of m c would count: differences first
 #pragma unroll
@@ -375,249 +310,153 @@ __global__ void __launch_bounds__(256 * NH, 2) kernel(Params p) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) l += s[u][r];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {                          // half of chunk 2 u + qt / 2
-      const int ch = (2 * u + (qt >> 1)) ^ ((qr >> 2) & 3);
-      *(SPMLA_LDS i32x2*)(lds + L::P + qr * 64 + 16 * ch + 8 * (qt & 1)) = i32x2{(int)pk_f16(s[u][0], s[u][1]), (int)pk_f16(s[u][2], s[u][3])};
-    }
   };
 
-  // O += V^T P^T of tile j
-  auto values = [&](int j, int slot) {
-    const int lane = here(), l32 = lane & 31, hh = lane >> 5;
-    const int vrow = 8 * hh + ((lane & 15) >> 1);         // V^T: row of the transposing read
-    SPMLA_LDS uint8_t* d = lds + slot * L::TILE;
-    const int k0 = kb + j * TR;
-    const i32x4 fl = *(SPMLA_LDS i32x4*)(lds + L::FLAG + 16 * half);
-    const int any = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
-    float sc = 0.f;
-    if constexpr (!R5) {
-      sc = *(SPMLA_LDS float*)(d + L::CODE + L::RP + wl * 128 + l32 * 4);
-      const float fin = fabsf(sc) < __builtin_inff() ? fabsf(sc) : 0.f;
-      if (__builtin_expect(__any(fin * u2f((uint32_t)(127 - ex2) << 23) > 64.f), 0)) {      // a larger scale than any before: e follows
-        float top = fin;
+  // O += V^T P^T
+  auto values = [&](SPMLA_LDS uint8_t* d) {
+    f16x8 P[R5 ? 1 : 4];
+    if constexpr (R5) {
+      P[0] = __builtin_bit_cast(f16x8, u32x4{pk_f16(s[0][0], s[0][1]), pk_f16(s[0][2], s[0][3]), pk_f16(s[1][0], s[1][1]), pk_f16(s[1][2], s[1][3])});
+    } else {
+      SPMLA_LDS uint8_t* sa = d + L::CODE + L::RP;
+      const f32x2 two = *(SPMLA_LDS f32x2*)(sa + lane * 8);                 // the tile's 128 scales
+      float top = fmaxf(fabsf(two[0]) < __builtin_inff() ? fabsf(two[0]) : 0.f, fabsf(two[1]) < __builtin_inff() ? fabsf(two[1]) : 0.f);
+      if (__builtin_expect(__any(top * u2f((uint32_t)(127 - ex2) << 23) > 1.f), 0)) {        // a larger one than before: e follows
         asm volatile("" : "+v"(top));
 #pragma unroll
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        int e = (int)(f2u(top) >> 23) - 127 - 5;                            // scale * 2^-e < 64
-        e = __builtin_amdgcn_readfirstlane(e < -126 ? -126 : e);
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        int e = (int)(f2u(top) >> 23) - 127 + 1;                            // scale * 2^-e < 1
+        e = __builtin_amdgcn_readfirstlane(e < -126 ? -126 : e > 126 ? 126 : e);
         const float a = __builtin_amdgcn_exp2f((float)(ex2 - e));
         ex2 = e;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) O[x][i][r] *= a;
+        for (int n = 0; n < 32; ++n) O[n] *= a;
       }
-      const bool masked = k0 + TR > least && least < most && !(fabsf(sc) < __builtin_inff());
-      const _Float16 h = masked ? (_Float16)0.f : (_Float16)(sc * u2f((uint32_t)(127 - ex2) << 23));
-      ((SPMLA_LDS _Float16*)(lds + L::SCH))[w * TR + l32] = h;
-    }
-    if (__builtin_expect(any, 0)) {
+      const float down = u2f((uint32_t)(127 - ex2) << 23);
+      f32x4 t[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float a = ((SPMLA_LDS float*)(lds + L::FAC))[HR * half + 32 * i + l32];
+      for (int u = 0; u < 2; ++u) t[u] = s[u] * down;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) O[x][i][r] *= a;
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 a = *(SPMLA_LDS f32x4*)(sa + g * 128 + qt * 16) * t[0], b = *(SPMLA_LDS f32x4*)(sa + g * 128 + 64 + qt * 16) * t[1];
+        P[g] = __builtin_bit_cast(f16x8, u32x4{pk_f16(a[0], a[1]), pk_f16(a[2], a[3]), pk_f16(b[0], b[1]), pk_f16(b[2], b[3])});
       }
     }
-    if (__builtin_expect(k0 + TR > least && least < most, 0)) {
-      // the mask cuts this tile: codes that are no numbers become 0 in the wave's group, whose values alone are read from now on
-      // (8 waves: by the other half's wave of the group as well, whose turn comes later)
-      uint32_t odd = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(d + wl * 4096 + i * 1024 + lane * 16);
-        u32x4 y = *at;
-        uint32_t bad = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t nan = ((y[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-          bad |= nan;
-          y[e] &= ~((nan >> 7) * 255u);
-        }
-        odd |= bad;
-        if (bad) *at = y;
-      }
-      if constexpr (!R5) odd |= fabsf(sc) < __builtin_inff() ? 0u : 1u;     // (its f16 form is 0)
-      if (__any(odd != 0)) odd_from = odd_from < k0 ? odd_from : k0;
-    }
-    const int vo = wl * 4096 + vrow * 128 + 8 * (lane & 1), vs = swz(vrow) ^ ((lane >> 4) & 1);
-    auto vread = [&](int n) -> i32x2 {                    // unit n: positions 16 (n / 4) .., dims 32 (n % 4) ..
-      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((SPMLA_LDS i32x2*)(d + vo + 16 * (vs ^ (2 * (n & 3))) + (n >> 2) * 2048));
+    // transposing read: lanes 2 i and 2 i + 1 of a quarter supply row i of the k slots 8 qt ..: positions 4 qt + i, 16 + 4 qt + i - 4
+    const int i2 = l16 >> 1, vrow = 16 * (i2 >> 2) + 4 * qt + (i2 & 3);
+    const int va = vrow * 128 + 16 * swz(vrow) + 8 * (lane & 1);
+    auto vread = [&](int n) -> i32x2 {                    // unit n = 4 c + g: dims 128 g + 16 c ..
+      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((SPMLA_LDS i32x2*)(d + (n & 3) * 4096 + (va ^ (16 * (n >> 2)))));
     };
-    auto pread = [&](int ks, int i) -> f16x8 {
-      return __builtin_bit_cast(f16x8, *(SPMLA_LDS u32x4*)(lds + L::P + (HR * half + 32 * i + l32) * 64 + 16 * ((2 * ks + hh) ^ ((l32 >> 2) & 3))));
-    };
-    auto vconv = [&](i32x2 c, u32x4 f) -> u32x4 {
-      u32x4 v = {lo_f16x2((uint32_t)c[0]), hi_f16x2((uint32_t)c[0]), lo_f16x2((uint32_t)c[1]), hi_f16x2((uint32_t)c[1])};
-      if constexpr (!R5)
+    i32x2 t[4] = {vread(0), vread(1), vread(2), vread(3)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = mul_f16x2(v[e], f[e]);
-      return v;
-    };
-    auto sread = [&](int ks) -> u32x4 {
-      if constexpr (R5) return u32x4{};
-      else return *(SPMLA_LDS u32x4*)(lds + L::SCH + (w * TR + 16 * ks + 8 * hh) * 2);
-    };
-    u32x4 f[2] = {sread(0)};
-    i32x2 t[3] = {vread(0), vread(1), vread(2)};
-    f16x8 pb[2] = {pread(0, 0), pread(0, 1)};
-    u32x4 v[2];
-    v[0] = vconv(t[0], f[0]);
-    t[0] = vread(3);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {                         // the next unit's conversions under this one's products
-      if (n == 1) f[1] = sread(1);
-      if (n < 7) v[(n + 1) & 1] = vconv(t[(n + 1) % 3], f[n >= 3]);
-      if (n < 4) t[(n + 1) % 3] = vread(n + 4);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        O[n & 3][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[n & 1]), pb[i], O[n & 3][i], 0, 0, 0);
-        if (n == 3) pb[i] = pread(1, i);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, R5 ? 2 : 4, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int n = 0; n < 32; ++n) {
+      const f16x8 v = codes8_f16(t[n & 3][0], t[n & 3][1]);
+      if (n + 4 < 32) t[n & 3] = vread(n + 4);
+      f32x4& o = O[8 * (n & 3) + (n >> 2)];
+      o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, P[R5 ? 0 : n & 3], o, 0, 0, 0);
     }
   };
 
-  // ---- steps: half 0 takes the products of tile s / 2 in even steps and a softmax in odd ones, half 1 the other way round, so
-  // that one half's products run beside the other's softmax
-  const bool works = HR * half < live;
-  if (nt > 0) {
-    for (int j = 0; j < 3 && j < nt; ++j) issue(j, j);
-    if (nt > 2) wait_vm<2 * COPIES>(); else if (nt > 1) wait_vm<COPIES>(); else wait_vm<0>();
+  // ---- tiles PS at a time
+  constexpr int AHEAD = L::RING - PS;                     // tiles copied ahead
+  const bool works = 16 * wr < live;
+  for (int j = 0; j < AHEAD && j < nt; ++j) issue(j);
+  for (int j = 0; j < nt; j += PS) {
+    // rows of the next IDS positions: looked up as a part begins, noted two tiles later, copied from a later step on
+    const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
+    // tile j (and j + 1) is there: of the copies after it at most AHEAD - PS tiles' are on their way
+    if (j + AHEAD <= nt) wait_vm<(AHEAD - PS) * COPIES>(); else wait_vm<0>();
     lds_barrier();
-    if (works) partials(0);
-    lds_barrier();
-    if (half == 0) softmax(0);
-    if (nt > 2) wait_vm<COPIES>(); else wait_vm<0>();
-    lds_barrier();
-  }
-  int slot = 0;                                           // of tile s / 2; the next ones follow
-  for (int s = 0; s < 2 * nt; ++s) {
-    const int j = s >> 1;
-    if (!(s & 1)) {
-      // rows of the next IDS positions: looked up 7 tiles before a part ends, written 4 before, copied from 3 before
-      const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
-      if (in == IDS / TR - 7 && next * (IDS / TR) < nt) found = look(next);
-      if (in == IDS / TR - 4 && next * (IDS / TR) < nt) note(next, found);
-    }
-    if ((s & 1) == half) {
-      if (works) {
-        partials(slot + 1 == L::RING ? 0 : slot + 1);     // (behind the last tile: of what lies there, not used)
-        values(j, slot);
+    if (in == 0 && next * (IDS / TR) < nt) found = look(next);
+    if (in == 2 && next * (IDS / TR) < nt) note(next, found);
+#pragma unroll
+    for (int i = 0; i < PS; ++i)
+      if (j + AHEAD + i < nt) issue(j + AHEAD + i);
+    const int mine = j + wp;
+    SPMLA_LDS uint8_t* d = lds + (mine % L::RING) * L::TILE;
+    const bool go = works && mine < nt;
+    if (go) scores(d);
+    if (__builtin_expect(kb + (j + PS) * TR > least && least < most, 0)) {
+      // the mask cuts a tile: codes and scales that are no numbers become 0 once every wave has its scores
+      lds_barrier();
+      for (int i = 0; i < PS && j + i < nt; ++i) {
+        SPMLA_LDS uint8_t* c = lds + ((j + i) % L::RING) * L::TILE;
+        for (int at = tid * 16; at < L::CODE; at += 512 * 16) {
+          u32x4 y = *(SPMLA_LDS u32x4*)(c + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t nan = ((y[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            y[e] &= ~((nan >> 7) * 255u);
+          }
+          *(SPMLA_LDS u32x4*)(c + at) = y;
+        }
+        if (!R5 && tid < 128) {
+          SPMLA_LDS float* x = (SPMLA_LDS float*)(c + L::CODE + L::RP) + tid;
+          if (!(fabsf(*x) < __builtin_inff())) *x = 0.f;
+        }
       }
-    } else {
-      // tile j + 3 into the slot of tile j, whose values are taken (4 waves), or of tile j - 1
-      if (j + 3 < nt) issue(j + 3, NH == 1 ? slot : (slot + 3) & 3);
-      if (works && (s + 1) / 2 < nt) softmax((s + 1) / 2);
+      lds_barrier();
     }
-    if (s & 1) {                                          // tile j + 2 is there
-      if (j + 3 < nt) wait_vm<COPIES>(); else wait_vm<0>();
-      slot = slot + 1 == L::RING ? 0 : slot + 1;
+    if (go) {
+      softmax(mine);
+      values(d);
     }
-    lds_barrier();
   }
 
-  // ---- join of a row's four lanes, 1 / l for the waves that hold its dims
+  // ---- join of a row's four lanes, and (PS = 2) of the two waves of its rows
   l = quad_sum(l);
-  const float ln = m == -__builtin_inff() ? m : m * p.c * 0.69314718055994531f + (__builtin_log2f(l) - UP) * 0.69314718055994531f;
-  SPMLA_LDS float* inv = (SPMLA_LDS float*)(lds + L::FAC);
-  if (qt == 0) inv[qr] = l > 0.f || l != l ? 1.f / l : 0.f;
+  float e2 = R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23);
+  if constexpr (PS == 2) {
+    SPMLA_LDS f32x4* oj = (SPMLA_LDS f32x4*)(lds + wr * 32768);
+    SPMLA_LDS float* st = (SPMLA_LDS float*)(lds + L::JOIN) + wr * 128;
+    lds_barrier();
+    if (wp == 1 && works) {
+#pragma unroll
+      for (int n = 0; n < 32; ++n) oj[n * 64 + lane] = O[n] * e2;
+      st[lane] = m;
+      st[64 + lane] = l;
+    }
+    lds_barrier();
+    if (wp == 1 || !works) return;
+    const float mo = st[lane], lo = st[64 + lane], mn = fmaxf(m, mo);
+    const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * p.c), c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
+    l = (m == -__builtin_inff() ? l : l * a) + (mo == -__builtin_inff() ? lo : lo * c);
+#pragma unroll
+    for (int n = 0; n < 32; ++n) O[n] = O[n] * (e2 * a) + oj[n * 64 + lane] * c;
+    m = mn;
+    e2 = 1.f;
+  } else {
+    lds_barrier();
+    if (!works) return;
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float ln = m == -__builtin_inff() && l == l ? m : m * p.c * 0.69314718055994531f + (__builtin_log2f(l) - UP) * 0.69314718055994531f;
   const bool whole = p.S == 1;
+  const long long r = r0 + qr;
   if (qt == 0 && qr < live) {
-    const long long r = r0 + qr;
-    if (whole) {
-      if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
-    } else {
-      p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
-    }
+    if (!whole) p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
+    else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
-  if (lane == 0) ((SPMLA_LDS int*)(lds + L::FLAG))[w] = odd_from;
-  lds_barrier();
-  if constexpr (NH > 1) {                                 // (the wave of the same group that came first took them out for both)
-    const int other = __builtin_amdgcn_readfirstlane(((SPMLA_LDS int*)(lds + L::FLAG))[w ^ 4]);
-    odd_from = odd_from < other ? odd_from : other;
-  }
-  const float back = p.kv_scale;
-  float a[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) a[i] = inv[HR * half + 32 * i + l32] * back;
-  const float e2 = R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23);
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) O[x][i][r] = O[x][i][r] * e2 * a[i];
-  if (__builtin_expect(odd_from < ke, 0)) {               // V that is no number, for the rows that see it
-    int lim[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = HR * half + 32 * i + l32;
-      lim[i] = limit_of(row < live ? row : live - 1);
-    }
-    for (int pos = odd_from; pos < ke; ++pos) {
-      const int page = btrow[pos / p.bs];
-      const long long y = (long long)page * p.stride + pos % p.bs;
-      if (page < 0 || y >= p.rows) continue;
-      const uint8_t* row = p.cache + y * RB;
-      const float sc = R5 ? 1.f : *(const float*)(row + SC_OFF + 4 * wl);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float v = e4m3_to_f32(row[128 * wl + 32 * x + 8 * (r >> 2) + 4 * hh + (r & 3)]) * sc * p.kv_scale;
-          const float add = fabsf(v) < __builtin_inff() ? 0.f : v;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) O[x][i][r] += pos < lim[i] ? add : 0.f;
-        }
-    }
-  }
+  const float back = e2 * inv * p.kv_scale;
   if (!whole) {
+    float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r) * D_LAT + 4 * qt;
+    if (qr < live)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = HR * half + 32 * i + l32;
-      if (row >= live) continue;
-      float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r0 + row) * D_LAT + 128 * wl + 4 * hh;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *(f32x4*)(o + 32 * x + 8 * q) = f32x4{O[x][i][4 * q], O[x][i][4 * q + 1], O[x][i][4 * q + 2], O[x][i][4 * q + 3]};
-    }
+      for (int n = 0; n < 32; ++n) *(f32x4*)(o + 16 * n) = O[n] * back;
     return;
   }
-  // bf16 rows through LDS, 32 at a time: the wave's 128 dims, 16-byte chunks permuted by the row
-  SPMLA_LDS uint8_t* ob = lds + w * (32 * 256);
-  static_assert(4 * NH * 32 * 256 <= L::FAC, "the output's rows fit below the factors");
+  // bf16 rows through LDS: 16 of 1024 bytes, 16-byte chunks permuted by the row
+  SPMLA_LDS uint8_t* ob = lds + wr * 16384;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(SPMLA_LDS i32x2*)(ob + l32 * 256 + 16 * ((4 * x + q) ^ l16) + 8 * hh) =
-            i32x2{(int)pk_bf16(O[x][i][4 * q], O[x][i][4 * q + 1]), (int)pk_bf16(O[x][i][4 * q + 2], O[x][i][4 * q + 3])};
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int row = 4 * k + qt;
-      if (HR * half + 32 * i + row < live) {
-        const long long r = r0 + HR * half + 32 * i + row;
-        *(u32x4*)(p.out + (t0 + r / p.H) * p.o_st + (r % p.H) * p.o_sh + 128 * wl + 8 * l16) =
-            *(SPMLA_LDS u32x4*)(ob + row * 256 + 16 * (l16 ^ (row & 15)));
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int n = 0; n < 32; ++n) {
+    const f32x4 y = O[n] * back;
+    *(SPMLA_LDS i32x2*)(ob + l16 * 1024 + 16 * ((2 * n + (qt >> 1)) ^ l16) + 8 * (qt & 1)) = i32x2{(int)pk_bf16(y[0], y[1]), (int)pk_bf16(y[2], y[3])};
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int row = 0; row < 16 && 16 * wr + row < live; ++row) {
+    const long long y = r0 + 16 * wr + row;
+    *(u32x4*)(p.out + (t0 + y / p.H) * p.o_st + (y % p.H) * p.o_sh + 8 * lane) = *(SPMLA_LDS u32x4*)(ob + row * 1024 + 16 * (lane ^ row));
   }
 }
 
@@ -674,7 +513,7 @@ extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int S) {
 
 extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                                 int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, int wide, void* out,
+                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
                                 long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream) {
   if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || S < 1 || span < 1 ||
       span % chunk::TR || (row_bytes != ROW656 && row_bytes != ROW576))
@@ -687,8 +526,10 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
     return SPMLA_EALIGN;
   if (S > 1 && (!ws || ((uintptr_t)ws & 15))) return ws ? SPMLA_EALIGN : SPMLA_EARG;
   if (S > 1 && ws_bytes < spmla_attn_chunk_ws_bytes(T, H, S)) return SPMLA_EARG;
-  const int r5 = row_bytes == ROW576, nh = wide ? 2 : 1;
-  const long long tiles = (long long)T * H / (chunk::HR * nh) + B;
+  const int r5 = row_bytes == ROW576;
+  // requests of 64 (token, head) rows or fewer on average: workgroups of 64 rows whose waves share the positions
+  const int narrow = (long long)T * H <= 64ll * B;
+  const long long tiles = (long long)T * H / (narrow ? 64 : 128) + B;
   if (tiles * S > (1ll << 30)) return SPMLA_ELIMIT;
   float* opart = (float*)ws;
   float* lpart = opart ? opart + (long long)T * H * S * D_LAT : nullptr;
@@ -698,13 +539,13 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
                   l_st, opart, lpart};
   static DynLds attr[4];
   static Launcher go[4];
-  const int at = 2 * (nh - 1) + r5;
+  const int at = 2 * narrow + r5;
   const void* fn[4] = {(const void*)chunk::kernel<false, 1>, (const void*)chunk::kernel<true, 1>, (const void*)chunk::kernel<false, 2>,
                        (const void*)chunk::kernel<true, 2>};
-  const int lds[4] = {chunk::Lds<false, 1>::TOTAL, chunk::Lds<true, 1>::TOTAL, chunk::Lds<false, 2>::TOTAL, chunk::Lds<true, 2>::TOTAL};
+  const int lds[4] = {chunk::Lds<false, 1>::BYTES, chunk::Lds<true, 1>::BYTES, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES};
   if (const int rc = attr[at].ensure(fn[at], lds[at])) return rc;
   hipStream_t s = (hipStream_t)stream;
-  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), 256 * nh, lds[at], s, p)) return rc;
+  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), 512, lds[at], s, p)) return rc;
   if (S == 1) return SPMLA_OK;
   static Launcher join;
   const chunk::MergeParams mp{opart, lpart, start, B, T, H, S, (uint16_t*)out, o_st, o_sh, lse, l_st};

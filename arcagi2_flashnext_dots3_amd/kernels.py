@@ -1138,24 +1138,18 @@ def attend_prompt(q, k, v, start, scale, causal=True, out=None, lse=None):
     return out, lse
 
 
-def chunk_wide(T, H, B):
-    """Whether attend_chunk takes 128 (token, head) rows of a request per workgroup."""
-    return T * H >= 128 * B
-
-
 @functools.lru_cache(maxsize=4096)
 def chunk_split(T, H, B, longest, cus=256):
     """(splits, positions of each) of attend_chunk for T tokens of H heads in B requests of up to `longest` cached rows."""
-    tiles = T * H // 64 + min(B, T)
-    tiles = max(1, tiles)
+    tiles = max(1, T * H // 128 + (min(B, T) if H % 128 else 0))
     units = max(1, -(-longest // 32))                    # tiles of 32 positions
-    split = max(1, min(2 * cus // tiles, -(-units // 8), 128))
+    split = max(1, min(cus // tiles, -(-units // 8), 128))
     span = -(-units // split)
     return -(-units // span), 32 * span
 
 
 def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0, max_seq_len=None, out=None, lse=None,
-                 split=None, wide=None):
+                 split=None):
     """Attention of new tokens over every cached row of their request: tokens start[b] .. start[b + 1] - 1 of q [T, H, 576] bf16
     (start [B + 1] int32) are the last of the seq_lens[b] rows that request b has in cache [blocks, block_size, 656 or 576]
     uint8 (already written; block stride any whole number of rows) through block_table [B, columns] int32; each token sees
@@ -1177,6 +1171,5 @@ def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0,
     if lse is None:
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
     ws = torch.empty(T * H * split * (D_LAT + 1) * 4, dtype=torch.uint8, device=q.device) if split > 1 else None
-    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, split, span, out, lse, ws,
-                     chunk_wide(T, H, block_table.shape[0]) if wide is None else wide)
+    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, split, span, out, lse, ws)
     return out, lse

@@ -544,14 +544,12 @@ int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void*
  * bf16 = kv_scale * sum p latent, lse [T][H] optional, as spmla_attn_splitk over all of these rows; a token without one gets
  * 0 and -inf, tokens of no request nothing. Positions are cut into S splits of span each (a multiple of 32; the last one
  * takes the rest; S <= 256), joined by a second kernel through a workspace of spmla_attn_chunk_ws_bytes (S > 1).
- * wide: 128 (token, head) rows of a request per workgroup instead of 64 (faster where requests have that many; the result
- * is the same).
  * The dense counterpart of PortableSparseImpl.forward_mqa (dsa_sm89.py:379-470) for layers without an indexer. */
 long long spmla_attn_chunk_ws_bytes(int T, int H, int S);
 int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                      int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, int wide,
-                     void* out, long long o_st, long long o_sh, float* lse, long long l_st, void* ws,
+                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
+                     long long o_st, long long o_sh, float* lse, long long l_st, void* ws,
                      long long ws_bytes, void* stream);
 
 /* Build identification string (static storage). */

@@ -79,9 +79,8 @@ CASES = [  # rows cached (with the new ones), new tokens, heads, page
 
 @pytest.mark.parametrize("seqs,lens,H,bs", CASES)
 @pytest.mark.parametrize("row", [656, 576])
-@pytest.mark.parametrize("wide", [False, True])
-def test_against_64_bits(dev, seqs, lens, H, bs, row, wide):
-    _run(dev, _case(seqs, lens, H, row, bs, H + bs), bs, 1.0 if row == 656 else 0.25, wide=wide)
+def test_against_64_bits(dev, seqs, lens, H, bs, row):
+    _run(dev, _case(seqs, lens, H, row, bs, H + bs), bs, 1.0 if row == 656 else 0.25)
 
 
 @pytest.mark.parametrize("row", [656, 576])
@@ -144,8 +143,7 @@ def test_scales_far_apart(dev, spread):
 
 
 @pytest.mark.parametrize("row", [656, 576])
-@pytest.mark.parametrize("wide", [False, True])
-def test_no_numbers_in_rows_behind_a_token(dev, row, wide):
+def test_no_numbers_in_rows_behind_a_token(dev, row):
     """A chunk's row that is no number reaches the tokens at and behind it only."""
     q, cache, table, seqs, start = _case([150], [100], 4, row, 16, 2)
     at = 120                                                   # position of the chunk's token 70
@@ -153,7 +151,7 @@ def test_no_numbers_in_rows_behind_a_token(dev, row, wide):
     before = cache[page, off].clone()
     cache[page, off, 300] = 0x7F                               # a NaN code, dim 300
     from arcagi2_flashnext_dots3_amd import kernels
-    out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM, wide=wide)
+    out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM)
     torch.cuda.synchronize()
     assert bool(out[:70].isfinite().all()) and bool(lse[:70].isfinite().all())
     assert bool(out[70:, :, 300].isnan().all())
@@ -161,7 +159,7 @@ def test_no_numbers_in_rows_behind_a_token(dev, row, wide):
     _check(out[:70].cpu(), lse[:70].cpu(), q[:70], cache, table, torch.tensor([at]), torch.tensor([0, 70]), 1.0, 16)
     if row == 656:                                             # a scale that is infinite
         cache[page, off, 516:520] = torch.tensor([float("inf")]).view(torch.uint8)
-        out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM, wide=wide)
+        out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM)
         torch.cuda.synchronize()
         cache[page, off] = before
         _check(out[:70].cpu(), lse[:70].cpu(), q[:70], cache, table, torch.tensor([at]), torch.tensor([0, 70]), 1.0, 16)
