@@ -29,7 +29,7 @@ namespace chunk {
 
 constexpr int TR = 32;                // positions per tile
 constexpr int IDS = 256;              // positions whose rows are looked up at a time
-constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;
+constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f, WIDE = 64.f;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -42,7 +42,7 @@ struct Params {
   const int* table; long long t_st; int W;
   const int* seqs; const int* start; int B, T, H, S, span; // splits of span positions each (a multiple of TR)
   float c, kv_scale;                                       // |sm_scale kv_scale| log2(e)
-  int flip, tiles;
+  int flip, tiles, slack;                                  // slack: requests may end inside a tile of query rows
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
   float* opart; float* lpart;                              // [S][T][H][512], [S][T][H]
@@ -121,19 +121,19 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   const int wr = PS == 1 ? w : w & 3, wp = PS == 1 ? 0 : w >> 2;          // the wave's 16 rows; which of PS tiles it takes
   const int l16 = lane & 15, l32 = lane & 31, qt = lane >> 4;
 
-  // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / MR + b.
+  // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / MR (+ b where requests may end inside one).
   const int f = remap_xcd(blockIdx.x, p.tiles * p.S);
   if (f < 0) return;
   const int sp = f / p.tiles, ti = p.tiles - 1 - f % p.tiles;
   int nb = 0;
   for (int at = 0; at < p.B; at += 64) {
     const int b = at + lane;
-    const bool in = b < p.B && (long long)p.start[b] * p.H / MR + b <= ti;
+    const bool in = b < p.B && (long long)p.start[b] * p.H / MR + (p.slack ? b : 0) <= ti;
     nb += __popcll(__ballot(in));
   }
   const int b = nb > 0 ? nb - 1 : 0;
   int t0 = p.start[b], t1 = p.start[b + 1];
-  const long long r0 = (long long)(ti - (int)((long long)t0 * p.H / MR) - b) * MR;
+  const long long r0 = (long long)(ti - (int)((long long)t0 * p.H / MR) - (p.slack ? b : 0)) * MR;
   t0 = t0 < 0 ? 0 : t0;
   t1 = t1 > p.T ? p.T : t1;
   const long long nrows = (long long)(t1 - t0) * p.H;
@@ -460,6 +460,399 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   }
 }
 
+// ---- 65 rows and more of a request: workgroups of 128 rows, 4 waves of 32 rows (one a SIMD, 512 registers). The codes of a
+// tile are converted to bf16 once, into a tile in LDS that both products read: K by rows, V by the 16-bit transposing read.
+template <bool R5>
+struct WLds {
+  static constexpr int RING = 4;
+  static constexpr int CODE = 4 * TR * 128;                // codes by scale group, [4][32 rows][128]
+  static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
+  static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
+  static constexpr int TILE = CODE + RP + SC;
+  static constexpr int NG = R5 ? 9 : 8;                    // groups of 64 dims in bf16, [NG][32 rows][128 bytes]
+  static constexpr int B = RING * TILE;                    // two of them
+  static constexpr int ID = B + 2 * NG * 4096;             // addresses of the rows of two times IDS positions
+  static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
+  static constexpr int OVER = OK + 2 * IDS / 32 * 4;       // a row's scores have left its reference's range
+  static constexpr int TOTAL = OVER + 16;
+  static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// QK products with their sums in VGPRs (the builtin would put them into AGPRs, which O fills). What the compiler cannot see
+// inside asm: operands come from LDS or were written long before; a chain's result is read 12 wait states after it.
+__device__ inline f32x16 qk_first(bf16x8 a, bf16x8 b) {
+  f32x16 d;
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  return d;
+}
+__device__ inline f32x16 qk_next(bf16x8 a, bf16x8 b, f32x16 c) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  return c;
+}
+template <bool R5>
+__global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
+  using L = WLds<R5>;
+  constexpr int RB = R5 ? ROW576 : ROW656, MR = 128;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
+  SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, l32 = lane & 31, hh = lane >> 5;
+
+  // ---- work item, as above
+  const int f = remap_xcd(blockIdx.x, p.tiles * p.S);
+  if (f < 0) return;
+  const int sp = f / p.tiles, ti = p.tiles - 1 - f % p.tiles;
+  int nb = 0;
+  for (int at = 0; at < p.B; at += 64) {
+    const int b = at + lane;
+    const bool in = b < p.B && (long long)p.start[b] * p.H / MR + (p.slack ? b : 0) <= ti;
+    nb += __popcll(__ballot(in));
+  }
+  const int b = nb > 0 ? nb - 1 : 0;
+  int t0 = p.start[b], t1 = p.start[b + 1];
+  const long long r0 = (long long)(ti - (int)((long long)t0 * p.H / MR) - (p.slack ? b : 0)) * MR;
+  t0 = t0 < 0 ? 0 : t0;
+  t1 = t1 > p.T ? p.T : t1;
+  const long long nrows = (long long)(t1 - t0) * p.H;
+  if (r0 < 0 || r0 >= nrows) return;
+  const int live = nrows - r0 < MR ? (int)(nrows - r0) : MR;
+  const int past = p.seqs[b] - (t1 - t0);
+  const long long cap = (long long)p.W * p.bs;
+  auto limit_of = [&](int r) -> int {
+    const long long x = (long long)past + (r0 + r) / p.H + 1;
+    return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
+  };
+  const int least = limit_of(0), most = limit_of(live - 1);
+  const long long first = (long long)sp * p.span;
+  const int kb = first < most ? (int)first : most;
+  const int ke = sp + 1 < p.S && first + p.span < most ? (int)(first + p.span) : most;
+  const int nt = (ke - kb + TR - 1) / TR;
+  if (nt <= 0 && sp > 0) {
+    if (tid < live) p.lpart[((long long)sp * p.T + t0) * p.H + r0 + tid] = -__builtin_inff();
+    return;
+  }
+  const int* btrow = p.table + (long long)b * p.t_st;
+  // the lane id, opaque in every step: LDS places made of it are formed again, not kept (the query alone takes 144 registers)
+  auto here = [&]() -> int {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto look = [&](int part) -> int {
+    const int tid = 64 * w + here();
+    const int pos = kb + part * IDS + tid;
+    if (pos >= ke) return -1;
+    const int page = btrow[pos / p.bs];
+    const long long y = (long long)page * p.stride + pos % p.bs;
+    return page >= 0 && y < p.rows ? (int)y : -1;
+  };
+  auto note = [&](int part, int row) {
+    const int lane = here(), tid = 64 * w + lane, l32 = lane & 31;
+    const int at = (part & 1) * IDS + tid;
+    const uint64_t a = (uint64_t)(uintptr_t)p.cache + (uint64_t)(uint32_t)row * RB;
+    ((SPMLA_LDS uint64_t*)(lds + L::ID))[at] = row >= 0 ? a : (uint64_t)(uintptr_t)zero_row;
+    const uint64_t has = __ballot(row >= 0);
+    if (l32 == 0) ((SPMLA_LDS uint32_t*)(lds + L::OK))[at >> 5] = (uint32_t)(has >> (lane & 32));
+  };
+
+  // ---- query operands of rows 32 w + l32: B operands of 32x32x16, dims 16 ks + 8 hh ..
+  const int qr = 32 * w + l32;
+  bf16x8 qf[36];
+  {
+    const long long r = r0 + (qr < live ? qr : live - 1);
+    const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
+    const uint32_t turn = p.flip ? 0x80008000u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < 36; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + 16 * ks + 8 * hh) ^ turn);
+  }
+
+  // ---- copies of a tile, in COPIES pieces: wave w the codes of scale group w (piece i: rows 8 i + lane / 8, the chunk whose
+  // place is lane % 8), a share of the rope and of the scales. Behind the last tile they copy rows that are there, unused.
+  constexpr int COPIES = R5 ? 5 : 6;
+  auto address = [&](int j, int i) -> uint64_t {          // of the lane's source in piece i
+    const int lane = here(), r = lane >> 3, place = (lane & 7) ^ swz(r);
+    SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
+    if (i < 4) return id[8 * i + r] + (uint32_t)(128 * w + 16 * (place ^ ((i & 1) << 1)));
+    // Row576: 16 rows of 64 bytes, waves 2 and 3 repeat those of 0 and 1; Row656: 8 rows of rope, 64 scales
+    if constexpr (R5) return id[16 * (w & 1) + (lane >> 2)] + (uint32_t)(D_LAT + 16 * (lane & 3));
+    if (i == 4) return id[8 * w + r] + (uint32_t)(ROPE_OFF + 16 * (place ^ ((w & 1) << 1)));
+    return id[lane & 31] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + (lane >> 5)));
+  };
+  auto copy = [&](int j, int i, uint64_t from) {
+    SPMLA_LDS uint8_t* d = lds + (j & 3) * L::TILE;
+    if (i < 4) dma16((const void*)from, d + w * 4096 + i * 1024);
+    else if (R5) dma16((const void*)from, d + L::CODE + (w & 1) * 1024);
+    else if (i == 4) dma16((const void*)from, d + L::CODE + w * 1024);
+    else dma4((const void*)from, d + L::CODE + L::RP + (w & 1) * 256);
+  };
+
+  // ---- codes of tile j to bf16: piece i of 4 of the wave's group (16 codes a lane: row 8 i + lane / 8), piece 4: rope (Row576)
+  auto codes = [&](int j, int i) -> i32x4 {
+    const int lane = here();
+    SPMLA_LDS uint8_t* d = lds + (j & 3) * L::TILE;
+    if (i < 4) return *(SPMLA_LDS i32x4*)(d + w * 4096 + i * 1024 + lane * 16);
+    const i32x2 y = *(SPMLA_LDS i32x2*)(d + L::CODE + w * 512 + lane * 8);
+    return i32x4{y[0], y[1], 0, 0};
+  };
+  auto convert = [&](int j, int i, i32x4 y) {
+    const int lane = here(), r = lane >> 3, x = swz(r);
+    SPMLA_LDS uint8_t* to = lds + L::B + (j & 1) * (L::NG * 4096);
+    if (i < 4) {
+      const int c = (lane & 7) ^ x;
+      const int at = (c >> 2) * 4096 + r * 128 + ((16 * ((2 * (c & 3)) ^ x)) ^ ((i & 1) * 96));
+      *(SPMLA_LDS bf16x8*)(to + w * 8192 + i * 1024 + at) = codes8_bf16(y[0], y[1]);
+      *(SPMLA_LDS bf16x8*)(to + w * 8192 + i * 1024 + (at ^ 16)) = codes8_bf16(y[2], y[3]);
+    } else if constexpr (R5) {
+      *(SPMLA_LDS bf16x8*)(to + 8 * 4096 + w * 1024 + r * 128 + 16 * ((lane & 7) ^ swz(8 * w + r))) = codes8_bf16(y[0], y[1]);
+    }
+  };
+  constexpr int PIECES = R5 ? 5 : 4;                      // of a tile's conversion
+
+  // ---- passes: a row's reference is the first maximum it meets and does not move (weights in bf16 have fp32's range, so O,
+  // which fills the AGPRs, is not rescaled). Where scores rise by more than 2^WIDE over it (rare), a pass takes the maxima
+  // alone and another one starts from those.
+  f32x16 O[16];                                           // O^T: dims 32 n + 8 a + 4 hh + b, query row qr
+  float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, of both halves; l: this half's)
+  SPMLA_LDS int* over = (SPMLA_LDS int*)(lds + L::OVER);
+  bool maxima = false;
+  for (;;) {
+  if (tid == 0) *over = 0;
+  int found = -1;
+  note(0, look(0));
+  note(1, -1);                                            // (addresses that a copy may take, whatever the tile)
+  l = 0.f;
+#pragma unroll
+  for (int n = 0; n < 16; ++n) O[n] = f32x16{};
+  lds_barrier();
+  for (int j = 0; j < 3; ++j)
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) copy(j, i, address(j, i));
+  wait_vm<2 * COPIES>();
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) convert(0, i, codes(0, i));
+#pragma unroll 1
+  for (int j = 0; j < nt; ++j) {
+    const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
+    wait_vm<COPIES>();                                    // tile j + 1 is there
+    lds_barrier();                                        // and tile j in bf16
+    if (in == 0 && next * (IDS / TR) < nt) found = look(next);
+    if (in == 2 && next * (IDS / TR) < nt) note(next, found);
+    SPMLA_LDS uint8_t* kt = lds + L::B + (j & 1) * (L::NG * 4096);
+    SPMLA_LDS uint8_t* raw = lds + (j & 3) * L::TILE;
+    // ---- S^T = K Q^T; beside it the copies of tile j + 3 and the conversion of tile j + 1, piece by piece
+    f32x16 S;
+    {
+      const int lane = here(), l32 = lane & 31, hh = lane >> 5;
+      const int ka = l32 * 128 + 16 * (hh ^ swz(l32));
+      auto kread = [&](int ks) -> bf16x8 {
+        SPMLA_LDS uint8_t* at = !R5 && ks >= 32 ? raw + L::CODE : kt + (ks >> 2) * 4096;
+        return *(SPMLA_LDS bf16x8*)(at + (ka ^ (32 * (ks & 3))));
+      };
+      constexpr int KD = R5 ? 8 : 6;
+      bf16x8 k[KD];
+#pragma unroll
+      for (int n = 0; n < KD; ++n) k[n] = kread(n);
+      uint64_t from = 0;
+      i32x4 y = {};
+      auto beside = [&](int ks) {                         // what runs beside product ks: piece ks / 6 of copies and codes
+        const int i = ks / 6, at = ks % 6;
+        if (at == 0 && i < COPIES) from = address(j + 3, i);
+        if (at == 1 && i < PIECES) y = codes(j + 1, i);
+        if (at == 3 && i < COPIES) copy(j + 3, i, from);
+        if (at == 4 && i < PIECES) convert(j + 1, i, y);
+      };
+      if constexpr (R5) {
+#pragma unroll
+        for (int ks = 0; ks < 36; ++ks) {
+          S = ks == 0 ? qk_first(k[0], qf[0]) : qk_next(k[ks % KD], qf[ks], S);
+          if (ks + KD < 36) k[ks % KD] = kread(ks + KD);
+          beside(ks);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        f32x16 acc[2];
+        S = f32x16{};
+#pragma unroll
+        for (int g = 0; g < 5; ++g) {
+          if (g < 4) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              const int ks = 8 * g + n;
+              acc[g & 1] = n == 0 ? qk_first(k[ks % KD], qf[ks]) : qk_next(k[ks % KD], qf[ks], acc[g & 1]);
+              if (ks + KD < 36) k[ks % KD] = kread(ks + KD);
+              beside(ks);
+              if (g > 0 && n >= 4) {                      // a quarter of the group before: its products are done
+                const int a = n - 4;
+                asm volatile("" : "+v"(acc[(g - 1) & 1]));
+                const f32x4 sc = *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + (g - 1) * 128 + 32 * a + 16 * hh);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[4 * a + r] = __builtin_fmaf(acc[(g - 1) & 1][4 * a + r], sc[r], S[4 * a + r]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          } else {
+            f32x4 sc[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) sc[a] = *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + 3 * 128 + 32 * a + 16 * hh);
+            beside(33);
+            asm volatile("s_nop 15" : "+v"(acc[1]));
+            beside(34);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] = __builtin_fmaf(acc[1][r], sc[r >> 2][r & 3], S[r]);
+          }
+        }
+        asm volatile("s_nop 1" : "+v"(S));                // (written by the VALU just before)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) S = qk_next(k[(32 + n) % KD], qf[32 + n], S);
+      }
+      asm volatile("s_nop 15" : "+v"(S));
+    }
+    // ---- softmax
+    const int lane = here(), l16 = lane & 15, l32 = lane & 31, hh = lane >> 5, qr = 32 * w + l32;
+    const uint32_t has = __builtin_amdgcn_readfirstlane(((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
+    const int k0 = kb + j * TR;
+    if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
+      asm volatile("" : "+v"(S));
+      const int limit = limit_of(qr < live ? qr : live - 1);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = 8 * (r >> 2) + 4 * hh + (r & 3);
+        S[r] = (has >> x & 1) && k0 + x < limit ? S[r] : -__builtin_inff();
+      }
+    }
+    if (__builtin_expect(k0 + TR > least && least < most, 0)) {
+      // the mask cuts this tile: values that are no numbers become 0 once every wave has its scores
+      lds_barrier();
+      for (int i = 0; i < 8; ++i) {                       // (every wave all of them: others read them beside this)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(kt + i * 4096 + r * 1024 + lane * 16);
+          u32x4 y = *at;
+          uint32_t bad = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t keep = ((y[e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((y[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+            bad |= ~keep;
+            y[e] &= keep;
+          }
+          if (bad) *at = y;
+        }
+      }
+      if (!R5) {
+        SPMLA_LDS f32x2* at = (SPMLA_LDS f32x2*)(raw + L::CODE + L::RP) + lane;
+        f32x2 y = *at;
+        const bool bad = !(fabsf(y[0]) < __builtin_inff()) || !(fabsf(y[1]) < __builtin_inff());
+        y[0] = fabsf(y[0]) < __builtin_inff() ? y[0] : 0.f;
+        y[1] = fabsf(y[1]) < __builtin_inff() ? y[1] : 0.f;
+        if (bad) *at = y;
+      }
+    }
+    float mx = S[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
+    mx = swap32_max(mx);
+    m = m == -__builtin_inff() ? mx : m;
+    if (__builtin_expect(maxima, 0)) m = fmaxf(m, mx);
+    if (__builtin_expect(__any((mx - m) * p.c > WIDE), 0) && lane == 0) *over = 1;
+    const float base = m == -__builtin_inff() ? 0.f : m, ref = -base * p.c;
+    if (__builtin_expect(__any(fabsf(ref) > FAR), 0)) {    // the rounding of m c would count: differences first
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f((S[r] - base) * p.c);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, ref));
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += S[r];
+    l += sum;
+    // ---- O^T += V^T P^T
+    {
+      bf16x8 P[2];
+      auto weights = [&](int g) {
+        f32x4 t[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          t[a] = f32x4{S[4 * a], S[4 * a + 1], S[4 * a + 2], S[4 * a + 3]};
+          if constexpr (!R5) t[a] *= *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + g * 128 + 32 * a + 16 * hh);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+          P[ks] = __builtin_bit_cast(bf16x8, u32x4{pk_bf16(t[2 * ks][0], t[2 * ks][1]), pk_bf16(t[2 * ks][2], t[2 * ks][3]),
+                                                   pk_bf16(t[2 * ks + 1][0], t[2 * ks + 1][1]), pk_bf16(t[2 * ks + 1][2], t[2 * ks + 1][3])});
+      };
+      const int vrow = 4 * hh + (l16 >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const int v0 = vrow * 128 + 16 * (vch ^ swz(vrow)) + 8 * (lane & 1);  // (rows 8 on: places ^ 2; the group's other half: ^ 4)
+      auto vread = [&](int n) -> bf16x8 {                  // unit n = 2 d + ks: dims 32 d + l32, positions 16 ks ..
+        SPMLA_LDS uint8_t* at = kt + (n >> 2) * 4096 + (n & 1) * 2048;
+        const int c = (n >> 1 & 1) * 64;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SPMLA_LDS s16x4*)(at + (v0 ^ c)));
+        const s16x4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SPMLA_LDS s16x4*)(at + 1024 + (v0 ^ c ^ 32)));
+        const auto x = __builtin_bit_cast(i32x2, a), y = __builtin_bit_cast(i32x2, e);
+        return __builtin_bit_cast(bf16x8, i32x4{x[0], x[1], y[0], y[1]});
+      };
+      constexpr int VD = 6;
+      bf16x8 v[VD];
+#pragma unroll
+      for (int n = 0; n < VD; ++n) v[n] = vread(n);
+      if constexpr (R5) weights(0);
+#pragma unroll
+      for (int n = 0; n < 32; ++n) {
+        if (!R5 && n % 8 == 0) weights(n / 8);
+        O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % VD], P[n & 1], O[n >> 1], 0, 0, 0);
+        if (n + VD < 32) v[n % VD] = vread(n + VD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  wait_vm<0>();
+  lds_barrier();
+  const int gone = __builtin_amdgcn_readfirstlane(*over);
+  if (__builtin_expect(!gone && !maxima, 1)) break;
+  maxima = gone != 0;
+  lds_barrier();
+  }
+
+  // ---- output
+  l = swap32_sum(l);
+  if (32 * w >= live) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float ln = m == -__builtin_inff() && l == l ? m : m * p.c * 0.69314718055994531f + __builtin_log2f(l) * 0.69314718055994531f;
+  const bool whole = p.S == 1;
+  const long long r = r0 + qr;
+  if (hh == 0 && qr < live) {
+    if (!whole) p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
+    else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
+  }
+  const float back = inv * p.kv_scale;
+  if (!whole) {
+    float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r) * D_LAT + 4 * hh;
+    if (qr < live)
+#pragma unroll
+      for (int n = 0; n < 16; ++n)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *(f32x4*)(o + 32 * n + 8 * a) = f32x4{O[n][4 * a], O[n][4 * a + 1], O[n][4 * a + 2], O[n][4 * a + 3]} * back;
+    return;
+  }
+  SPMLA_LDS uint8_t* ob = lds + w * 32768;                // 32 rows of 1024 bytes, 16-byte chunks permuted by the row
+#pragma unroll
+  for (int n = 0; n < 16; ++n)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      *(SPMLA_LDS i32x2*)(ob + l32 * 1024 + 16 * ((4 * n + a) ^ l32) + 8 * hh) =
+          i32x2{(int)pk_bf16(O[n][4 * a] * back, O[n][4 * a + 1] * back), (int)pk_bf16(O[n][4 * a + 2] * back, O[n][4 * a + 3] * back)};
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int row = 0; row < 32 && 32 * w + row < live; ++row) {
+    const long long y = r0 + 32 * w + row;
+    *(u32x4*)(p.out + (t0 + y / p.H) * p.o_st + (y % p.H) * p.o_sh + 8 * lane) = *(SPMLA_LDS u32x4*)(ob + row * 1024 + 16 * (lane ^ row));
+  }
+}
+
 // Joins the splits of query row (t, h): weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
 // was not written, is not read. One wave a row, 8 dims a lane.
 struct MergeParams {
@@ -529,23 +922,24 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const int r5 = row_bytes == ROW576;
   // requests of 64 (token, head) rows or fewer on average: workgroups of 64 rows whose waves share the positions
   const int narrow = (long long)T * H <= 64ll * B;
-  const long long tiles = (long long)T * H / (narrow ? 64 : 128) + B;
+  const int mr = narrow ? 64 : 128, slack = H % mr != 0;
+  const long long tiles = (long long)T * H / mr + (slack ? B : 0);
   if (tiles * S > (1ll << 30)) return SPMLA_ELIMIT;
   float* opart = (float*)ws;
   float* lpart = opart ? opart + (long long)T * H * S * D_LAT : nullptr;
   const float sc = sm_scale * kv_scale;
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
-                  H, S, span, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)tiles, (uint16_t*)out, o_st, o_sh, lse,
+                  H, S, span, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)tiles, slack, (uint16_t*)out, o_st, o_sh, lse,
                   l_st, opart, lpart};
   static DynLds attr[4];
   static Launcher go[4];
   const int at = 2 * narrow + r5;
-  const void* fn[4] = {(const void*)chunk::kernel<false, 1>, (const void*)chunk::kernel<true, 1>, (const void*)chunk::kernel<false, 2>,
+  const void* fn[4] = {(const void*)chunk::wide_kernel<false>, (const void*)chunk::wide_kernel<true>, (const void*)chunk::kernel<false, 2>,
                        (const void*)chunk::kernel<true, 2>};
-  const int lds[4] = {chunk::Lds<false, 1>::BYTES, chunk::Lds<true, 1>::BYTES, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES};
+  const int lds[4] = {chunk::WLds<false>::TOTAL, chunk::WLds<true>::TOTAL, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES};
   if (const int rc = attr[at].ensure(fn[at], lds[at])) return rc;
   hipStream_t s = (hipStream_t)stream;
-  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), 512, lds[at], s, p)) return rc;
+  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), narrow ? 512 : 256, lds[at], s, p)) return rc;
   if (S == 1) return SPMLA_OK;
   static Launcher join;
   const chunk::MergeParams mp{opart, lpart, start, B, T, H, S, (uint16_t*)out, o_st, o_sh, lse, l_st};

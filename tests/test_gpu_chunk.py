@@ -53,11 +53,11 @@ def _check(out, lse, q, cache, table, seqs, start, kv_scale, bs):
         seen = (x <= (L - n + torch.arange(n))[:, None]) & has
         qs = q[t0:t1].double().transpose(0, 1)
         r = ref.softmax_product(qs, rows[None], rows[None, :, :512], seen, SM)
-        # weights in f16, the largest of a row 2^9 at least: a subnormal one loses 2^-25; values in f16 too (Row656: half a
-        # step for the scale and half for the product), below their normal range 2^-39 of the largest magnitude
+        # weights (times the row's scale in Row656) are rounded once to bf16, or in workgroups of 64 rows to f16, where the
+        # largest of a row is 2^9 at least and a subnormal one loses 2^-25, times what the largest scale so far is
         top = float(rows.abs().max()) if L > 0 else 0.0
-        half = ref.HALF[torch.float16] * (1 if cache.shape[2] == 576 else 3)
-        floor = L * 2.0 ** -34 * top + 2.0 ** -38 * top
+        half = ref.HALF[torch.bfloat16]
+        floor = L * 2.0 ** -33 * top
         ref.check(out[t0:t1].transpose(0, 1), lse[t0:t1].transpose(0, 1), r, 576, max(L, 1), torch.bfloat16, half, floor, f"request {b}: {n} of {L}")
 
 
