@@ -73,7 +73,7 @@ struct Entry<R (*)(A...)> {
   X(spmla_bmm_fp8) X(spmla_mla_query) X(spmla_topk_overlap) X(spmla_mtp_union) X(spmla_attn_packed)                 \
   X(spmla_index_key_write_shuffle) X(spmla_mqa_logits) X(spmla_paged_mqa_logits) X(spmla_paged_mqa_logits_seq)   \
   X(spmla_rms_norm) X(spmla_quant_fp8) X(spmla_linear_fp8) X(spmla_rope) X(spmla_latent_write)  \
-  X(spmla_page_step) X(spmla_page_trim) X(spmla_attn_prompt) X(spmla_attn_chunk_ws_bytes) X(spmla_attn_chunk)
+  X(spmla_page_step) X(spmla_page_trim) X(spmla_attn_prompt) X(spmla_attn_chunk_items) X(spmla_attn_chunk_ws_bytes) X(spmla_attn_chunk)
 
 #define SLOT(name)                                                                                                  \
   decltype(&::name) fn_##name = nullptr;                                                                            \

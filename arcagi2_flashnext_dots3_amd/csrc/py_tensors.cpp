@@ -33,6 +33,7 @@ decltype(&::spmla_page_step) f_page_step = nullptr;
 decltype(&::spmla_page_trim) f_page_trim = nullptr;
 decltype(&::spmla_attn_prompt) f_attn_prompt = nullptr;
 decltype(&::spmla_attn_chunk) f_attn_chunk = nullptr;
+decltype(&::spmla_attn_chunk_ws_bytes) f_attn_chunk_ws_bytes = nullptr;
 PyObject *raw_stream = nullptr, *get_device = nullptr;
 
 // ---- arguments
@@ -479,12 +480,12 @@ long attend_prompt(PyObject* const* a) {
   });
 }
 
-// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, split, span, out, lse, ws)
+// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, items, out, lse, ws)
 long attend_chunk(PyObject* const* a) {
   const at::Tensor *q = tensor(a[0], "q"), *cache = tensor(a[1], "cache"), *table = tensor(a[2], "block_table"), *seqs = tensor(a[3], "seq_lens");
-  const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[9], "out"), *lse = maybe(a[10], "lse"), *ws = maybe(a[11], "ws");
+  const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[8], "out"), *lse = maybe(a[9], "lse"), *ws = maybe(a[10], "ws");
   const double sm = number(a[5]), kvs = number(a[6]);
-  const long long split = integer(a[7]), span = integer(a[8]);
+  const long long items = integer(a[7]);
   if (q->dim() != 3 || type_of(*q) != BF16 || q->size(2) != 576) refuse("q [T, H, 576] bf16: got " + shown(*q));
   const int64_t T = q->size(0), H = q->size(1), B = starts(*start);
   at_most(T, MAX_TOKENS, "T");
@@ -506,11 +507,11 @@ long attend_chunk(PyObject* const* a) {
   at_most(W * bs, 0x7fffff00, "positions of a block table's row");
   line(*seqs, B, B, I32, "seq_lens [requests] int32");
   if (!((float)(sm * kvs) - (float)(sm * kvs) == 0.f)) refuse("sm_scale, kv_scale: finite numbers");
-  if (split < 1 || split > 256) refuse("split of 1 to 256: got " + std::to_string(split));
-  if (span < 32 || span % 32 || span > 0x7fffffe0) refuse("span: a positive multiple of 32");
-  if (split > 1) {
-    if (!ws) refuse("ws: a workspace for split > 1");
-    line(*ws, T * H * split * 513 * 4, ANY, U8, "ws [T * H * split * 2052] uint8");
+  if (items < 0 || items > 65536) refuse("items of 0 to 65536: got " + std::to_string(items));
+  const long long need = f_attn_chunk_ws_bytes((int)T, (int)H, (int)B, (int)rowb, (int)items);
+  if (need > 0) {
+    if (!ws) refuse("ws: a workspace of " + std::to_string(need) + " bytes");
+    line(*ws, need, ANY, U8, "ws uint8 (spmla_attn_chunk_ws_bytes)");
     on_bytes(*ws, 0, 16, "ws");
   }
   const int dev = gpu_of(*q);
@@ -519,7 +520,7 @@ long attend_chunk(PyObject* const* a) {
   return launch(dev, [&](void* s) {
     return f_attn_chunk(address(q), qs.st, qs.sh, address(cache), total, (int)rowb, as_int(bs, "block_size"), stride,
                         (const int*)address(table), tst, (int)W, (const int*)address(seqs), (const int*)address(start), (int)B, (int)T,
-                        (int)H, (float)sm, (float)kvs, (int)split, (int)span, address(out), os.st, os.sh, (float*)address(lse), ls,
+                        (int)H, (float)sm, (float)kvs, (int)items, address(out), os.st, os.sh, (float*)address(lse), ls,
                         address(ws), ws ? ws->numel() : 0, s);
   });
 }
@@ -542,7 +543,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define CALLABLE(name, n) {#name, (PyCFunction)(void (*)())entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(linear_quant, 6),
                        CALLABLE(rope, 8), CALLABLE(latent_write, 13), CALLABLE(page_step, 11), CALLABLE(page_trim, 7),
-                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 12)};
+                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 11)};
 
 PyObject* load(PyObject*, PyObject* args) {
   const char* path;
@@ -554,7 +555,7 @@ PyObject* load(PyObject*, PyObject* args) {
   f_##name = (decltype(f_##name))dlsym(h, "spmla_" #name);                                           \
   if (!f_##name) return PyErr_Format(PyExc_OSError, "%s: no spmla_" #name, path);
   BIND(rms_norm) BIND(quant_fp8) BIND(linear_fp8) BIND(rope) BIND(latent_write) BIND(page_step) BIND(page_trim)
-  BIND(attn_prompt) BIND(attn_chunk)
+  BIND(attn_prompt) BIND(attn_chunk) BIND(attn_chunk_ws_bytes)
   Py_INCREF(rs);
   Py_INCREF(gd);
   raw_stream = rs;

@@ -40,18 +40,130 @@ struct Params {
   const uint8_t* cache; long long rows, stride;            // rows of the cache, rows from a block to the next
   int bs;
   const int* table; long long t_st; int W;
-  const int* seqs; const int* start; int B, T, H, S, span; // splits of span positions each (a multiple of TR)
+  const int* seqs; const int* start; int B, T, H;
   float c, kv_scale;                                       // |sm_scale kv_scale| log2(e)
-  int flip, tiles, slack;                                  // slack: requests may end inside a tile of query rows
+  int flip;
+  int tiles, slack;                                        // slack: requests may end inside a tile of query rows
+  int items, extra;                                        // workgroups that share the positions, those beyond one a tile (0: no splits)
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
-  float* opart; float* lpart;                              // [S][T][H][512], [S][T][H]
+  float* opart; float* lpart; i32x2* parts;                // [slot][MR][512], [slot][MR]; of a (token, head): first row, splits
 };
+
+// ---- which tile of query rows (MR of one request) and which of its splits a workgroup takes.
+// Without splits: request b starts at tile start[b] H / MR (+ b where requests may end inside a tile), found by a search of 64
+// places a step. With them (B <= PLAN): span is the least number of position tiles, no less than an even share, for which
+// splitting every request's positions by it takes at most `extra` workgroups more than one a tile; a request's tiles x splits
+// follow the last request's, and so do the places of partial results, which only split tiles have (at most 2 extra).
+struct Item {
+  int b, tile, sp, splits, span, slot;                     // slot: the tile's first partial result
+};
+constexpr int PLAN = 256, CUS = 256, LEAST = 4;                     // (a split of fewer tiles costs more to join than it saves)
+
+__device__ inline int wave_sum(int x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+__device__ inline int wave_scan(int x, int lane) {         // inclusive
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    x += lane >= d ? y : 0;
+  }
+  return x;
+}
+
+template <int MR>
+__device__ inline bool find_item(const Params& p, int lane, Item& o) {
+  if (p.extra == 0) {
+    const int ti = p.tiles - 1 - (int)blockIdx.x;          // (round robin over the XCDs: they get even shares of long requests)
+    if (ti < 0) return false;
+    int lo = 0, hi = p.B, step;
+    do {
+      step = (hi - lo + 63) >> 6;
+      const int b = lo + lane * step;
+      const int n = __popcll(__ballot(b < hi && (long long)p.start[b] * p.H / MR + (p.slack ? b : 0) <= ti));
+      lo += (n > 0 ? n - 1 : 0) * step;
+      hi = lo + step < hi ? lo + step : hi;
+    } while (step > 1);
+    const long long tile = ti - (long long)p.start[lo] * p.H / MR - (p.slack ? lo : 0);
+    o = Item{lo, (int)tile, 0, 1, 0x7fffffff / TR, 0};
+    return tile >= 0;
+  }
+  int n[PLAN / 64], u[PLAN / 64];                          // of request 64 k + lane: tiles of query rows, tiles of positions
+  const long long cap = (long long)p.W * p.bs;
+  long long work = 0;
+  int top = 1;
+#pragma unroll
+  for (int k = 0; k < PLAN / 64; ++k) {
+    n[k] = 0;
+    u[k] = 1;
+    const int b = 64 * k + lane;
+    if (b < p.B) {
+      const int t0 = p.start[b], t1 = p.start[b + 1], len = p.seqs[b];
+      const long long r = (long long)((t1 > p.T ? p.T : t1) - (t0 < 0 ? 0 : t0)) * p.H, x = len < cap ? len : cap;
+      n[k] = r > 0 ? (int)((r + MR - 1) / MR) : 0;
+      u[k] = x > 0 ? (int)((x + TR - 1) / TR) : 1;
+      work += (long long)n[k] * u[k];
+      top = n[k] > 0 && u[k] > top ? u[k] : top;
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    work += __shfl_xor(work, d);
+    const int y = __shfl_xor(top, d);
+    top = y > top ? y : top;
+  }
+  work = __builtin_amdgcn_readfirstlane((int)work) & 0xffffffffll | (long long)__builtin_amdgcn_readfirstlane((int)(work >> 32)) << 32;
+  top = __builtin_amdgcn_readfirstlane(top);
+  const long long even = (work + p.items - 1) / p.items, most = (work + p.extra - 1) / p.extra;
+  int lo = even < LEAST ? LEAST : even < top ? (int)even : top;
+  int hi = lo < most ? (most < top ? (int)most : top) : lo;
+  if (hi < lo) hi = lo;
+  while (lo < hi) {
+    const unsigned mid = (unsigned)(lo + hi) >> 1;
+    int e = 0;
+#pragma unroll
+    for (int k = 0; k < PLAN / 64; ++k)
+      if (64 * k < p.B) e += n[k] * (int)(((unsigned)u[k] - 1) / mid);
+    e = __builtin_amdgcn_readfirstlane(wave_sum(e));
+    if (e <= p.extra) hi = mid; else lo = mid + 1;
+  }
+  o.span = lo;
+  int total = 0, f = -1, slots = 0;
+#pragma unroll
+  for (int k = 0; k < PLAN / 64; ++k)
+    if (64 * k < p.B) total += n[k] * (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1);
+  total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+  const int per = (total + 7) >> 3, x = blockIdx.x & 7, y = blockIdx.x >> 3;       // consecutive items on one XCD: they read the same rows
+  if (y >= per || (f = x * per + y) >= total) return false;
+  o.b = -1;
+#pragma unroll
+  for (int k = 0; k < PLAN / 64; ++k)
+    if (64 * k < p.B && o.b < 0) {
+      const int c = (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1), mine = n[k] * c, parts = c > 1 ? mine : 0;
+      const int end = wave_scan(mine, lane), send = wave_scan(parts, lane);
+      const uint64_t hit = __ballot(f < end && f >= end - mine);
+      if (hit) {
+        const int at = __builtin_ctzll(hit), g = f - __builtin_amdgcn_readlane(end - mine, at), nn = __builtin_amdgcn_readlane(n[k], at);
+        o.b = 64 * k + at;
+        o.sp = g / nn;
+        o.tile = nn - 1 - g % nn;
+        o.splits = __builtin_amdgcn_readlane(c, at);
+        o.slot = slots + __builtin_amdgcn_readlane(send - parts, at) + o.tile * o.splits;
+      } else {
+        f -= __builtin_amdgcn_readlane(end, 63);
+        slots += __builtin_amdgcn_readlane(send, 63);
+      }
+    }
+  return o.b >= 0;
+}
 
 template <bool R5, int PS>
 struct Lds {
   static constexpr int MR = 128 / PS;                      // query rows
-  static constexpr int RING = 6;
+  static constexpr int RING = PS == 4 ? 8 : 6;
   static constexpr int CODE = 4 * TR * 128;                // codes by scale group, [4][32 rows][128]
   static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
   static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
@@ -59,9 +171,9 @@ struct Lds {
   static constexpr int ID = RING * TILE;                   // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
   static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
-  static constexpr int JOIN = 4 * 32768;                   // at the end, PS = 2: O of 4 waves; then maxima and sums
+  static constexpr int JOIN = 4 * 32768;                   // at the end: O of 4 waves, then maxima and sums
   static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0, "one workgroup a compute unit");
-  static constexpr int BYTES = PS == 2 && TOTAL < JOIN + 2048 ? JOIN + 2048 : TOTAL < 131072 ? 131072 : TOTAL;
+  static constexpr int BYTES = TOTAL < JOIN + 2048 ? JOIN + 2048 : TOTAL;
 };
 
 __device__ __attribute__((aligned(16))) uint8_t zero_row[ROW656];
@@ -118,22 +230,14 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = PS == 1 ? w : w & 3, wp = PS == 1 ? 0 : w >> 2;          // the wave's 16 rows; which of PS tiles it takes
-  const int l16 = lane & 15, l32 = lane & 31, qt = lane >> 4;
+  const int wr = w / PS, wp = w % PS;                     // the wave's 16 rows; which of PS tiles it takes
+  const int l16 = lane & 15, qt = lane >> 4;
 
-  // ---- work item: split and tile of query rows. Request b starts at tile start[b] * H / MR (+ b where requests may end inside one).
-  const int f = remap_xcd(blockIdx.x, p.tiles * p.S);
-  if (f < 0) return;
-  const int sp = f / p.tiles, ti = p.tiles - 1 - f % p.tiles;
-  int nb = 0;
-  for (int at = 0; at < p.B; at += 64) {
-    const int b = at + lane;
-    const bool in = b < p.B && (long long)p.start[b] * p.H / MR + (p.slack ? b : 0) <= ti;
-    nb += __popcll(__ballot(in));
-  }
-  const int b = nb > 0 ? nb - 1 : 0;
+  Item it;
+  if (!find_item<MR>(p, lane, it)) return;
+  const int b = it.b;
   int t0 = p.start[b], t1 = p.start[b + 1];
-  const long long r0 = (long long)(ti - (int)((long long)t0 * p.H / MR) - (p.slack ? b : 0)) * MR;
+  const long long r0 = (long long)it.tile * MR;
   t0 = t0 < 0 ? 0 : t0;
   t1 = t1 > p.T ? p.T : t1;
   const long long nrows = (long long)(t1 - t0) * p.H;
@@ -146,18 +250,27 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
   };
   const int least = limit_of(0), most = limit_of(live - 1);
-  const long long first = (long long)sp * p.span;
+  const long long first = (long long)it.sp * it.span * TR, last = first + (long long)it.span * TR;
   const int kb = first < most ? (int)first : most;
-  const int ke = sp + 1 < p.S && first + p.span < most ? (int)(first + p.span) : most;       // (the last split takes the rest)
+  const int ke = it.sp + 1 < it.splits && last < most ? (int)last : most;                    // (the last split takes the rest)
   const int nt = (ke - kb + TR - 1) / TR;
-  if (nt <= 0 && sp > 0) {                                                 // nothing of this split: no weight in the join
-    if (tid < live) p.lpart[((long long)sp * p.T + t0) * p.H + r0 + tid] = -__builtin_inff();
+  if (p.extra && it.sp == 0 && tid < live)
+    p.parts[(long long)t0 * p.H + r0 + tid] = i32x2{it.slot * MR + tid, it.splits};
+  if (nt <= 0 && it.sp > 0) {                             // nothing of this split: no weight in the join
+    if (tid < live) p.lpart[((long long)it.slot + it.sp) * MR + tid] = -__builtin_inff();
     return;
   }
   const int* btrow = p.table + (long long)b * p.t_st;
 
+  // the lane id, opaque in every step: LDS places made of it are formed again, not kept (and spilled)
+  auto here = [&]() -> int {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   // ---- rows of IDS positions: looked up (x beyond ke: none), then their addresses written with a bit per position
   auto look = [&](int part) -> int {
+    const int tid = 64 * w + here();
     const int pos = kb + part * IDS + tid;
     if (pos >= ke || tid >= IDS) return -1;
     const int page = btrow[pos / p.bs];
@@ -165,6 +278,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     return page >= 0 && y < p.rows ? (int)y : -1;
   };
   auto note = [&](int part, int row) {
+    const int lane = here(), tid = 64 * w + lane, l32 = lane & 31;
     if (tid >= IDS) return;
     const int at = (part & 1) * IDS + tid;
     const uint64_t a = (uint64_t)(uintptr_t)p.cache + (uint64_t)(uint32_t)row * RB;
@@ -199,7 +313,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   auto issue = [&](int j) {
     SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
     SPMLA_LDS uint8_t* d = lds + (j % L::RING) * L::TILE;
-    const int r = lane >> 3, place = (lane & 7) ^ swz(r), wl = w & 3, half = w >> 2;
+    const int lane = here(), r = lane >> 3, place = (lane & 7) ^ swz(r), wl = w & 3, half = w >> 2;
     auto copy = [&](int row, uint32_t off, SPMLA_LDS uint8_t* to) { dma16((const void*)(id[row] + off), to); };
 #pragma unroll
     for (int n = 0; n < 2; ++n) copy(8 * (n + 2 * half) + r, 128 * wl + 16 * (place ^ (n << 1)), d + wl * 4096 + (n + 2 * half) * 1024);
@@ -222,6 +336,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   f32x4 s[2];                                             // scores, then weights: value 4 u + r is position 16 u + 4 qt + r
 
   auto scores = [&](SPMLA_LDS uint8_t* d) {
+    const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     SPMLA_LDS uint8_t* at = d + l16 * 128;
     const int x0 = 16 * (qt ^ swz(l16)), x1 = x0 ^ 64;
     // unit n = 9 u + i: positions 16 u .., dims 64 i .. (i = 8: rope)
@@ -267,6 +382,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
 
   // softmax of tile j: s becomes the weights, O and l follow a moved maximum
   auto softmax = [&](int j) {
+    const int lane = here(), qt = lane >> 4, qr = 16 * wr + (lane & 15);
     const uint32_t has = __builtin_amdgcn_readfirstlane(((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
     const int k0 = kb + j * TR;
     if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
@@ -314,6 +430,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
 
   // O += V^T P^T
   auto values = [&](SPMLA_LDS uint8_t* d) {
+    const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     f16x8 P[R5 ? 1 : 4];
     if constexpr (R5) {
       P[0] = __builtin_bit_cast(f16x8, u32x4{pk_f16(s[0][0], s[0][1]), pk_f16(s[0][2], s[0][3]), pk_f16(s[1][0], s[1][1]), pk_f16(s[1][2], s[1][3])});
@@ -363,13 +480,13 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   const bool works = 16 * wr < live;
   for (int j = 0; j < AHEAD && j < nt; ++j) issue(j);
   for (int j = 0; j < nt; j += PS) {
-    // rows of the next IDS positions: looked up as a part begins, noted two tiles later, copied from a later step on
+    // rows of the next IDS positions: looked up as a part begins, noted at the end of the step, copied from a later one on
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
     // tile j (and j + 1) is there: of the copies after it at most AHEAD - PS tiles' are on their way
     if (j + AHEAD <= nt) wait_vm<(AHEAD - PS) * COPIES>(); else wait_vm<0>();
     lds_barrier();
-    if (in == 0 && next * (IDS / TR) < nt) found = look(next);
-    if (in == 2 && next * (IDS / TR) < nt) note(next, found);
+    const bool more = in == 0 && next * (IDS / TR) < nt;
+    if (more) found = look(next);
 #pragma unroll
     for (int i = 0; i < PS; ++i)
       if (j + AHEAD + i < nt) issue(j + AHEAD + i);
@@ -382,6 +499,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
       lds_barrier();
       for (int i = 0; i < PS && j + i < nt; ++i) {
         SPMLA_LDS uint8_t* c = lds + ((j + i) % L::RING) * L::TILE;
+        const int tid = 64 * w + here();
         for (int at = tid * 16; at < L::CODE; at += 512 * 16) {
           u32x4 y = *(SPMLA_LDS u32x4*)(c + at);
 #pragma unroll
@@ -402,45 +520,48 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
       softmax(mine);
       values(d);
     }
+    if (more) note(next, found);
   }
 
-  // ---- join of a row's four lanes, and (PS = 2) of the two waves of its rows
+  // ---- join of a row's four lanes, and of the waves of its rows
   l = quad_sum(l);
   float e2 = R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23);
-  if constexpr (PS == 2) {
-    SPMLA_LDS f32x4* oj = (SPMLA_LDS f32x4*)(lds + wr * 32768);
-    SPMLA_LDS float* st = (SPMLA_LDS float*)(lds + L::JOIN) + wr * 128;
+  bool done = !works;
+#pragma unroll
+  for (int half = PS / 2; half >= 1; half /= 2) {
+    SPMLA_LDS f32x4* oj = (SPMLA_LDS f32x4*)(lds + (wr * half + wp % half) * 32768);
+    SPMLA_LDS float* st = (SPMLA_LDS float*)(lds + L::JOIN) + (wr * half + wp % half) * 128;
     lds_barrier();
-    if (wp == 1 && works) {
+    if (!done && wp >= half) {
 #pragma unroll
       for (int n = 0; n < 32; ++n) oj[n * 64 + lane] = O[n] * e2;
       st[lane] = m;
       st[64 + lane] = l;
+      done = true;
     }
     lds_barrier();
-    if (wp == 1 || !works) return;
-    const float mo = st[lane], lo = st[64 + lane], mn = fmaxf(m, mo);
-    const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * p.c), c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
-    l = (m == -__builtin_inff() ? l : l * a) + (mo == -__builtin_inff() ? lo : lo * c);
+    if (!done) {
+      const float mo = st[lane], lo = st[64 + lane], mn = fmaxf(m, mo);
+      const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * p.c), c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
+      l = (m == -__builtin_inff() ? l : l * a) + (mo == -__builtin_inff() ? lo : lo * c);
 #pragma unroll
-    for (int n = 0; n < 32; ++n) O[n] = O[n] * (e2 * a) + oj[n * 64 + lane] * c;
-    m = mn;
-    e2 = 1.f;
-  } else {
-    lds_barrier();
-    if (!works) return;
+      for (int n = 0; n < 32; ++n) O[n] = O[n] * (e2 * a) + oj[n * 64 + lane] * c;
+      m = mn;
+      e2 = 1.f;
+    }
   }
+  if (done) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   const float ln = m == -__builtin_inff() && l == l ? m : m * p.c * 0.69314718055994531f + (__builtin_log2f(l) - UP) * 0.69314718055994531f;
-  const bool whole = p.S == 1;
+  const bool whole = it.splits == 1;
   const long long r = r0 + qr;
   if (qt == 0 && qr < live) {
-    if (!whole) p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
+    if (!whole) p.lpart[((long long)it.slot + it.sp) * MR + qr] = ln;
     else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
   const float back = e2 * inv * p.kv_scale;
   if (!whole) {
-    float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r) * D_LAT + 4 * qt;
+    float* o = p.opart + (((long long)it.slot + it.sp) * MR + qr) * D_LAT + 4 * qt;
     if (qr < live)
 #pragma unroll
       for (int n = 0; n < 32; ++n) *(f32x4*)(o + 16 * n) = O[n] * back;
@@ -500,19 +621,11 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, l32 = lane & 31, hh = lane >> 5;
 
-  // ---- work item, as above
-  const int f = remap_xcd(blockIdx.x, p.tiles * p.S);
-  if (f < 0) return;
-  const int sp = f / p.tiles, ti = p.tiles - 1 - f % p.tiles;
-  int nb = 0;
-  for (int at = 0; at < p.B; at += 64) {
-    const int b = at + lane;
-    const bool in = b < p.B && (long long)p.start[b] * p.H / MR + (p.slack ? b : 0) <= ti;
-    nb += __popcll(__ballot(in));
-  }
-  const int b = nb > 0 ? nb - 1 : 0;
+  Item it;
+  if (!find_item<MR>(p, lane, it)) return;
+  const int b = it.b;
   int t0 = p.start[b], t1 = p.start[b + 1];
-  const long long r0 = (long long)(ti - (int)((long long)t0 * p.H / MR) - (p.slack ? b : 0)) * MR;
+  const long long r0 = (long long)it.tile * MR;
   t0 = t0 < 0 ? 0 : t0;
   t1 = t1 > p.T ? p.T : t1;
   const long long nrows = (long long)(t1 - t0) * p.H;
@@ -525,12 +638,14 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
   };
   const int least = limit_of(0), most = limit_of(live - 1);
-  const long long first = (long long)sp * p.span;
+  const long long first = (long long)it.sp * it.span * TR, last = first + (long long)it.span * TR;
   const int kb = first < most ? (int)first : most;
-  const int ke = sp + 1 < p.S && first + p.span < most ? (int)(first + p.span) : most;
+  const int ke = it.sp + 1 < it.splits && last < most ? (int)last : most;                    // (the last split takes the rest)
   const int nt = (ke - kb + TR - 1) / TR;
-  if (nt <= 0 && sp > 0) {
-    if (tid < live) p.lpart[((long long)sp * p.T + t0) * p.H + r0 + tid] = -__builtin_inff();
+  if (p.extra && it.sp == 0 && tid < live)
+    p.parts[(long long)t0 * p.H + r0 + tid] = i32x2{it.slot * MR + tid, it.splits};
+  if (nt <= 0 && it.sp > 0) {                             // nothing of this split: no weight in the join
+    if (tid < live) p.lpart[((long long)it.slot + it.sp) * MR + tid] = -__builtin_inff();
     return;
   }
   const int* btrow = p.table + (long long)b * p.t_st;
@@ -822,15 +937,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   if (32 * w >= live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   const float ln = m == -__builtin_inff() && l == l ? m : m * p.c * 0.69314718055994531f + __builtin_log2f(l) * 0.69314718055994531f;
-  const bool whole = p.S == 1;
+  const bool whole = it.splits == 1;
   const long long r = r0 + qr;
   if (hh == 0 && qr < live) {
-    if (!whole) p.lpart[((long long)sp * p.T + t0) * p.H + r] = ln;
+    if (!whole) p.lpart[((long long)it.slot + it.sp) * MR + qr] = ln;
     else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
   const float back = inv * p.kv_scale;
   if (!whole) {
-    float* o = p.opart + (((long long)sp * p.T + t0) * p.H + r) * D_LAT + 4 * hh;
+    float* o = p.opart + (((long long)it.slot + it.sp) * MR + qr) * D_LAT + 4 * hh;
     if (qr < live)
 #pragma unroll
       for (int n = 0; n < 16; ++n)
@@ -853,20 +968,28 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   }
 }
 
-// Joins the splits of query row (t, h): weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
-// was not written, is not read. One wave a row, 8 dims a lane.
+// Joins the splits of (token, head) row r: weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
+// was not written, is not read. A workgroup a row and half of its dims, every fourth split a wave, 4 dims a lane. Bound by
+// the partials' bytes.
 struct MergeParams {
-  const float* opart; const float* lpart; const int* start; int B, T, H, S;
+  const float* opart; const float* lpart; const i32x2* parts; long long rows; int items;
+  const int* start; int B, T, H;
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
 };
 __global__ void __launch_bounds__(256) merge_kernel(MergeParams p) {
-  const int lane = threadIdx.x & 63;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long long)p.T * p.H;
-  if (r >= n || r / p.H < p.start[0] || r / p.H >= p.start[p.B]) return;      // rows of no request stay as they are
+  __shared__ float wgt[512];
+  __shared__ f32x4 sums[4][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long r = blockIdx.x >> 1, t = r / p.H, h = r % p.H;
+  if (t < p.start[0] || t >= p.start[p.B]) return;        // rows of no request stay as they are
+  const i32x2 part = p.parts[r];
+  const long long first = part[0] & 0x7fffffff, step = p.rows;
+  const int n = part[1];
+  if (n < 2 || n > 512 || (first / step + n) > p.items) return;
   float top = -__builtin_inff();
-  for (int s = lane; s < p.S; s += 64) {
-    const float x = p.lpart[s * n + r];
+  for (int s = lane; s < n; s += 64) {
+    const float x = p.lpart[first + s * step];
     top = x > top || x != x ? x : top;
   }
 #pragma unroll
@@ -876,72 +999,103 @@ __global__ void __launch_bounds__(256) merge_kernel(MergeParams p) {
   }
   const float ref = top == -__builtin_inff() ? 0.f : top;
   float sum = 0.f;
-  f32x4 a = {}, b = {};
-  for (int s = 0; s < p.S; ++s) {
-    const float x = p.lpart[s * n + r];
-    if (x == -__builtin_inff()) continue;
-    const float wgt = __expf(x - ref);
-    const f32x4* o = (const f32x4*)(p.opart + (s * n + r) * D_LAT + 8 * lane);
-    a += wgt * o[0];
-    b += wgt * o[1];
-    sum += wgt;
+  for (int s = lane; s < n; s += 64) {
+    const float x = p.lpart[first + s * step], y = x == -__builtin_inff() ? 0.f : __expf(x - ref);
+    if (w == 0) wgt[s] = x == -__builtin_inff() ? -1.f : y;
+    sum += y;
   }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+  __syncthreads();
+  const float* o = p.opart + first * D_LAT + (blockIdx.x & 1) * 256 + 4 * lane;
+  f32x4 a = {};
+#pragma unroll 4
+  for (int s = w; s < n; s += 4)
+    if (wgt[s] >= 0.f || wgt[s] != wgt[s]) a += wgt[s] * *(const f32x4*)(o + s * step * D_LAT);
+  sums[w][lane] = a;
+  __syncthreads();
+  if (w) return;
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  a *= inv;
-  b *= inv;
-  const long long t = r / p.H, h = r % p.H;
-  *(u32x4*)(p.out + t * p.o_st + h * p.o_sh + 8 * lane) = u32x4{pk_bf16(a[0], a[1]), pk_bf16(a[2], a[3]), pk_bf16(b[0], b[1]), pk_bf16(b[2], b[3])};
-  if (p.lse && lane == 0) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
+  a = (sums[0][lane] + sums[1][lane] + (sums[2][lane] + sums[3][lane])) * inv;
+  *(i32x2*)(p.out + t * p.o_st + h * p.o_sh + (blockIdx.x & 1) * 256 + 4 * lane) = i32x2{(int)pk_bf16(a[0], a[1]), (int)pk_bf16(a[2], a[3])};
+  if (p.lse && threadIdx.x == 0 && !(blockIdx.x & 1)) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
 }
+
+// Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions;
+// of 32 or fewer of 32 rows and four (Row576: eight tiles in LDS; of Row656 seven would fit).
+struct Shape {
+  int rows, slack;
+  long long tiles;
+};
+static Shape shape_of(int T, int H, int B, int row_bytes) {
+  const long long n = (long long)T * H;
+  const int mr = n <= 32ll * B && row_bytes == ROW576 ? 32 : n <= 64ll * B ? 64 : 128, slack = H % mr != 0;
+  return Shape{mr, slack, n / mr + (slack ? B : 0)};
+}
+// splits need a place for each (token, head), and for the partial results of a split tile's rows
+static long long part_slots(const Shape& s, int items) { return items < 2 * (items - s.tiles) ? items : 2 * (items - s.tiles); }
 
 }  // namespace chunk
 }  // namespace spmla
 
 using namespace spmla;
 
-extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int S) {
-  if (T <= 0 || H <= 0 || S <= 1) return 0;
-  return (long long)T * H * S * (D_LAT + 1) * 4;
+extern "C" int spmla_attn_chunk_items(int T, int H, int B, int row_bytes, int longest) {
+  if (T <= 0 || H <= 0 || B <= 0 || B > chunk::PLAN || longest <= 2 * chunk::LEAST * chunk::TR) return 0;
+  const long long tiles = chunk::shape_of(T, H, B, row_bytes).tiles, full = (tiles + chunk::CUS - 1) / chunk::CUS * chunk::CUS;
+  // whole rounds of workgroups, a few beyond one a tile for the longest requests; from four rounds on no tile is split
+  return tiles >= 4 * chunk::CUS ? 0 : (int)(full - tiles >= chunk::CUS / 4 ? full : full + chunk::CUS / 4);
+}
+
+extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int items) {
+  if (T <= 0 || H <= 0 || B <= 0 || items <= 0 || B > chunk::PLAN) return 0;
+  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes);
+  if (items <= s.tiles) return 0;
+  return (long long)T * H * 8 + 16 + chunk::part_slots(s, items) * s.rows * (D_LAT + 1) * 4;
 }
 
 extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                                 int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
+                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int items, void* out,
                                 long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream) {
-  if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || S < 1 || span < 1 ||
-      span % chunk::TR || (row_bytes != ROW656 && row_bytes != ROW576))
+  if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || items < 0 ||
+      (row_bytes != ROW656 && row_bytes != ROW576))
     return SPMLA_EARG;
-  if (T > MAX_TOKENS || B > MAX_TOKENS || H > 65536 || S > 256 || rows > 0x7fffffffll || (long long)W * block_size > 0x7fffff00ll) return SPMLA_ELIMIT;
+  if (T > MAX_TOKENS || B > MAX_TOKENS || H > 65536 || items > 65536 || rows > 0x7fffffffll || (long long)W * block_size > 0x7fffff00ll) return SPMLA_ELIMIT;
   if (B == 0 || T == 0 || H == 0) return SPMLA_OK;
   if (!q || !start || !seqs || !out || (rows && !cache) || (W && !table)) return SPMLA_EARG;
   if (((q_st | q_sh | o_st | o_sh) & 7) || (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out) & 15) ||
       (((uintptr_t)start | (uintptr_t)seqs | (uintptr_t)table | (uintptr_t)lse) & 3))
     return SPMLA_EALIGN;
-  if (S > 1 && (!ws || ((uintptr_t)ws & 15))) return ws ? SPMLA_EALIGN : SPMLA_EARG;
-  if (S > 1 && ws_bytes < spmla_attn_chunk_ws_bytes(T, H, S)) return SPMLA_EARG;
-  const int r5 = row_bytes == ROW576;
-  // requests of 64 (token, head) rows or fewer on average: workgroups of 64 rows whose waves share the positions
-  const int narrow = (long long)T * H <= 64ll * B;
-  const int mr = narrow ? 64 : 128, slack = H % mr != 0;
-  const long long tiles = (long long)T * H / mr + (slack ? B : 0);
-  if (tiles * S > (1ll << 30)) return SPMLA_ELIMIT;
-  float* opart = (float*)ws;
-  float* lpart = opart ? opart + (long long)T * H * S * D_LAT : nullptr;
+  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes);
+  if (s.tiles > (1ll << 30)) return SPMLA_ELIMIT;
+  const long long need = spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, items);
+  const int extra = need ? (int)(items - s.tiles) : 0;
+  if (extra > 511) return SPMLA_ELIMIT;
+  if (need && !ws) return SPMLA_EARG;
+  if (need && ((uintptr_t)ws & 15)) return SPMLA_EALIGN;
+  if (need && ws_bytes < need) return SPMLA_EARG;
+  const long long slots = need ? chunk::part_slots(s, items) : 0;
+  float* opart = need ? (float*)ws : nullptr;
+  float* lpart = need ? opart + slots * s.rows * D_LAT : nullptr;
+  i32x2* parts = need ? (i32x2*)(lpart + slots * s.rows) : nullptr;
   const float sc = sm_scale * kv_scale;
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
-                  H, S, span, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)tiles, slack, (uint16_t*)out, o_st, o_sh, lse,
-                  l_st, opart, lpart};
-  static DynLds attr[4];
-  static Launcher go[4];
-  const int at = 2 * narrow + r5;
-  const void* fn[4] = {(const void*)chunk::wide_kernel<false>, (const void*)chunk::wide_kernel<true>, (const void*)chunk::kernel<false, 2>,
-                       (const void*)chunk::kernel<true, 2>};
-  const int lds[4] = {chunk::WLds<false>::TOTAL, chunk::WLds<true>::TOTAL, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES};
+                  H, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)s.tiles, s.slack,
+                  extra ? items : 0, extra, (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts};
+  static DynLds attr[5];
+  static Launcher go[5];
+  const int r5 = row_bytes == ROW576, at = s.rows == 32 ? 4 : 2 * (s.rows == 64) + r5;
+  const void* fn[5] = {(const void*)chunk::wide_kernel<false>, (const void*)chunk::wide_kernel<true>, (const void*)chunk::kernel<false, 2>,
+                       (const void*)chunk::kernel<true, 2>, (const void*)chunk::kernel<true, 4>};
+  const int lds[5] = {chunk::WLds<false>::TOTAL, chunk::WLds<true>::TOTAL, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES,
+                      chunk::Lds<true, 4>::BYTES};
   if (const int rc = attr[at].ensure(fn[at], lds[at])) return rc;
-  hipStream_t s = (hipStream_t)stream;
-  if (const int rc = go[at](fn[at], dim3((unsigned)((tiles * S + 7) / 8 * 8)), narrow ? 512 : 256, lds[at], s, p)) return rc;
-  if (S == 1) return SPMLA_OK;
+  hipStream_t stm = (hipStream_t)stream;
+  const long long grid = extra ? (items + 7) / 8 * 8 : s.tiles;
+  if (const int rc = go[at](fn[at], dim3((unsigned)grid), s.rows == 128 ? 256 : 512, lds[at], stm, p)) return rc;
+  if (!extra) return SPMLA_OK;
   static Launcher join;
-  const chunk::MergeParams mp{opart, lpart, start, B, T, H, S, (uint16_t*)out, o_st, o_sh, lse, l_st};
-  return join((const void*)chunk::merge_kernel, dim3((unsigned)(((long long)T * H + 3) / 4)), 256, 0, s, mp);
+  const chunk::MergeParams mp{opart, lpart, parts, s.rows, (int)slots, start, B, T, H, (uint16_t*)out, o_st, o_sh, lse, l_st};
+  return join((const void*)chunk::merge_kernel, dim3((unsigned)(2 * (long long)T * H)), 256, 0, stm, mp);
 }

@@ -1139,37 +1139,39 @@ def attend_prompt(q, k, v, start, scale, causal=True, out=None, lse=None):
 
 
 @functools.lru_cache(maxsize=4096)
-def chunk_split(T, H, B, longest, cus=256):
-    """(splits, positions of each) of attend_chunk for T tokens of H heads in B requests of up to `longest` cached rows."""
-    tiles = max(1, T * H // 128 + (min(B, T) if H % 128 else 0))
-    units = max(1, -(-longest // 32))                    # tiles of 32 positions
-    split = max(1, min(cus // tiles, -(-units // 8), 128))
-    span = -(-units // split)
-    return -(-units // span), 32 * span
+@functools.lru_cache(maxsize=4096)
+def chunk_items(T, H, B, row_bytes, longest):
+    """Workgroups that attend_chunk has share the positions of T tokens of H heads in B requests (spmla_attn_chunk_items)."""
+    return int(_lib.lib().spmla_attn_chunk_items(T, H, B, row_bytes, min(longest, 1 << 20)))
+
+
+@functools.lru_cache(maxsize=4096)
+def chunk_ws_bytes(T, H, B, row_bytes, items):
+    """Bytes of the workspace attend_chunk needs (spmla_attn_chunk_ws_bytes)."""
+    return int(_lib.lib().spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, items))
 
 
 def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0, max_seq_len=None, out=None, lse=None,
-                 split=None):
+                 items=None):
     """Attention of new tokens over every cached row of their request: tokens start[b] .. start[b + 1] - 1 of q [T, H, 576] bf16
     (start [B + 1] int32) are the last of the seq_lens[b] rows that request b has in cache [blocks, block_size, 656 or 576]
     uint8 (already written; block stride any whole number of rows) through block_table [B, columns] int32; each token sees
     its own position and those before it, but for pages that are not there (-1). Returns (out [T, H, 512] bf16, lse [T, H]
     fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: about the
-    longest seq_lens, known on the host (None: what the table can hold), by which the positions are split; the result does
-    not depend on it. split: splits of the positions (None: chunk_split), joined through a temporary workspace."""
+    longest seq_lens, known on the host (None: what the table can hold): short ones are not split. items: workgroups that the
+    kernel makes of the requests' positions, in even shares (None: chunk_items; 0: one a tile of query rows); their partial
+    results are joined through a temporary workspace. The result does not depend on either, but for the order of its sums."""
     _need(q.dim() == 3 and cache.dim() == 3 and block_table.dim() == 2, "q [T, H, 576], cache [blocks, block_size, row], block_table [B, columns]")
-    T, H = q.shape[0], q.shape[1]
-    room = block_table.shape[1] * cache.shape[1]
-    longest = max(1, room if max_seq_len is None else min(int(max_seq_len), room))
-    if split is None:
-        split, span = chunk_split(T, H, block_table.shape[0], longest)
-    else:
-        _need(1 <= split <= 256, "split of 1 to 256")
-        span = -(-longest // (32 * split)) * 32
+    T, H, B, row = q.shape[0], q.shape[1], block_table.shape[0], cache.shape[2]
+    if items is None:
+        room = block_table.shape[1] * cache.shape[1]
+        items = chunk_items(T, H, B, row, max(0, room if max_seq_len is None else min(int(max_seq_len), room)))
+    _need(0 <= items <= 65536, "items of 0 to 65536")
     if out is None:
         out = torch.empty(T, H, D_LAT, dtype=torch.bfloat16, device=q.device)
     if lse is None:
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
-    ws = torch.empty(T * H * split * (D_LAT + 1) * 4, dtype=torch.uint8, device=q.device) if split > 1 else None
-    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, split, span, out, lse, ws)
+    nb = chunk_ws_bytes(T, H, B, row, items) if items else 0
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, items, out, lse, ws)
     return out, lse

@@ -542,15 +542,18 @@ int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void*
  * (row stride t_st, W columns) is not negative: cache row page * stride_rows + x % block_size (stride_rows: rows from a block
  * to the next; rows beyond `rows` are not read). row_bytes 656 or 576; s = sm_scale * kv_scale * (q . row), out [T][H][512]
  * bf16 = kv_scale * sum p latent, lse [T][H] optional, as spmla_attn_splitk over all of these rows; a token without one gets
- * 0 and -inf, tokens of no request nothing. Positions are cut into S splits of span each (a multiple of 32; the last one
- * takes the rest; S <= 256), joined by a second kernel through a workspace of spmla_attn_chunk_ws_bytes (S > 1).
+ * 0 and -inf, tokens of no request nothing. Codes are exact in bf16, scores, sums and statistics in fp32; weights (Row656:
+ * times the row's scale) are rounded to bf16, or to fp16 where requests have 64 (token, head) rows or fewer on average.
+ * items: workgroups that the requests' positions are shared out to on the device, by their lengths (0, B > 256, or no more
+ * than the tiles of query rows: one a tile; ELIMIT beyond 511 more), partial results joined by a second kernel through a
+ * workspace of spmla_attn_chunk_ws_bytes. spmla_attn_chunk_items: a good number of them, longest: about the longest seqs.
  * The dense counterpart of PortableSparseImpl.forward_mqa (dsa_sm89.py:379-470) for layers without an indexer. */
-long long spmla_attn_chunk_ws_bytes(int T, int H, int S);
+int spmla_attn_chunk_items(int T, int H, int B, int row_bytes, int longest);
+long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int items);
 int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                      int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int S, int span, void* out,
-                     long long o_st, long long o_sh, float* lse, long long l_st, void* ws,
-                     long long ws_bytes, void* stream);
+                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int items, void* out,
+                     long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream);
 
 /* Build identification string (static storage). */
 const char* spmla_version(void);

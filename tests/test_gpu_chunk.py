@@ -84,17 +84,18 @@ def test_against_64_bits(dev, seqs, lens, H, bs, row):
 
 
 @pytest.mark.parametrize("row", [656, 576])
-@pytest.mark.parametrize("split", [1, 2, 3, 7, 40])
-def test_splits(dev, row, split):
-    """Splits without positions among them (40 of 1000 rows, of 31 and of none)."""
-    case = _case([1000, 31, 640, 0], [1, 2, 33, 0], 16, row, 64, split)
-    _run(dev, case, 64, 0.5, split=split, max_seq_len=1000)
+@pytest.mark.parametrize("items", [0, 15, 16, 19, 27, 256, 500])
+@pytest.mark.parametrize("heads,lens", [(16, [1, 2, 33, 0]), (128, [1, 2, 33, 0]), (16, [1, 1, 2, 0]), (60, [1, 1, 1, 1])])
+def test_splits(dev, row, items, heads, lens):
+    """From no splits to as many as there can be, of 1000 rows, of 31 and of none; some without positions that a token sees."""
+    case = _case([1000, 31, 640, 0], lens, heads, row, 64, items)
+    _run(dev, case, 64, 0.5, items=items)
 
 
 def test_result_does_not_depend_on_max_seq_len(dev):
-    """Rows beyond a max_seq_len that is too small are still seen (the last split takes the rest)."""
+    """Rows beyond a max_seq_len that is too small are still seen."""
     case = _case([1500, 900], [2, 1], 32, 656, 64, 3)
-    _run(dev, case, 64, split=4, max_seq_len=256)
+    _run(dev, case, 64, items=40, max_seq_len=256)
     _run(dev, case, 64, max_seq_len=1)
     _run(dev, case, 64)
 
@@ -105,7 +106,7 @@ def test_pages_that_are_not_there(dev, row):
     case = _case([300, 64, 200, 10], [2, 1, 150, 1], 16, row, 16, 8, missing=[(0, 0), (0, 7), (0, 18), (1, 0), (1, 1), (1, 2), (1, 3), (2, 5), (3, 0)])
     out, lse = _run(dev, case, 16)
     assert bool((out[2] == 0).all()) and bool((lse[2] == -torch.inf).all()) and bool((lse[-1] == -torch.inf).all())
-    _run(dev, case, 16, split=5, max_seq_len=300)
+    _run(dev, case, 16, items=60, max_seq_len=300)
 
 
 def test_more_new_tokens_than_rows(dev):
@@ -124,11 +125,11 @@ def test_padded_block_stride_and_strided_query(dev):
     T, H = q.shape[:2]
     wide = torch.full((T + 7, H + 1, 584), float("nan"), dtype=torch.bfloat16, device=dev)
     wide[2:2 + T, :H, 8:] = q.to(dev)
-    for split in (1, 3):
+    for items in (0, 40):
         out = torch.full((T + 7, H, 520), 7.0, dtype=torch.bfloat16, device=dev)
         lse = torch.full((T + 7, H), 7.0, device=dev)
         kernels.attend_chunk(wide[:, :H, 8:], _device(cache, dev), table.to(dev), seqs.to(dev), (start + 2).to(dev), SM, out=out[..., 8:],
-                             lse=lse, split=split)
+                             lse=lse, items=items)
         torch.cuda.synchronize()
         o, z = out.cpu(), lse.cpu()
         _check(o[2:2 + T, :, 8:], z[2:2 + T], q, cache, table, seqs, start, 1.0, 16)
