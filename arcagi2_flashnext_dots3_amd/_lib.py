@@ -74,8 +74,8 @@ SIGNATURES = {
     "spmla_page_trim": [P, I, P, P, P, LL, I, P, I, P, I, P],
     "spmla_attn_prompt": [P, LL, LL, P, LL, LL, P, LL, LL, P, I, I, I, I, I, I, F, I, I, P, LL, LL, P, LL, P],
     "spmla_attn_chunk_items": [I, I, I, I, I],
-    "spmla_attn_chunk_ws_bytes": [I, I, I, I, I],
-    "spmla_attn_chunk": [P, LL, LL, P, LL, I, I, LL, P, LL, I, P, P, I, I, I, F, F, I, P, LL, LL, P, LL, P, LL, P],
+    "spmla_attn_chunk_ws_bytes": [I, I, I, I, I, I],
+    "spmla_attn_chunk": [P, LL, LL, P, LL, I, I, LL, P, LL, I, P, P, I, I, I, F, F, I, I, P, LL, LL, P, LL, P, LL, P],
     "spmla_version": [],
     "spmla_host_e4m3_encode": [P, P, LL],
 }

@@ -480,12 +480,12 @@ long attend_prompt(PyObject* const* a) {
   });
 }
 
-// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, items, out, lse, ws)
+// attend_chunk(q, cache, table, seqs, start, sm_scale, kv_scale, longest, items, out, lse, ws)
 long attend_chunk(PyObject* const* a) {
   const at::Tensor *q = tensor(a[0], "q"), *cache = tensor(a[1], "cache"), *table = tensor(a[2], "block_table"), *seqs = tensor(a[3], "seq_lens");
-  const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[8], "out"), *lse = maybe(a[9], "lse"), *ws = maybe(a[10], "ws");
+  const at::Tensor *start = tensor(a[4], "start"), *out = tensor(a[9], "out"), *lse = maybe(a[10], "lse"), *ws = maybe(a[11], "ws");
   const double sm = number(a[5]), kvs = number(a[6]);
-  const long long items = integer(a[7]);
+  const long long longest = integer(a[7]), items = integer(a[8]);
   if (q->dim() != 3 || type_of(*q) != BF16 || q->size(2) != 576) refuse("q [T, H, 576] bf16: got " + shown(*q));
   const int64_t T = q->size(0), H = q->size(1), B = starts(*start);
   at_most(T, MAX_TOKENS, "T");
@@ -507,8 +507,9 @@ long attend_chunk(PyObject* const* a) {
   at_most(W * bs, 0x7fffff00, "positions of a block table's row");
   line(*seqs, B, B, I32, "seq_lens [requests] int32");
   if (!((float)(sm * kvs) - (float)(sm * kvs) == 0.f)) refuse("sm_scale, kv_scale: finite numbers");
+  if (longest < 0 || longest > 0x7fffffff) refuse("longest of 0 to 2^31 - 1: got " + std::to_string(longest));
   if (items < 0 || items > 65536) refuse("items of 0 to 65536: got " + std::to_string(items));
-  const long long need = f_attn_chunk_ws_bytes((int)T, (int)H, (int)B, (int)rowb, (int)items);
+  const long long need = f_attn_chunk_ws_bytes((int)T, (int)H, (int)B, (int)rowb, (int)(longest < W * bs ? longest : W * bs), (int)items);
   if (need > 0) {
     if (!ws) refuse("ws: a workspace of " + std::to_string(need) + " bytes");
     line(*ws, need, ANY, U8, "ws uint8 (spmla_attn_chunk_ws_bytes)");
@@ -520,7 +521,7 @@ long attend_chunk(PyObject* const* a) {
   return launch(dev, [&](void* s) {
     return f_attn_chunk(address(q), qs.st, qs.sh, address(cache), total, (int)rowb, as_int(bs, "block_size"), stride,
                         (const int*)address(table), tst, (int)W, (const int*)address(seqs), (const int*)address(start), (int)B, (int)T,
-                        (int)H, (float)sm, (float)kvs, (int)items, address(out), os.st, os.sh, (float*)address(lse), ls,
+                        (int)H, (float)sm, (float)kvs, (int)longest, (int)items, address(out), os.st, os.sh, (float*)address(lse), ls,
                         address(ws), ws ? ws->numel() : 0, s);
   });
 }
@@ -543,7 +544,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define CALLABLE(name, n) {#name, (PyCFunction)(void (*)())entry<name, n>, METH_FASTCALL, nullptr}
 PyMethodDef calls[] = {CALLABLE(rms_norm, 9), CALLABLE(quant_fp8, 4), CALLABLE(linear_fp8, 5), CALLABLE(linear_quant, 6),
                        CALLABLE(rope, 8), CALLABLE(latent_write, 13), CALLABLE(page_step, 11), CALLABLE(page_trim, 7),
-                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 11)};
+                       CALLABLE(attend_prompt, 8), CALLABLE(attend_chunk, 12)};
 
 PyObject* load(PyObject*, PyObject* args) {
   const char* path;

@@ -48,6 +48,8 @@ struct Params {
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
   float* opart; float* lpart; i32x2* parts;                // [slot][MR][512], [slot][MR]; of a (token, head): first row, splits
+  int longest;                                             // positions from here on are not seen
+  uint8_t* images; int img_tiles;                          // [request][img_tiles][IMAGE], see image_kernel
 };
 
 // ---- which tile of query rows (MR of one request) and which of its splits a workgroup takes.
@@ -92,9 +94,9 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
     return tile >= 0;
   }
   int n[PLAN / 64], u[PLAN / 64];                          // of request 64 k + lane: tiles of query rows, tiles of positions
-  const long long cap = (long long)p.W * p.bs;
+  const long long cap = p.longest;
   long long work = 0;
-  int top = 1;
+  int top = 1, tiles = 0;
 #pragma unroll
   for (int k = 0; k < PLAN / 64; ++k) {
     n[k] = 0;
@@ -106,18 +108,21 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
       n[k] = r > 0 ? (int)((r + MR - 1) / MR) : 0;
       u[k] = x > 0 ? (int)((x + TR - 1) / TR) : 1;
       work += (long long)n[k] * u[k];
+      tiles += n[k];
       top = n[k] > 0 && u[k] > top ? u[k] : top;
     }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     work += __shfl_xor(work, d);
+    tiles += __shfl_xor(tiles, d);
     const int y = __shfl_xor(top, d);
     top = y > top ? y : top;
   }
+  const int extra = p.extra < p.items - tiles ? p.extra : p.items - tiles;     // (fewer tiles where requests fill theirs)
   work = __builtin_amdgcn_readfirstlane((int)work) & 0xffffffffll | (long long)__builtin_amdgcn_readfirstlane((int)(work >> 32)) << 32;
   top = __builtin_amdgcn_readfirstlane(top);
-  const long long even = (work + p.items - 1) / p.items, most = (work + p.extra - 1) / p.extra;
+  const long long even = (work + p.items - 1) / p.items, most = extra > 0 ? (work + extra - 1) / extra : top;
   int lo = even < LEAST ? LEAST : even < top ? (int)even : top;
   int hi = lo < most ? (most < top ? (int)most : top) : lo;
   if (hi < lo) hi = lo;
@@ -128,7 +133,7 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
     for (int k = 0; k < PLAN / 64; ++k)
       if (64 * k < p.B) e += n[k] * (int)(((unsigned)u[k] - 1) / mid);
     e = __builtin_amdgcn_readfirstlane(wave_sum(e));
-    if (e <= p.extra) hi = mid; else lo = mid + 1;
+    if (e <= extra) hi = mid; else lo = mid + 1;
   }
   o.span = lo;
   int total = 0, f = -1, slots = 0;
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   if (r0 < 0 || r0 >= nrows) return;
   const int live = nrows - r0 < MR ? (int)(nrows - r0) : MR;               // query rows here
   const int past = p.seqs[b] - (t1 - t0);                                  // rows before the new ones
-  const long long cap = (long long)p.W * p.bs;
+  const long long cap = p.longest;
   auto limit_of = [&](int r) -> int {                                      // positions that row r sees
     const long long x = (long long)past + (r0 + r) / p.H + 1;
     return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
@@ -599,6 +604,58 @@ struct WLds {
   static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
 };
 
+// Where a request has many query rows, a kernel before this one gathers and converts its tiles once for all of them, as they
+// lie in LDS: nine groups of 64 dims in bf16, scales by group [4][32], a word of which positions have rows.
+constexpr int IMG_SC = 9 * 4096, IMG_OK = IMG_SC + 512, IMAGE = IMG_SC + 1024;
+struct ILds {
+  static constexpr int OVER = 4 * IMAGE;
+  static constexpr int TOTAL = OVER + 16;
+  static_assert(TOTAL <= 160 * 1024 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
+};
+
+template <bool R5>
+__global__ void __launch_bounds__(256) image_kernel(Params p) {
+  constexpr int RB = R5 ? ROW576 : ROW656;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.y, j = blockIdx.x;
+  const int len = p.seqs[b] < p.longest ? p.seqs[b] : p.longest;
+  if (j * TR >= len) return;
+  const int r = tid >> 3, e = tid & 7, pos = j * TR + r;  // 8 threads a row
+  const uint8_t* row = zero_row;
+  bool has = false;
+  if (pos < len) {
+    const int page = p.table[(long long)b * p.t_st + pos / p.bs];
+    const long long y = (long long)page * p.stride + pos % p.bs;
+    has = page >= 0 && y < p.rows;
+    if (has) row = p.cache + y * RB;
+  }
+  uint8_t* img = p.images + ((long long)b * p.img_tiles + j) * IMAGE;
+  uint8_t* to = img + r * 128;
+  const int x = swz(r);
+  i32x4 y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = *(const i32x4*)(row + 128 * i + 16 * e);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int g = 2 * i + (e >> 2), c = 2 * (e & 3);
+    *(bf16x8*)(to + g * 4096 + 16 * (c ^ x)) = codes8_bf16(y[i][0], y[i][1]);
+    *(bf16x8*)(to + g * 4096 + 16 * ((c ^ x) ^ 1)) = codes8_bf16(y[i][2], y[i][3]);
+  }
+  if constexpr (R5) {
+    const i32x2 z = *(const i32x2*)(row + D_LAT + 8 * e);
+    *(bf16x8*)(to + 8 * 4096 + 16 * (e ^ x)) = codes8_bf16(z[0], z[1]);
+  } else {
+    *(u32x4*)(to + 8 * 4096 + 16 * (e ^ x)) = *(const u32x4*)(row + ROPE_OFF + 16 * e);
+    if (e < 4) ((float*)(img + IMG_SC))[e * 32 + r] = *(const float*)(row + SC_OFF + 4 * e);
+  }
+  const uint64_t bits = __ballot(has && e == 0);          // rows 8 w .. 8 w + 7, a bit each in lanes 8 k
+  if (lane == 0) {
+    uint32_t y8 = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y8 |= (uint32_t)(bits >> (8 * k) & 1) << k;
+    img[IMG_OK + w] = (uint8_t)y8;
+  }
+}
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // QK products with their sums in VGPRs (the builtin would put them into AGPRs, which O fills). What the compiler cannot see
@@ -612,9 +669,10 @@ __device__ inline f32x16 qk_next(bf16x8 a, bf16x8 b, f32x16 c) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
   return c;
 }
-template <bool R5>
+template <bool R5, bool IMG>
 __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   using L = WLds<R5>;
+  constexpr int OVER = IMG ? ILds::OVER : L::OVER;
   constexpr int RB = R5 ? ROW576 : ROW656, MR = 128;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
@@ -632,7 +690,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   if (r0 < 0 || r0 >= nrows) return;
   const int live = nrows - r0 < MR ? (int)(nrows - r0) : MR;
   const int past = p.seqs[b] - (t1 - t0);
-  const long long cap = (long long)p.W * p.bs;
+  const long long cap = p.longest;
   auto limit_of = [&](int r) -> int {
     const long long x = (long long)past + (r0 + r) / p.H + 1;
     return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
@@ -685,8 +743,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 
   // ---- copies of a tile, in COPIES pieces: wave w the codes of scale group w (piece i: rows 8 i + lane / 8, the chunk whose
   // place is lane % 8), a share of the rope and of the scales. Behind the last tile they copy rows that are there, unused.
-  constexpr int COPIES = R5 ? 5 : 6;
+  constexpr int COPIES = IMG ? 10 : R5 ? 5 : 6;
+  const uint8_t* image = IMG ? p.images + ((long long)b * p.img_tiles) * IMAGE : nullptr;
   auto address = [&](int j, int i) -> uint64_t {          // of the lane's source in piece i
+    if constexpr (IMG) {                                  // (pieces 0, 3, 6 and 9; those behind them by the instruction's offset)
+      const int t = kb / TR + j < p.img_tiles ? kb / TR + j : p.img_tiles - 1;
+      return (uint64_t)(uintptr_t)(image + (long long)t * IMAGE + (i < 9 ? w * 9216 + i * 1024 : IMG_SC + w * 256)) + (uint32_t)(here() * (i < 9 ? 16 : 4));
+    }
     const int lane = here(), r = lane >> 3, place = (lane & 7) ^ swz(r);
     SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
     if (i < 4) return id[8 * i + r] + (uint32_t)(128 * w + 16 * (place ^ ((i & 1) << 1)));
@@ -696,6 +759,14 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     return id[lane & 31] + (uint32_t)(SC_OFF + 4 * (2 * (w & 1) + (lane >> 5)));
   };
   auto copy = [&](int j, int i, uint64_t from) {
+    if constexpr (IMG) {
+      SPMLA_LDS uint8_t* d = lds + (j & 3) * IMAGE;
+      if (i == 9) dma4((const void*)from, d + IMG_SC + w * 256);
+      else if (i % 3 == 0) dma16((const void*)from, d + w * 9216 + i * 1024);
+      else if (i % 3 == 1) dma16_off<1024, 1024>(from, d + w * 9216 + (i - 1) * 1024);
+      else dma16_off<2048, 2048>(from, d + w * 9216 + (i - 2) * 1024);
+      return;
+    }
     SPMLA_LDS uint8_t* d = lds + (j & 3) * L::TILE;
     if (i < 4) dma16((const void*)from, d + w * 4096 + i * 1024);
     else if (R5) dma16((const void*)from, d + L::CODE + (w & 1) * 1024);
@@ -723,47 +794,57 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       *(SPMLA_LDS bf16x8*)(to + 8 * 4096 + w * 1024 + r * 128 + 16 * ((lane & 7) ^ swz(8 * w + r))) = codes8_bf16(y[0], y[1]);
     }
   };
-  constexpr int PIECES = R5 ? 5 : 4;                      // of a tile's conversion
+  constexpr int PIECES = IMG ? 0 : R5 ? 5 : 4;            // of a tile's conversion
 
   // ---- passes: a row's reference is the first maximum it meets and does not move (weights in bf16 have fp32's range, so O,
   // which fills the AGPRs, is not rescaled). Where scores rise by more than 2^WIDE over it (rare), a pass takes the maxima
   // alone and another one starts from those.
   f32x16 O[16];                                           // O^T: dims 32 n + 8 a + 4 hh + b, query row qr
   float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, of both halves; l: this half's)
-  SPMLA_LDS int* over = (SPMLA_LDS int*)(lds + L::OVER);
+  SPMLA_LDS int* over = (SPMLA_LDS int*)(lds + OVER);
   bool maxima = false;
   for (;;) {
   if (tid == 0) *over = 0;
   int found = -1;
-  note(0, look(0));
-  note(1, -1);                                            // (addresses that a copy may take, whatever the tile)
+  if constexpr (!IMG) {
+    note(0, look(0));
+    note(1, -1);                                          // (addresses that a copy may take, whatever the tile)
+  }
   l = 0.f;
 #pragma unroll
   for (int n = 0; n < 16; ++n) O[n] = f32x16{};
   lds_barrier();
-  for (int j = 0; j < 3; ++j)
+  for (int j = 0; j < 3; ++j) {
+    uint64_t from = 0;
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) copy(j, i, address(j, i));
+    for (int i = 0; i < COPIES; ++i) {
+      if (!IMG || i % 3 == 0) from = address(j, i);
+      copy(j, i, from);
+    }
+  }
   wait_vm<2 * COPIES>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i) convert(0, i, codes(0, i));
+  for (int i = 0; i < (IMG ? 0 : R5 ? 5 : 4); ++i) convert(0, i, codes(0, i));
 #pragma unroll 1
   for (int j = 0; j < nt; ++j) {
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
-    wait_vm<COPIES>();                                    // tile j + 1 is there
+    wait_vm<(IMG ? 2 : 1) * COPIES>();                    // tile j + 1 (of an image: j) is there
     lds_barrier();                                        // and tile j in bf16
+    if constexpr (!IMG) {
     if (in == 0 && next * (IDS / TR) < nt) found = look(next);
     if (in == 2 && next * (IDS / TR) < nt) note(next, found);
-    SPMLA_LDS uint8_t* kt = lds + L::B + (j & 1) * (L::NG * 4096);
-    SPMLA_LDS uint8_t* raw = lds + (j & 3) * L::TILE;
+    }
+    SPMLA_LDS uint8_t* kt = IMG ? lds + (j & 3) * IMAGE : lds + L::B + (j & 1) * (L::NG * 4096);
+    SPMLA_LDS uint8_t* rope = IMG ? kt + 8 * 4096 : R5 ? kt + 8 * 4096 : lds + (j & 3) * L::TILE + L::CODE;
+    SPMLA_LDS uint8_t* scales = IMG ? kt + IMG_SC : lds + (j & 3) * L::TILE + L::CODE + L::RP;
     // ---- S^T = K Q^T; beside it the copies of tile j + 3 and the conversion of tile j + 1, piece by piece
     f32x16 S;
     {
       const int lane = here(), l32 = lane & 31, hh = lane >> 5;
       const int ka = l32 * 128 + 16 * (hh ^ swz(l32));
       auto kread = [&](int ks) -> bf16x8 {
-        SPMLA_LDS uint8_t* at = !R5 && ks >= 32 ? raw + L::CODE : kt + (ks >> 2) * 4096;
+        SPMLA_LDS uint8_t* at = ks >= 32 ? rope : kt + (ks >> 2) * 4096;
         return *(SPMLA_LDS bf16x8*)(at + (ka ^ (32 * (ks & 3))));
       };
       constexpr int KD = R5 ? 8 : 6;
@@ -773,6 +854,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       uint64_t from = 0;
       i32x4 y = {};
       auto beside = [&](int ks) {                         // what runs beside product ks: piece ks / 6 of copies and codes
+        if constexpr (IMG) {
+          if (ks % 3 == 0 && ks / 3 < COPIES) {
+            if (ks / 3 % 3 == 0) from = address(j + 3, ks / 3);
+            copy(j + 3, ks / 3, from);
+          }
+          return;
+        }
         const int i = ks / 6, at = ks % 6;
         if (at == 0 && i < COPIES) from = address(j + 3, i);
         if (at == 1 && i < PIECES) y = codes(j + 1, i);
@@ -802,7 +890,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
               if (g > 0 && n >= 4) {                      // a quarter of the group before: its products are done
                 const int a = n - 4;
                 asm volatile("" : "+v"(acc[(g - 1) & 1]));
-                const f32x4 sc = *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + (g - 1) * 128 + 32 * a + 16 * hh);
+                const f32x4 sc = *(SPMLA_LDS f32x4*)(scales + (g - 1) * 128 + 32 * a + 16 * hh);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) S[4 * a + r] = __builtin_fmaf(acc[(g - 1) & 1][4 * a + r], sc[r], S[4 * a + r]);
               }
@@ -811,7 +899,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
           } else {
             f32x4 sc[4];
 #pragma unroll
-            for (int a = 0; a < 4; ++a) sc[a] = *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + 3 * 128 + 32 * a + 16 * hh);
+            for (int a = 0; a < 4; ++a) sc[a] = *(SPMLA_LDS f32x4*)(scales + 3 * 128 + 32 * a + 16 * hh);
             beside(33);
             asm volatile("s_nop 15" : "+v"(acc[1]));
             beside(34);
@@ -827,7 +915,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     }
     // ---- softmax
     const int lane = here(), l16 = lane & 15, l32 = lane & 31, hh = lane >> 5, qr = 32 * w + l32;
-    const uint32_t has = __builtin_amdgcn_readfirstlane(((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
+    const uint32_t has = __builtin_amdgcn_readfirstlane(IMG ? *(SPMLA_LDS uint32_t*)(kt + IMG_OK) : ((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
     const int k0 = kb + j * TR;
     if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
       asm volatile("" : "+v"(S));
@@ -857,7 +945,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         }
       }
       if (!R5) {
-        SPMLA_LDS f32x2* at = (SPMLA_LDS f32x2*)(raw + L::CODE + L::RP) + lane;
+        SPMLA_LDS f32x2* at = (SPMLA_LDS f32x2*)(scales) + lane;
         f32x2 y = *at;
         const bool bad = !(fabsf(y[0]) < __builtin_inff()) || !(fabsf(y[1]) < __builtin_inff());
         y[0] = fabsf(y[0]) < __builtin_inff() ? y[0] : 0.f;
@@ -892,7 +980,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           t[a] = f32x4{S[4 * a], S[4 * a + 1], S[4 * a + 2], S[4 * a + 3]};
-          if constexpr (!R5) t[a] *= *(SPMLA_LDS f32x4*)(raw + L::CODE + L::RP + g * 128 + 32 * a + 16 * hh);
+          if constexpr (!R5) t[a] *= *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh);
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -1024,16 +1112,21 @@ __global__ void __launch_bounds__(256) merge_kernel(MergeParams p) {
 // Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions;
 // of 32 or fewer of 32 rows and four (Row576: eight tiles in LDS; of Row656 seven would fit).
 struct Shape {
-  int rows, slack;
+  int rows, slack, images;                                 // images: tiles of each request that are gathered first (0: none)
   long long tiles;
 };
-static Shape shape_of(int T, int H, int B, int row_bytes) {
+static Shape shape_of(int T, int H, int B, int row_bytes, int longest) {
   const long long n = (long long)T * H;
   const int mr = n <= 32ll * B && row_bytes == ROW576 ? 32 : n <= 64ll * B ? 64 : 128, slack = H % mr != 0;
-  return Shape{mr, slack, n / mr + (slack ? B : 0)};
+  const long long units = ((long long)longest + TR - 1) / TR;
+  const bool images = n >= 512ll * B && B < 65536 && units * B * IMAGE <= 4ll << 30;
+  return Shape{mr, slack, images ? (int)units : 0, n / mr + (slack ? B : 0)};
 }
 // splits need a place for each (token, head), and for the partial results of a split tile's rows
-static long long part_slots(const Shape& s, int items) { return items < 2 * (items - s.tiles) ? items : 2 * (items - s.tiles); }
+static long long part_slots(const Shape& s, int items, int B) {
+  const long long e = items - s.tiles + (s.slack ? B : 0);
+  return items < 2 * e ? items : 2 * e;
+}
 
 }  // namespace chunk
 }  // namespace spmla
@@ -1042,23 +1135,24 @@ using namespace spmla;
 
 extern "C" int spmla_attn_chunk_items(int T, int H, int B, int row_bytes, int longest) {
   if (T <= 0 || H <= 0 || B <= 0 || B > chunk::PLAN || longest <= 2 * chunk::LEAST * chunk::TR) return 0;
-  const long long tiles = chunk::shape_of(T, H, B, row_bytes).tiles, full = (tiles + chunk::CUS - 1) / chunk::CUS * chunk::CUS;
+  const long long tiles = chunk::shape_of(T, H, B, row_bytes, longest).tiles, full = (tiles + chunk::CUS - 1) / chunk::CUS * chunk::CUS;
   // whole rounds of workgroups, a few beyond one a tile for the longest requests; from four rounds on no tile is split
   return tiles >= 4 * chunk::CUS ? 0 : (int)(full - tiles >= chunk::CUS / 4 ? full : full + chunk::CUS / 4);
 }
 
-extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int items) {
-  if (T <= 0 || H <= 0 || B <= 0 || items <= 0 || B > chunk::PLAN) return 0;
-  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes);
-  if (items <= s.tiles) return 0;
-  return (long long)T * H * 8 + 16 + chunk::part_slots(s, items) * s.rows * (D_LAT + 1) * 4;
+extern "C" long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int longest, int items) {
+  if (T <= 0 || H <= 0 || B <= 0 || longest <= 0) return 0;
+  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes, longest);
+  const long long images = (long long)B * s.images * chunk::IMAGE;
+  if (B > chunk::PLAN || items <= s.tiles) return images;
+  return images + (long long)T * H * 8 + 16 + chunk::part_slots(s, items, B) * s.rows * (D_LAT + 1) * 4;
 }
 
 extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                                 int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int items, void* out,
+                                const int* start, int B, int T, int H, float sm_scale, float kv_scale, int longest, int items, void* out,
                                 long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream) {
-  if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || items < 0 ||
+  if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || items < 0 || longest < 0 ||
       (row_bytes != ROW656 && row_bytes != ROW576))
     return SPMLA_EARG;
   if (T > MAX_TOKENS || B > MAX_TOKENS || H > 65536 || items > 65536 || rows > 0x7fffffffll || (long long)W * block_size > 0x7fffff00ll) return SPMLA_ELIMIT;
@@ -1067,31 +1161,39 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   if (((q_st | q_sh | o_st | o_sh) & 7) || (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out) & 15) ||
       (((uintptr_t)start | (uintptr_t)seqs | (uintptr_t)table | (uintptr_t)lse) & 3))
     return SPMLA_EALIGN;
-  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes);
+  const long long room = (long long)W * block_size;
+  if (longest > room) longest = (int)room;
+  const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes, longest);
   if (s.tiles > (1ll << 30)) return SPMLA_ELIMIT;
-  const long long need = spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, items);
-  const int extra = need ? (int)(items - s.tiles) : 0;
+  const long long need = spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, longest, items);
+  const int extra = B <= chunk::PLAN && longest > 0 && items > s.tiles ? (int)(items - s.tiles) : 0;
   if (extra > 511) return SPMLA_ELIMIT;
   if (need && !ws) return SPMLA_EARG;
   if (need && ((uintptr_t)ws & 15)) return SPMLA_EALIGN;
   if (need && ws_bytes < need) return SPMLA_EARG;
-  const long long slots = need ? chunk::part_slots(s, items) : 0;
-  float* opart = need ? (float*)ws : nullptr;
-  float* lpart = need ? opart + slots * s.rows * D_LAT : nullptr;
-  i32x2* parts = need ? (i32x2*)(lpart + slots * s.rows) : nullptr;
+  const long long slots = extra ? chunk::part_slots(s, items, B) : 0;
+  uint8_t* images = s.images ? (uint8_t*)ws : nullptr;
+  float* opart = extra ? (float*)((uint8_t*)ws + (long long)B * s.images * chunk::IMAGE) : nullptr;
+  float* lpart = extra ? opart + slots * s.rows * D_LAT : nullptr;
+  i32x2* parts = extra ? (i32x2*)(lpart + slots * s.rows) : nullptr;
   const float sc = sm_scale * kv_scale;
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
                   H, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)s.tiles, s.slack,
-                  extra ? items : 0, extra, (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts};
-  static DynLds attr[5];
-  static Launcher go[5];
-  const int r5 = row_bytes == ROW576, at = s.rows == 32 ? 4 : 2 * (s.rows == 64) + r5;
-  const void* fn[5] = {(const void*)chunk::wide_kernel<false>, (const void*)chunk::wide_kernel<true>, (const void*)chunk::kernel<false, 2>,
-                       (const void*)chunk::kernel<true, 2>, (const void*)chunk::kernel<true, 4>};
-  const int lds[5] = {chunk::WLds<false>::TOTAL, chunk::WLds<true>::TOTAL, chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES,
-                      chunk::Lds<true, 4>::BYTES};
+                  extra ? items : 0, extra + (extra && s.slack ? B : 0), (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts, longest, images, s.images};
+  static DynLds attr[7];
+  static Launcher go[7], first[2];
+  const int r5 = row_bytes == ROW576, at = s.rows == 32 ? 6 : s.rows == 64 ? 4 + r5 : 2 * (s.images > 0) + r5;
+  const void* fn[7] = {(const void*)chunk::wide_kernel<false, false>, (const void*)chunk::wide_kernel<true, false>,
+                       (const void*)chunk::wide_kernel<false, true>, (const void*)chunk::wide_kernel<true, true>,
+                       (const void*)chunk::kernel<false, 2>, (const void*)chunk::kernel<true, 2>, (const void*)chunk::kernel<true, 4>};
+  const int lds[7] = {chunk::WLds<false>::TOTAL, chunk::WLds<true>::TOTAL, chunk::ILds::TOTAL, chunk::ILds::TOTAL,
+                      chunk::Lds<false, 2>::BYTES, chunk::Lds<true, 2>::BYTES, chunk::Lds<true, 4>::BYTES};
   if (const int rc = attr[at].ensure(fn[at], lds[at])) return rc;
   hipStream_t stm = (hipStream_t)stream;
+  if (images) {
+    const void* f = r5 ? (const void*)chunk::image_kernel<true> : (const void*)chunk::image_kernel<false>;
+    if (const int rc = first[r5](f, dim3((unsigned)s.images, (unsigned)B), 256, 0, stm, p)) return rc;
+  }
   const long long grid = extra ? (items + 7) / 8 * 8 : s.tiles;
   if (const int rc = go[at](fn[at], dim3((unsigned)grid), s.rows == 128 ? 256 : 512, lds[at], stm, p)) return rc;
   if (!extra) return SPMLA_OK;

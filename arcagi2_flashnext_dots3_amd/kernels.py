@@ -1142,13 +1142,13 @@ def attend_prompt(q, k, v, start, scale, causal=True, out=None, lse=None):
 @functools.lru_cache(maxsize=4096)
 def chunk_items(T, H, B, row_bytes, longest):
     """Workgroups that attend_chunk has share the positions of T tokens of H heads in B requests (spmla_attn_chunk_items)."""
-    return int(_lib.lib().spmla_attn_chunk_items(T, H, B, row_bytes, min(longest, 1 << 20)))
+    return int(_lib.lib().spmla_attn_chunk_items(T, H, B, row_bytes, longest))
 
 
 @functools.lru_cache(maxsize=4096)
-def chunk_ws_bytes(T, H, B, row_bytes, items):
+def chunk_ws_bytes(T, H, B, row_bytes, longest, items):
     """Bytes of the workspace attend_chunk needs (spmla_attn_chunk_ws_bytes)."""
-    return int(_lib.lib().spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, items))
+    return int(_lib.lib().spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, longest, items))
 
 
 def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0, max_seq_len=None, out=None, lse=None,
@@ -1157,21 +1157,23 @@ def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0,
     (start [B + 1] int32) are the last of the seq_lens[b] rows that request b has in cache [blocks, block_size, 656 or 576]
     uint8 (already written; block stride any whole number of rows) through block_table [B, columns] int32; each token sees
     its own position and those before it, but for pages that are not there (-1). Returns (out [T, H, 512] bf16, lse [T, H]
-    fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: about the
-    longest seq_lens, known on the host (None: what the table can hold): short ones are not split. items: workgroups that the
-    kernel makes of the requests' positions, in even shares (None: chunk_items; 0: one a tile of query rows); their partial
-    results are joined through a temporary workspace. The result does not depend on either, but for the order of its sums."""
+    fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: at least the longest
+    seq_lens, known on the host (None: what the table can hold); positions from it on are not seen. Temporary workspace: for
+    512 (token, head) rows or more a request, max_seq_len rows of each request in 16 bits (up to 4 GiB; beyond, rows are
+    converted where they are used); for few rows, partial results. items: workgroups that the kernel makes of the requests'
+    positions, in even shares (None: chunk_items; 0: one a tile of query rows); it changes the order of sums alone."""
     _need(q.dim() == 3 and cache.dim() == 3 and block_table.dim() == 2, "q [T, H, 576], cache [blocks, block_size, row], block_table [B, columns]")
     T, H, B, row = q.shape[0], q.shape[1], block_table.shape[0], cache.shape[2]
+    room = block_table.shape[1] * cache.shape[1]
+    longest = room if max_seq_len is None else max(0, min(int(max_seq_len), room))
     if items is None:
-        room = block_table.shape[1] * cache.shape[1]
-        items = chunk_items(T, H, B, row, max(0, room if max_seq_len is None else min(int(max_seq_len), room)))
+        items = chunk_items(T, H, B, row, longest)
     _need(0 <= items <= 65536, "items of 0 to 65536")
     if out is None:
         out = torch.empty(T, H, D_LAT, dtype=torch.bfloat16, device=q.device)
     if lse is None:
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
-    nb = chunk_ws_bytes(T, H, B, row, items) if items else 0
+    nb = chunk_ws_bytes(T, H, B, row, longest, items)
     ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, items, out, lse, ws)
+    _lib.tensor_call("attend_chunk", q, q, cache, block_table, seq_lens, start, sm_scale, kv_scale, longest, items, out, lse, ws)
     return out, lse

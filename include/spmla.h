@@ -546,13 +546,15 @@ int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void*
  * times the row's scale) are rounded to bf16, or to fp16 where requests have 64 (token, head) rows or fewer on average.
  * items: workgroups that the requests' positions are shared out to on the device, by their lengths (0, B > 256, or no more
  * than the tiles of query rows: one a tile; ELIMIT beyond 511 more), partial results joined by a second kernel through a
- * workspace of spmla_attn_chunk_ws_bytes. spmla_attn_chunk_items: a good number of them, longest: about the longest seqs.
+ * workspace of spmla_attn_chunk_ws_bytes. spmla_attn_chunk_items: a good number of them.
+ * longest: positions from there on are not seen; where requests have 512 (token, head) rows or more on average, as many rows
+ * of each are gathered and converted into the workspace first (up to 4 GiB).
  * The dense counterpart of PortableSparseImpl.forward_mqa (dsa_sm89.py:379-470) for layers without an indexer. */
 int spmla_attn_chunk_items(int T, int H, int B, int row_bytes, int longest);
-long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int items);
+long long spmla_attn_chunk_ws_bytes(int T, int H, int B, int row_bytes, int longest, int items);
 int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, const void* cache, long long rows, int row_bytes,
                      int block_size, long long stride_rows, const int* table, long long t_st, int W, const int* seqs,
-                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int items, void* out,
+                     const int* start, int B, int T, int H, float sm_scale, float kv_scale, int longest, int items, void* out,
                      long long o_st, long long o_sh, float* lse, long long l_st, void* ws, long long ws_bytes, void* stream);
 
 /* Build identification string (static storage). */

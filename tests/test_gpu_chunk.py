@@ -92,12 +92,20 @@ def test_splits(dev, row, items, heads, lens):
     _run(dev, case, 64, 0.5, items=items)
 
 
-def test_result_does_not_depend_on_max_seq_len(dev):
-    """Rows beyond a max_seq_len that is too small are still seen."""
-    case = _case([1500, 900], [2, 1], 32, 656, 64, 3)
-    _run(dev, case, 64, items=40, max_seq_len=256)
-    _run(dev, case, 64, max_seq_len=1)
+def test_max_seq_len(dev):
+    """What it is does not change a result, as long as no request has more rows; positions from it on are not seen."""
+    q, cache, table, seqs, start = case = _case([1500, 900], [2, 1], 32, 656, 64, 3)
     _run(dev, case, 64)
+    _run(dev, case, 64, max_seq_len=1500)
+    _run(dev, case, 64, max_seq_len=10 ** 6)
+    from arcagi2_flashnext_dots3_amd import kernels
+    for lens, heads in (([2, 1], 32), ([40, 3], 64)):
+        q, cache, table, seqs, start = _case([1500, 900], lens, heads, 656, 64, 4)
+        out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), seqs.to(dev), start.to(dev), SM, max_seq_len=1000)
+        t = sum(lens) - lens[1] - 1                          # the first request's last token: positions 0 .. 999
+        r = kernels.attend_chunk(q[t:t + 1].to(dev), cache.to(dev), table[:1].to(dev), seqs[:1].clamp(max=1000).to(dev),
+                                 torch.tensor([0, 1], dtype=torch.int32, device=dev), SM)
+        assert torch.allclose(out[t:t + 1].float(), r[0].float(), rtol=2 ** -6, atol=2 ** -7) and torch.allclose(lse[t:t + 1], r[1], rtol=1e-5, atol=1e-5)
 
 
 @pytest.mark.parametrize("row", [656, 576])
