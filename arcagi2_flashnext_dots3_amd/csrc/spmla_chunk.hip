@@ -1033,13 +1033,23 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   }
   const float back = inv * p.kv_scale;
   if (!whole) {
-    float* o = p.opart + (((long long)it.slot + it.sp) * MR + qr) * D_LAT + 4 * hh;
-    if (qr < live)
+    // through LDS, 256 dims of a row at a time: 32 rows of 1024 bytes, 16-byte chunks permuted by the row
+    SPMLA_LDS uint8_t* ob = lds + w * 32768;
+    float* to = p.opart + (((long long)it.slot + it.sp) * MR + 32 * w) * D_LAT + 4 * lane;
 #pragma unroll
-      for (int n = 0; n < 16; ++n)
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-          *(f32x4*)(o + 32 * n + 8 * a) = f32x4{O[n][4 * a], O[n][4 * a + 1], O[n][4 * a + 2], O[n][4 * a + 3]} * back;
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x16& y = O[8 * half + n];
+          *(SPMLA_LDS f32x4*)(ob + l32 * 1024 + 16 * ((8 * n + 2 * a + hh) ^ l32)) = f32x4{y[4 * a], y[4 * a + 1], y[4 * a + 2], y[4 * a + 3]} * back;
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int row = 0; row < 32 && 32 * w + row < live; ++row)
+        *(f32x4*)(to + (long long)row * D_LAT + 256 * half) = *(SPMLA_LDS f32x4*)(ob + row * 1024 + 16 * (lane ^ row));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     return;
   }
   SPMLA_LDS uint8_t* ob = lds + w * 32768;                // 32 rows of 1024 bytes, 16-byte chunks permuted by the row
@@ -1057,27 +1067,27 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 }
 
 // Joins the splits of (token, head) row r: weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
-// was not written, is not read. A workgroup a row and half of its dims, every fourth split a wave, 4 dims a lane. Bound by
-// the partials' bytes.
+// was not written, is not read. 8 waves a row, or one (many rows, that have few splits each); 8 dims a lane. Bound by the
+// partials' bytes.
 struct MergeParams {
-  const float* opart; const float* lpart; const i32x2* parts; long long rows; int items;
+  const float* opart; const float* lpart; const i32x2* parts; long long rows; int slots;
   const int* start; int B, T, H;
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
 };
-__global__ void __launch_bounds__(256) merge_kernel(MergeParams p) {
-  __shared__ float wgt[512];
-  __shared__ f32x4 sums[4][64];
+template <int WAVES>                                       // of a row
+__global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
+  __shared__ float wgt[8][512];
+  __shared__ f32x4 sums[WAVES == 1 ? 1 : 8][2][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long r = blockIdx.x >> 1, t = r / p.H, h = r % p.H;
-  if (t < p.start[0] || t >= p.start[p.B]) return;        // rows of no request stay as they are
+  const long long r = WAVES == 1 ? (long long)blockIdx.x * 8 + w : blockIdx.x, t = r / p.H, h = r % p.H;
+  if (t >= p.T || t < p.start[0] || t >= p.start[p.B]) return;               // rows of no request stay as they are
   const i32x2 part = p.parts[r];
-  const long long first = part[0] & 0x7fffffff, step = p.rows;
-  const int n = part[1];
-  if (n < 2 || n > 512 || (first / step + n) > p.items) return;
+  const int first = __builtin_amdgcn_readfirstlane(part[0]), n = __builtin_amdgcn_readfirstlane(part[1]);
+  if (first < 0 || n < 2 || n > 512 || first / p.rows + n > p.slots) return;
   float top = -__builtin_inff();
   for (int s = lane; s < n; s += 64) {
-    const float x = p.lpart[first + s * step];
+    const float x = p.lpart[first + s * p.rows];
     top = x > top || x != x ? x : top;
   }
 #pragma unroll
@@ -1087,26 +1097,42 @@ __global__ void __launch_bounds__(256) merge_kernel(MergeParams p) {
   }
   const float ref = top == -__builtin_inff() ? 0.f : top;
   float sum = 0.f;
-  for (int s = lane; s < n; s += 64) {
-    const float x = p.lpart[first + s * step], y = x == -__builtin_inff() ? 0.f : __expf(x - ref);
-    if (w == 0) wgt[s] = x == -__builtin_inff() ? -1.f : y;
+  for (int s = lane; s < n; s += 64) {                    // (every wave all of them, in memory of its own)
+    const float x = p.lpart[first + s * p.rows], y = x == -__builtin_inff() ? 0.f : __expf(x - ref);
+    wgt[w][s] = x == -__builtin_inff() ? -1.f : y;
     sum += y;
   }
 #pragma unroll
   for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-  __syncthreads();
-  const float* o = p.opart + first * D_LAT + (blockIdx.x & 1) * 256 + 4 * lane;
-  f32x4 a = {};
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  const float* o = p.opart + (long long)first * D_LAT + 4 * lane;
+  f32x4 a = {}, b = {};
 #pragma unroll 4
-  for (int s = w; s < n; s += 4)
-    if (wgt[s] >= 0.f || wgt[s] != wgt[s]) a += wgt[s] * *(const f32x4*)(o + s * step * D_LAT);
-  sums[w][lane] = a;
-  __syncthreads();
-  if (w) return;
+  for (int s = WAVES == 1 ? 0 : w; s < n; s += WAVES) {
+    const float y = wgt[w][s];
+    if (y >= 0.f || y != y) {
+      a += y * *(const f32x4*)(o + s * p.rows * D_LAT);
+      b += y * *(const f32x4*)(o + s * p.rows * D_LAT + 256);
+    }
+  }
+  if constexpr (WAVES > 1) {
+    sums[w][0][lane] = a;
+    sums[w][1][lane] = b;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      a += sums[i][0][lane];
+      b += sums[i][1][lane];
+    }
+  }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  a = (sums[0][lane] + sums[1][lane] + (sums[2][lane] + sums[3][lane])) * inv;
-  *(i32x2*)(p.out + t * p.o_st + h * p.o_sh + (blockIdx.x & 1) * 256 + 4 * lane) = i32x2{(int)pk_bf16(a[0], a[1]), (int)pk_bf16(a[2], a[3])};
-  if (p.lse && threadIdx.x == 0 && !(blockIdx.x & 1)) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
+  a *= inv;
+  b *= inv;
+  uint16_t* to = p.out + t * p.o_st + h * p.o_sh + 4 * lane;
+  *(i32x2*)to = i32x2{(int)pk_bf16(a[0], a[1]), (int)pk_bf16(a[2], a[3])};
+  *(i32x2*)(to + 256) = i32x2{(int)pk_bf16(b[0], b[1]), (int)pk_bf16(b[2], b[3])};
+  if (p.lse && lane == 0) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
 }
 
 // Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions;
@@ -1197,7 +1223,9 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const long long grid = extra ? (items + 7) / 8 * 8 : s.tiles;
   if (const int rc = go[at](fn[at], dim3((unsigned)grid), s.rows == 128 ? 256 : 512, lds[at], stm, p)) return rc;
   if (!extra) return SPMLA_OK;
-  static Launcher join;
+  static Launcher join[2];
+  const long long n = (long long)T * H;
+  const int many = n > 4096;
   const chunk::MergeParams mp{opart, lpart, parts, s.rows, (int)slots, start, B, T, H, (uint16_t*)out, o_st, o_sh, lse, l_st};
-  return join((const void*)chunk::merge_kernel, dim3((unsigned)(2 * (long long)T * H)), 256, 0, stm, mp);
+  return join[many](many ? (const void*)chunk::merge_kernel<1> : (const void*)chunk::merge_kernel<8>, dim3((unsigned)(many ? (n + 7) / 8 : n)), 512, 0, stm, mp);
 }
