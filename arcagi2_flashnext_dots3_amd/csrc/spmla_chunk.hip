@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         SPMLA_LDS uint8_t* at = ks >= 32 ? rope : kt + (ks >> 2) * 4096;
         return *(SPMLA_LDS bf16x8*)(at + (ka ^ (32 * (ks & 3))));
       };
-      constexpr int KD = R5 ? 8 : 6;
+      constexpr int KD = R5 ? 8 : IMG ? 6 : 5;
       bf16x8 k[KD];
 #pragma unroll
       for (int n = 0; n < KD; ++n) k[n] = kread(n);
@@ -877,6 +877,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         }
       } else {
         f32x16 acc[2];
+        f32x4 sc[2];
         S = f32x16{};
 #pragma unroll
         for (int g = 0; g < 5; ++g) {
@@ -890,10 +891,10 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
               if (g > 0 && n >= 4) {                      // a quarter of the group before: its products are done
                 const int a = n - 4;
                 asm volatile("" : "+v"(acc[(g - 1) & 1]));
-                const f32x4 sc = *(SPMLA_LDS f32x4*)(scales + (g - 1) * 128 + 32 * a + 16 * hh);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[4 * a + r] = __builtin_fmaf(acc[(g - 1) & 1][4 * a + r], sc[r], S[4 * a + r]);
+                for (int r = 0; r < 4; ++r) S[4 * a + r] = __builtin_fmaf(acc[(g - 1) & 1][4 * a + r], sc[a & 1][r], S[4 * a + r]);
               }
+              if (g > 0 && n >= 2 && n < 6) sc[n & 1] = *(SPMLA_LDS f32x4*)(scales + (g - 1) * 128 + 32 * (n - 2) + 16 * hh);
               __builtin_amdgcn_sched_barrier(0);
             }
           } else {
@@ -929,29 +930,23 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     if (__builtin_expect(k0 + TR > least && least < most, 0)) {
       // the mask cuts this tile: values that are no numbers become 0 once every wave has its scores
       lds_barrier();
-      for (int i = 0; i < 8; ++i) {                       // (every wave all of them: others read them beside this)
+      u32x4 y[8];
+      SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(kt + w * 8192) + lane;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          SPMLA_LDS u32x4* at = (SPMLA_LDS u32x4*)(kt + i * 4096 + r * 1024 + lane * 16);
-          u32x4 y = *at;
-          uint32_t bad = 0;
+      for (int i = 0; i < 8; ++i) y[i] = at[64 * i];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t keep = ((y[e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((y[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
-            bad |= ~keep;
-            y[e] &= keep;
-          }
-          if (bad) *at = y;
-        }
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[i][e] &= ((y[i][e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((y[i][e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+        at[64 * i] = y[i];
       }
-      if (!R5) {
-        SPMLA_LDS f32x2* at = (SPMLA_LDS f32x2*)(scales) + lane;
-        f32x2 y = *at;
-        const bool bad = !(fabsf(y[0]) < __builtin_inff()) || !(fabsf(y[1]) < __builtin_inff());
-        y[0] = fabsf(y[0]) < __builtin_inff() ? y[0] : 0.f;
-        y[1] = fabsf(y[1]) < __builtin_inff() ? y[1] : 0.f;
-        if (bad) *at = y;
+      if (!R5 && w == 0) {
+        SPMLA_LDS f32x2* x = (SPMLA_LDS f32x2*)scales + lane;
+        const f32x2 z = *x;
+        *x = f32x2{fabsf(z[0]) < __builtin_inff() ? z[0] : 0.f, fabsf(z[1]) < __builtin_inff() ? z[1] : 0.f};
       }
+      lds_barrier();
     }
     float mx = S[0];
 #pragma unroll
@@ -974,19 +969,16 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     l += sum;
     // ---- O^T += V^T P^T
     {
-      bf16x8 P[2];
-      auto weights = [&](int g) {
-        f32x4 t[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          t[a] = f32x4{S[4 * a], S[4 * a + 1], S[4 * a + 2], S[4 * a + 3]};
-          if constexpr (!R5) t[a] *= *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-          P[ks] = __builtin_bit_cast(bf16x8, u32x4{pk_bf16(t[2 * ks][0], t[2 * ks][1]), pk_bf16(t[2 * ks][2], t[2 * ks][3]),
-                                                   pk_bf16(t[2 * ks + 1][0], t[2 * ks + 1][1]), pk_bf16(t[2 * ks + 1][2], t[2 * ks + 1][3])});
+      bf16x8 P[R5 ? 1 : 2][2];                            // (Row656: weights times the scales of a group, the next one's beside its products)
+      f32x4 sc[2];
+      auto half_of = [&](int g, int a) {                   // positions 8 a + 4 hh .. + 3
+        const f32x4 t = f32x4{S[4 * a], S[4 * a + 1], S[4 * a + 2], S[4 * a + 3]} * (R5 ? f32x4{1.f, 1.f, 1.f, 1.f} : sc[a & 1]);
+        u32x4 y = __builtin_bit_cast(u32x4, P[R5 ? 0 : g & 1][a >> 1]);
+        y[2 * (a & 1)] = pk_bf16(t[0], t[1]);
+        y[2 * (a & 1) + 1] = pk_bf16(t[2], t[3]);
+        P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(bf16x8, y);
       };
+      auto scale_of = [&](int g, int a) { sc[a & 1] = *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh); };
       const int vrow = 4 * hh + (l16 >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
       const int v0 = vrow * 128 + 16 * (vch ^ swz(vrow)) + 8 * (lane & 1);  // (rows 8 on: places ^ 2; the group's other half: ^ 4)
       auto vread = [&](int n) -> bf16x8 {                  // unit n = 2 d + ks: dims 32 d + l32, positions 16 ks ..
@@ -1001,12 +993,23 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       bf16x8 v[VD];
 #pragma unroll
       for (int n = 0; n < VD; ++n) v[n] = vread(n);
-      if constexpr (R5) weights(0);
+      if (!R5) {
+        scale_of(0, 0);
+        scale_of(0, 1);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        half_of(0, a);
+        if (!R5 && a < 2) scale_of(0, a + 2);
+      }
 #pragma unroll
       for (int n = 0; n < 32; ++n) {
-        if (!R5 && n % 8 == 0) weights(n / 8);
-        O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % VD], P[n & 1], O[n >> 1], 0, 0, 0);
+        O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % VD], P[R5 ? 0 : (n >> 3) & 1][n & 1], O[n >> 1], 0, 0, 0);
         if (n + VD < 32) v[n % VD] = vread(n + VD);
+        if (!R5 && n < 24) {
+          if (n % 8 >= 2 && n % 8 < 6) half_of(n / 8 + 1, n % 8 - 2);
+          if (n % 8 < 4) scale_of(n / 8 + 1, n % 8);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
