@@ -120,12 +120,23 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
     top = y > top ? y : top;
   }
   const int extra = p.extra < p.items - tiles ? p.extra : p.items - tiles;     // (fewer tiles where requests fill theirs)
+  tiles = __builtin_amdgcn_readfirstlane(tiles);
   work = __builtin_amdgcn_readfirstlane((int)work) & 0xffffffffll | (long long)__builtin_amdgcn_readfirstlane((int)(work >> 32)) << 32;
   top = __builtin_amdgcn_readfirstlane(top);
   const long long even = (work + p.items - 1) / p.items, most = extra > 0 ? (work + extra - 1) / extra : top;
   int lo = even < LEAST ? LEAST : even < top ? (int)even : top;
   int hi = lo < most ? (most < top ? (int)most : top) : lo;
   if (hi < lo) hi = lo;
+  // more than a round of workgroups, but no more than one of long tiles: one a tile, the long ones first, beats two of halves
+  // (1009 tokens in 10 requests, 259 tiles, 251 of them long: 260 us, in the requests' order 322, split 374)
+  bool plain = false;
+  if (tiles > CUS) {
+    int y = 0;
+#pragma unroll
+    for (int k = 0; k < PLAN / 64; ++k) y += u[k] > top / 2 ? n[k] : 0;
+    plain = __builtin_amdgcn_readfirstlane(wave_sum(y)) <= CUS;
+    if (plain) lo = hi = top;
+  }
   while (lo < hi) {
     const unsigned mid = (unsigned)(lo + hi) >> 1;
     int e = 0;
@@ -141,27 +152,31 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
   for (int k = 0; k < PLAN / 64; ++k)
     if (64 * k < p.B) total += n[k] * (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1);
   total = __builtin_amdgcn_readfirstlane(wave_sum(total));
-  const int per = (total + 7) >> 3, x = blockIdx.x & 7, y = blockIdx.x >> 3;       // consecutive items on one XCD: they read the same rows
-  if (y >= per || (f = x * per + y) >= total) return false;
+  // consecutive items on one XCD: they read the same rows
+  const int per = (total + 7) >> 3, x = blockIdx.x & 7, y = blockIdx.x >> 3;
+  f = plain ? (int)blockIdx.x : y < per ? x * per + y : total;
+  if (f >= total) return false;
   o.b = -1;
+  for (int turn = plain ? 0 : 1; turn < 2; ++turn)
 #pragma unroll
-  for (int k = 0; k < PLAN / 64; ++k)
-    if (64 * k < p.B && o.b < 0) {
-      const int c = (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1), mine = n[k] * c, parts = c > 1 ? mine : 0;
-      const int end = wave_scan(mine, lane), send = wave_scan(parts, lane);
-      const uint64_t hit = __ballot(f < end && f >= end - mine);
-      if (hit) {
-        const int at = __builtin_ctzll(hit), g = f - __builtin_amdgcn_readlane(end - mine, at), nn = __builtin_amdgcn_readlane(n[k], at);
-        o.b = 64 * k + at;
-        o.sp = g / nn;
-        o.tile = nn - 1 - g % nn;
-        o.splits = __builtin_amdgcn_readlane(c, at);
-        o.slot = slots + __builtin_amdgcn_readlane(send - parts, at) + o.tile * o.splits;
-      } else {
-        f -= __builtin_amdgcn_readlane(end, 63);
-        slots += __builtin_amdgcn_readlane(send, 63);
+    for (int k = 0; k < PLAN / 64; ++k)
+      if (64 * k < p.B && o.b < 0) {
+        const int c = (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1);
+        const int mine = plain && (u[k] > top / 2) != (turn == 0) ? 0 : n[k] * c, parts = c > 1 ? mine : 0;
+        const int end = wave_scan(mine, lane), send = wave_scan(parts, lane);
+        const uint64_t hit = __ballot(f < end && f >= end - mine);
+        if (hit) {
+          const int at = __builtin_ctzll(hit), g = f - __builtin_amdgcn_readlane(end - mine, at), nn = __builtin_amdgcn_readlane(n[k], at);
+          o.b = 64 * k + at;
+          o.sp = g / nn;
+          o.tile = nn - 1 - g % nn;
+          o.splits = __builtin_amdgcn_readlane(c, at);
+          o.slot = slots + __builtin_amdgcn_readlane(send - parts, at) + o.tile * o.splits;
+        } else {
+          f -= __builtin_amdgcn_readlane(end, 63);
+          slots += __builtin_amdgcn_readlane(send, 63);
+        }
       }
-    }
   return o.b >= 0;
 }
 
@@ -300,13 +315,12 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   {
     const long long r = r0 + (qr < live ? qr : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
-    const uint32_t turn = p.flip ? 0x80008000u : 0u;
 #pragma unroll
     for (int n = 0; n < 9; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int at = n == 8 && !R5 ? D_LAT + 32 * e + 8 * qt : 64 * n + 16 * qt + 8 * e;
-        qf[n][e] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + at) ^ turn);
+        qf[n][e] = *(const bf16x8*)(qp + at);
       }
   }
   note(0, found);
@@ -484,6 +498,13 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   constexpr int AHEAD = L::RING - PS;                     // tiles copied ahead
   const bool works = 16 * wr < live;
   for (int j = 0; j < AHEAD && j < nt; ++j) issue(j);
+#pragma unroll
+  for (int n = 0; n < 9; ++n) asm volatile("" : "+v"(qf[n][0]), "+v"(qf[n][1]));       // (the query is there; negated where scores are)
+  if (p.flip)
+#pragma unroll
+    for (int n = 0; n < 9; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[n][e] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[n][e]) ^ 0x80008000u);
   for (int j = 0; j < nt; j += PS) {
     // rows of the next IDS positions: looked up as a part begins, noted at the end of the step, copied from a later one on
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
@@ -730,15 +751,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     if (l32 == 0) ((SPMLA_LDS uint32_t*)(lds + L::OK))[at >> 5] = (uint32_t)(has >> (lane & 32));
   };
 
-  // ---- query operands of rows 32 w + l32: B operands of 32x32x16, dims 16 ks + 8 hh ..
+  // ---- query operands of rows 32 w + l32: B operands of 32x32x16, dims 16 ks + 8 hh .. (on their way until the first copies are)
   const int qr = 32 * w + l32;
   bf16x8 qf[36];
+  int found = IMG ? -1 : look(0);
   {
     const long long r = r0 + (qr < live ? qr : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
-    const uint32_t turn = p.flip ? 0x80008000u : 0u;
 #pragma unroll
-    for (int ks = 0; ks < 36; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + 16 * ks + 8 * hh) ^ turn);
+    for (int ks = 0; ks < 36; ++ks) qf[ks] = *(const bf16x8*)(qp + 16 * ks + 8 * hh);
   }
 
   // ---- copies of a tile, in COPIES pieces: wave w the codes of scale group w (piece i: rows 8 i + lane / 8, the chunk whose
@@ -802,12 +823,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   f32x16 O[16];                                           // O^T: dims 32 n + 8 a + 4 hh + b, query row qr
   float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, of both halves; l: this half's)
   SPMLA_LDS int* over = (SPMLA_LDS int*)(lds + OVER);
-  bool maxima = false;
+  bool maxima = false, again = false;
+  uint32_t turn = p.flip ? 0x80008000u : 0u;
   for (;;) {
   if (tid == 0) *over = 0;
-  int found = -1;
   if constexpr (!IMG) {
-    note(0, look(0));
+    if (maxima || again) found = look(0);
+    note(0, found);
     note(1, -1);                                          // (addresses that a copy may take, whatever the tile)
   }
   l = 0.f;
@@ -822,6 +844,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       copy(j, i, from);
     }
   }
+#pragma unroll
+  for (int ks = 0; ks < 36; ++ks) asm volatile("" : "+v"(qf[ks]));           // (the query is there; negated where scores are, once)
+  if (turn)
+#pragma unroll
+    for (int ks = 0; ks < 36; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[ks]) ^ turn);
+  turn = 0;
+  again = true;
   wait_vm<2 * COPIES>();
   lds_barrier();
 #pragma unroll
