@@ -62,20 +62,6 @@ struct Item {
 };
 constexpr int PLAN = 256, CUS = 256, LEAST = 4;                     // (a split of fewer tiles costs more to join than it saves)
 
-__device__ inline int wave_sum(int x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ inline int wave_scan(int x, int lane) {         // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    x += lane >= d ? y : 0;
-  }
-  return x;
-}
-
 template <int MR>
 __device__ inline bool find_item(const Params& p, int lane, Item& o) {
   if (p.extra == 0) {
@@ -112,17 +98,12 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
       top = n[k] > 0 && u[k] > top ? u[k] : top;
     }
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    work += __shfl_xor(work, d);
-    tiles += __shfl_xor(tiles, d);
-    const int y = __shfl_xor(top, d);
-    top = y > top ? y : top;
-  }
+  // (in two parts: a lane has 4 products of less than 2^42)
+  const int wl = wave_total((int)(work & 0xffffff)), wh = wave_total((int)(work >> 24));
+  work = ((long long)wh << 24) + wl;
+  tiles = wave_total(tiles);
+  top = wave_top(top);
   const int extra = p.extra < p.items - tiles ? p.extra : p.items - tiles;     // (fewer tiles where requests fill theirs)
-  tiles = __builtin_amdgcn_readfirstlane(tiles);
-  work = __builtin_amdgcn_readfirstlane((int)work) & 0xffffffffll | (long long)__builtin_amdgcn_readfirstlane((int)(work >> 32)) << 32;
-  top = __builtin_amdgcn_readfirstlane(top);
   const long long even = (work + p.items - 1) / p.items, most = extra > 0 ? (work + extra - 1) / extra : top;
   int lo = even < LEAST ? LEAST : even < top ? (int)even : top;
   int hi = lo < most ? (most < top ? (int)most : top) : lo;
@@ -134,7 +115,7 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
     int y = 0;
 #pragma unroll
     for (int k = 0; k < PLAN / 64; ++k) y += u[k] > top / 2 ? n[k] : 0;
-    plain = __builtin_amdgcn_readfirstlane(wave_sum(y)) <= CUS;
+    plain = wave_total(y) <= CUS;
     if (plain) lo = hi = top;
   }
   while (lo < hi) {
@@ -143,7 +124,7 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
 #pragma unroll
     for (int k = 0; k < PLAN / 64; ++k)
       if (64 * k < p.B) e += n[k] * (int)(((unsigned)u[k] - 1) / mid);
-    e = __builtin_amdgcn_readfirstlane(wave_sum(e));
+    e = wave_total(e);
     if (e <= extra) hi = mid; else lo = mid + 1;
   }
   o.span = lo;
@@ -151,7 +132,7 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
 #pragma unroll
   for (int k = 0; k < PLAN / 64; ++k)
     if (64 * k < p.B) total += n[k] * (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1);
-  total = __builtin_amdgcn_readfirstlane(wave_sum(total));
+  total = wave_total(total);
   // consecutive items on one XCD: they read the same rows
   const int per = (total + 7) >> 3, x = blockIdx.x & 7, y = blockIdx.x >> 3;
   f = plain ? (int)blockIdx.x : y < per ? x * per + y : total;
@@ -163,7 +144,7 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
       if (64 * k < p.B && o.b < 0) {
         const int c = (int)(((unsigned)u[k] - 1) / (unsigned)lo + 1);
         const int mine = plain && (u[k] > top / 2) != (turn == 0) ? 0 : n[k] * c, parts = c > 1 ? mine : 0;
-        const int end = wave_scan(mine, lane), send = wave_scan(parts, lane);
+        const int end = (int)wave_incl_scan((uint32_t)mine), send = (int)wave_incl_scan((uint32_t)parts);
         const uint64_t hit = __ballot(f < end && f >= end - mine);
         if (hit) {
           const int at = __builtin_ctzll(hit), g = f - __builtin_amdgcn_readlane(end - mine, at), nn = __builtin_amdgcn_readlane(n[k], at);

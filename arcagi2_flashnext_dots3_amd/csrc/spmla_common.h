@@ -102,6 +102,30 @@ __host__ __device__ inline uint8_t e2m2_to_e4m3(uint32_t code, int k) {
 }
 
 // ---- XCD-aware workgroup order ---------------------------------------------------------------------------
+// Inclusive prefix sum over the 64 lanes of a wave on the VALU: DPP row shifts 1, 2, 4, 8 scan each 16-lane row,
+// then row_bcast:15 adds row 0's total to row 1 and row 2's to row 3, and row_bcast:31 adds rows 0-1's total to rows
+// 2 and 3 (gfx9 DPP controls). A lane whose DPP source is outside its row adds 0.
+__device__ inline uint32_t wave_incl_scan(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);   // row_shr:1
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);   // row_shr:2
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);   // row_shr:4
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);   // row_shr:8
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);   // row_bcast:15, rows 1, 3
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);   // row_bcast:31, rows 2, 3
+  return x;
+}
+__device__ inline int wave_total(int x) { return __builtin_amdgcn_readlane((int)wave_incl_scan((uint32_t)x), 63); }
+__device__ inline int wave_top(int x) {                    // the largest, of values >= 0
+  auto up = [&](int y) { x = y > x ? y : x; };
+  up(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  up(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  up(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  up(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  up(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  up(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The dispatcher hands workgroup i to XCD (i % 8). remap_xcd(i, n) gives the logical work index so that
 // each XCD receives a contiguous block of ceil(n / 8) logical items: consecutive logical items (e.g. the
 // head groups of one token, which gather the same rows) then share one XCD's L2. Returns -1 for the padding

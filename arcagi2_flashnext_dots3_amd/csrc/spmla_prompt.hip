@@ -36,7 +36,7 @@ struct Params {
   const int* start; int B, T, H, group, D, Dv;
   float c;                            // |scale| log2(e)
   int flip;                           // scale < 0: queries with their signs turned
-  int causal, tiles, order;
+  int causal, tiles, together;        // together: heads that one XCD takes tile by tile (0: H is no multiple of 8)
   uint16_t* out; long long o_st, o_sh;
   float* lse; long long l_st;
 };
@@ -80,6 +80,72 @@ __device__ inline float half_sum(float x) {
   return u2f(a) + u2f(b);
 }
 
+// Tile `rank` (MQ queries) of a head, the longest first: up to SORTED sequences by a search for the level x (causal: tiles of
+// index x - 1; full: sequences of x tiles) that the rank falls into, v(x) tiles of a sequence being at levels >= x; more
+// sequences from the last to the first, sequence b from tile start[b] / MQ + b (as many tiles lie between two sequences as
+// the first one has). 17 ragged sequences, 32 heads: see the kernel.
+constexpr int SORTED = 256;
+
+template <int MQ>
+__device__ inline bool place(const Params& p, int lane, int rank, int& b, int& q0) {
+  if (p.B > SORTED) {
+    const int ti = p.tiles - 1 - rank;
+    int lo = 0, hi = p.B, step;
+    if (ti < 0) return false;
+    do {                              // the last b whose first tile is no later, 64 places a step
+      step = (hi - lo + 63) >> 6;
+      const int at = lo + lane * step;
+      const int n = __popcll(__ballot(at < hi && p.start[at] / MQ + at <= ti));
+      lo += (n > 0 ? n - 1 : 0) * step;
+      hi = lo + step < hi ? lo + step : hi;
+    } while (step > 1);
+    b = lo;
+    q0 = (ti - p.start[lo] / MQ - lo) * MQ;
+    return q0 >= 0;
+  }
+  int n[SORTED / 64], top = 0;
+#pragma unroll
+  for (int k = 0; k < SORTED / 64; ++k) {
+    n[k] = 0;
+    const int at = 64 * k + lane;
+    if (at < p.B) {
+      const int s0 = p.start[at], s1 = p.start[at + 1], len = (s1 > p.T ? p.T : s1) - (s0 < 0 ? 0 : s0);
+      n[k] = len > 0 ? (len + MQ - 1) / MQ : 0;
+    }
+    top = n[k] > top ? n[k] : top;
+  }
+  top = wave_top(top);
+  auto from = [&](int x) {            // tiles at levels >= x
+    int y = 0;
+#pragma unroll
+    for (int k = 0; k < SORTED / 64; ++k)
+      if (64 * k < p.B) y += n[k] < x ? 0 : p.causal ? n[k] - x + 1 : n[k];
+    return wave_total(y);
+  };
+  int lo = 1, hi = top + 1;             // from(hi) = 0
+  if (from(1) <= rank) return false;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > rank) lo = mid; else hi = mid;
+  }
+  const int g = rank - from(hi), each = p.causal ? 1 : lo;                 // of the level's tiles
+  int member = g / each, found = -1;
+#pragma unroll
+  for (int k = 0; k < SORTED / 64; ++k) {
+    const uint64_t has = __ballot(p.causal ? n[k] >= lo : n[k] == lo);
+    const int c = __popcll(has);
+    if (found < 0 && member < c) {    // its lane: the one with `member` members before it
+      const int before = __popcll(has & ((1ull << lane) - 1));
+      found = 64 * k + __builtin_ctzll(__ballot((has >> lane & 1) && before == member));
+    }
+    member -= c;
+  }
+  if (found < 0) return false;
+  b = found;
+  q0 = (p.causal ? lo - 1 : g % each) * MQ;
+  return true;
+}
+
 template <int DK, int DV>
 struct Lds {
   static constexpr int K = TK * DK * 2, V = TK * DV * 2, BUF = K + V, TOTAL = 2 * BUF;
@@ -95,32 +161,24 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hh = lane >> 5, l32 = lane & 31;
 
-  // ---- work item: head and tile, the tiles of a head from its last (the longest rows of a causal sequence) to its first
-  int f = blockIdx.x;
-  int h, ti;
-  if (p.order) {                      // heads in turn on one XCD
-    f = remap_xcd(f, p.H * p.tiles);
-    if (f < 0) return;
-    h = f / p.tiles;
-    ti = p.tiles - 1 - f % p.tiles;
+  // ---- work item: head and tile, a head's longest tiles first
+  int h, rank;
+  if (p.together) {                   // an XCD's heads in groups that read the same or few keys
+    const int per = p.H >> 3, y = blockIdx.x >> 3, g = y / (p.together * p.tiles), x = y % (p.together * p.tiles);
+    if (g * p.together >= per) return;
+    h = (blockIdx.x & 7) * per + g * p.together + x % p.together;
+    rank = x / p.together;
   } else {
-    h = f % p.H;
-    ti = p.tiles - 1 - f / p.H;
+    h = blockIdx.x % p.H;
+    rank = blockIdx.x / p.H;
   }
-  // sequence b starts at tile start[b] / MQ + b: at least as many tiles lie between two sequences as the first one has
-  int nb = 0;
-  for (int at = 0; at < p.B; at += 64) {
-    const int b = at + lane;
-    const bool in = b < p.B && p.start[b] / MQ + b <= ti;
-    nb += __popcll(__ballot(in));
-  }
-  const int b = nb > 0 ? nb - 1 : 0;
+  int b, q0;
+  if (!place<MQ>(p, lane, rank, b, q0)) return;
   int s0 = p.start[b], s1 = p.start[b + 1];
-  const int q0 = (ti - (s0 / MQ + b)) * MQ;
   s0 = s0 < 0 ? 0 : s0;
   s1 = s1 > p.T ? p.T : s1;
   const int len = s1 - s0;
-  if (q0 < 0 || q0 >= len) return;
+  if (q0 >= len) return;
 
   const int qw = q0 + 32 * w;                              // the wave's first query
   const int qi = qw + l32;                                 // the lane's
@@ -339,14 +397,14 @@ int launch(Params& p, hipStream_t s) {
   p.tiles = p.T / (32 * NW) + p.B;
   const long long n = (long long)p.tiles * p.H;
   if (n > (1ll << 30)) return SPMLA_ELIMIT;
-  return start(fn, dim3((unsigned)((n + 7) / 8 * 8)), 64 * NW, lds, s, p);
+  return start(fn, dim3((unsigned)n), 64 * NW, lds, s, p);
 }
 
 template <bool BF>
 int go(Params& p, hipStream_t s) {
   if (p.D <= 64 && p.Dv <= 64) return launch<BF, 64, 64, 4>(p, s);
-  if (p.D <= 128 && p.Dv <= 128) return launch<BF, 128, 128, 8>(p, s);
-  if (p.D <= 192 && p.Dv <= 128) return launch<BF, 192, 128, 8>(p, s);
+  if (p.D <= 128 && p.Dv <= 128) return launch<BF, 128, 128, 4>(p, s);
+  if (p.D <= 192 && p.Dv <= 128) return launch<BF, 192, 128, 4>(p, s);
   return launch<BF, 256, 256, 4>(p, s);
 }
 
@@ -367,7 +425,7 @@ extern "C" int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, 
       (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) || (((uintptr_t)start | (uintptr_t)lse) & 3))
     return SPMLA_EALIGN;
   prompt::Params p{(const uint16_t*)q, q_st, q_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh, start, B, T, H,
-                   H / Hk, D, Dv, fmaxf((scale < 0.f ? -scale : scale) * 1.4426950408889634f, 1e-30f), scale < 0.f, causal != 0, 0, Hk >= 8,
+                   H / Hk, D, Dv, fmaxf((scale < 0.f ? -scale : scale) * 1.4426950408889634f, 1e-30f), scale < 0.f, causal != 0, 0, H % 8 ? 0 : H % 32 == 0 ? 4 : H % 16 == 0 ? 2 : 1,
                    (uint16_t*)out, o_st, o_sh, lse, l_st};
   return dtype == DT_BF16 ? prompt::go<true>(p, (hipStream_t)stream) : prompt::go<false>(p, (hipStream_t)stream);
 }
