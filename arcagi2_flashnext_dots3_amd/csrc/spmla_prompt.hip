@@ -17,6 +17,7 @@
 //     their place, and the queries that see such a value get it at the end.
 #include "spmla_common.h"
 #include "spmla_quant.h"
+#include <type_traits>
 
 namespace spmla {
 namespace prompt {
@@ -151,6 +152,14 @@ struct Lds {
   static constexpr int K = TK * DK * 2, V = TK * DV * 2, BUF = K + V, TOTAL = 2 * BUF;
 };
 
+template <int G, int I = 0>
+__device__ inline void copies(uint64_t from, SPMLA_LDS uint8_t* to) {      // a row's chunk of G groups
+  if constexpr (I < G) {
+    dma16_off<128 * I, 8192 * I>(from, to);
+    copies<G, I + 1>(from, to);
+  }
+}
+
 template <bool BF, int DK, int DV, int NW>
 __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   using E = Type<BF>;
@@ -188,8 +197,10 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   const int kend = p.causal && q0 + MQ < len ? q0 + MQ : len;
   const int nt = (kend + TK - 1) / TK;
 
-  // ---- copies: a lane copies from row 8 i + lane / 8 of a group of columns, the chunk whose place is lane % 8
-  auto issue = [&](const uint8_t* base, long long st, int dim, int groups, int k0, int dst) {
+  // ---- copies: a lane copies from row 8 i + lane / 8 of a group of columns, the chunk whose place is lane % 8. Whole tiles of
+  // whole heads: rows 8 w + lane / 8 (+ 32 with four waves) of every group, one address for them; otherwise one by one.
+  auto issue_some = [&](const uint8_t* base, long long st, int dim, int groups, int k0, int dst) {
+#pragma unroll 1
     for (int i = w; i < 8 * groups; i += NW) {             // (wave-uniform)
       const int g = i >> 3, row = (i & 7) * 8 + (lane >> 3);
       const int col = 64 * g + 8 * ((lane & 7) ^ swz(row));
@@ -197,10 +208,29 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
       dma16(k0 + row < len && col < dim ? (const void*)src : (const void*)zeros, lds + dst + i * 1024);
     }
   };
+  constexpr int RS = 8 / NW;
+  const int crow = 8 * w + (lane >> 3), cch = 16 * ((lane & 7) ^ swz(crow));
+  const uint64_t ksrc = (uint64_t)(uintptr_t)kp + (uint64_t)((long long)crow * p.k_st * 2 + cch);
+  const uint64_t vsrc = (uint64_t)(uintptr_t)vp + (uint64_t)((long long)crow * p.v_st * 2 + cch);
+  const bool heads = p.D == DK && p.Dv == DV;
   auto issue_tile = [&](int j) {
     const int buf = (j & 1) * L::BUF;
-    issue(kp, p.k_st, p.D, GK, j * TK, buf);
-    issue(vp, p.v_st, p.Dv, GV, j * TK, buf + L::K);
+    if (heads && (j + 1) * TK <= len) {
+      SPMLA_LDS uint8_t* to = lds + buf + w * 1024;
+#pragma unroll
+      for (int i = 0; i < RS; ++i) {
+        const uint64_t k = ksrc + (uint64_t)((long long)(j * TK + 32 * i) * p.k_st * 2);
+        copies<GK>(k, to + i * 4096);
+      }
+#pragma unroll
+      for (int i = 0; i < RS; ++i) {
+        const uint64_t v = vsrc + (uint64_t)((long long)(j * TK + 32 * i) * p.v_st * 2);
+        copies<GV>(v, to + L::K + i * 4096);
+      }
+    } else {
+      issue_some(kp, p.k_st, p.D, GK, j * TK, buf);
+      issue_some(vp, p.v_st, p.Dv, GV, j * TK, buf + L::K);
+    }
   };
   issue_tile(0);
 
@@ -234,12 +264,14 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) va[i][e] = (vrow + 8 * e) * 128 + (((4 * i + vch) ^ swz(vrow + 8 * e)) * 16) + 8 * (lane & 1);
 
-  for (int j = 0; j < nt; ++j) {
+  // a tile; CUT: one that the wave's mask may cut (loops of their own, or every tile would pay for the other path's O)
+  auto tile = [&](int j, auto cutting) {
+    constexpr bool CUT = decltype(cutting)::value;
     wait_vm<0>();
     lds_barrier();                                         // tile j is there, tile j - 1 is done with
     if (j + 1 < nt) issue_tile(j + 1);
     const int k0 = j * TK;
-    if (!active || (p.causal && k0 > qw + 31)) continue;
+    if (CUT && (!active || (p.causal && k0 > qw + 31))) return;
     SPMLA_LDS uint8_t* kb = lds + (j & 1) * L::BUF;
     SPMLA_LDS uint8_t* vb = kb + L::K;
 
@@ -251,8 +283,7 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
       for (int ks = 0; ks < DK / 16; ++ks)
         S[u] = E::mfma(*(SPMLA_LDS u32x4*)(kb + ka[ks & 3] + (ks >> 2) * (TK * 128) + u * 4096), qf[ks], S[u]);
     }
-    const bool cut = p.causal && k0 + TK - 1 > qw;         // the mask cuts this tile
-    if (cut || k0 + TK > len) {
+    if constexpr (CUT) {
       const int last = p.causal ? (qi < len ? qi : len - 1) : len - 1;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -311,7 +342,7 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
       const auto a = __builtin_bit_cast(i32x2, x), c = __builtin_bit_cast(i32x2, y);
       return u32x4{(uint32_t)a[0], (uint32_t)a[1], (uint32_t)c[0], (uint32_t)c[1]};
     };
-    if (cut) {
+    if constexpr (CUT) {
       uint32_t odd = 0;
 #pragma unroll
       for (int d = 0; d < DV / 32; ++d) {
@@ -339,14 +370,18 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
           }
           asm volatile("" ::: "memory");
         }
-        continue;
+        return;
       }
     }
 #pragma unroll
     for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) O[d] = E::mfma(vread(d, i >> 1, i & 1), P[i >> 1][i & 1], O[d]);
-  }
+  };
+  const int full = len / TK, clear = p.causal && (qw + 1) / TK < full ? (qw + 1) / TK : full;
+  int j = 0;
+  for (; j < nt && j < clear; ++j) tile(j, std::false_type());
+  for (; j < nt; ++j) tile(j, std::true_type());
 
   if (__builtin_expect(odd_from < kend, 0)) {              // those values for the queries that see them
     for (int key = odd_from; key < kend && key <= qw + 31; ++key)
@@ -400,11 +435,15 @@ int launch(Params& p, hipStream_t s) {
   return start(fn, dim3((unsigned)n), 64 * NW, lds, s, p);
 }
 
+// Eight waves read a tile of keys for 256 queries, four for 128: long prompts take eight (4096 tokens, 128 heads of 192 + 128:
+// 735 us against 770), short ones and few of them four, whose last tiles hold fewer queries that are none and fill the chip
+// (17 prompts of 8003 tokens, 32 heads of 128: 144 us against 163).
 template <bool BF>
 int go(Params& p, hipStream_t s) {
+  const bool wide = (long long)p.T >= 1024ll * p.B && (long long)p.T * p.H >= 256ll * 1024;
   if (p.D <= 64 && p.Dv <= 64) return launch<BF, 64, 64, 4>(p, s);
-  if (p.D <= 128 && p.Dv <= 128) return launch<BF, 128, 128, 4>(p, s);
-  if (p.D <= 192 && p.Dv <= 128) return launch<BF, 192, 128, 4>(p, s);
+  if (p.D <= 128 && p.Dv <= 128) return wide ? launch<BF, 128, 128, 8>(p, s) : launch<BF, 128, 128, 4>(p, s);
+  if (p.D <= 192 && p.Dv <= 128) return wide ? launch<BF, 192, 128, 8>(p, s) : launch<BF, 192, 128, 4>(p, s);
   return launch<BF, 256, 256, 4>(p, s);
 }
 
