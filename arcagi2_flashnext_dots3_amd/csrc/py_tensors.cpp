@@ -376,10 +376,10 @@ long latent_write(PyObject* const* a) {
 struct Pool {
   const at::Tensor *table, *lens, *held, *free, *state;
   int64_t M, W, st, P;
-  int bs, dev;
+  int bs;
 };
 Pool pool_of(PyObject* const* a, PyObject* block) {
-  Pool p{tensor(a[0], "table"), tensor(a[1], "lens"), tensor(a[2], "held"), tensor(a[3], "free"), tensor(a[4], "state"), 0, 0, 0, 0, 0, 0};
+  Pool p{tensor(a[0], "table"), tensor(a[1], "lens"), tensor(a[2], "held"), tensor(a[3], "free"), tensor(a[4], "state"), 0, 0, 0, 0, 0};
   if (p.table->dim() != 2) refuse("table [requests, pages of a request] int32: got " + shown(*p.table));
   p.M = p.table->size(0), p.W = p.table->size(1);
   if (p.M == 0) refuse("table: at least one request");
@@ -393,9 +393,13 @@ Pool pool_of(PyObject* const* a, PyObject* block) {
   const long long bs = integer(block);
   if (bs < 1 || bs > 1 << 20) refuse("block_size of 1 to 2^20: got " + std::to_string(bs));
   p.bs = (int)bs;
-  p.dev = gpu_of(*p.table);
-  for (const at::Tensor* t : {p.table, p.lens, p.held, p.free, p.state}) same_gpu(*t, p.dev, "pool");
   return p;
+}
+int gpu_with(const Pool& p, std::initializer_list<const at::Tensor*> more, const char* what) {
+  const int dev = gpu_of(*p.table);
+  for (const at::Tensor* t : {p.table, p.lens, p.held, p.free, p.state}) same_gpu(*t, dev, what);
+  for (const at::Tensor* t : more) same_gpu(*t, dev, what);
+  return dev;
 }
 
 // page_step(table, lens, held, free, state, block_size, new, start, req, positions, slots)
@@ -409,8 +413,8 @@ long page_step(PyObject* const* a) {
   const int64_t n = req->size(0);
   line(*pos, n, n, I64, "positions [n] int64");
   line(*slots, n, n, I64, "slots [n] int64");
-  for (const at::Tensor* t : {fresh, start, req, pos, slots}) same_gpu(*t, p.dev, "page_step");
-  return launch(p.dev, [&](void* s) {
+  const int dev = gpu_with(p, {fresh, start, req, pos, slots}, "page_step");
+  return launch(dev, [&](void* s) {
     return f_page_step((const int*)address(fresh), (int)p.M, (int*)address(p.lens), (int*)address(p.held), (int*)address(p.table), p.st,
                        as_int(p.W, "W"), (int*)address(p.free), (int)p.P, (int*)address(p.state), p.bs, (int)n, (int*)address(start),
                        (int*)address(req), (long long*)address(pos), (long long*)address(slots), s);
@@ -422,8 +426,8 @@ long page_trim(PyObject* const* a) {
   const Pool p = pool_of(a, a[5]);
   const at::Tensor* keep = tensor(a[6], "keep");
   line(*keep, p.M, p.M, I32, "keep [requests] int32");
-  same_gpu(*keep, p.dev, "page_trim");
-  return launch(p.dev, [&](void* s) {
+  const int dev = gpu_with(p, {keep}, "page_trim");
+  return launch(dev, [&](void* s) {
     return f_page_trim((const int*)address(keep), (int)p.M, (int*)address(p.lens), (int*)address(p.held), (int*)address(p.table), p.st,
                        as_int(p.W, "W"), (int*)address(p.free), (int)p.P, (int*)address(p.state), p.bs, s);
   });

@@ -115,11 +115,15 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
       b = find(st, M, t);
       const int len = clamp0(p.lens[b], 0x7fffffff), held = clamp0(p.held[b], p.W);
       pos = (long long)len + (t - st[b]);
-      const long long c = pos / p.bs;
+      const uint32_t c = (uint32_t)pos / (uint32_t)p.bs;           // (two lengths below 2^31: 32 bits without a sign)
       int page = -1;
-      if (c < held) page = p.table[b * p.t_st + c];
-      else if (c < p.W && off[b] + (c - held) < got && c - held < off[b + 1] - off[b]) page = p.free[count - 1 - (off[b] + (int)(c - held))];
-      if (page >= 0) slot = (long long)page * p.bs + pos % p.bs;
+      if (c < (uint32_t)held) {
+        page = p.table[b * p.t_st + c];
+      } else if (c < (uint32_t)p.W) {
+        const int i = (int)c - held;                // of the pages that the request takes
+        if (i < off[b + 1] - off[b] && i < got - off[b]) page = p.free[count - 1 - (off[b] + i)];
+      }
+      if (page >= 0) slot = (long long)page * p.bs + (uint32_t)pos % (uint32_t)p.bs;
     }
     req[t] = b;
     positions[t] = pos;

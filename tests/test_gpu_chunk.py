@@ -145,6 +145,54 @@ def test_padded_block_stride_and_strided_query(dev):
             assert bool((x == 7.0).all())
 
 
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads", [16, 128])
+def test_many_requests(dev, row, heads):
+    """More requests than the shares are formed for; some without tokens, some without rows."""
+    n = 300
+    seqs, lens = [(37 * b) % 100 for b in range(n)], [0 if b % 7 == 3 else 1 for b in range(n)]
+    _run(dev, _case(seqs, lens, heads, row, 16, heads), 16)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads", [40, 128])
+def test_rows_gathered_first(dev, row, heads):
+    """Requests of 512 (token, head) rows or more: pages that end inside a tile, some missing, positions split."""
+    case = _case([700, 300, 77], [40, 33, 30], heads, row, 48, heads, missing=[(0, 0), (0, 14), (1, 3)])
+    for kw in (dict(), dict(items=0), dict(items=130), dict(max_seq_len=700)):
+        _run(dev, case, 48, **kw)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads,lens", [(4, [1, 1]), (16, [1, 1]), (128, [1, 1]), (64, [20, 11])])
+def test_scores_rise_far_over_the_first_tile(dev, row, heads, lens):
+    """Scores that climb by hundreds behind the first positions, past what a reference that does not move can hold."""
+    q, cache, table, seqs, start = _case([300, 200], lens, heads, row, 16, 17)
+    q = (q.float() + 6.0 * torch.arange(576).remainder(2).mul(2).sub(1)).to(torch.bfloat16)
+    sign = torch.arange(576).remainder(2).mul(2).sub(1)
+    for b, at in ((0, 90), (0, 91), (0, 200), (1, 64)):          # rows along the queries' common direction, larger later
+        page, off = int(table[b, at // 16]), at % 16
+        x = sign * (1.0 + at / 100.0)
+        if row == 576:
+            cache[page, off] = x.to(ref.E4M3).view(torch.uint8)
+        else:
+            sc = torch.full((4,), float(x.abs().max()) / 448.0)
+            cache[page, off, :512] = (x[:512] / sc[0]).to(ref.E4M3).view(torch.uint8)
+            cache[page, off, 512:528] = sc.view(torch.uint8)
+            cache[page, off, 528:] = x[512:].to(torch.bfloat16).view(torch.uint8)
+    case = (q, cache, table, seqs, start)
+    _run(dev, case, 16)
+    _run(dev, case, 16, items=20)
+    _run(dev, case, 16, 0.5, items=0)
+
+
+@pytest.mark.parametrize("scale", [-1.0, 0.0])
+def test_kv_scales(dev, scale):
+    """A negative scale turns the order of the scores, zero makes all weights equal (and the output 0)."""
+    for heads, lens in ((16, [1, 1]), (128, [1, 1]), (64, [20, 11])):
+        _run(dev, _case([300, 200], lens, heads, 576, 16, 18), 16, scale)
+
+
 @pytest.mark.parametrize("spread", [3.0, 8.0])
 def test_scales_far_apart(dev, spread):
     """Latents of very different sizes in one context (scale ratios up to e^40): bounded by the largest."""

@@ -37,6 +37,7 @@ SIZES = [  # lengths around the tiles of 64 keys and 128 / 256 queries, heads, w
     ([1], 1, 1, 64, 64), ([2, 1, 63], 4, 2, 64, 64), ([64, 65, 1, 127], 3, 1, 128, 128), ([256, 257, 255], 2, 2, 192, 128),
     ([700], 2, 1, 192, 128), ([130, 3, 90], 16, 8, 128, 128), ([33, 129], 5, 1, 72, 40), ([100, 28], 2, 2, 256, 256),
     ([200], 2, 2, 96, 96), ([50, 0, 77], 2, 1, 8, 8), ([300, 20], 2, 2, 64, 128), ([150], 2, 1, 192, 192), ([1] * 70, 2, 2, 128, 64),
+    ([300, 2, 130], 32, 4, 128, 128), ([130, 40], 64, 64, 64, 64), ([170], 24, 8, 192, 128),
 ]
 
 
@@ -49,6 +50,39 @@ def test_against_64_bits(dev, lens, H, Hk, D, Dv, causal, dt):
     out, lse = kernels.attend_prompt(q.to(dev), k.to(dev), v.to(dev), start.to(dev), D ** -0.5, causal=causal)
     torch.cuda.synchronize()
     _check(out.cpu(), lse.cpu(), q, k, v, lens, D ** -0.5, causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(dev, causal):
+    """More sequences than the kernel sorts, many of them empty."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    lens = [(7 * b * b + b) % 11 % 6 for b in range(300)] + [140, 0, 0]
+    q, k, v, start = _inputs(lens, 3, 1, 64, 64, torch.bfloat16, 13)
+    out, lse = kernels.attend_prompt(q.to(dev), k.to(dev), v.to(dev), start.to(dev), 0.125, causal=causal)
+    torch.cuda.synchronize()
+    _check(out.cpu(), lse.cpu(), q, k, v, lens, 0.125, causal)
+
+
+@pytest.mark.parametrize("D,Dv", [(128, 128), (192, 128), (120, 104)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_long_prompts_of_many_heads(dev, D, Dv, causal):
+    """Enough work for workgroups of eight waves: some heads against 64 bits; a value that is no number reaches those behind
+    it only."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    lens, H, Hk, at = [2100, 1], 128, 8, 1333
+    q, k, v, start = _inputs(lens, H, Hk, D, Dv, torch.bfloat16, D)
+    args = (q.to(dev), k.to(dev), v.to(dev), start.to(dev), D ** -0.5)
+    out, lse = kernels.attend_prompt(*args, causal=causal)
+    torch.cuda.synchronize()
+    for h in (0, 37, 127):
+        g = h // (H // Hk)
+        _check(out[:, h:h + 1].cpu(), lse[:, h:h + 1].cpu(), q[:, h:h + 1], k[:, g:g + 1], v[:, g:g + 1], lens, D ** -0.5, causal)
+    args[2][at, 3, 5] = float("inf")
+    o2, z2 = kernels.attend_prompt(*args, causal=causal)
+    torch.cuda.synchronize()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[at if causal else 0:2100, 3 * 16:4 * 16, 5] = True
+    assert bool((o2[hit] == float("inf")).all()) and torch.equal(o2[~hit], out[~hit]) and torch.equal(z2, lse)
 
 
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
