@@ -747,12 +747,12 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   // place is lane % 8), a share of the rope and of the scales. Behind the last tile they copy rows that are there, unused.
   constexpr int COPIES = IMG ? 10 : R5 ? 5 : 6;
   const uint8_t* image = IMG ? p.images + ((long long)b * p.img_tiles) * IMAGE : nullptr;
-  auto address = [&](int j, int i) -> uint64_t {          // of the lane's source in piece i
+  auto address = [&](int lane, int j, int i) -> uint64_t { // of the lane's source in piece i
     if constexpr (IMG) {                                  // (pieces 0, 3, 6 and 9; those behind them by the instruction's offset)
       const int t = kb / TR + j < p.img_tiles ? kb / TR + j : p.img_tiles - 1;
-      return (uint64_t)(uintptr_t)(image + (long long)t * IMAGE + (i < 9 ? w * 9216 + i * 1024 : IMG_SC + w * 256)) + (uint32_t)(here() * (i < 9 ? 16 : 4));
+      return (uint64_t)(uintptr_t)(image + (long long)t * IMAGE + (i < 9 ? w * 9216 + i * 1024 : IMG_SC + w * 256)) + (uint32_t)(lane * (i < 9 ? 16 : 4));
     }
-    const int lane = here(), r = lane >> 3, place = (lane & 7) ^ swz(r);
+    const int r = lane >> 3, place = (lane & 7) ^ swz(r);
     SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
     if (i < 4) return id[8 * i + r] + (uint32_t)(128 * w + 16 * (place ^ ((i & 1) << 1)));
     // Row576: 16 rows of 64 bytes, waves 2 and 3 repeat those of 0 and 1; Row656: 8 rows of rope, 64 scales
@@ -776,24 +776,25 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     else dma4((const void*)from, d + L::CODE + L::RP + (w & 1) * 256);
   };
 
-  // ---- codes of tile j to bf16: piece i of 4 of the wave's group (16 codes a lane: row 8 i + lane / 8), piece 4: rope (Row576)
-  auto codes = [&](int j, int i) -> i32x4 {
-    const int lane = here();
+  // ---- codes of tile j to bf16, by half pieces of 8 codes a lane: piece i of the wave's group (row 8 i + lane / 8, 16 codes),
+  // piece 4: the rope (Row576, one half)
+  auto codes = [&](int lane, int j, int i, int half) -> i32x2 {
     SPMLA_LDS uint8_t* d = lds + (j & 3) * L::TILE;
-    if (i < 4) return *(SPMLA_LDS i32x4*)(d + w * 4096 + i * 1024 + lane * 16);
-    const i32x2 y = *(SPMLA_LDS i32x2*)(d + L::CODE + w * 512 + lane * 8);
-    return i32x4{y[0], y[1], 0, 0};
+    return *(SPMLA_LDS i32x2*)(i < 4 ? d + w * 4096 + i * 1024 + lane * 16 + 8 * half : d + L::CODE + w * 512 + lane * 8);
   };
-  auto convert = [&](int j, int i, i32x4 y) {
-    const int lane = here(), r = lane >> 3, x = swz(r);
+  auto two = [&](u32x4& z, i32x2 y, int e) {              // four codes
+    z[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y[e], 1.0f, false));
+    z[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y[e], 1.0f, true));
+  };
+  auto put = [&](int lane, int j, int i, int half, u32x4 z) {
+    const int r = lane >> 3, x = swz(r);
     SPMLA_LDS uint8_t* to = lds + L::B + (j & 1) * (L::NG * 4096);
     if (i < 4) {
       const int c = (lane & 7) ^ x;
       const int at = (c >> 2) * 4096 + r * 128 + ((16 * ((2 * (c & 3)) ^ x)) ^ ((i & 1) * 96));
-      *(SPMLA_LDS bf16x8*)(to + w * 8192 + i * 1024 + at) = codes8_bf16(y[0], y[1]);
-      *(SPMLA_LDS bf16x8*)(to + w * 8192 + i * 1024 + (at ^ 16)) = codes8_bf16(y[2], y[3]);
-    } else if constexpr (R5) {
-      *(SPMLA_LDS bf16x8*)(to + 8 * 4096 + w * 1024 + r * 128 + 16 * ((lane & 7) ^ swz(8 * w + r))) = codes8_bf16(y[0], y[1]);
+      *(SPMLA_LDS u32x4*)(to + w * 8192 + i * 1024 + (at ^ (16 * half))) = z;
+    } else {
+      *(SPMLA_LDS u32x4*)(to + 8 * 4096 + w * 1024 + r * 128 + 16 * ((lane & 7) ^ swz(8 * w + r))) = z;
     }
   };
   constexpr int PIECES = IMG ? 0 : R5 ? 5 : 4;            // of a tile's conversion
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     uint64_t from = 0;
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
-      if (!IMG || i % 3 == 0) from = address(j, i);
+      if (!IMG || i % 3 == 0) from = address(lane, j, i);
       copy(j, i, from);
     }
   }
@@ -835,7 +836,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   wait_vm<2 * COPIES>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < (IMG ? 0 : R5 ? 5 : 4); ++i) convert(0, i, codes(0, i));
+  for (int i = 0; i < (IMG ? 0 : R5 ? 5 : 4); ++i)
+#pragma unroll
+    for (int half = 0; half < (i < 4 ? 2 : 1); ++half) {
+      const i32x2 y = codes(lane, 0, i, half);
+      u32x4 z;
+      two(z, y, 0);
+      two(z, y, 1);
+      put(lane, 0, i, half, z);
+    }
 #pragma unroll 1
   for (int j = 0; j < nt; ++j) {
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
@@ -857,25 +866,34 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         SPMLA_LDS uint8_t* at = ks >= 32 ? rope : kt + (ks >> 2) * 4096;
         return *(SPMLA_LDS bf16x8*)(at + (ka ^ (32 * (ks & 3))));
       };
-      constexpr int KD = R5 ? 8 : IMG ? 6 : 5;
+      constexpr int KD = R5 ? 8 : IMG ? 6 : 4;
       bf16x8 k[KD];
 #pragma unroll
       for (int n = 0; n < KD; ++n) k[n] = kread(n);
       uint64_t from = 0;
-      i32x4 y = {};
+      i32x2 y0 = {}, y1 = {};
+      u32x4 z = {};
       auto beside = [&](int ks) {                         // what runs beside product ks: piece ks / 6 of copies and codes
         if constexpr (IMG) {
           if (ks % 3 == 0 && ks / 3 < COPIES) {
-            if (ks / 3 % 3 == 0) from = address(j + 3, ks / 3);
+            if (ks / 3 % 3 == 0) from = address(lane, j + 3, ks / 3);
             copy(j + 3, ks / 3, from);
           }
           return;
         }
-        const int i = ks / 6, at = ks % 6;
-        if (at == 0 && i < COPIES) from = address(j + 3, i);
-        if (at == 1 && i < PIECES) y = codes(j + 1, i);
+        // an address and a copy every six products; a piece's codes are read beside six of them and converted beside the next
+        // six, four at a time: a conversion takes the VALU for as long as half a product (all 16 beside one: + 1000 cycles a tile)
+        const int i = ks / 6, at = ks % 6, q = i - 1;
+        if (at == 0 && i < COPIES) from = address(lane, j + 3, i);
         if (at == 3 && i < COPIES) copy(j + 3, i, from);
-        if (at == 4 && i < PIECES) convert(j + 1, i, y);
+        if (q >= 0 && q < PIECES) {
+          if (at < 2) two(z, y0, at);
+          if (at == 2) put(lane, j + 1, q, 0, z);
+          if (q < 4 && (at == 3 || at == 4)) two(z, y1, at - 3);
+          if (q < 4 && at == 5) put(lane, j + 1, q, 1, z);
+        }
+        if (at == 2 && i < PIECES) y0 = codes(lane, j + 1, i, 0);
+        if (at == 5 && i < PIECES && i < 4) y1 = codes(lane, j + 1, i, 1);
       };
       if constexpr (R5) {
 #pragma unroll
@@ -981,12 +999,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     {
       bf16x8 P[R5 ? 1 : 2][2];                            // (Row656: weights times the scales of a group, the next one's beside its products)
       f32x4 sc[2];
-      auto half_of = [&](int g, int a) {                   // positions 8 a + 4 hh .. + 3
-        const f32x4 t = f32x4{S[4 * a], S[4 * a + 1], S[4 * a + 2], S[4 * a + 3]} * (R5 ? f32x4{1.f, 1.f, 1.f, 1.f} : sc[a & 1]);
-        u32x4 y = __builtin_bit_cast(u32x4, P[R5 ? 0 : g & 1][a >> 1]);
-        y[2 * (a & 1)] = pk_bf16(t[0], t[1]);
-        y[2 * (a & 1) + 1] = pk_bf16(t[2], t[3]);
-        P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(bf16x8, y);
+      auto half_of = [&](int g, int a, int e) {            // positions 8 a + 4 hh + 2 e, + 1
+        float x = S[4 * a + 2 * e], y = S[4 * a + 2 * e + 1];
+        if constexpr (!R5) {
+          x *= sc[a & 1][2 * e];
+          y *= sc[a & 1][2 * e + 1];
+        }
+        u32x4 u = __builtin_bit_cast(u32x4, P[R5 ? 0 : g & 1][a >> 1]);
+        u[2 * (a & 1) + e] = pk_bf16(x, y);
+        P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(bf16x8, u);
       };
       auto scale_of = [&](int g, int a) { sc[a & 1] = *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh); };
       const int vrow = 4 * hh + (l16 >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -1009,16 +1030,18 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       }
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        half_of(0, a);
-        if (!R5 && a < 2) scale_of(0, a + 2);
+        half_of(0, a, 0);
+        half_of(0, a, 1);
+        if (!R5 && a < 3) scale_of(a < 2 ? 0 : 1, a < 2 ? a + 2 : 0);
       }
 #pragma unroll
       for (int n = 0; n < 32; ++n) {
         O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % VD], P[R5 ? 0 : (n >> 3) & 1][n & 1], O[n >> 1], 0, 0, 0);
         if (n + VD < 32) v[n % VD] = vread(n + VD);
         if (!R5 && n < 24) {
-          if (n % 8 >= 2 && n % 8 < 6) half_of(n / 8 + 1, n % 8 - 2);
-          if (n % 8 < 4) scale_of(n / 8 + 1, n % 8);
+          const int g = n / 8 + 1, e = n % 8;
+          half_of(g, e >> 1, e & 1);
+          if (e % 2 == 0 && (e < 6 || g < 3)) scale_of(e < 6 ? g : g + 1, e < 6 ? e / 2 + 1 : 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
