@@ -12,6 +12,7 @@
 // is new, so nothing waits for the table's new entries. lens, held and the count change only after every workgroup
 // has read them: the one that arrives last at a counter in the pool's state writes them (and clears the counter).
 #include "spmla_common.h"
+#include "spmla_quant.h"
 
 namespace spmla {
 namespace pages {
@@ -40,12 +41,13 @@ __device__ inline void scan(int* v, int M, int* part) {
   int base = 0;
   for (int at = 0; at < M; at += blockDim.x) {
     const int x = at + tid < M ? v[at + tid] : 0;
-    int s = x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(s, d);
-      if (lane >= d) s = sat_add(s, y);
-    }
+    int s = x;                                      // (wave_incl_scan with sums that saturate)
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x111, 0xf, 0xf, false));
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x112, 0xf, 0xf, false));
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x114, 0xf, 0xf, false));
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x118, 0xf, 0xf, false));
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x142, 0xa, 0xf, false));
+    s = sat_add(s, __builtin_amdgcn_update_dpp(0, s, 0x143, 0xc, 0xf, false));
     int ex = __shfl_up(s, 1);                       // (not s - x: the sums stay ascending where they saturate)
     ex = lane ? ex : 0;
     if (lane == 63) part[w] = s;
@@ -93,13 +95,17 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
   extern __shared__ int lds[];
   int* st = lds;                                    // [M + 1] sums of the new tokens
   int* off = lds + M + 1;                           // [M + 1] sums of the needed pages
-  int* part = lds + 2 * M + 2;
+  int* lens = lds + 2 * M + 2;                      // [M] lengths and pages before the step
+  int* helds = lds + 3 * M + 2;
+  int* part = lds + 4 * M + 2;
   const int tid = threadIdx.x, G = gridDim.x;
   for (int b = tid; b < M; b += blockDim.x) {
     const int x = clamp0(fresh[b], 0x7fffffff), len = clamp0(p.lens[b], 0x7fffffff), held = clamp0(p.held[b], p.W);
     const int want = pages_of(sat_add(len, x), p.bs, p.W);
     st[b] = x;
     off[b] = want > held ? want - held : 0;
+    lens[b] = len;
+    helds[b] = held;
   }
   const int count = clamp0(p.state[0], p.P);
   __syncthreads();
@@ -113,7 +119,7 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
     long long pos = 0, slot = -1;
     if (t < st[M]) {
       b = find(st, M, t);
-      const int len = clamp0(p.lens[b], 0x7fffffff), held = clamp0(p.held[b], p.W);
+      const int len = lens[b], held = helds[b];
       pos = (long long)len + (t - st[b]);
       const uint32_t c = (uint32_t)pos / (uint32_t)p.bs;           // (two lengths below 2^31: 32 bits without a sign)
       int page = -1;
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
     slots[t] = slot;
   }
   for (int i = at0; i < got; i += step) {
-    const int b = find(off, M, i), c = clamp0(p.held[b], p.W) + (i - off[b]);
+    const int b = find(off, M, i), c = helds[b] + (i - off[b]);
     p.table[b * p.t_st + c] = p.free[count - 1 - i];
   }
   for (int b = at0; b <= M; b += step) start[b] = st[b];
@@ -138,8 +144,8 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
   if (!last_reader(p.state)) return;
   for (int b = tid; b < M; b += blockDim.x) {
     const int need = off[b + 1] - off[b], left = got - off[b];
-    p.lens[b] = sat_add(clamp0(p.lens[b], 0x7fffffff), st[b + 1] - st[b]);
-    p.held[b] = clamp0(p.held[b], p.W) + (left < need ? clamp0(left, need) : need);
+    p.lens[b] = sat_add(lens[b], st[b + 1] - st[b]);
+    p.held[b] = helds[b] + (left < need ? clamp0(left, need) : need);
   }
   if (tid == 0) {
     p.state[0] = count - got;
@@ -150,7 +156,8 @@ __global__ void __launch_bounds__(TPB) step_kernel(const int* fresh, int M, Pool
 __global__ void __launch_bounds__(TPB) trim_kernel(const int* keep, int M, Pool p) {
   extern __shared__ int lds[];
   int* off = lds;                                   // [M + 1] sums of the pages that go back
-  int* part = lds + M + 1;
+  int* lefts = lds + M + 1;                         // [M] pages that stay
+  int* part = lds + 2 * M + 1;
   const int tid = threadIdx.x, G = gridDim.x;
   auto left_of = [&](int b, int& len) {             // pages that request b keeps
     len = clamp0(p.lens[b], 0x7fffffff);
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(TPB) trim_kernel(const int* keep, int M, Pool 
     int len;
     const int left = left_of(b, len);
     off[b] = clamp0(p.held[b], p.W) - left;
+    lefts[b] = left;
   }
   const int count = clamp0(p.state[0], p.P);
   __syncthreads();
@@ -171,8 +179,7 @@ __global__ void __launch_bounds__(TPB) trim_kernel(const int* keep, int M, Pool 
   const int at0 = blockIdx.x * blockDim.x + tid, step = G * blockDim.x;
   for (int i = at0; i < R; i += step) {
     const int b = find(off, M, i);
-    int len;
-    int* e = p.table + b * p.t_st + left_of(b, len) + (i - off[b]);
+    int* e = p.table + b * p.t_st + lefts[b] + (i - off[b]);
     const long long to = (long long)count + R - 1 - i;
     if (to < p.P) p.free[to] = *e;                  // (a pool whose pages are all its own has room)
     *e = -1;
@@ -194,6 +201,7 @@ int check(const int* in, int M, const Pool& p) {
   return SPMLA_OK;
 }
 int threads_of(long long work) { return work <= 256 ? 256 : TPB; }
+constexpr int most_lds(int per) { return (per * MAXM + 2 + TPB / 64) * 4; }
 
 }  // namespace pages
 }  // namespace spmla
@@ -209,12 +217,13 @@ int spmla_page_step(const int* fresh, int M, int* lens, int* held, int* table, l
   if (const int rc = check(fresh, M, p)) return rc;
   if (n < 0 || !start || (n && (!req || !positions || !slots))) return SPMLA_EARG;
   static DynLds attr;
-  if (const int rc = attr.ensure((const void*)step_kernel, (2 * MAXM + 2 + TPB / 64) * 4)) return rc;
+  static Launcher go;
+  if (const int rc = attr.ensure((const void*)step_kernel, most_lds(4))) return rc;
   const int tpb = threads_of(n > M ? n : M);
   int G = (n + tpb - 1) / tpb;
   G = G < 1 ? 1 : G > 64 ? 64 : G;
-  step_kernel<<<G, tpb, (2 * M + 2 + TPB / 64) * 4, (hipStream_t)stream>>>(fresh, M, p, n, start, req, positions, slots);
-  return (int)hipGetLastError();
+  return go((const void*)step_kernel, dim3((unsigned)G), (unsigned)tpb, (size_t)(4 * M + 2 + TPB / 64) * 4, (hipStream_t)stream, fresh, M, p, n, start,
+            req, positions, slots);
 }
 
 int spmla_page_trim(const int* keep, int M, int* lens, int* held, int* table, long long table_st, int W, int* free, int P, int* state,
@@ -222,12 +231,13 @@ int spmla_page_trim(const int* keep, int M, int* lens, int* held, int* table, lo
   const Pool p{lens, held, table, table_st, W, free, P, state, block_size};
   if (const int rc = check(keep, M, p)) return rc;
   static DynLds attr;
-  if (const int rc = attr.ensure((const void*)trim_kernel, (MAXM + 1 + TPB / 64) * 4)) return rc;
+  static Launcher go;
+  if (const int rc = attr.ensure((const void*)trim_kernel, most_lds(2))) return rc;
   const long long most = (long long)M * W;                       // pages that may go back
-  long long G = (most + 65535) / 65536;
-  G = G < 1 ? 1 : G > 32 ? 32 : G;
-  trim_kernel<<<(int)G, threads_of(most / 64 > M ? most / 64 : M), (M + 1 + TPB / 64) * 4, (hipStream_t)stream>>>(keep, M, p);
-  return (int)hipGetLastError();
+  const int tpb = threads_of(most / 8 > M ? most / 8 : M);
+  int G = (int)((most + 32 * TPB - 1) / (32 * TPB) < 32 ? (most + 32 * TPB - 1) / (32 * TPB) : 32);
+  G = G < 1 ? 1 : G;
+  return go((const void*)trim_kernel, dim3((unsigned)G), (unsigned)tpb, (size_t)(2 * M + 1 + TPB / 64) * 4, (hipStream_t)stream, keep, M, p);
 }
 
 }  // extern "C"

@@ -31,7 +31,8 @@ def _trim(pool, ref, keep, dev):
 
 # one request; more than a workgroup's; many workgroups of tokens; odd pages, pages of one row
 @pytest.mark.parametrize("M,bs,W,pages,most", [(1, 64, 8, 8, 200), (5, 1, 40, 120, 12), (17, 48, 30, 400, 300),
-                                               (300, 16, 12, 2500, 40), (1500, 64, 6, 9000, 9), (40, 7, 4000, 60000, 9000)])
+                                               (300, 16, 12, 2500, 40), (1500, 64, 6, 9000, 9), (40, 7, 4000, 60000, 9000),
+                                               (8192, 16, 3, 20000, 7)])
 def test_steps_and_trims(dev, M, bs, W, pages, most):
     from arcagi2_flashnext_dots3_amd.paging import PagePool
     rng = random.Random(M * bs)
