@@ -6,20 +6,30 @@
 //   s = sm_scale kv_scale (q[:512] . latent + q[512:] . rope),  p = exp(s - m),  o = kv_scale sum p latent / sum p,
 //   lse = ln sum exp(s)
 //
-// One workgroup = up to 128 rows of (token, head) of one request, token by token, over one split of the positions: whatever
-// the number of heads, a cached row is copied once for them. 8 waves of 16 rows each; where a request has 64 rows or fewer
-// (PS = 2) 4 of them take every other tile, and both join at the end. Tiles of 32 positions in a ring in LDS, filled by
-// direct copies, one barrier a tile; otherwise a wave is on its own, from the scores to its output:
-//   * QK: S^T = K Q^T in bf16 MFMA 16x16x32, codes converted exactly, the query in 72 registers. (8-bit MFMA would take the
-//     codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of the summed magnitudes, 1.3e-5 at most,
-//     against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales;
-//   * softmax: one query row per lane (and three others); base 2, 32 bits; the reference maximum moves only past TAU. A lane's
-//     weights are the operand it needs: the k slots of V^T follow the rows of the accumulator, P never leaves its registers;
-//   * PV: O^T = V^T P^T in f16 MFMA 16x16x32, V^T by the 8-bit transposing read, converted exactly; P in f16 times 2^UP so
-//     that few weights are f16 subnormals. Row656: P times the scales of the four groups times 2^-e, e following the largest
-//     scale so far (a product p * scale is off by half an f16 step, or 2^-34 of the largest scale).
-// Masked positions take no part: scores of -inf, and where the mask cuts a tile codes and scales that are no numbers become 0
-// after the scores (a row that sees one has a score that is none).
+// One workgroup = a tile of (token, head) rows of one request, token by token, over one split of the positions: whatever the
+// number of heads, a cached row is copied once for all of them. A position costs 2 (576 + 512) operations a row: with 128 rows
+// 425 to 484 a byte, matrix cores and HBM alike; with fewer HBM, with several tiles of a request the matrix cores.
+//   * products: S^T = K Q^T and O^T = V^T P^T, both with a query row in a lane, so that maxima, sums and factors are one
+//     register a lane, and the weights that a lane forms are the operand it needs: P never leaves its registers. Codes are exact in
+//     bf16 and fp16. (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
+//     the summed magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales;
+//     for PV the weight times the group's scale.
+//   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale) are rounded to bf16,
+//     or to fp16 in the kernel of few rows, once.
+//   * masked positions take no part: scores of -inf, and where the mask cuts a tile codes and scales that are no numbers
+//     become 0 after the scores (a row that sees one has a score that is none).
+//
+// Three kernels by the rows of a request, on average:
+//   * `kernel`, up to 64: 8 waves of 16 rows, 2 or 4 of them on the same rows with every second or fourth tile of 32 positions,
+//     joined in LDS. A wave converts what it reads. Bound by HBM (48 requests of 16 heads, 364 MB: 98 us = 3.7 TB/s).
+//   * `wide_kernel<R5, false>`: 4 waves of 32 rows, 512 registers (O in the 256 accumulation registers, the query in 144 others).
+//     A tile's codes are converted to bf16 once for all waves, beside the score products. Bound by the issue of one
+//     wave a SIMD: matrix cores busy for 29% (64 requests of 128 heads: 115 us = 560 TFLOP/s). Two waves a SIMD leave 16 rows
+//     a wave, each of which converts everything again (267 us).
+//   * from 1024 on, `image_kernel` gathers and converts the tiles first, `wide_kernel<R5, true>` copies them as they lie
+//     in LDS: no conversions, addresses without tables (1024 tokens of 128 heads over 16384 rows: 3.74 ms = 1210 TFLOP/s, of
+//     which the images take 0.01; converted in the kernel 5.3). Bound by the power limit: the clock falls to 1.8 - 2.0
+//     GHz, and a form that runs the softmax beside the next tile's score products takes as long.
 // Splits leave normalized fp32 partials and their lse in a workspace; a second kernel joins them.
 #include "spmla_common.h"
 #include "spmla_quant.h"
@@ -60,7 +70,10 @@ struct Params {
 struct Item {
   int b, tile, sp, splits, span, slot;                     // slot: the tile's first partial result
 };
-constexpr int PLAN = 256, CUS = 256, LEAST = 4;                     // (a split of fewer tiles costs more to join than it saves)
+constexpr int PLAN = 256, CUS = 256;
+// A split of fewer tiles costs more to join than it saves: one token of 128 heads over 1000 / 16000 rows with two tiles at least
+// 27 / 43 us, with four 30 / 40, with eight 39 / 45.
+constexpr int LEAST = 3;
 
 template <int MR>
 __device__ inline bool find_item(const Params& p, int lane, Item& o) {
@@ -224,6 +237,10 @@ __device__ inline f16x8 codes8_f16(int a, int b) {
 // place of chunk c (16 bytes) in a row of 128 bytes: c ^ swz(row); 16 rows' chunks c lie in all 64 banks
 __device__ inline int swz(int row) { return ((row & 2) << 1) | ((row & 4) >> 2) | ((row & 8) >> 2); }
 
+// ---- 64 rows or fewer of a request. PV: V^T by the 8-bit transposing read, converted exactly to f16; P in f16 times 2^UP so that
+// few weights are f16 subnormals (Row656: P times the scales of the four groups times 2^-e, e following the largest
+// scale so far: a product p * scale is off by half an f16 step, or 2^-34 of the largest scale). The reference maximum
+// moves only past TAU.
 template <bool R5, int PS>
 __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   using L = Lds<R5, PS>;
@@ -588,8 +605,10 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   }
 }
 
-// ---- 65 rows and more of a request: workgroups of 128 rows, 4 waves of 32 rows (one a SIMD, 512 registers). The codes of a
-// tile are converted to bf16 once, into a tile in LDS that both products read: K by rows, V by the 16-bit transposing read.
+// ---- more than 64 rows of a request: workgroups of 128 rows, 4 waves of 32 rows (one a SIMD, 512 registers). The codes of a
+// tile are in bf16 in a tile in LDS that both products read: K by rows, V by the 16-bit transposing read (chunks permuted by the
+// row: neither meets in a bank). A step of 32 positions takes 36 + 32 matrix instructions of 32 clocks a wave; what
+// else a wave does in it is spread between them, a few instructions each.
 template <bool R5>
 struct WLds {
   static constexpr int RING = 4;
@@ -1171,8 +1190,11 @@ __global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
   if (p.lse && lane == 0) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
 }
 
-// Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions;
-// of 32 or fewer of 32 rows and four (Row576: eight tiles in LDS; of Row656 seven would fit).
+// Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions (48
+// requests of 64 rows, 4000 cached ones on average: 90 us, in tiles of 128 rows 115; of 128 rows 146 against 122); of 32
+// or fewer of 32 rows and four (16 rows: 45 us against 55; Row576 alone: of Row656 seven tiles fit into LDS, not the eight).
+// Tiles are gathered first for requests of 1024 rows and more (16 requests, 2000 cached rows on average: with 256 rows 83 us
+// against 73 without, with 512 103 against 100, with 1024 163 against 174), while their images take 4 GiB at most.
 struct Shape {
   int rows, slack, images;                                 // images: tiles of each request that are gathered first (0: none)
   long long tiles;
@@ -1181,7 +1203,7 @@ static Shape shape_of(int T, int H, int B, int row_bytes, int longest) {
   const long long n = (long long)T * H;
   const int mr = n <= 32ll * B && row_bytes == ROW576 ? 32 : n <= 64ll * B ? 64 : 128, slack = H % mr != 0;
   const long long units = ((long long)longest + TR - 1) / TR;
-  const bool images = n >= 512ll * B && B < 65536 && units * B * IMAGE <= 4ll << 30;
+  const bool images = n >= 1024ll * B && B < 65536 && units * B * IMAGE <= 4ll << 30;
   return Shape{mr, slack, images ? (int)units : 0, n / mr + (slack ? B : 0)};
 }
 // splits need a place for each (token, head), and for the partial results of a split tile's rows

@@ -1159,7 +1159,7 @@ def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0,
     its own position and those before it, but for pages that are not there (-1). Returns (out [T, H, 512] bf16, lse [T, H]
     fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: at least the longest
     seq_lens, known on the host (None: what the table can hold); positions from it on are not seen. Temporary workspace: for
-    512 (token, head) rows or more a request, max_seq_len rows of each request in 16 bits (up to 4 GiB; beyond, rows are
+    1024 (token, head) rows or more a request, max_seq_len rows of each request in 16 bits (up to 4 GiB; beyond, rows are
     converted where they are used); for few rows, partial results. items: workgroups that the kernel makes of the requests'
     positions, in even shares (None: chunk_items; 0: one a tile of query rows); it changes the order of sums alone."""
     _need(q.dim() == 3 and cache.dim() == 3 and block_table.dim() == 2, "q [T, H, 576], cache [blocks, block_size, row], block_table [B, columns]")

@@ -547,7 +547,7 @@ int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void*
  * items: workgroups that the requests' positions are shared out to on the device, by their lengths (0, B > 256, or no more
  * than the tiles of query rows: one a tile; ELIMIT beyond 511 more), partial results joined by a second kernel through a
  * workspace of spmla_attn_chunk_ws_bytes. spmla_attn_chunk_items: a good number of them.
- * longest: positions from there on are not seen; where requests have 512 (token, head) rows or more on average, as many rows
+ * longest: positions from there on are not seen; where requests have 1024 (token, head) rows or more on average, as many rows
  * of each are gathered and converted into the workspace first (up to 4 GiB).
  * The dense counterpart of PortableSparseImpl.forward_mqa (dsa_sm89.py:379-470) for layers without an indexer. */
 int spmla_attn_chunk_items(int T, int H, int B, int row_bytes, int longest);

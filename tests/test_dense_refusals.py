@@ -138,13 +138,13 @@ def test_chunk_workgroups_and_workspace():
     assert items(250, 128, 250, 656, 6000) == 256 + 64            # few beyond one a tile: some for the longest requests
     assert items(1024, 128, 1, 576, 16384) == 0                   # four rounds and more: no splits
     assert items(257, 128, 257, 656, 6000) == 0                   # more requests than the shares are formed for
-    assert items(1, 128, 1, 656, 256) == 0 and items(0, 128, 1, 656, 9999) == 0
+    assert items(1, 128, 1, 656, 192) == 0 and items(1, 128, 1, 656, 193) == 256 and items(0, 128, 1, 656, 9999) == 0
     assert ws(1, 128, 1, 656, 65536, 0) == 0 and ws(1, 128, 1, 656, 0, 256) == 0
     assert ws(1, 128, 1, 656, 65536, 1) == 0                      # no more workgroups than tiles
     assert ws(1, 128, 1, 656, 65536, 256) == 128 * 8 + 16 + 256 * 128 * 513 * 4
     images = 512 * (9 * 4096 + 1024)                              # 16384 rows, gathered first
     assert ws(1024, 128, 1, 576, 16384, 0) == images
-    assert ws(3, 128, 1, 576, 16384, 0) == 0 and ws(4, 128, 1, 576, 16384, 0) == images
+    assert ws(7, 128, 1, 576, 16384, 0) == 0 and ws(8, 128, 1, 576, 16384, 0) == images
     assert ws(1024, 128, 8, 656, 1 << 20, 0) == 0                 # beyond 4 GiB: rows are converted where they are used
 
 

@@ -157,14 +157,14 @@ def test_many_requests(dev, row, heads):
 @pytest.mark.parametrize("row", [656, 576])
 @pytest.mark.parametrize("heads", [40, 128])
 def test_rows_gathered_first(dev, row, heads):
-    """Requests of 512 (token, head) rows or more: pages that end inside a tile, some missing, positions split."""
+    """Requests of 1024 (token, head) rows or more: pages that end inside a tile, some missing, positions split."""
     case = _case([700, 300, 77], [40, 33, 30], heads, row, 48, heads, missing=[(0, 0), (0, 14), (1, 3)])
     for kw in (dict(), dict(items=0), dict(items=130), dict(max_seq_len=700)):
         _run(dev, case, 48, **kw)
 
 
 @pytest.mark.parametrize("row", [656, 576])
-@pytest.mark.parametrize("heads,lens", [(4, [1, 1]), (16, [1, 1]), (128, [1, 1]), (64, [20, 11])])
+@pytest.mark.parametrize("heads,lens", [(4, [1, 1]), (16, [1, 1]), (128, [1, 1]), (64, [20, 13])])
 def test_scores_rise_far_over_the_first_tile(dev, row, heads, lens):
     """Scores that climb by hundreds behind the first positions, past what a reference that does not move can hold."""
     q, cache, table, seqs, start = _case([300, 200], lens, heads, row, 16, 17)
@@ -189,7 +189,7 @@ def test_scores_rise_far_over_the_first_tile(dev, row, heads, lens):
 @pytest.mark.parametrize("scale", [-1.0, 0.0])
 def test_kv_scales(dev, scale):
     """A negative scale turns the order of the scores, zero makes all weights equal (and the output 0)."""
-    for heads, lens in ((16, [1, 1]), (128, [1, 1]), (64, [20, 11])):
+    for heads, lens in ((16, [1, 1]), (128, [1, 1]), (64, [20, 13])):
         _run(dev, _case([300, 200], lens, heads, 576, 16, 18), 16, scale)
 
 
