@@ -11,10 +11,16 @@
 //     16-byte chunks are permuted by its number, so that neither K's reads (32 rows, one chunk) nor V's transposing reads
 //     (4 rows, 32 bytes) meet in a bank. Rows behind the sequence and columns behind the head are copied from zeros.
 //   * one pass, running maximum and sum in base 2 and 32 bits; the reference maximum moves only when a tile
-//     exceeds it by more than TAU (P <= 2^(TAU + UP)), so O is rescaled rarely.
+//     exceeds it by more than TAU (P <= 2^(TAU + UP)), so O is rescaled rarely. Weights are rounded once, to the inputs' type.
 //   * masked scores are -inf whatever their values; a masked key's V takes no part either, though 0 * inf is no number:
 //     tiles that the mask cuts look at V's exponents, and where one is all ones (rare) the products run with zeros in
 //     their place, and the queries that see such a value get it at the end.
+//
+// Two waves a SIMD (three with heads of 64, one with heads of 256): the matrix products of one run beside the softmax of the
+// other. Heads of 128 and 192: 950 - 1140 TFLOP/s on long prompts, the matrix cores busy for half of the time at the clock
+// that the power limit leaves; of 64: 860, bound by the VALU (per 64 keys 32 exponentials of 16 clocks and 120 instructions of 4
+// against 512 clocks of products); of 256: 775 (one wave a SIMD, O in accumulation registers). Short prompts: the
+// launch, the search for the tile, two dependent loads and cold code, 11 us.
 #include "spmla_common.h"
 #include "spmla_quant.h"
 #include <type_traits>
