@@ -11,11 +11,12 @@
 // 425 to 484 a byte, matrix cores and HBM alike; with fewer HBM, with several tiles of a request the matrix cores.
 //   * products: S^T = K Q^T and O^T = V^T P^T, both with a query row in a lane, so that maxima, sums and factors are one
 //     register a lane, and the weights that a lane forms are the operand it needs: P never leaves its registers. Codes are exact in
-//     bf16 and fp16. (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
+//     bf16 and in fp16, and so is the query but for fp16's range (the wide kernel takes rows out of it times a power of two). (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
 //     the summed magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales;
 //     for PV the weight times the group's scale.
-//   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale) are rounded to bf16,
-//     or to fp16 in the kernel of few rows, once.
+//   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale) are rounded to fp16,
+//     once. (In bf16 they need no care for their range and cost as much, but put as large an error on the output as its
+//     own rounding does.)
 //   * masked positions take no part: scores of -inf, and where the mask cuts a tile codes and scales that are no numbers
 //     become 0 after the scores (a row that sees one has a score that is none).
 //
@@ -23,7 +24,7 @@
 //   * `kernel`, up to 64: 8 waves of 16 rows, 2 or 4 of them on the same rows with every second or fourth tile of 32 positions,
 //     joined in LDS. A wave converts what it reads. Bound by HBM (48 requests of 16 heads, 364 MB: 98 us = 3.7 TB/s).
 //   * `wide_kernel<R5, false>`: 4 waves of 32 rows, 512 registers (O in the 256 accumulation registers, the query in 144 others).
-//     A tile's codes are converted to bf16 once for all waves, beside the score products. Bound by the issue of one
+//     A tile's codes are converted to fp16 once for all waves, beside the score products. Bound by the issue of one
 //     wave a SIMD: matrix cores busy for 29% (64 requests of 128 heads: 115 us = 560 TFLOP/s). Two waves a SIMD leave 16 rows
 //     a wave, each of which converts everything again (267 us).
 //   * from 1024 on, `image_kernel` gathers and converts the tiles first, `wide_kernel<R5, true>` copies them as they lie
@@ -39,11 +40,13 @@ namespace chunk {
 
 constexpr int TR = 32;                // positions per tile
 constexpr int IDS = 256;              // positions whose rows are looked up at a time
-constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f, WIDE = 64.f;
+constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;     // the reference maximum moves past 2^TAU; weights are times 2^UP
+constexpr float WTAU = 10.0f, WUP = 5.0f;                // of the wide kernel, where moving it costs more
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 struct Params {
   const uint16_t* q; long long q_st, q_sh;
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
 }
 
 // ---- more than 64 rows of a request: workgroups of 128 rows, 4 waves of 32 rows (one a SIMD, 512 registers). The codes of a
-// tile are in bf16 in a tile in LDS that both products read: K by rows, V by the 16-bit transposing read (chunks permuted by the
+// tile are in fp16 in a tile in LDS that both products read: K by rows, V by the 16-bit transposing read (chunks permuted by the
 // row: neither meets in a bank). A step of 32 positions takes 36 + 32 matrix instructions of 32 clocks a wave; what
 // else a wave does in it is spread between them, a few instructions each.
 template <bool R5>
@@ -620,17 +623,15 @@ struct WLds {
   static constexpr int B = RING * TILE;                    // two of them
   static constexpr int ID = B + 2 * NG * 4096;             // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
-  static constexpr int OVER = OK + 2 * IDS / 32 * 4;       // a row's scores have left its reference's range
-  static constexpr int TOTAL = OVER + 16;
+  static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
   static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
 };
 
 // Where a request has many query rows, a kernel before this one gathers and converts its tiles once for all of them, as they
-// lie in LDS: nine groups of 64 dims in bf16, scales by group [4][32], a word of which positions have rows.
+// lie in LDS: nine groups of 64 dims in fp16 (Row656's rope in bf16, as it is), scales by group [4][32], a word of which positions have rows.
 constexpr int IMG_SC = 9 * 4096, IMG_OK = IMG_SC + 512, IMAGE = IMG_SC + 1024;
 struct ILds {
-  static constexpr int OVER = 4 * IMAGE;
-  static constexpr int TOTAL = OVER + 16;
+  static constexpr int TOTAL = 4 * IMAGE;
   static_assert(TOTAL <= 160 * 1024 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
 };
 
@@ -658,12 +659,12 @@ __global__ void __launch_bounds__(256) image_kernel(Params p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int g = 2 * i + (e >> 2), c = 2 * (e & 3);
-    *(bf16x8*)(to + g * 4096 + 16 * (c ^ x)) = codes8_bf16(y[i][0], y[i][1]);
-    *(bf16x8*)(to + g * 4096 + 16 * ((c ^ x) ^ 1)) = codes8_bf16(y[i][2], y[i][3]);
+    *(f16x8*)(to + g * 4096 + 16 * (c ^ x)) = codes8_f16(y[i][0], y[i][1]);
+    *(f16x8*)(to + g * 4096 + 16 * ((c ^ x) ^ 1)) = codes8_f16(y[i][2], y[i][3]);
   }
   if constexpr (R5) {
     const i32x2 z = *(const i32x2*)(row + D_LAT + 8 * e);
-    *(bf16x8*)(to + 8 * 4096 + 16 * (e ^ x)) = codes8_bf16(z[0], z[1]);
+    *(f16x8*)(to + 8 * 4096 + 16 * (e ^ x)) = codes8_f16(z[0], z[1]);
   } else {
     *(u32x4*)(to + 8 * 4096 + 16 * (e ^ x)) = *(const u32x4*)(row + ROPE_OFF + 16 * e);
     if (e < 4) ((float*)(img + IMG_SC))[e * 32 + r] = *(const float*)(row + SC_OFF + 4 * e);
@@ -681,19 +682,22 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // QK products with their sums in VGPRs (the builtin would put them into AGPRs, which O fills). What the compiler cannot see
 // inside asm: operands come from LDS or were written long before; a chain's result is read 12 wait states after it.
-__device__ inline f32x16 qk_first(bf16x8 a, bf16x8 b) {
+__device__ inline f32x16 qk_first(u32x4 a, u32x4 b) {
   f32x16 d;
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "v"(b));
   return d;
 }
-__device__ inline f32x16 qk_next(bf16x8 a, bf16x8 b, f32x16 c) {
+__device__ inline f32x16 qk_next(u32x4 a, u32x4 b, f32x16 c) {
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  return c;
+}
+__device__ inline f32x16 qk_rope(u32x4 a, u32x4 b, f32x16 c) {             // Row656: in bf16
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
   return c;
 }
 template <bool R5, bool IMG>
 __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   using L = WLds<R5>;
-  constexpr int OVER = IMG ? ILds::OVER : L::OVER;
   constexpr int RB = R5 ? ROW576 : ROW656, MR = 128;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
@@ -753,13 +757,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 
   // ---- query operands of rows 32 w + l32: B operands of 32x32x16, dims 16 ks + 8 hh .. (on their way until the first copies are)
   const int qr = 32 * w + l32;
-  bf16x8 qf[36];
+  u32x4 qf[36];
   int found = IMG ? -1 : look(0);
   {
     const long long r = r0 + (qr < live ? qr : live - 1);
     const uint16_t* qp = p.q + (t0 + r / p.H) * p.q_st + (r % p.H) * p.q_sh;
 #pragma unroll
-    for (int ks = 0; ks < 36; ++ks) qf[ks] = *(const bf16x8*)(qp + 16 * ks + 8 * hh);
+    for (int ks = 0; ks < 36; ++ks) qf[ks] = *(const u32x4*)(qp + 16 * ks + 8 * hh);
   }
 
   // ---- copies of a tile, in COPIES pieces: wave w the codes of scale group w (piece i: rows 8 i + lane / 8, the chunk whose
@@ -795,15 +799,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     else dma4((const void*)from, d + L::CODE + L::RP + (w & 1) * 256);
   };
 
-  // ---- codes of tile j to bf16, by half pieces of 8 codes a lane: piece i of the wave's group (row 8 i + lane / 8, 16 codes),
+  // ---- codes of tile j to f16, by half pieces of 8 codes a lane: piece i of the wave's group (row 8 i + lane / 8, 16 codes),
   // piece 4: the rope (Row576, one half)
   auto codes = [&](int lane, int j, int i, int half) -> i32x2 {
     SPMLA_LDS uint8_t* d = lds + (j & 3) * L::TILE;
     return *(SPMLA_LDS i32x2*)(i < 4 ? d + w * 4096 + i * 1024 + lane * 16 + 8 * half : d + L::CODE + w * 512 + lane * 8);
   };
   auto two = [&](u32x4& z, i32x2 y, int e) {              // four codes
-    z[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y[e], 1.0f, false));
-    z[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y[e], 1.0f, true));
+    z[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y[e], 1.0f, false));
+    z[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y[e], 1.0f, true));
   };
   auto put = [&](int lane, int j, int i, int half, u32x4 z) {
     const int r = lane >> 3, x = swz(r);
@@ -818,18 +822,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   };
   constexpr int PIECES = IMG ? 0 : R5 ? 5 : 4;            // of a tile's conversion
 
-  // ---- passes: a row's reference is the first maximum it meets and does not move (weights in bf16 have fp32's range, so O,
-  // which fills the AGPRs, is not rescaled). Where scores rise by more than 2^WIDE over it (rare), a pass takes the maxima
-  // alone and another one starts from those.
+  // ---- softmax state. The reference maximum is the first one that a row meets and moves past 2^WTAU over it only (O, which fills
+  // the AGPRs, takes 800 instructions to rescale); Row656: O is times 2^-ex2, ex2 following the largest scale so far.
   f32x16 O[16];                                           // O^T: dims 32 n + 8 a + 4 hh + b, query row qr
-  float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, of both halves; l: this half's)
-  SPMLA_LDS int* over = (SPMLA_LDS int*)(lds + OVER);
-  bool maxima = false, again = false;
-  uint32_t turn = p.flip ? 0x80008000u : 0u;
-  for (;;) {
-  if (tid == 0) *over = 0;
+  float m = -__builtin_inff(), l;                         // of query row qr (m: as scores are, of both halves; l: this half's)
+  float c = p.c;                                          // (per row: the query is times a power of two)
+  int ex2 = -126;
   if constexpr (!IMG) {
-    if (maxima || again) found = look(0);
     note(0, found);
     note(1, -1);                                          // (addresses that a copy may take, whatever the tile)
   }
@@ -846,12 +845,35 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     }
   }
 #pragma unroll
-  for (int ks = 0; ks < 36; ++ks) asm volatile("" : "+v"(qf[ks]));           // (the query is there; negated where scores are, once)
-  if (turn)
+  for (int ks = 0; ks < 36; ++ks) asm volatile("" : "+v"(qf[ks]));           // (the query is there)
+  {
+    // The query in f16: its 8 bits are exact there, but for the range: a row whose largest value lies outside of 2^0 .. 2^15 is
+    // taken times a power of two. (What is smaller than 2^-14 of f16 is off by 2^-24 then, against a largest one of 1.)
+    u16x2 top = {};
 #pragma unroll
-    for (int ks = 0; ks < 36; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[ks]) ^ turn);
-  turn = 0;
-  again = true;
+    for (int ks = 0; ks < 36; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, qf[ks][e] & 0x7fff7fffu));
+    int ex = (top[0] > top[1] ? top[0] : top[1]) >> 7;
+    const int other = __shfl_xor(ex, 32);
+    ex = other > ex ? other : ex;
+    const uint32_t turn = p.flip ? 0x80008000u : 0u;       // negated where scores are
+    float up = 1.f;
+    if (__any((ex < 127 || ex >= 127 + 15) && ex != 255)) {
+      int e = ex == 255 || ex == 0 ? 0 : 127 + 10 - ex;    // (subnormal ones as they are)
+      e = e > 120 ? 120 : e;
+      up = __builtin_amdgcn_ldexpf(1.f, e);
+      c = p.c * __builtin_amdgcn_ldexpf(1.f, -e);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 36; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = qf[ks][e] ^ turn;
+        const float lo = u2f(x << 16) * up, hi = u2f(x & 0xffff0000u) * up;
+        qf[ks][e] = ks < 32 || R5 ? pk_f16(lo, hi) : pk_bf16(lo, hi);
+      }
+  }
   wait_vm<2 * COPIES>();
   lds_barrier();
 #pragma unroll
@@ -881,12 +903,12 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     {
       const int lane = here(), l32 = lane & 31, hh = lane >> 5;
       const int ka = l32 * 128 + 16 * (hh ^ swz(l32));
-      auto kread = [&](int ks) -> bf16x8 {
+      auto kread = [&](int ks) -> u32x4 {
         SPMLA_LDS uint8_t* at = ks >= 32 ? rope : kt + (ks >> 2) * 4096;
-        return *(SPMLA_LDS bf16x8*)(at + (ka ^ (32 * (ks & 3))));
+        return *(SPMLA_LDS u32x4*)(at + (ka ^ (32 * (ks & 3))));
       };
       constexpr int KD = R5 ? 8 : IMG ? 6 : 4;
-      bf16x8 k[KD];
+      u32x4 k[KD];
 #pragma unroll
       for (int n = 0; n < KD; ++n) k[n] = kread(n);
       uint64_t from = 0;
@@ -957,7 +979,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         }
         asm volatile("s_nop 1" : "+v"(S));                // (written by the VALU just before)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) S = qk_next(k[(32 + n) % KD], qf[32 + n], S);
+        for (int n = 0; n < 4; ++n) S = qk_rope(k[(32 + n) % KD], qf[32 + n], S);
       }
       asm volatile("s_nop 15" : "+v"(S));
     }
@@ -985,7 +1007,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       for (int i = 0; i < 8; ++i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          y[i][e] &= ((y[i][e] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((y[i][e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+          y[i][e] &= ((y[i][e] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((y[i][e] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
         at[64 * i] = y[i];
       }
       if (!R5 && w == 0) {
@@ -1000,23 +1022,52 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
     mx = swap32_max(mx);
     m = m == -__builtin_inff() ? mx : m;
-    if (__builtin_expect(maxima, 0)) m = fmaxf(m, mx);
-    if (__builtin_expect(__any((mx - m) * p.c > WIDE), 0) && lane == 0) *over = 1;
-    const float base = m == -__builtin_inff() ? 0.f : m, ref = -base * p.c;
+    float f = 1.f;
+    bool grows = false;
+    if constexpr (!R5) {                                  // scale * 2^-ex2 < 1
+      const f32x2 two = *((SPMLA_LDS f32x2*)scales + lane);
+      float top = fmaxf(fabsf(two[0]) < __builtin_inff() ? fabsf(two[0]) : 0.f, fabsf(two[1]) < __builtin_inff() ? fabsf(two[1]) : 0.f);
+      if (__builtin_expect(__any(top * u2f((uint32_t)(127 - ex2) << 23) > 1.f), 0)) {
+        asm volatile("" : "+v"(top));
+#pragma unroll
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        int e = (int)(f2u(top) >> 23) - 127 + 1;
+        e = __builtin_amdgcn_readfirstlane(e < -126 ? -126 : e > 126 ? 126 : e);
+        f = __builtin_amdgcn_exp2f((float)(ex2 - e));
+        ex2 = e;
+        grows = j > 0;                                    // (before the first products O is zero)
+      }
+    }
+    if (__builtin_expect(__any((mx - m) * c > WTAU) || grows, 0)) {
+      const float mn = fmaxf(m, mx), a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= a;
+      f *= a;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        f32x16 y = O[n];
+        asm volatile("" : "+v"(y));                        // (one after the other: there are 16 registers for it)
+        y *= f;
+        asm volatile("" : "+v"(y));
+        O[n] = y;
+      }
+    }
+    const float base = m == -__builtin_inff() ? 0.f : m, ref = WUP - base * c;
     if (__builtin_expect(__any(fabsf(ref) > FAR), 0)) {    // the rounding of m c would count: differences first
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f((S[r] - base) * p.c);
+      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r] - base, c, WUP));
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], p.c, ref));
+      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], c, ref));
     }
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum += S[r];
     l += sum;
+    if constexpr (!R5) S *= u2f((uint32_t)(127 - ex2) << 23);
     // ---- O^T += V^T P^T
     {
-      bf16x8 P[R5 ? 1 : 2][2];                            // (Row656: weights times the scales of a group, the next one's beside its products)
+      f16x8 P[R5 ? 1 : 2][2];                            // (Row656: weights times the scales of a group, the next one's beside its products)
       f32x4 sc[2];
       auto half_of = [&](int g, int a, int e) {            // positions 8 a + 4 hh + 2 e, + 1
         float x = S[4 * a + 2 * e], y = S[4 * a + 2 * e + 1];
@@ -1025,22 +1076,22 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
           y *= sc[a & 1][2 * e + 1];
         }
         u32x4 u = __builtin_bit_cast(u32x4, P[R5 ? 0 : g & 1][a >> 1]);
-        u[2 * (a & 1) + e] = pk_bf16(x, y);
-        P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(bf16x8, u);
+        u[2 * (a & 1) + e] = pk_f16(x, y);
+        P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(f16x8, u);
       };
       auto scale_of = [&](int g, int a) { sc[a & 1] = *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh); };
       const int vrow = 4 * hh + (l16 >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
       const int v0 = vrow * 128 + 16 * (vch ^ swz(vrow)) + 8 * (lane & 1);  // (rows 8 on: places ^ 2; the group's other half: ^ 4)
-      auto vread = [&](int n) -> bf16x8 {                  // unit n = 2 d + ks: dims 32 d + l32, positions 16 ks ..
+      auto vread = [&](int n) -> f16x8 {                  // unit n = 2 d + ks: dims 32 d + l32, positions 16 ks ..
         SPMLA_LDS uint8_t* at = kt + (n >> 2) * 4096 + (n & 1) * 2048;
         const int c = (n >> 1 & 1) * 64;
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SPMLA_LDS s16x4*)(at + (v0 ^ c)));
         const s16x4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SPMLA_LDS s16x4*)(at + 1024 + (v0 ^ c ^ 32)));
         const auto x = __builtin_bit_cast(i32x2, a), y = __builtin_bit_cast(i32x2, e);
-        return __builtin_bit_cast(bf16x8, i32x4{x[0], x[1], y[0], y[1]});
+        return __builtin_bit_cast(f16x8, i32x4{x[0], x[1], y[0], y[1]});
       };
       constexpr int VD = 6;
-      bf16x8 v[VD];
+      f16x8 v[VD];
 #pragma unroll
       for (int n = 0; n < VD; ++n) v[n] = vread(n);
       if (!R5) {
@@ -1055,7 +1106,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       }
 #pragma unroll
       for (int n = 0; n < 32; ++n) {
-        O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[n % VD], P[R5 ? 0 : (n >> 3) & 1][n & 1], O[n >> 1], 0, 0, 0);
+        O[n >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[n % VD], P[R5 ? 0 : (n >> 3) & 1][n & 1], O[n >> 1], 0, 0, 0);
         if (n + VD < 32) v[n % VD] = vread(n + VD);
         if (!R5 && n < 24) {
           const int g = n / 8 + 1, e = n % 8;
@@ -1069,24 +1120,19 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 
   wait_vm<0>();
   lds_barrier();
-  const int gone = __builtin_amdgcn_readfirstlane(*over);
-  if (__builtin_expect(!gone && !maxima, 1)) break;
-  maxima = gone != 0;
-  lds_barrier();
-  }
 
   // ---- output
   l = swap32_sum(l);
   if (32 * w >= live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const float ln = m == -__builtin_inff() && l == l ? m : m * p.c * 0.69314718055994531f + __builtin_log2f(l) * 0.69314718055994531f;
+  const float ln = m == -__builtin_inff() && l == l ? m : m * c * 0.69314718055994531f + (__builtin_log2f(l) - WUP) * 0.69314718055994531f;
   const bool whole = it.splits == 1;
   const long long r = r0 + qr;
   if (hh == 0 && qr < live) {
     if (!whole) p.lpart[((long long)it.slot + it.sp) * MR + qr] = ln;
     else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
-  const float back = inv * p.kv_scale;
+  const float back = inv * p.kv_scale * (R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23));
   if (!whole) {
     // through LDS, 256 dims of a row at a time: 32 rows of 1024 bytes, 16-byte chunks permuted by the row
     SPMLA_LDS uint8_t* ob = lds + w * 32768;

@@ -20,6 +20,6 @@ def test_compiled_order_of_asm_statements(tmp_path):
     for s in starts:
         end = next(i for i in range(s, len(text)) if ".Lfunc_end" in text[i])
         body = text[s:end]
-        assert sum("v_mfma_f32_32x32x16_bf16" in l for l in body) == 36 + 32
+        assert sum("v_mfma_f32_32x32x16_" in l for l in body) == 36 + 32
         assert not hazards(body), text[s]
         assert not branch_hazards(body), text[s]

@@ -53,11 +53,11 @@ def _check(out, lse, q, cache, table, seqs, start, kv_scale, bs):
         seen = (x <= (L - n + torch.arange(n))[:, None]) & has
         qs = q[t0:t1].double().transpose(0, 1)
         r = ref.softmax_product(qs, rows[None], rows[None, :, :512], seen, SM)
-        # weights (times the row's scale in Row656) are rounded once to bf16, or in workgroups of 64 rows to f16, where the
-        # largest of a row is 2^9 at least and a subnormal one loses 2^-25, times what the largest scale so far is
+        # weights (times the row's scale in Row656) are rounded once to f16, where the largest of a row is 2^5 at least and a
+        # subnormal one loses 2^-25, times less than twice the largest scale so far: 2^-29 of the largest latent a position
         top = float(rows.abs().max()) if L > 0 else 0.0
-        half = ref.HALF[torch.bfloat16]
-        floor = L * 2.0 ** -33 * top
+        half = ref.HALF[torch.float16]
+        floor = L * 2.0 ** -29 * top
         ref.check(out[t0:t1].transpose(0, 1), lse[t0:t1].transpose(0, 1), r, 576, max(L, 1), torch.bfloat16, half, floor, f"request {b}: {n} of {L}")
 
 
@@ -154,6 +154,20 @@ def test_many_requests(dev, row, heads):
     _run(dev, _case(seqs, lens, heads, row, 16, heads), 16)
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 3e-2, 3e3, 1e6, 1e20])
+def test_queries_of_any_size(dev, size):
+    """Queries far from 1 (the kernel's own type for them holds 2^-24 to 2^16), against a kv_scale that brings the scores back."""
+    q, cache, table, seqs, start = _case([300, 77], [20, 13], 64, 656, 16, 19)
+    q = (q.double() * size).to(torch.bfloat16)
+    from arcagi2_flashnext_dots3_amd import kernels
+    for t in (slice(None), slice(20, 21)):
+        qs, tb, sq = (q, table, seqs) if t == slice(None) else (q[t], table[1:], torch.tensor([65], dtype=torch.int32))
+        st = start if t == slice(None) else torch.tensor([0, 1], dtype=torch.int32)
+        out, lse = kernels.attend_chunk(qs.to(dev), cache.to(dev), tb.to(dev), sq.to(dev), st.to(dev), SM / size)
+        torch.cuda.synchronize()
+        _check(out.cpu(), lse.cpu(), (qs.double() / size), cache, tb, sq, st, 1.0, 16)
+
+
 @pytest.mark.parametrize("row", [656, 576])
 @pytest.mark.parametrize("heads", [40, 128])
 def test_rows_gathered_first(dev, row, heads):
@@ -166,7 +180,7 @@ def test_rows_gathered_first(dev, row, heads):
 @pytest.mark.parametrize("row", [656, 576])
 @pytest.mark.parametrize("heads,lens", [(4, [1, 1]), (16, [1, 1]), (128, [1, 1]), (64, [20, 13])])
 def test_scores_rise_far_over_the_first_tile(dev, row, heads, lens):
-    """Scores that climb by hundreds behind the first positions, past what a reference that does not move can hold."""
+    """Scores that climb by hundreds behind the first positions: the reference maximum moves, in every kernel."""
     q, cache, table, seqs, start = _case([300, 200], lens, heads, row, 16, 17)
     q = (q.float() + 6.0 * torch.arange(576).remainder(2).mul(2).sub(1)).to(torch.bfloat16)
     sign = torch.arange(576).remainder(2).mul(2).sub(1)
@@ -184,6 +198,33 @@ def test_scores_rise_far_over_the_first_tile(dev, row, heads, lens):
     _run(dev, case, 16)
     _run(dev, case, 16, items=20)
     _run(dev, case, 16, 0.5, items=0)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads,tokens", [(16, 1), (128, 1), (128, 8)])
+def test_small_weights_are_kept(dev, row, heads, tokens):
+    """One position with nearly all of the weight, at the context's begin; 20,000 others of 2^-22 and 2^-27 of it, that some
+    dims of the output are made of alone."""
+    L, bs = 20000, 64
+    blocks = -(-L // bs)
+    x = torch.zeros(blocks * bs, 576)
+    x[1::2, 256:384] = 1.0
+    x[2::2, 384:512] = 1.0
+    x[1::2, 128:256] = 0.25
+    x[0, :256] = 1.0
+    cache = torch.zeros(blocks * bs, row, dtype=torch.uint8)
+    if row == 576:
+        cache[:] = x.to(ref.E4M3).view(torch.uint8)
+    else:
+        cache[:, :512] = (x[:, :512] * 256).to(ref.E4M3).view(torch.uint8)
+        cache[:, 512:528] = torch.full((4,), 2.0 ** -8).view(torch.uint8)
+    q = torch.zeros(tokens, heads, 576)
+    q[..., :128] = 22 * 0.6931 / (SM * 128)
+    q[..., 128:256] = 5 * 0.6931 / (SM * 128)
+    case = (q.to(torch.bfloat16), cache.view(blocks, bs, row), torch.arange(blocks, dtype=torch.int32)[None], torch.tensor([L], dtype=torch.int32),
+            torch.tensor([0, tokens], dtype=torch.int32))
+    _run(dev, case, bs)
+    _run(dev, case, bs, items=0)
 
 
 @pytest.mark.parametrize("scale", [-1.0, 0.0])
