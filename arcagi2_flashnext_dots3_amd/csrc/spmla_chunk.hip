@@ -10,10 +10,11 @@
 // number of heads, a cached row is copied once for all of them. A position costs 2 (576 + 512) operations a row: with 128 rows
 // 425 to 484 a byte, matrix cores and HBM alike; with fewer HBM, with several tiles of a request the matrix cores.
 //   * products: S^T = K Q^T and O^T = V^T P^T, both with a query row in a lane, so that maxima, sums and factors are one
-//     register a lane, and the weights that a lane forms are the operand it needs: P never leaves its registers. Codes are exact in
-//     bf16 and in fp16, and so is the query but for fp16's range (the wide kernel takes rows out of it times a power of two). (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of
-//     the summed magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales;
-//     for PV the weight times the group's scale.
+//     register a lane, and the weights that a lane forms are the operand it needs: P never leaves its registers. Codes are exact
+//     in bf16 and in fp16, and so is the query but for fp16's range (the wide kernel takes rows out of it times a power of
+//     two). (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of the summed
+//     magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales; for PV
+//     the weight times the group's scale.
 //   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale) are rounded to fp16,
 //     once. (In bf16 they need no care for their range and cost as much, but put as large an error on the output as its
 //     own rounding does.)
@@ -25,10 +26,10 @@
 //     joined in LDS. A wave converts what it reads. Bound by HBM (48 requests of 16 heads, 364 MB: 98 us = 3.7 TB/s).
 //   * `wide_kernel<R5, false>`: 4 waves of 32 rows, 512 registers (O in the 256 accumulation registers, the query in 144 others).
 //     A tile's codes are converted to fp16 once for all waves, beside the score products. Bound by the issue of one
-//     wave a SIMD: matrix cores busy for 29% (64 requests of 128 heads: 115 us = 560 TFLOP/s). Two waves a SIMD leave 16 rows
+//     wave a SIMD: matrix cores busy for 28% (64 requests of 128 heads: 119 us = 540 TFLOP/s). Two waves a SIMD leave 16 rows
 //     a wave, each of which converts everything again (267 us).
 //   * from 1024 on, `image_kernel` gathers and converts the tiles first, `wide_kernel<R5, true>` copies them as they lie
-//     in LDS: no conversions, addresses without tables (1024 tokens of 128 heads over 16384 rows: 3.74 ms = 1210 TFLOP/s, of
+//     in LDS: no conversions, addresses without tables (1024 tokens of 128 heads over 16384 rows: 3.78 ms = 1200 TFLOP/s, of
 //     which the images take 0.01; converted in the kernel 5.3). Bound by the power limit: the clock falls to 1.8 - 2.0
 //     GHz, and a form that runs the softmax beside the next tile's score products takes as long.
 // Splits leave normalized fp32 partials and their lse in a workspace; a second kernel joins them.
@@ -453,7 +454,8 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     f16x8 P[R5 ? 1 : 4];
     if constexpr (R5) {
-      P[0] = __builtin_bit_cast(f16x8, u32x4{pk_f16(s[0][0], s[0][1]), pk_f16(s[0][2], s[0][3]), pk_f16(s[1][0], s[1][1]), pk_f16(s[1][2], s[1][3])});
+      P[0] = __builtin_bit_cast(f16x8, u32x4{pk_f16(s[0][0], s[0][1]), pk_f16(s[0][2], s[0][3]), pk_f16(s[1][0], s[1][1]),
+                                             pk_f16(s[1][2], s[1][3])});
     } else {
       SPMLA_LDS uint8_t* sa = d + L::CODE + L::RP;
       const f32x2 two = *(SPMLA_LDS f32x2*)(sa + lane * 8);                 // the tile's 128 scales
@@ -569,7 +571,8 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     lds_barrier();
     if (!done) {
       const float mo = st[lane], lo = st[64 + lane], mn = fmaxf(m, mo);
-      const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * p.c), c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
+      const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - mn) * p.c);
+      const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
       l = (m == -__builtin_inff() ? l : l * a) + (mo == -__builtin_inff() ? lo : lo * c);
 #pragma unroll
       for (int n = 0; n < 32; ++n) O[n] = O[n] * (e2 * a) + oj[n * 64 + lane] * c;
@@ -599,7 +602,8 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
 #pragma unroll
   for (int n = 0; n < 32; ++n) {
     const f32x4 y = O[n] * back;
-    *(SPMLA_LDS i32x2*)(ob + l16 * 1024 + 16 * ((2 * n + (qt >> 1)) ^ l16) + 8 * (qt & 1)) = i32x2{(int)pk_bf16(y[0], y[1]), (int)pk_bf16(y[2], y[3])};
+    *(SPMLA_LDS i32x2*)(ob + l16 * 1024 + 16 * ((2 * n + (qt >> 1)) ^ l16) + 8 * (qt & 1)) =
+        i32x2{(int)pk_bf16(y[0], y[1]), (int)pk_bf16(y[2], y[3])};
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   for (int row = 0; row < 16 && 16 * wr + row < live; ++row) {
@@ -619,7 +623,7 @@ struct WLds {
   static constexpr int RP = TR * (R5 ? 64 : 128);          // rope
   static constexpr int SC = R5 ? 0 : 4 * TR * 4;           // scales by group, [4][32]
   static constexpr int TILE = CODE + RP + SC;
-  static constexpr int NG = R5 ? 9 : 8;                    // groups of 64 dims in bf16, [NG][32 rows][128 bytes]
+  static constexpr int NG = R5 ? 9 : 8;                    // groups of 64 dims in fp16, [NG][32 rows][128 bytes]
   static constexpr int B = RING * TILE;                    // two of them
   static constexpr int ID = B + 2 * NG * 4096;             // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
@@ -628,7 +632,8 @@ struct WLds {
 };
 
 // Where a request has many query rows, a kernel before this one gathers and converts its tiles once for all of them, as they
-// lie in LDS: nine groups of 64 dims in fp16 (Row656's rope in bf16, as it is), scales by group [4][32], a word of which positions have rows.
+// lie in LDS: nine groups of 64 dims in fp16 (Row656's rope in bf16, as it is), scales by group [4][32], a word of which
+// positions have rows. Bound by the images' bytes (16384 Row576 rows, 28 MB: 11 us).
 constexpr int IMG_SC = 9 * 4096, IMG_OK = IMG_SC + 512, IMAGE = IMG_SC + 1024;
 struct ILds {
   static constexpr int TOTAL = 4 * IMAGE;
@@ -773,7 +778,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   auto address = [&](int lane, int j, int i) -> uint64_t { // of the lane's source in piece i
     if constexpr (IMG) {                                  // (pieces 0, 3, 6 and 9; those behind them by the instruction's offset)
       const int t = kb / TR + j < p.img_tiles ? kb / TR + j : p.img_tiles - 1;
-      return (uint64_t)(uintptr_t)(image + (long long)t * IMAGE + (i < 9 ? w * 9216 + i * 1024 : IMG_SC + w * 256)) + (uint32_t)(lane * (i < 9 ? 16 : 4));
+      return (uint64_t)(uintptr_t)(image + (long long)t * IMAGE + (i < 9 ? w * 9216 + i * 1024 : IMG_SC + w * 256)) +
+             (uint32_t)(lane * (i < 9 ? 16 : 4));
     }
     const int r = lane >> 3, place = (lane & 7) ^ swz(r);
     SPMLA_LDS uint64_t* id = (SPMLA_LDS uint64_t*)(lds + L::ID) + (j * TR & (2 * IDS - 1));
@@ -890,7 +896,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   for (int j = 0; j < nt; ++j) {
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
     wait_vm<(IMG ? 2 : 1) * COPIES>();                    // tile j + 1 (of an image: j) is there
-    lds_barrier();                                        // and tile j in bf16
+    lds_barrier();                                        // and tile j converted
     if constexpr (!IMG) {
     if (in == 0 && next * (IDS / TR) < nt) found = look(next);
     if (in == 2 && next * (IDS / TR) < nt) note(next, found);
@@ -985,7 +991,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     }
     // ---- softmax
     const int lane = here(), l16 = lane & 15, l32 = lane & 31, hh = lane >> 5, qr = 32 * w + l32;
-    const uint32_t has = __builtin_amdgcn_readfirstlane(IMG ? *(SPMLA_LDS uint32_t*)(kt + IMG_OK) : ((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
+    const uint32_t has = __builtin_amdgcn_readfirstlane(IMG ? *(SPMLA_LDS uint32_t*)(kt + IMG_OK)
+                                                            : ((SPMLA_LDS uint32_t*)(lds + L::OK))[j & (2 * IDS / TR - 1)]);
     const int k0 = kb + j * TR;
     if (__builtin_expect(has != 0xffffffffu || k0 + TR > least, 0)) {
       asm volatile("" : "+v"(S));
@@ -1067,7 +1074,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     if constexpr (!R5) S *= u2f((uint32_t)(127 - ex2) << 23);
     // ---- O^T += V^T P^T
     {
-      f16x8 P[R5 ? 1 : 2][2];                            // (Row656: weights times the scales of a group, the next one's beside its products)
+      f16x8 P[R5 ? 1 : 2][2];                            // (Row656: times a group's scales, the next one's beside its products)
       f32x4 sc[2];
       auto half_of = [&](int g, int a, int e) {            // positions 8 a + 4 hh + 2 e, + 1
         float x = S[4 * a + 2 * e], y = S[4 * a + 2 * e + 1];
@@ -1144,7 +1151,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const f32x16& y = O[8 * half + n];
-          *(SPMLA_LDS f32x4*)(ob + l32 * 1024 + 16 * ((8 * n + 2 * a + hh) ^ l32)) = f32x4{y[4 * a], y[4 * a + 1], y[4 * a + 2], y[4 * a + 3]} * back;
+          *(SPMLA_LDS f32x4*)(ob + l32 * 1024 + 16 * ((8 * n + 2 * a + hh) ^ l32)) =
+              f32x4{y[4 * a], y[4 * a + 1], y[4 * a + 2], y[4 * a + 3]} * back;
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       for (int row = 0; row < 32 && 32 * w + row < live; ++row)
@@ -1285,7 +1293,8 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   if (B < 0 || T < 0 || H < 0 || W < 0 || rows < 0 || block_size <= 0 || stride_rows < block_size || items < 0 || longest < 0 ||
       (row_bytes != ROW656 && row_bytes != ROW576))
     return SPMLA_EARG;
-  if (T > MAX_TOKENS || B > MAX_TOKENS || H > 65536 || items > 65536 || rows > 0x7fffffffll || (long long)W * block_size > 0x7fffff00ll) return SPMLA_ELIMIT;
+  if (T > MAX_TOKENS || B > MAX_TOKENS || H > 65536 || items > 65536 || rows > 0x7fffffffll || (long long)W * block_size > 0x7fffff00ll)
+    return SPMLA_ELIMIT;
   if (B == 0 || T == 0 || H == 0) return SPMLA_OK;
   if (!q || !start || !seqs || !out || (rows && !cache) || (W && !table)) return SPMLA_EARG;
   if (((q_st | q_sh | o_st | o_sh) & 7) || (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out) & 15) ||
@@ -1309,7 +1318,8 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const float sc = sm_scale * kv_scale;
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
                   H, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)s.tiles, s.slack,
-                  extra ? items : 0, extra + (extra && s.slack ? B : 0), (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts, longest, images, s.images};
+                  extra ? items : 0, extra + (extra && s.slack ? B : 0), (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts,
+                  longest, images, s.images};
   static DynLds attr[7];
   static Launcher go[7], first[2];
   const int r5 = row_bytes == ROW576, at = s.rows == 32 ? 6 : s.rows == 64 ? 4 + r5 : 2 * (s.images > 0) + r5;
@@ -1331,5 +1341,6 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const long long n = (long long)T * H;
   const int many = n > 4096;
   const chunk::MergeParams mp{opart, lpart, parts, s.rows, (int)slots, start, B, T, H, (uint16_t*)out, o_st, o_sh, lse, l_st};
-  return join[many](many ? (const void*)chunk::merge_kernel<1> : (const void*)chunk::merge_kernel<8>, dim3((unsigned)(many ? (n + 7) / 8 : n)), 512, 0, stm, mp);
+  const void* f = many ? (const void*)chunk::merge_kernel<1> : (const void*)chunk::merge_kernel<8>;
+  return join[many](f, dim3((unsigned)(many ? (n + 7) / 8 : n)), 512, 0, stm, mp);
 }

@@ -222,8 +222,8 @@ int spmla_page_step(const int* fresh, int M, int* lens, int* held, int* table, l
   const int tpb = threads_of(n > M ? n : M);
   int G = (n + tpb - 1) / tpb;
   G = G < 1 ? 1 : G > 64 ? 64 : G;
-  return go((const void*)step_kernel, dim3((unsigned)G), (unsigned)tpb, (size_t)(4 * M + 2 + TPB / 64) * 4, (hipStream_t)stream, fresh, M, p, n, start,
-            req, positions, slots);
+  return go((const void*)step_kernel, dim3((unsigned)G), tpb, (4 * M + 2 + TPB / 64) * 4, (hipStream_t)stream, fresh, M, p, n, start, req,
+            positions, slots);
 }
 
 int spmla_page_trim(const int* keep, int M, int* lens, int* held, int* table, long long table_st, int W, int* free, int P, int* state,
@@ -237,7 +237,7 @@ int spmla_page_trim(const int* keep, int M, int* lens, int* held, int* table, lo
   const int tpb = threads_of(most / 8 > M ? most / 8 : M);
   int G = (int)((most + 32 * TPB - 1) / (32 * TPB) < 32 ? (most + 32 * TPB - 1) / (32 * TPB) : 32);
   G = G < 1 ? 1 : G;
-  return go((const void*)trim_kernel, dim3((unsigned)G), (unsigned)tpb, (size_t)(2 * M + 1 + TPB / 64) * 4, (hipStream_t)stream, keep, M, p);
+  return go((const void*)trim_kernel, dim3((unsigned)G), tpb, (2 * M + 1 + TPB / 64) * 4, (hipStream_t)stream, keep, M, p);
 }
 
 }  // extern "C"

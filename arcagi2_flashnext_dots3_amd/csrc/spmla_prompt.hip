@@ -418,13 +418,15 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
       const uint32_t x = E::pack(O[d][4 * a] * inv, O[d][4 * a + 1] * inv), y = E::pack(O[d][4 * a + 2] * inv, O[d][4 * a + 3] * inv);
       *(SPMLA_LDS i32x2*)(ob + l32 * OROW + ((4 * d + a) ^ (l32 & 7)) * 16 + 8 * hh) = i32x2{(int)x, (int)y};
     }
-  if (p.lse && hh == 0 && qi < len) p.lse[(long long)(s0 + qi) * p.l_st + h] = m * p.c * 0.69314718055994531f + (__builtin_log2f(l) - E::UP) * 0.69314718055994531f;
+  if (p.lse && hh == 0 && qi < len)
+    p.lse[(long long)(s0 + qi) * p.l_st + h] = m * p.c * 0.69314718055994531f + (__builtin_log2f(l) - E::UP) * 0.69314718055994531f;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own rows only
   constexpr int CH = DV / 8;                               // 16-byte chunks a row
   for (int i = lane; i < 32 * CH; i += 64) {
     const int r = i / CH, c = i % CH;
     if (qw + r < len && 8 * c < p.Dv)
-      *(u32x4*)(p.out + (long long)(s0 + qw + r) * p.o_st + (long long)h * p.o_sh + 8 * c) = *(SPMLA_LDS u32x4*)(ob + r * OROW + (c ^ (r & 7)) * 16);
+      *(u32x4*)(p.out + (long long)(s0 + qw + r) * p.o_st + (long long)h * p.o_sh + 8 * c) =
+          *(SPMLA_LDS u32x4*)(ob + r * OROW + (c ^ (r & 7)) * 16);
   }
 }
 
@@ -470,7 +472,8 @@ extern "C" int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, 
       (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) || (((uintptr_t)start | (uintptr_t)lse) & 3))
     return SPMLA_EALIGN;
   prompt::Params p{(const uint16_t*)q, q_st, q_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh, start, B, T, H,
-                   H / Hk, D, Dv, fmaxf((scale < 0.f ? -scale : scale) * 1.4426950408889634f, 1e-30f), scale < 0.f, causal != 0, 0, H % 8 ? 0 : H % 32 == 0 ? 4 : H % 16 == 0 ? 2 : 1,
+                   H / Hk, D, Dv, fmaxf((scale < 0.f ? -scale : scale) * 1.4426950408889634f, 1e-30f), scale < 0.f, causal != 0, 0,
+                   H % 8 ? 0 : H % 32 == 0 ? 4 : H % 16 == 0 ? 2 : 1,
                    (uint16_t*)out, o_st, o_sh, lse, l_st};
   return dtype == DT_BF16 ? prompt::go<true>(p, (hipStream_t)stream) : prompt::go<false>(p, (hipStream_t)stream);
 }
