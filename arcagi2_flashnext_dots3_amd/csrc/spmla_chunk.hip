@@ -1339,7 +1339,7 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   if (!extra) return SPMLA_OK;
   static Launcher join[2];
   const long long n = (long long)T * H;
-  const int many = n > 4096;
+  const int many = n >= 2048;                             // (whole call, 8 / 32 requests of 128 rows: 8 waves a row 48 / 86 us, one 56 / 80)
   const chunk::MergeParams mp{opart, lpart, parts, s.rows, (int)slots, start, B, T, H, (uint16_t*)out, o_st, o_sh, lse, l_st};
   const void* f = many ? (const void*)chunk::merge_kernel<1> : (const void*)chunk::merge_kernel<8>;
   return join[many](f, dim3((unsigned)(many ? (n + 7) / 8 : n)), 512, 0, stm, mp);

@@ -90,7 +90,8 @@ __device__ inline float half_sum(float x) {
 // Tile `rank` (MQ queries) of a head, the longest first: up to SORTED sequences by a search for the level x (causal: tiles of
 // index x - 1; full: sequences of x tiles) that the rank falls into, v(x) tiles of a sequence being at levels >= x; more
 // sequences from the last to the first, sequence b from tile start[b] / MQ + b (as many tiles lie between two sequences as
-// the first one has). 17 ragged sequences, 32 heads: see the kernel.
+// the first one has). With the longest first (17 ragged sequences, 32 heads: 194 -> 172 us) an XCD also takes the tiles of a few
+// heads in turn: of one head after the other 4096 tokens of 128 heads took 849 us, of four together 807, of all 16 840.
 constexpr int SORTED = 256;
 
 template <int MQ>
