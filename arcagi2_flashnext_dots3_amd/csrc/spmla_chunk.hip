@@ -1247,6 +1247,8 @@ __global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
 // Requests of 64 (token, head) rows or fewer on average take workgroups of 64 rows, two waves a row sharing the positions (48
 // requests of 64 rows, 4000 cached ones on average: 90 us, in tiles of 128 rows 115; of 128 rows 146 against 122); of 32
 // or fewer of 32 rows and four (16 rows: 45 us against 55; Row576 alone: of Row656 seven tiles fit into LDS, not the eight).
+// Tiles of 64 rows also where contexts are short and one round takes them: more waves, and less to start and to leave (65 tokens of
+// 128 heads over up to 300 rows: 37 us against 45; 77 over 600: 52 against 56, over 1000: 70 against 64).
 // Tiles are gathered first for requests of 1024 rows and more (16 requests, 2000 cached rows on average: with 256 rows 83 us
 // against 73 without, with 512 103 against 100, with 1024 163 against 174), while their images take 4 GiB at most.
 struct Shape {
@@ -1255,9 +1257,10 @@ struct Shape {
 };
 static Shape shape_of(int T, int H, int B, int row_bytes, int longest) {
   const long long n = (long long)T * H;
-  const int mr = n <= 32ll * B && row_bytes == ROW576 ? 32 : n <= 64ll * B ? 64 : 128, slack = H % mr != 0;
+  const bool little = longest <= 20 * TR && n / 64 + (H % 64 ? B : 0) <= CUS;
+  const int mr = n <= 32ll * B && row_bytes == ROW576 ? 32 : n <= 64ll * B || little ? 64 : 128, slack = H % mr != 0;
   const long long units = ((long long)longest + TR - 1) / TR;
-  const bool images = n >= 1024ll * B && B < 65536 && units * B * IMAGE <= 4ll << 30;
+  const bool images = mr == 128 && n >= 1024ll * B && B < 65536 && units * B * IMAGE <= 4ll << 30;
   return Shape{mr, slack, images ? (int)units : 0, n / mr + (slack ? B : 0)};
 }
 // splits need a place for each (token, head), and for the partial results of a split tile's rows

@@ -89,13 +89,13 @@ def test_a_serving_loop(dev, row):
         seen_lens = list(book.lens)
 
 
-@pytest.mark.parametrize("heads", [16, 128])
-def test_a_captured_decode_step(dev, heads):
+@pytest.mark.parametrize("heads,most", [(16, 600), (128, 600), (128, 700)])
+def test_a_captured_decode_step(dev, heads, most):
     """A decode step with a draft (tables, rows written, attention, one draft rejected) captured once and replayed: every replay
     is the eager step over a copy of the pool and the cache, while eager calls run between."""
     from arcagi2_flashnext_dots3_amd import kernels
     from arcagi2_flashnext_dots3_amd.paging import PagePool
-    M, W, most = 3, 40, 600
+    M, W = 3, 48
     g = torch.Generator().manual_seed(heads)
     pools = [PagePool(100, BS, M, W, dev) for _ in range(2)]
     caches = [torch.zeros(100, BS, 656, dtype=torch.uint8, device=dev) for _ in range(2)]
