@@ -96,6 +96,12 @@ constexpr int SORTED = 256;
 
 template <int MQ>
 __device__ inline bool place(const Params& p, int lane, int rank, int& b, int& q0) {
+  if (p.B == 1) {                     // (no search)
+    const int a = p.start[0], z = p.start[1], len = (z > p.T ? p.T : z) - (a < 0 ? 0 : a);
+    b = 0;
+    q0 = ((len + MQ - 1) / MQ - 1 - rank) * MQ;
+    return len > 0 && q0 >= 0;
+  }
   if (p.B > SORTED) {
     const int ti = p.tiles - 1 - rank;
     int lo = 0, hi = p.B, step;

@@ -1100,7 +1100,8 @@ def page_step(pool, new, n=None, start=None, req=None, positions=None, slots=Non
     """The tables of a step, built on the GPU: new [requests] int32 new tokens of each request of pool (paging.PagePool; <= 0:
     none) -> (start [requests + 1] int32 sums of the new tokens; req [n] int32, positions [n] int64 and slots [n] int64 of
     each token). Pages the tokens need come from the pool's free stack and are entered in its table; where the stack is
-    empty the rest go without (slot -1; pool.state[1] counts the missing pages, and a later step fills them in). n: places
+    empty the rest go without (slot -1; pool.state[1] counts the missing pages; a later step enters pages for them, but their
+    rows were not written: such a request is to be computed again). n: places
     for tokens (None: that of req); those behind the last token hold the last request, position 0 and slot -1, tokens
     beyond n have none."""
     dev = pool.table.device
