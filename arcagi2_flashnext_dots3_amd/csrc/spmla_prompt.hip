@@ -172,6 +172,11 @@ __device__ inline void copies(uint64_t from, SPMLA_LDS uint8_t* to) {      // a 
     copies<G, I + 1>(from, to);
   }
 }
+template <int G>
+__device__ inline void copies_up_to(uint64_t from, SPMLA_LDS uint8_t* to, int left) {     // those of `left` columns on, zeros behind
+#pragma unroll
+  for (int g = 0; g < G; ++g) dma16(64 * g < left ? (const void*)(from + 128 * g) : (const void*)zeros, to + 8192 * g);
+}
 
 template <bool BF, int DK, int DV, int NW>
 __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
@@ -210,8 +215,8 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   const int kend = p.causal && q0 + MQ < len ? q0 + MQ : len;
   const int nt = (kend + TK - 1) / TK;
 
-  // ---- copies: a lane copies from row 8 i + lane / 8 of a group of columns, the chunk whose place is lane % 8. Whole tiles of
-  // whole heads: rows 8 w + lane / 8 (+ 32 with four waves) of every group, one address for them; otherwise one by one.
+  // ---- copies: a lane copies from row 8 i + lane / 8 of a group of columns, the chunk whose place is lane % 8. Whole tiles: rows
+  // 8 w + lane / 8 (+ 32 with four waves) of every group, one address for them; the last tile's one by one.
   auto issue_some = [&](const uint8_t* base, long long st, int dim, int groups, int k0, int dst) {
 #pragma unroll 1
     for (int i = w; i < 8 * groups; i += NW) {             // (wave-uniform)
@@ -228,17 +233,17 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   const bool heads = p.D == DK && p.Dv == DV;
   auto issue_tile = [&](int j) {
     const int buf = (j & 1) * L::BUF;
-    if (heads && (j + 1) * TK <= len) {
-      SPMLA_LDS uint8_t* to = lds + buf + w * 1024;
+    const bool whole = (j + 1) * TK <= len;
+    SPMLA_LDS uint8_t* to = lds + buf + w * 1024;
+    if (__builtin_expect(heads && whole, 1)) {
 #pragma unroll
-      for (int i = 0; i < RS; ++i) {
-        const uint64_t k = ksrc + (uint64_t)((long long)(j * TK + 32 * i) * p.k_st * 2);
-        copies<GK>(k, to + i * 4096);
-      }
+      for (int i = 0; i < RS; ++i) copies<GK>(ksrc + (uint64_t)((long long)(j * TK + 32 * i) * p.k_st * 2), to + i * 4096);
 #pragma unroll
+      for (int i = 0; i < RS; ++i) copies<GV>(vsrc + (uint64_t)((long long)(j * TK + 32 * i) * p.v_st * 2), to + L::K + i * 4096);
+    } else if (whole) {
       for (int i = 0; i < RS; ++i) {
-        const uint64_t v = vsrc + (uint64_t)((long long)(j * TK + 32 * i) * p.v_st * 2);
-        copies<GV>(v, to + L::K + i * 4096);
+        copies_up_to<GK>(ksrc + (uint64_t)((long long)(j * TK + 32 * i) * p.k_st * 2), to + i * 4096, p.D - cch / 2);
+        copies_up_to<GV>(vsrc + (uint64_t)((long long)(j * TK + 32 * i) * p.v_st * 2), to + L::K + i * 4096, p.Dv - cch / 2);
       }
     } else {
       issue_some(kp, p.k_st, p.D, GK, j * TK, buf);
