@@ -254,7 +254,8 @@ class PortableSparseImpl:
         """forward_mqa without a selection (layers without an indexer, or contexts of at most topk rows): every token of
         q [T, H, 576] bf16 (or the pair (q_nope, q_pe)) attends all cached rows of its request up to its own -> (out [T, H,
         512] bf16, lse [T, H] fp32). attn_metadata: CommonAttentionMetadata (with seq_lens, none of them beyond
-        max_seq_len). The rows are in the paged cache: not for an offloaded layer."""
+        max_seq_len). Tokens of no request (a padded batch) get no output. The rows are in the paged cache: not for an
+        offloaded layer."""
         if self._offload:
             raise NotImplementedError("forward_dense: the rows of an offloaded layer are not in the paged cache")
         if isinstance(q, tuple):

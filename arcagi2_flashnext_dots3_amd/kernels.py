@@ -1158,11 +1158,13 @@ def attend_chunk(q, cache, block_table, seq_lens, start, sm_scale, kv_scale=1.0,
     (start [B + 1] int32) are the last of the seq_lens[b] rows that request b has in cache [blocks, block_size, 656 or 576]
     uint8 (already written; block stride any whole number of rows) through block_table [B, columns] int32; each token sees
     its own position and those before it, but for pages that are not there (-1). Returns (out [T, H, 512] bf16, lse [T, H]
-    fp32) as attend over the list of these rows; a token without rows gets 0 and -inf. max_seq_len: at least the longest
+    fp32) as attend over the list of these rows; a token without rows gets 0 and -inf, a token of no request (a padded batch)
+    nothing: its rows of out and lse stay as they are. max_seq_len: at least the longest
     seq_lens, known on the host (None: what the table can hold); positions from it on are not seen. Temporary workspace: for
     1024 (token, head) rows or more a request, max_seq_len rows of each request in 16 bits (up to 4 GiB; beyond, rows are
     converted where they are used); for few rows, partial results. items: workgroups that the kernel makes of the requests'
-    positions, in even shares (None: chunk_items; 0: one a tile of query rows); it changes the order of sums alone."""
+    positions, in even shares (None: chunk_items; 0: one a tile of query rows; 511 beyond those at most); it changes the order
+    of sums alone."""
     _need(q.dim() == 3 and cache.dim() == 3 and block_table.dim() == 2, "q [T, H, 576], cache [blocks, block_size, row], block_table [B, columns]")
     T, H, B, row = q.shape[0], q.shape[1], block_table.shape[0], cache.shape[2]
     room = block_table.shape[1] * cache.shape[1]

@@ -128,14 +128,15 @@ def test_more_new_tokens_than_rows(dev):
     _run(dev, (q, cache, table, torch.tensor([5, 40, -3], dtype=torch.int32), start), 16)
 
 
-def test_padded_block_stride_and_strided_query(dev):
+@pytest.mark.parametrize("heads,lens", [(12, [40, 3]), (128, [40, 3]), (128, [1, 1]), (4, [2, 3])])
+def test_padded_block_stride_and_strided_query(dev, heads, lens):
     """Blocks with rows between them; queries and outputs inside wider tensors; tokens of no request stay as they were."""
     from arcagi2_flashnext_dots3_amd import kernels
-    q, cache, table, seqs, start = _case([200, 77], [40, 3], 12, 656, 16, 6, gap=2)
+    q, cache, table, seqs, start = _case([200, 77], lens, heads, 656, 16, 6, gap=2)
     T, H = q.shape[:2]
     wide = torch.full((T + 7, H + 1, 584), float("nan"), dtype=torch.bfloat16, device=dev)
     wide[2:2 + T, :H, 8:] = q.to(dev)
-    for items in (0, 40):
+    for items in (0, 100):
         out = torch.full((T + 7, H, 520), 7.0, dtype=torch.bfloat16, device=dev)
         lse = torch.full((T + 7, H), 7.0, device=dev)
         kernels.attend_chunk(wide[:, :H, 8:], _device(cache, dev), table.to(dev), seqs.to(dev), (start + 2).to(dev), SM, out=out[..., 8:],
