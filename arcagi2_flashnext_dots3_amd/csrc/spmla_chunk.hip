@@ -96,6 +96,21 @@ __device__ inline bool find_item(const Params& p, int lane, Item& o) {
     o = Item{lo, (int)tile, 0, 1, 0x7fffffff / TR, 0};
     return tile >= 0;
   }
+  if (p.B == 1) {                                         // (the same without sums and search)
+    const int a = p.start[0] < 0 ? 0 : p.start[0], z = p.start[1] > p.T ? p.T : p.start[1];
+    const int n = z > a ? (int)(((long long)(z - a) * p.H + MR - 1) / MR) : 0, len = p.seqs[0] < p.longest ? p.seqs[0] : p.longest;
+    if (n == 0 || n > p.items) return false;
+    const int u = len > 0 ? (len + TR - 1) / TR : 1, room = p.extra < p.items - n ? p.extra : p.items - n;
+    int c = room / n + 1;
+    c = c < (u + LEAST - 1) / LEAST ? c : (u + LEAST - 1) / LEAST;
+    const int span = (u + c - 1) / c;
+    c = (u + span - 1) / span;
+    const int total = n * c, per = (total + 7) >> 3, y = blockIdx.x >> 3, f = y < per ? (int)(blockIdx.x & 7) * per + y : total;
+    if (f >= total) return false;
+    const int tile = n - 1 - f % n;
+    o = Item{0, tile, f / n, c, span, c > 1 ? tile * c : 0};
+    return true;
+  }
   int n[PLAN / 64], u[PLAN / 64];                          // of request 64 k + lane: tiles of query rows, tiles of positions
   const long long cap = p.longest;
   long long work = 0;
@@ -1176,8 +1191,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 }
 
 // Joins the splits of (token, head) row r: weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
-// was not written, is not read. 8 waves a row, or one (many rows, that have few splits each); 8 dims a lane. Bound by the
-// partials' bytes.
+// was not written, does not count. 8 waves a row, or one (many rows, that have few splits each); 8 dims a lane. Bound by the
+// partials' bytes and the chain to them (128 rows of 256 splits, 67 MB: 16 us; with a load that waits for its weight 18).
 struct MergeParams {
   const float* opart; const float* lpart; const i32x2* parts; long long rows; int slots;
   const int* start; int B, T, H;
@@ -1186,8 +1201,9 @@ struct MergeParams {
 };
 template <int WAVES>                                       // of a row
 __global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
+  constexpr int PARTS = 2;                                // 4 dims a lane each
   __shared__ float wgt[8][512];
-  __shared__ f32x4 sums[WAVES == 1 ? 1 : 8][2][64];
+  __shared__ f32x4 sums[WAVES == 1 ? 1 : 8][PARTS][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long r = WAVES == 1 ? (long long)blockIdx.x * 8 + w : blockIdx.x, t = r / p.H, h = r % p.H;
   if (t >= p.T || t < p.start[0] || t >= p.start[p.B]) return;               // rows of no request stay as they are
@@ -1215,32 +1231,35 @@ __global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
   for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   const float* o = p.opart + (long long)first * D_LAT + 4 * lane;
-  f32x4 a = {}, b = {};
-#pragma unroll 4
+  f32x4 a[PARTS] = {};
+#pragma unroll 8
   for (int s = WAVES == 1 ? 0 : w; s < n; s += WAVES) {
     const float y = wgt[w][s];
-    if (y >= 0.f || y != y) {
-      a += y * *(const f32x4*)(o + s * p.rows * D_LAT);
-      b += y * *(const f32x4*)(o + s * p.rows * D_LAT + 256);
+    const bool has = !(y < 0.f);                          // (the load does not wait for it: what was not written is there, unused)
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const f32x4 v = *(const f32x4*)(o + s * p.rows * D_LAT + 256 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[i][e] = has ? __builtin_fmaf(y, v[e], a[i][e]) : a[i][e];
     }
   }
   if constexpr (WAVES > 1) {
-    sums[w][0][lane] = a;
-    sums[w][1][lane] = b;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) sums[w][i][lane] = a[i];
     __syncthreads();
     if (w) return;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-      a += sums[i][0][lane];
-      b += sums[i][1][lane];
-    }
+    for (int k = 1; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) a[i] += sums[k][i][lane];
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  a *= inv;
-  b *= inv;
   uint16_t* to = p.out + t * p.o_st + h * p.o_sh + 4 * lane;
-  *(i32x2*)to = i32x2{(int)pk_bf16(a[0], a[1]), (int)pk_bf16(a[2], a[3])};
-  *(i32x2*)(to + 256) = i32x2{(int)pk_bf16(b[0], b[1]), (int)pk_bf16(b[2], b[3])};
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    a[i] *= inv;
+    *(i32x2*)(to + 256 * i) = i32x2{(int)pk_bf16(a[i][0], a[i][1]), (int)pk_bf16(a[i][2], a[i][3])};
+  }
   if (p.lse && lane == 0) p.lse[t * p.l_st + h] = sum > 0.f || sum != sum ? ref + __logf(sum) : -__builtin_inff();
 }
 
