@@ -1192,7 +1192,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 
 // Joins the splits of (token, head) row r: weights exp(lse_s - max); a split without keys has lse -inf and its partial, which
 // was not written, does not count. 8 waves a row, or one (many rows, that have few splits each); 8 dims a lane. Bound by the
-// partials' bytes and the chain to them (128 rows of 256 splits, 67 MB: 16 us; with a load that waits for its weight 18).
+// partials' bytes and the chain to them (128 rows of 256 splits, 67 MB: 14 us; with loads that wait for their weights 18).
 struct MergeParams {
   const float* opart; const float* lpart; const i32x2* parts; long long rows; int slots;
   const int* start; int B, T, H;
