@@ -35,6 +35,7 @@
 // Splits leave normalized fp32 partials and their lse in a workspace; a second kernel joins them.
 #include "spmla_common.h"
 #include "spmla_quant.h"
+#include "spmla_rules.h"
 
 namespace spmla {
 namespace chunk {
@@ -204,7 +205,7 @@ struct Lds {
   static constexpr int ID = RING * TILE;                   // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
   static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
-  static constexpr int JOIN = 4 * 32768;                   // at the end: O of 4 waves, then maxima and sums
+  static constexpr int JOIN = 4 * rules::CHUNK_JOIN;       // at the end: O of 4 waves, then maxima and sums
   static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0, "one workgroup a compute unit");
   static constexpr int BYTES = TOTAL < JOIN + 2048 ? JOIN + 2048 : TOTAL;
 };
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   bool done = !works;
 #pragma unroll
   for (int half = PS / 2; half >= 1; half /= 2) {
-    SPMLA_LDS f32x4* oj = (SPMLA_LDS f32x4*)(lds + (wr * half + wp % half) * 32768);
+    SPMLA_LDS f32x4* oj = (SPMLA_LDS f32x4*)(lds + rules::chunk_join_at(wr, half, wp));
     SPMLA_LDS float* st = (SPMLA_LDS float*)(lds + L::JOIN) + (wr * half + wp % half) * 128;
     lds_barrier();
     if (!done && wp >= half) {
@@ -612,8 +613,8 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
       for (int n = 0; n < 32; ++n) *(f32x4*)(o + 16 * n) = O[n] * back;
     return;
   }
-  // bf16 rows through LDS: 16 of 1024 bytes, 16-byte chunks permuted by the row
-  SPMLA_LDS uint8_t* ob = lds + wr * 16384;
+  // bf16 rows through LDS, in the place that this wave alone read last: 16 of 1024 bytes, 16-byte chunks permuted by the row
+  SPMLA_LDS uint8_t* ob = lds + rules::chunk_rows_at(wr);
 #pragma unroll
   for (int n = 0; n < 32; ++n) {
     const f32x4 y = O[n] * back;

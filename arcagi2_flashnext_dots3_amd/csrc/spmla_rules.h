@@ -82,5 +82,14 @@ inline int linear_kernel(int T, int N, int K) {
   return best;
 }
 
+
+// LDS places (bytes) at the end of the small-row kernel over all cached rows (spmla_chunk.hip), whose PS waves of the same 16
+// query rows (wave w: rows w / PS, share w % PS) are joined two by two and the first of them writes the rows out. In the round
+// that leaves `half` of them wave wp takes the 32 KB that wave wp + half left at chunk_join_at(wr, half, wp). Its bf16 rows (16
+// KB) go where it alone reads in the last round: no barrier stands between.
+constexpr int CHUNK_JOIN = 32768;                        // O of 16 rows of 512 dims in fp32
+inline constexpr int chunk_join_at(int wr, int half, int wp) { return (wr * half + wp % half) * CHUNK_JOIN; }
+inline constexpr int chunk_rows_at(int wr) { return chunk_join_at(wr, 1, 0); }
+
 }  // namespace rules
 }  // namespace spmla
