@@ -742,6 +742,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     return x < 0 ? 0 : x > cap ? (int)cap : (int)x;
   };
   const int least = limit_of(0), most = limit_of(live - 1);
+  // where the rows of a tile end: an image holds the request's rows behind `most` too (those of its later tokens)
+  const int there = !IMG ? most : p.seqs[b] < p.longest ? p.seqs[b] : p.longest;
   const long long first = (long long)it.sp * it.span * TR, last = first + (long long)it.span * TR;
   const int kb = first < most ? (int)first : most;
   const int ke = it.sp + 1 < it.splits && last < most ? (int)last : most;                    // (the last split takes the rest)
@@ -1019,7 +1021,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         S[r] = (has >> x & 1) && k0 + x < limit ? S[r] : -__builtin_inff();
       }
     }
-    if (__builtin_expect(k0 + TR > least && least < most, 0)) {
+    if (__builtin_expect(k0 + TR > least && least < there, 0)) {
       // the mask cuts this tile: values that are no numbers become 0 once every wave has its scores
       lds_barrier();
       u32x4 y[8];
