@@ -1205,14 +1205,14 @@ struct MergeParams {
 template <int WAVES>                                       // of a row
 __global__ void __launch_bounds__(512) merge_kernel(MergeParams p) {
   constexpr int PARTS = 2;                                // 4 dims a lane each
-  __shared__ float wgt[8][512];
+  __shared__ float wgt[8][rules::CHUNK_SPLITS];
   __shared__ f32x4 sums[WAVES == 1 ? 1 : 8][PARTS][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long r = WAVES == 1 ? (long long)blockIdx.x * 8 + w : blockIdx.x, t = r / p.H, h = r % p.H;
   if (t >= p.T || t < p.start[0] || t >= p.start[p.B]) return;               // rows of no request stay as they are
   const i32x2 part = p.parts[r];
   const int first = __builtin_amdgcn_readfirstlane(part[0]), n = __builtin_amdgcn_readfirstlane(part[1]);
-  if (first < 0 || n < 2 || n > 512 || first / p.rows + n > p.slots) return;
+  if (first < 0 || n < 2 || n > rules::CHUNK_SPLITS || first / p.rows + n > p.slots) return;
   float top = -__builtin_inff();
   for (int s = lane; s < n; s += 64) {
     const float x = p.lpart[first + s * p.rows];
@@ -1287,7 +1287,7 @@ static Shape shape_of(int T, int H, int B, int row_bytes, int longest) {
 }
 // splits need a place for each (token, head), and for the partial results of a split tile's rows
 static long long part_slots(const Shape& s, int items, int B) {
-  const long long e = items - s.tiles + (s.slack ? B : 0);
+  const int e = rules::chunk_extra(items - s.tiles, s.slack, B);
   return items < 2 * e ? items : 2 * e;
 }
 
@@ -1331,7 +1331,7 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   if (s.tiles > (1ll << 30)) return SPMLA_ELIMIT;
   const long long need = spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, longest, items);
   const int extra = B <= chunk::PLAN && longest > 0 && items > s.tiles ? (int)(items - s.tiles) : 0;
-  if (extra > 511) return SPMLA_ELIMIT;
+  if (extra >= rules::CHUNK_SPLITS) return SPMLA_ELIMIT;
   if (need && !ws) return SPMLA_EARG;
   if (need && ((uintptr_t)ws & 15)) return SPMLA_EALIGN;
   if (need && ws_bytes < need) return SPMLA_EARG;
@@ -1343,7 +1343,7 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const float sc = sm_scale * kv_scale;
   chunk::Params p{(const uint16_t*)q, q_st, q_sh, (const uint8_t*)cache, rows, stride_rows, block_size, table, t_st, W, seqs, start, B, T,
                   H, fmaxf((sc < 0.f ? -sc : sc) * 1.4426950408889634f, 1e-30f), kv_scale, sc < 0.f, (int)s.tiles, s.slack,
-                  extra ? items : 0, extra + (extra && s.slack ? B : 0), (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts,
+                  extra ? items : 0, extra ? rules::chunk_extra(extra, s.slack, B) : 0, (uint16_t*)out, o_st, o_sh, lse, l_st, opart, lpart, parts,
                   longest, images, s.images};
   static DynLds attr[7];
   static Launcher go[7], first[2];

@@ -91,5 +91,14 @@ constexpr int CHUNK_JOIN = 32768;                        // O of 16 rows of 512 
 inline constexpr int chunk_join_at(int wr, int half, int wp) { return (wr * half + wp % half) * CHUNK_JOIN; }
 inline constexpr int chunk_rows_at(int wr) { return chunk_join_at(wr, 1, 0); }
 
+// Of spmla_chunk.hip's launches: the most partial results of a (token, head) row that the join takes, and how many workgroups
+// beyond one a tile share out the positions, all of which one tile may take: `beyond` of the counted tiles (one less than
+// those results at most), and as many more as there are requests where these are counted with a tile too many each.
+constexpr int CHUNK_SPLITS = 512;
+inline int chunk_extra(long long beyond, int slack, int B) {
+  const long long x = beyond + (slack ? B : 0);
+  return (int)(x < CHUNK_SPLITS - 1 ? x : CHUNK_SPLITS - 1);
+}
+
 }  // namespace rules
 }  // namespace spmla

@@ -17,7 +17,9 @@ def lib(tmp_path_factory):
     (d / "r.cpp").write_text('#include "spmla_rules.h"\n'
                              'extern "C" int join_at(int wr, int half, int wp) { return spmla::rules::chunk_join_at(wr, half, wp); }\n'
                              'extern "C" int join_bytes() { return spmla::rules::CHUNK_JOIN; }\n'
-                             'extern "C" int rows_at(int wr) { return spmla::rules::chunk_rows_at(wr); }\n')
+                             'extern "C" int rows_at(int wr) { return spmla::rules::chunk_rows_at(wr); }\n'
+                             'extern "C" int splits() { return spmla::rules::CHUNK_SPLITS; }\n'
+                             'extern "C" int extra(int beyond, int slack, int B) { return spmla::rules::chunk_extra(beyond, slack, B); }\n')
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I", build.CSRC, str(d / "r.cpp"), "-o",
                     str(d / "r.so")], check=True, capture_output=True)
     return ctypes.CDLL(str(d / "r.so"))
@@ -43,3 +45,12 @@ def test_partial_sums_of_a_round_do_not_overlap(lib, shares):
         places.sort()
         assert all(b - a >= lib.join_bytes() for a, b in zip(places, places[1:])) and places[-1] + lib.join_bytes() <= 4 * 32768
         half //= 2
+
+
+@pytest.mark.parametrize("beyond", [1, 255, 300, 510, 511])
+@pytest.mark.parametrize("slack,requests", [(0, 1), (1, 1), (1, 2), (1, 200), (1, 256)])
+def test_no_row_has_more_parts_than_the_join_takes(lib, beyond, slack, requests):
+    """One tile may take all of the workgroups beyond one a tile."""
+    extra = lib.extra(beyond, slack, requests)
+    assert extra + 1 <= lib.splits()
+    assert extra >= beyond
