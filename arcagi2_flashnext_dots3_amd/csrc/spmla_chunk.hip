@@ -43,7 +43,7 @@ namespace chunk {
 constexpr int TR = 32;                // positions per tile
 constexpr int IDS = 256;              // positions whose rows are looked up at a time
 constexpr float TAU = 6.0f, UP = 9.0f, FAR = 65536.f;     // the reference maximum moves past 2^TAU; weights are times 2^UP
-constexpr float WTAU = 10.0f, WUP = 5.0f;                // of the wide kernel, where moving it costs more
+constexpr float WTAU = 10.0f, WUP = 5.0f;                // of the wide kernel, where moving it costs more (Row656: 9 and 6, see raise)
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -257,10 +257,36 @@ __device__ inline f16x8 codes8_f16(int a, int b) {
 // place of chunk c (16 bytes) in a row of 128 bytes: c ^ swz(row); 16 rows' chunks c lie in all 64 banks
 __device__ inline int swz(int row) { return ((row & 2) << 1) | ((row & 4) >> 2) | ((row & 8) >> 2); }
 
+// ---- Row656: weights times scales in f16's range. A query row's weight times the scale of group g is taken times 2^-e, e following
+// the group's largest scale among the positions that the row sees (scale * 2^-e <= 1): per lane four bytes 127 - e, and O
+// holds its dims of the group times 2^-e. e starts at LOW: a weight (up to 2^15) times 2^-LOW is finite, so that scales of zero
+// give zeros; it moves when a scale passes 2^e, to twice what that takes, so that it moves rarely (64 requests of 128
+// heads: 112 us; to just what it takes 122). Rows that see the same positions have the same e; they differ behind a tile that the mask cuts.
+constexpr int LOW = -100;
+constexpr uint32_t LOWS = 0x01010101u * (127 - LOW);
+__device__ inline float down_of(uint32_t ex, int g) { return u2f((ex >> (8 * g) & 255u) << 23); }               // 2^-e of group g
+__device__ inline float up_of(uint32_t ex, int g) { return u2f((254u - (ex >> (8 * g) & 255u)) << 23); }
+__device__ inline float finite_size(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.f; }
+// top: per lane the largest scale of each group that its row has come to see. Returns the rows' new bytes, factor: what O's dims of
+// a group are to be multiplied by, down: the largest 2^-e of any row in the group of the scales 2 lane, 2 lane + 1.
+__device__ inline uint32_t raise(uint32_t ex, const float (&top)[4], int lane, float (&factor)[4], float& down) {
+  uint32_t to = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int old = (int)(ex >> (8 * g) & 255u), e = (int)(f2u(top[g]) >> 23) - 125;                  // top * 2^-e < 1 / 2
+    int now = 127 - (e < 126 ? e : 126);
+    now = now < old ? now : old;
+    to |= (uint32_t)now << (8 * g);
+    factor[g] = __builtin_amdgcn_ldexpf(1.f, now - old);
+    const int most = wave_top(now);
+    if (lane >> 4 == g) down = u2f((uint32_t)most << 23);
+  }
+  return to;
+}
+
 // ---- 64 rows or fewer of a request. PV: V^T by the 8-bit transposing read, converted exactly to f16; P in f16 times 2^UP so that
-// few weights are f16 subnormals (Row656: P times the scales of the four groups times 2^-e, e following the largest
-// scale so far: a product p * scale is off by half an f16 step, or 2^-34 of the largest scale). The reference maximum
-// moves only past TAU.
+// few weights are f16 subnormals (Row656: P times the scales of the four groups times 2^-e: a product p * scale is off by half
+// an f16 step, or 2^-32 of the largest scale of the group that the row has seen). The reference maximum moves only past TAU.
 template <bool R5, int PS>
 __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   using L = Lds<R5, PS>;
@@ -364,12 +390,13 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     }
   };
 
-  f32x4 O[32];                                            // O^T: dims 16 n + 4 qt .., query row qr; times 2^-ex2 (Row656)
+  f32x4 O[32];                                            // O^T: dims 16 n + 4 qt .., query row qr; times 2^-e (Row656)
 #pragma unroll
   for (int n = 0; n < 32; ++n) O[n] = f32x4{};
   float m = -__builtin_inff(), l = 0.f;                   // of query row qr (m: as scores are, shared by its four lanes; l: this lane's)
   bool far = false;                                       // a reference is beyond FAR
-  int ex2 = -126;
+  uint32_t ex = LOWS;                                     // 127 - e of the four groups
+  float down = u2f((uint32_t)(127 - LOW) << 23);          // the largest 2^-e in the group of this lane's two scales
   f32x4 s[2];                                             // scores, then weights: value 4 u + r is position 16 u + 4 qt + r
 
   auto scores = [&](SPMLA_LDS uint8_t* d) {
@@ -465,8 +492,8 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
       for (int r = 0; r < 4; ++r) l += s[u][r];
   };
 
-  // O += V^T P^T
-  auto values = [&](SPMLA_LDS uint8_t* d) {
+  // O += V^T P^T of tile j
+  auto values = [&](SPMLA_LDS uint8_t* d, int j) {
     const int lane = here(), l16 = lane & 15, qt = lane >> 4;
     f16x8 P[R5 ? 1 : 4];
     if constexpr (R5) {
@@ -475,25 +502,36 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     } else {
       SPMLA_LDS uint8_t* sa = d + L::CODE + L::RP;
       const f32x2 two = *(SPMLA_LDS f32x2*)(sa + lane * 8);                 // the tile's 128 scales
-      float top = fmaxf(fabsf(two[0]) < __builtin_inff() ? fabsf(two[0]) : 0.f, fabsf(two[1]) < __builtin_inff() ? fabsf(two[1]) : 0.f);
-      if (__builtin_expect(__any(top * u2f((uint32_t)(127 - ex2) << 23) > 1.f), 0)) {        // a larger one than before: e follows
-        asm volatile("" : "+v"(top));
+      const float most = fmaxf(finite_size(two[0]), finite_size(two[1]));
+      if (__builtin_expect(__any(most * down > 1.f), 0)) {                  // a larger one than before
+        float top[4], factor[4];
+        if (kb + (j + 1) * TR > least) {                                    // the mask cuts the tile: each row for itself
 #pragma unroll
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        int e = (int)(f2u(top) >> 23) - 127 + 1;                            // scale * 2^-e < 1
-        e = __builtin_amdgcn_readfirstlane(e < -126 ? -126 : e > 126 ? 126 : e);
-        const float a = __builtin_amdgcn_exp2f((float)(ex2 - e));
-        ex2 = e;
+          for (int g = 0; g < 4; ++g) {
+            top[g] = 0.f;
 #pragma unroll
-        for (int n = 0; n < 32; ++n) O[n] *= a;
+            for (int u = 0; u < 2; ++u) {
+              const f32x4 x = *(SPMLA_LDS f32x4*)(sa + g * 128 + 64 * u + qt * 16);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) top[g] = s[u][r] > 0.f ? fmaxf(top[g], finite_size(x[r])) : top[g];
+            }
+            top[g] = quad_max(top[g]);
+          }
+        } else {
+          float y = most;
+#pragma unroll
+          for (int x = 8; x; x >>= 1) y = fmaxf(y, __shfl_xor(y, x));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) top[g] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(y), 16 * g));
+        }
+        ex = raise(ex, top, lane, factor, down);
+#pragma unroll
+        for (int n = 0; n < 32; ++n) O[n] *= factor[n >> 3];
       }
-      const float down = u2f((uint32_t)(127 - ex2) << 23);
-      f32x4 t[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) t[u] = s[u] * down;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 a = *(SPMLA_LDS f32x4*)(sa + g * 128 + qt * 16) * t[0], b = *(SPMLA_LDS f32x4*)(sa + g * 128 + 64 + qt * 16) * t[1];
+      for (int g = 0; g < 4; ++g) {                                         // (weights first: 0 * scale stays 0)
+        const f32x4 a = s[0] * down_of(ex, g) * *(SPMLA_LDS f32x4*)(sa + g * 128 + qt * 16);
+        const f32x4 b = s[1] * down_of(ex, g) * *(SPMLA_LDS f32x4*)(sa + g * 128 + 64 + qt * 16);
         P[g] = __builtin_bit_cast(f16x8, u32x4{pk_f16(a[0], a[1]), pk_f16(a[2], a[3]), pk_f16(b[0], b[1]), pk_f16(b[2], b[3])});
       }
     }
@@ -563,14 +601,16 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     }
     if (go) {
       softmax(mine);
-      values(d);
+      values(d, mine);
     }
     if (more) note(next, found);
   }
 
   // ---- join of a row's four lanes, and of the waves of its rows
   l = quad_sum(l);
-  float e2 = R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23);
+  float up[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) up[g] = R5 ? 1.f : up_of(ex, g);
   bool done = !works;
 #pragma unroll
   for (int half = PS / 2; half >= 1; half /= 2) {
@@ -579,7 +619,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     lds_barrier();
     if (!done && wp >= half) {
 #pragma unroll
-      for (int n = 0; n < 32; ++n) oj[n * 64 + lane] = O[n] * e2;
+      for (int n = 0; n < 32; ++n) oj[n * 64 + lane] = O[n] * up[n >> 3];
       st[lane] = m;
       st[64 + lane] = l;
       done = true;
@@ -591,9 +631,10 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
       const float c = mo == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mo - mn) * p.c);
       l = (m == -__builtin_inff() ? l : l * a) + (mo == -__builtin_inff() ? lo : lo * c);
 #pragma unroll
-      for (int n = 0; n < 32; ++n) O[n] = O[n] * (e2 * a) + oj[n * 64 + lane] * c;
+      for (int n = 0; n < 32; ++n) O[n] = O[n] * (up[n >> 3] * a) + oj[n * 64 + lane] * c;
       m = mn;
-      e2 = 1.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) up[g] = 1.f;
     }
   }
   if (done) return;
@@ -605,7 +646,7 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
     if (!whole) p.lpart[((long long)it.slot + it.sp) * MR + qr] = ln;
     else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
-  const float back = e2 * inv * p.kv_scale;
+  const float back = inv * p.kv_scale;                    // (the join has taken 2^-e from O)
   if (!whole) {
     float* o = p.opart + (((long long)it.slot + it.sp) * MR + qr) * D_LAT + 4 * qt;
     if (qr < live)
@@ -643,7 +684,8 @@ struct WLds {
   static constexpr int B = RING * TILE;                    // two of them
   static constexpr int ID = B + 2 * NG * 4096;             // addresses of the rows of two times IDS positions
   static constexpr int OK = ID + 2 * IDS * 8;              // which of a tile's positions have rows, a bit each
-  static constexpr int TOTAL = OK + 2 * IDS / 32 * 4;
+  static constexpr int PV = OK + 2 * IDS / 32 * 4;         // Row656: each wave's scales of a tile for the second product
+  static constexpr int TOTAL = PV + (R5 ? 0 : 4 * 512);
   static_assert(TOTAL <= 160 * 1024 && ID % 8 == 0 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
 };
 
@@ -652,7 +694,8 @@ struct WLds {
 // positions have rows. Bound by the images' bytes (16384 Row576 rows, 28 MB: 11 us).
 constexpr int IMG_SC = 9 * 4096, IMG_OK = IMG_SC + 512, IMAGE = IMG_SC + 1024;
 struct ILds {
-  static constexpr int TOTAL = 4 * IMAGE;
+  static constexpr int PV = 4 * IMAGE;                     // (as above)
+  static constexpr int TOTAL = PV + 4 * 512;
   static_assert(TOTAL <= 160 * 1024 && TOTAL >= 4 * 32768, "one workgroup a compute unit");
 };
 
@@ -720,6 +763,7 @@ template <bool R5, bool IMG>
 __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   using L = WLds<R5>;
   constexpr int RB = R5 ? ROW576 : ROW656, MR = 128;
+  constexpr float TAU = R5 ? WTAU : WTAU - 1.f, UP = R5 ? WUP : WUP + 1.f;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem_generic[];
   SPMLA_LDS uint8_t* lds = (SPMLA_LDS uint8_t*)smem_generic;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -846,12 +890,15 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   };
   constexpr int PIECES = IMG ? 0 : R5 ? 5 : 4;            // of a tile's conversion
 
-  // ---- softmax state. The reference maximum is the first one that a row meets and moves past 2^WTAU over it only (O, which fills
-  // the AGPRs, takes 800 instructions to rescale); Row656: O is times 2^-ex2, ex2 following the largest scale so far.
+  // ---- softmax state. The reference maximum is the first one that a row meets and moves past 2^TAU over it only (O, which fills
+  // the AGPRs, takes 800 instructions to rescale); Row656: O is times 2^-e (see raise).
   f32x16 O[16];                                           // O^T: dims 32 n + 8 a + 4 hh + b, query row qr
   float m = -__builtin_inff(), l;                         // of query row qr (m: as scores are, of both halves; l: this half's)
   float c = p.c;                                          // (per row: the query is times a power of two)
-  int ex2 = -126;
+  uint32_t ex = LOWS;
+  float down = u2f((uint32_t)(127 - LOW) << 23);          // 2^-e of the two scales of a tile that this lane copies
+  bool apart = false;
+  SPMLA_LDS uint8_t* copied = lds + (IMG ? ILds::PV : L::PV) + w * 512;
   if constexpr (!IMG) {
     note(0, found);
     note(1, -1);                                          // (addresses that a copy may take, whatever the tile)
@@ -910,8 +957,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       two(z, y, 1);
       put(lane, 0, i, half, z);
     }
+  // Row656: the second product takes the scales times 2^-e (weights times 2^-e of every group instead: 64 requests of 128 heads 2.4
+  // us more). Rows apart, from a tile on that the mask cuts and where e moves: a tile is taken four times (copies and conversions
+  // that are repeated leave what is there), each time with the weights times the row's own 2^-e of one group and zeros for the scales of
+  // the others. `apart` is the same for all waves: up to that tile they have met the same scales.
+  int pass = 0;
 #pragma unroll 1
-  for (int j = 0; j < nt; ++j) {
+  for (int j = 0; j < nt;) {
     const int in = j & (IDS / TR - 1), next = j / (IDS / TR) + 1;
     wait_vm<(IMG ? 2 : 1) * COPIES>();                    // tile j + 1 (of an image: j) is there
     lds_barrier();                                        // and tile j converted
@@ -922,6 +974,13 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     SPMLA_LDS uint8_t* kt = IMG ? lds + (j & 3) * IMAGE : lds + L::B + (j & 1) * (L::NG * 4096);
     SPMLA_LDS uint8_t* rope = IMG ? kt + 8 * 4096 : R5 ? kt + 8 * 4096 : lds + (j & 3) * L::TILE + L::CODE;
     SPMLA_LDS uint8_t* scales = IMG ? kt + IMG_SC : lds + (j & 3) * L::TILE + L::CODE + L::RP;
+    // ---- Row656: the wave's copy of the scales times 2^-e, beside the first products (and again behind them where e moves or the
+    // mask cuts the tile)
+    bool grows = false;
+    auto copy_scales = [&](f32x2 two) {
+      *((SPMLA_LDS f32x2*)copied + here()) = two * down;
+      asm volatile("" ::: "memory");                       // (the wave's own, in order)
+    };
     // ---- S^T = K Q^T; beside it the copies of tile j + 3 and the conversion of tile j + 1, piece by piece
     f32x16 S;
     {
@@ -938,7 +997,11 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
       uint64_t from = 0;
       i32x2 y0 = {}, y1 = {};
       u32x4 z = {};
+      f32x2 both = {};
       auto beside = [&](int ks) {                         // what runs beside product ks: piece ks / 6 of copies and codes
+        if (!R5 && ks == 1) both = *((SPMLA_LDS f32x2*)scales + lane);
+        if (!R5 && ks == 7) grows = apart | (__any(fmaxf(finite_size(both[0]), finite_size(both[1])) * down > 1.f) != 0);
+        if (!R5 && ks == 8) copy_scales(both);
         if constexpr (IMG) {
           if (ks % 3 == 0 && ks / 3 < COPIES) {
             if (ks / 3 % 3 == 0) from = address(lane, j + 3, ks / 3);
@@ -1047,49 +1110,70 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
     mx = swap32_max(mx);
     m = m == -__builtin_inff() ? mx : m;
-    float f = 1.f;
-    bool grows = false;
-    if constexpr (!R5) {                                  // scale * 2^-ex2 < 1
+    float by[4] = {1.f, 1.f, 1.f, 1.f};                     // factors of O's dims of the groups
+    bool moved = false;
+    const bool cut = k0 + TR > least;
+    if (!R5 && __builtin_expect(grows || cut, 0)) {
       const f32x2 two = *((SPMLA_LDS f32x2*)scales + lane);
-      float top = fmaxf(fabsf(two[0]) < __builtin_inff() ? fabsf(two[0]) : 0.f, fabsf(two[1]) < __builtin_inff() ? fabsf(two[1]) : 0.f);
-      if (__builtin_expect(__any(top * u2f((uint32_t)(127 - ex2) << 23) > 1.f), 0)) {
-        asm volatile("" : "+v"(top));
+      if (grows) {
+        float top[4];
+        if (cut) {                                         // each row for itself
+          apart = true;
 #pragma unroll
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        int e = (int)(f2u(top) >> 23) - 127 + 1;
-        e = __builtin_amdgcn_readfirstlane(e < -126 ? -126 : e > 126 ? 126 : e);
-        f = __builtin_amdgcn_exp2f((float)(ex2 - e));
-        ex2 = e;
-        grows = j > 0;                                    // (before the first products O is zero)
+          for (int g = 0; g < 4; ++g) {
+            top[g] = 0.f;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+              const f32x4 x = *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) top[g] = S[4 * a + r] > -__builtin_inff() ? fmaxf(top[g], finite_size(x[r])) : top[g];
+            }
+            top[g] = swap32_max(top[g]);
+          }
+        } else {
+          float y = fmaxf(finite_size(two[0]), finite_size(two[1]));
+#pragma unroll
+          for (int x = 8; x; x >>= 1) y = fmaxf(y, __shfl_xor(y, x));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) top[g] = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(y), 16 * g));
+        }
+        const uint32_t was = ex;
+        ex = raise(ex, top, lane, by, down);
+        moved = (j > 0 || pass > 0) && __any(ex != was);   // (before the first products O is zero)
+        if (apart) down = lane >> 4 == pass ? 1.f : 0.f;
       }
+      copy_scales(two);
     }
-    if (__builtin_expect(__any((mx - m) * c > WTAU) || grows, 0)) {
+    if (__builtin_expect(__any((mx - m) * c > TAU) || moved, 0)) {
       const float mn = fmaxf(m, mx), a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       l *= a;
-      f *= a;
 #pragma unroll
       for (int n = 0; n < 16; ++n) {
         f32x16 y = O[n];
         asm volatile("" : "+v"(y));                        // (one after the other: there are 16 registers for it)
-        y *= f;
+        y *= a * by[n >> 2];
         asm volatile("" : "+v"(y));
         O[n] = y;
       }
     }
-    const float base = m == -__builtin_inff() ? 0.f : m, ref = WUP - base * c;
-    if (__builtin_expect(__any(fabsf(ref) > FAR), 0)) {    // the rounding of m c would count: differences first
+    const float base = m == -__builtin_inff() ? 0.f : m, ref = UP - base * c;
+    auto total = [&]() {
+      float sum = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r] - base, c, WUP));
+      for (int r = 0; r < 16; ++r) sum += S[r];
+      return sum;
+    };
+    if (__builtin_expect(__any(fabsf(ref) > FAR) || apart, 0)) {           // the rounding of m c would count: differences first
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r] - base, c, UP));
+      l += pass == 0 ? total() : 0.f;
+      if (!R5 && apart) S *= down_of(ex, pass);            // (before the scales: 0 * scale stays 0)
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], c, ref));
+      l += total();
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum += S[r];
-    l += sum;
-    if constexpr (!R5) S *= u2f((uint32_t)(127 - ex2) << 23);
     // ---- O^T += V^T P^T
     {
       f16x8 P[R5 ? 1 : 2][2];                            // (Row656: times a group's scales, the next one's beside its products)
@@ -1104,7 +1188,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         u[2 * (a & 1) + e] = pk_f16(x, y);
         P[R5 ? 0 : g & 1][a >> 1] = __builtin_bit_cast(f16x8, u);
       };
-      auto scale_of = [&](int g, int a) { sc[a & 1] = *(SPMLA_LDS f32x4*)(scales + g * 128 + 32 * a + 16 * hh); };
+      auto scale_of = [&](int g, int a) { sc[a & 1] = *(SPMLA_LDS f32x4*)(copied + g * 128 + 32 * a + 16 * hh); };
       const int vrow = 4 * hh + (l16 >> 2), vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
       const int v0 = vrow * 128 + 16 * (vch ^ swz(vrow)) + 8 * (lane & 1);  // (rows 8 on: places ^ 2; the group's other half: ^ 4)
       auto vread = [&](int n) -> f16x8 {                  // unit n = 2 d + ks: dims 32 d + l32, positions 16 ks ..
@@ -1141,6 +1225,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if constexpr (!R5) pass = apart ? (pass + 1) & 3 : 0;
+    j += pass == 0;
   }
 
   wait_vm<0>();
@@ -1150,14 +1236,16 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   l = swap32_sum(l);
   if (32 * w >= live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const float ln = m == -__builtin_inff() && l == l ? m : m * c * 0.69314718055994531f + (__builtin_log2f(l) - WUP) * 0.69314718055994531f;
+  const float ln = m == -__builtin_inff() && l == l ? m : m * c * 0.69314718055994531f + (__builtin_log2f(l) - UP) * 0.69314718055994531f;
   const bool whole = it.splits == 1;
   const long long r = r0 + qr;
   if (hh == 0 && qr < live) {
     if (!whole) p.lpart[((long long)it.slot + it.sp) * MR + qr] = ln;
     else if (p.lse) p.lse[(t0 + r / p.H) * p.l_st + r % p.H] = ln;
   }
-  const float back = inv * p.kv_scale * (R5 ? 1.f : u2f((uint32_t)(ex2 + 127) << 23));
+  float back[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) back[g] = inv * p.kv_scale * (R5 ? 1.f : up_of(ex, g));
   if (!whole) {
     // through LDS, 256 dims of a row at a time: 32 rows of 1024 bytes, 16-byte chunks permuted by the row
     SPMLA_LDS uint8_t* ob = lds + w * 32768;
@@ -1170,7 +1258,7 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
         for (int a = 0; a < 4; ++a) {
           const f32x16& y = O[8 * half + n];
           *(SPMLA_LDS f32x4*)(ob + l32 * 1024 + 16 * ((8 * n + 2 * a + hh) ^ l32)) =
-              f32x4{y[4 * a], y[4 * a + 1], y[4 * a + 2], y[4 * a + 3]} * back;
+              f32x4{y[4 * a], y[4 * a + 1], y[4 * a + 2], y[4 * a + 3]} * back[2 * half + (n >> 2)];
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       for (int row = 0; row < 32 && 32 * w + row < live; ++row)
@@ -1185,7 +1273,8 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
 #pragma unroll
     for (int a = 0; a < 4; ++a)
       *(SPMLA_LDS i32x2*)(ob + l32 * 1024 + 16 * ((4 * n + a) ^ l32) + 8 * hh) =
-          i32x2{(int)pk_bf16(O[n][4 * a] * back, O[n][4 * a + 1] * back), (int)pk_bf16(O[n][4 * a + 2] * back, O[n][4 * a + 3] * back)};
+          i32x2{(int)pk_bf16(O[n][4 * a] * back[n >> 2], O[n][4 * a + 1] * back[n >> 2]),
+                (int)pk_bf16(O[n][4 * a + 2] * back[n >> 2], O[n][4 * a + 3] * back[n >> 2])};
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   for (int row = 0; row < 32 && 32 * w + row < live; ++row) {
     const long long y = r0 + 32 * w + row;
