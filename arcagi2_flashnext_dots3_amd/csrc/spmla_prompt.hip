@@ -402,17 +402,21 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   for (; j < nt; ++j) tile(j, std::true_type());
 
   if (__builtin_expect(odd_from < kend, 0)) {              // those values for the queries that see them
-    for (int key = odd_from; key < kend && key <= qw + 31; ++key)
+    const int upto = p.causal ? qi : len - 1;              // the last key that the lane's query sees
+    for (int key = odd_from; key < kend && (!p.causal || key <= qw + 31); ++key) {
+      int width = p.Dv;
+      asm volatile("" : "+s"(width));                      // (else the compiler keeps a mask for each column over the tiles)
 #pragma unroll
       for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int col = 32 * d + 8 * (r >> 2) + 4 * hh + (r & 3);
-          const uint32_t x = col < p.Dv ? *(const uint16_t*)(vp + ((long long)key * p.v_st + col) * 2) : 0u;
+          const uint32_t x = col < width ? *(const uint16_t*)(vp + ((long long)key * p.v_st + col) * 2) : 0u;
           const uint32_t ex = E::EXPO & 0xffffu;
           const float bad = (x & 0x7fffu) != ex ? __builtin_nanf("") : x >> 15 ? -__builtin_inff() : __builtin_inff();
-          O[d][r] += (x & ex) == ex && key <= qi ? bad : 0.f;
+          O[d][r] += (x & ex) == ex && key <= upto ? bad : 0.f;
         }
+    }
   }
 
   // ---- output: through LDS (the tiles are done with), a query's values in one row
