@@ -303,11 +303,11 @@ __global__ void __launch_bounds__(512, 2) kernel(Params p) {
   int t0 = p.start[b], t1 = p.start[b + 1];
   const long long r0 = (long long)it.tile * MR;
   t0 = t0 < 0 ? 0 : t0;
+  const int past = p.seqs[b] - (t1 - t0);                 // rows before the new ones (all of them, places for them or not)
   t1 = t1 > p.T ? p.T : t1;
   const long long nrows = (long long)(t1 - t0) * p.H;
   if (r0 < 0 || r0 >= nrows) return;
   const int live = nrows - r0 < MR ? (int)(nrows - r0) : MR;               // query rows here
-  const int past = p.seqs[b] - (t1 - t0);                                  // rows before the new ones
   const long long cap = p.longest;
   auto limit_of = [&](int r) -> int {                                      // positions that row r sees
     const long long x = (long long)past + (r0 + r) / p.H + 1;
@@ -775,11 +775,11 @@ __global__ void __launch_bounds__(256, 1) wide_kernel(Params p) {
   int t0 = p.start[b], t1 = p.start[b + 1];
   const long long r0 = (long long)it.tile * MR;
   t0 = t0 < 0 ? 0 : t0;
+  const int past = p.seqs[b] - (t1 - t0);                 // rows before the new ones (all of them, places for them or not)
   t1 = t1 > p.T ? p.T : t1;
   const long long nrows = (long long)(t1 - t0) * p.H;
   if (r0 < 0 || r0 >= nrows) return;
   const int live = nrows - r0 < MR ? (int)(nrows - r0) : MR;
-  const int past = p.seqs[b] - (t1 - t0);
   const long long cap = p.longest;
   auto limit_of = [&](int r) -> int {
     const long long x = (long long)past + (r0 + r) / p.H + 1;

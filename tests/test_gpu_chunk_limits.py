@@ -23,3 +23,20 @@ def test_as_many_workgroups_as_may_be(dev, row, heads, lens, seqs, items):
     _check(out.cpu(), lse.cpu(), q, cache, table, s, start, 1.0, 64)
     with pytest.raises(Exception, match="limit"):
         kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), s.to(dev), start.to(dev), SM, items=items + 300)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads,lens,seqs,T", [(16, [2, 9], [300, 150], 7), (128, [1, 3], [300, 400], 3), (128, [4, 30], [700, 900], 20),
+                                               (24, [5, 6, 7], [300, 200, 100], 8), (16, [60], [90], 1)])
+def test_fewer_places_than_tokens(dev, row, heads, lens, seqs, T):
+    """A step cut to T places (page_step: tokens beyond have none): the tokens that are there see what they would see in the
+    whole step."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, s, start = _case(seqs, lens, heads, row, 16, T)
+    args = [x.to(dev) for x in (q[:T], cache, table, s, start)] + [SM]
+    short = start.clamp(max=T)
+    cut = (start[1:] - start[:-1]) - (short[1:] - short[:-1])
+    for items in (None, 0, 40):
+        out, lse = kernels.attend_chunk(*args, items=items)
+        torch.cuda.synchronize()
+        _check(out.cpu(), lse.cpu(), q[:T], cache, table, s - cut, short, 1.0, 16)
