@@ -1417,7 +1417,8 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
   const long long room = (long long)W * block_size;
   if (longest > room) longest = (int)room;
   const chunk::Shape s = chunk::shape_of(T, H, B, row_bytes, longest);
-  if (s.tiles > (1ll << 30)) return SPMLA_ELIMIT;
+  const int threads = s.rows == 128 ? 256 : 512;
+  if (s.tiles * threads >= 1ll << 32) return SPMLA_ELIMIT;   // a grid of 2^32 threads or more is not launched
   const long long need = spmla_attn_chunk_ws_bytes(T, H, B, row_bytes, longest, items);
   const int extra = B <= chunk::PLAN && longest > 0 && items > s.tiles ? (int)(items - s.tiles) : 0;
   if (extra >= rules::CHUNK_SPLITS) return SPMLA_ELIMIT;
@@ -1449,7 +1450,7 @@ extern "C" int spmla_attn_chunk(const void* q, long long q_st, long long q_sh, c
     if (const int rc = first[r5](f, dim3((unsigned)s.images, (unsigned)B), 256, 0, stm, p)) return rc;
   }
   const long long grid = extra ? (items + 7) / 8 * 8 : s.tiles;
-  if (const int rc = go[at](fn[at], dim3((unsigned)grid), s.rows == 128 ? 256 : 512, lds[at], stm, p)) return rc;
+  if (const int rc = go[at](fn[at], dim3((unsigned)grid), threads, lds[at], stm, p)) return rc;
   if (!extra) return SPMLA_OK;
   static Launcher join[2];
   const long long n = (long long)T * H;

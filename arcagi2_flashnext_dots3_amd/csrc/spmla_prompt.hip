@@ -455,7 +455,7 @@ int launch(Params& p, hipStream_t s) {
   if (const int rc = attr.ensure(fn, lds)) return rc;
   p.tiles = p.T / (32 * NW) + p.B;
   const long long n = (long long)p.tiles * p.H;
-  if (n > (1ll << 30)) return SPMLA_ELIMIT;
+  if (n * (64 * NW) >= 1ll << 32) return SPMLA_ELIMIT;     // a grid of 2^32 threads or more is not launched
   return start(fn, dim3((unsigned)n), 64 * NW, lds, s, p);
 }
 
