@@ -452,10 +452,10 @@ int launch(Params& p, hipStream_t s) {
   static Launcher start;
   const void* fn = (const void*)kernel<BF, DK, DV, NW>;
   constexpr int lds = Lds<DK, DV>::TOTAL;
-  if (const int rc = attr.ensure(fn, lds)) return rc;
   p.tiles = p.T / (32 * NW) + p.B;
   const long long n = (long long)p.tiles * p.H;
   if (n * (64 * NW) >= 1ll << 32) return SPMLA_ELIMIT;     // a grid of 2^32 threads or more is not launched
+  if (const int rc = attr.ensure(fn, lds)) return rc;
   return start(fn, dim3((unsigned)n), 64 * NW, lds, s, p);
 }
 
