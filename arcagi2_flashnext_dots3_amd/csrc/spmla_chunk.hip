@@ -212,23 +212,11 @@ struct Lds {
 
 __device__ __attribute__((aligned(16))) uint8_t zero_row[ROW656];
 
-__device__ inline float swap32_max(float x) {
-  const uint32_t u = f2u(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t a = r[0], b = r[1];
-  return fmaxf(u2f(a), u2f(b));
-}
 __device__ inline float swap16_max(float x) {
   const uint32_t u = f2u(x);
   const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   const uint32_t a = r[0], b = r[1];
   return fmaxf(u2f(a), u2f(b));
-}
-__device__ inline float swap32_sum(float x) {
-  const uint32_t u = f2u(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t a = r[0], b = r[1];
-  return u2f(a) + u2f(b);
 }
 __device__ inline float swap16_sum(float x) {
   const uint32_t u = f2u(x);

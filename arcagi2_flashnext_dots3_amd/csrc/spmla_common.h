@@ -101,7 +101,7 @@ __host__ __device__ inline uint8_t e2m2_to_e4m3(uint32_t code, int k) {
   return (uint8_t)(c | ((code & 16u) << 3));     // the sign survives rounding to zero (-0 -> 0x80)
 }
 
-// ---- XCD-aware workgroup order ---------------------------------------------------------------------------
+// ---- sums and maxima of a wave on the VALU ---------------------------------------------------------------
 // Inclusive prefix sum over the 64 lanes of a wave on the VALU: DPP row shifts 1, 2, 4, 8 scan each 16-lane row,
 // then row_bcast:15 adds row 0's total to row 1 and row 2's to row 3, and row_bcast:31 adds rows 0-1's total to rows
 // 2 and 3 (gfx9 DPP controls). A lane whose DPP source is outside its row adds 0.
@@ -125,7 +125,20 @@ __device__ inline int wave_top(int x) {                    // the largest, of va
   up(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
   return __builtin_amdgcn_readlane(x, 63);
 }
+__device__ inline float swap32_max(float x) {              // over lanes l, l ^ 32
+  const uint32_t u = f2u(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  return fmaxf(u2f(a), u2f(b));
+}
+__device__ inline float swap32_sum(float x) {
+  const uint32_t u = f2u(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  return u2f(a) + u2f(b);
+}
 
+// ---- XCD-aware workgroup order ---------------------------------------------------------------------------
 // The dispatcher hands workgroup i to XCD (i % 8). remap_xcd(i, n) gives the logical work index so that
 // each XCD receives a contiguous block of ceil(n / 8) logical items: consecutive logical items (e.g. the
 // head groups of one token, which gather the same rows) then share one XCD's L2. Returns -1 for the padding

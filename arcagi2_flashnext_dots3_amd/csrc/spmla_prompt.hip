@@ -74,19 +74,6 @@ struct Type<false> {                  // P up to 2^13: small weights stay above 
 // place of a row's 16-byte chunk c: c ^ swz(row)
 __device__ inline int swz(int row) { return ((row & 2) << 1) | ((row & 4) >> 2) | ((row & 8) >> 2); }
 
-__device__ inline float half_max(float x) {                // over lanes l, l ^ 32
-  const uint32_t u = f2u(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t a = r[0], b = r[1];
-  return fmaxf(u2f(a), u2f(b));
-}
-__device__ inline float half_sum(float x) {
-  const uint32_t u = f2u(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t a = r[0], b = r[1];
-  return u2f(a) + u2f(b);
-}
-
 // Tile `rank` (MQ queries) of a head, the longest first: up to SORTED sequences by a search for the level x (causal: tiles of
 // index x - 1; full: sequences of x tiles) that the rank falls into, v(x) tiles of a sequence being at levels >= x; more
 // sequences from the last to the first, sequence b from tile start[b] / MQ + b (as many tiles lie between two sequences as
@@ -316,7 +303,7 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[u][r]);
-    mx = half_max(mx);
+    mx = swap32_max(mx);
     if (__any(mx * p.c > m * p.c + TAU)) {                 // (also the first tile: m = -inf)
       const float mn = fmaxf(m, mx);
       const float a = mn == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.c);
@@ -420,7 +407,7 @@ __global__ void __launch_bounds__(64 * NW, DK > 192 ? 1 : 2) kernel(Params p) {
   }
 
   // ---- output: through LDS (the tiles are done with), a query's values in one row
-  l = half_sum(l);
+  l = swap32_sum(l);
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   lds_barrier();
   constexpr int OROW = DV * 2;                             // its chunks permuted by the query

@@ -1140,7 +1140,6 @@ def attend_prompt(q, k, v, start, scale, causal=True, out=None, lse=None):
 
 
 @functools.lru_cache(maxsize=4096)
-@functools.lru_cache(maxsize=4096)
 def chunk_items(T, H, B, row_bytes, longest):
     """Workgroups that attend_chunk has share the positions of T tokens of H heads in B requests (spmla_attn_chunk_items)."""
     return int(_lib.lib().spmla_attn_chunk_items(T, H, B, row_bytes, longest))

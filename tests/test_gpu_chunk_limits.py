@@ -40,3 +40,19 @@ def test_fewer_places_than_tokens(dev, row, heads, lens, seqs, T):
         out, lse = kernels.attend_chunk(*args, items=items)
         torch.cuda.synchronize()
         _check(out.cpu(), lse.cpu(), q[:T], cache, table, s - cut, short, 1.0, 16)
+
+
+@pytest.mark.parametrize("row", [656, 576])
+@pytest.mark.parametrize("heads,lens,seqs,items", [(16, [2] * 40, [100] * 40, 0), (32, [2] * 60, [70] * 60, 0), (40, [1] * 30, [150] * 30, None),
+                                                   (128, [1, 2, 1], [2000, 500, 60], None), (128, [9, 10], [700, 800], None)])
+def test_same_bits_again(dev, row, heads, lens, seqs, items):
+    """The same inputs give the same bits, whatever the waves' order (tiles of 32, 64 and 128 rows, splits, gathered rows)."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, s, start = case = _case(seqs, lens, heads, row, 16, heads)
+    args = [x.to(dev) for x in case] + [SM]
+    out, lse = kernels.attend_chunk(*args, items=items)
+    torch.cuda.synchronize()
+    _check(out.cpu(), lse.cpu(), q, cache, table, s, start, 1.0, 16)
+    more = [kernels.attend_chunk(*args, items=items) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) and torch.equal(z, lse) for o, z in more)
