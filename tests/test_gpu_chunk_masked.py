@@ -43,3 +43,22 @@ def test_rows_gathered_first(dev, heads, tokens, row, spoil, items):
         out, lse = _behind(dev, case, i, spoil, 16, items=items)
         if spoil is not infinite_scale:                        # (of scores that may be -inf)
             assert bool(out[i:].isnan().any(2).all())
+
+
+def nan_rope(row):
+    row[-64:] = 0x7F if len(row) == 576 else 0xFF
+
+
+def infinite_rope(row):
+    row[-64:] = 0x7F if len(row) == 576 else torch.tensor([float("inf")], dtype=torch.bfloat16).view(torch.uint8).repeat(32)
+
+
+@pytest.mark.parametrize("seqs,heads,tokens,longest", [(300, 16, 5, 300), (300, 128, 3, 300), (300, 4, 70, None), (900, 128, 5, None), (900, 16, 9, None),
+                                                       (40, 40, 40, None), (900, 1, 200, None), (700, 64, 20, None)])
+@pytest.mark.parametrize("row,spoil", [(576, nan_code), (576, nan_rope), (656, nan_code), (656, infinite_scale), (656, nan_scale), (656, nan_rope),
+                                       (656, infinite_rope)])
+def test_every_kernel(dev, seqs, heads, tokens, longest, row, spoil):
+    """Tiles of 32, 64 and 128 rows, of one token and of several, split or not."""
+    case = _case([seqs], [tokens], heads, row, 16, heads + tokens)
+    for items in (None, 0):
+        _behind(dev, case, max(1, tokens // 2), spoil, 16, items=items, max_seq_len=longest)

@@ -93,3 +93,33 @@ def test_large_scales_behind_a_token(dev, seqs, lens, heads):
         out, lse = kernels.attend_chunk(q.to(dev), far.to(dev), table.to(dev), s.to(dev), start.to(dev), SM, items=items)
         torch.cuda.synchronize()
         _check(out[:i].cpu(), lse[:i].cpu(), q[:i], cache, table, torch.tensor([at]), torch.tensor([0, i]), 16)
+
+
+@pytest.mark.parametrize("seqs,lens,heads,items", [([150], [150], 1, None), ([40], [40], 4, None), ([300], [130], 2, 0), ([300], [130], 2, 30),
+                                                   ([330], [300], 16, None), ([700], [200], 8, 40), ([1000, 200], [100, 50], 16, None),
+                                                   ([64, 30], [5, 30], 6, None), ([25], [25], 128, None)])
+@pytest.mark.parametrize("spread", [2, 20, 60])
+def test_scales_of_every_size_in_a_chunk(dev, seqs, lens, heads, items, spread):
+    """Scales from 2^-spread to 2^spread of the ordinary ones at random, by position and group, under weights that do not depend on
+    them (rope alone): each token's output keeps the precision that the largest scale of the group among the rows it sees leaves."""
+    from arcagi2_flashnext_dots3_amd import kernels
+    q, cache, table, s, start = _case(seqs, lens, heads, 656, 16, heads + spread)
+    q[..., :512] = 0
+    g = torch.Generator().manual_seed(spread)
+    for b, L in enumerate(seqs):
+        old, put = _scales(cache, table, b, torch.arange(L), 16)
+        put(old * 2.0 ** (spread * (2 * torch.rand(L, 4, generator=g) - 1)))
+    out, lse = kernels.attend_chunk(q.to(dev), cache.to(dev), table.to(dev), s.to(dev), start.to(dev), SM, items=items)
+    torch.cuda.synchronize()
+    out, lse = out.cpu(), lse.cpu()
+    assert bool(out.isfinite().all())
+    for b, L in enumerate(seqs):
+        t0, t1 = int(start[b]), int(start[b + 1])
+        x = torch.arange(L)
+        raw = cache[table[b].long()[x // 16], x % 16]
+        rows = ref.rows64(raw)
+        last = L - (t1 - t0) + torch.arange(t1 - t0)
+        r = ref.softmax_product(q[t0:t1].double().transpose(0, 1), rows[None], rows[None, :, :512], x <= last[:, None], SM)
+        top = raw[:, 512:528].contiguous().view(torch.float32).double().abs().cummax(0).values[last].repeat_interleave(128, 1) * 448.0
+        ref.check(out[t0:t1].transpose(0, 1), lse[t0:t1].transpose(0, 1), r, 576, L, torch.bfloat16, ref.HALF[torch.float16],
+                  L * 2.0 ** -29 * top, f"request {b}")
