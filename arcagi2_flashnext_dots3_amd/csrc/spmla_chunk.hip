@@ -15,23 +15,23 @@
 //     two). (8-bit MFMA would take the codes as they are, the query in two e4m3 parts: its sums are off by 2e-6 of the summed
 //     magnitudes, 1.3e-5 at most, against 4e-9 and 1.2e-7 here.) Row656: a group's sum times the rows' fp32 scales; for PV
 //     the weight times the group's scale.
-//   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale) are rounded to fp16,
-//     once. (In bf16 they need no care for their range and cost as much, but put as large an error on the output as its
-//     own rounding does.)
+//   * roundings: scores, statistics, sums and partial results are fp32; weights (Row656: times a scale, in units that follow the
+//     largest scale of the group that the query row has seen) are rounded to fp16, once. (In bf16 they need no care for their
+//     range and cost as much, but put as large an error on the output as its own rounding does.)
 //   * masked positions take no part: scores of -inf, and where the mask cuts a tile codes and scales that are no numbers
-//     become 0 after the scores (a row that sees one has a score that is none).
+//     become 0 after the scores (a row that sees one has a score that is none); scales that a row does not see do not move its units.
 //
 // Three kernels by the rows of a request, on average:
 //   * `kernel`, up to 64: 8 waves of 16 rows, 2 or 4 of them on the same rows with every second or fourth tile of 32 positions,
 //     joined in LDS. A wave converts what it reads. Bound by HBM (48 requests of 16 heads, 364 MB: 98 us = 3.7 TB/s).
 //   * `wide_kernel<R5, false>`: 4 waves of 32 rows, 512 registers (O in the 256 accumulation registers, the query in 144 others).
 //     A tile's codes are converted to fp16 once for all waves, beside the score products. Bound by the issue of one
-//     wave a SIMD: matrix cores busy for 28% (64 requests of 128 heads: 119 us = 540 TFLOP/s). Two waves a SIMD leave 16 rows
+//     wave a SIMD: matrix cores busy for 29% (64 requests of 128 heads: 119 us = 540 TFLOP/s). Two waves a SIMD leave 16 rows
 //     a wave, each of which converts everything again (267 us).
 //   * from 1024 on, `image_kernel` gathers and converts the tiles first, `wide_kernel<R5, true>` copies them as they lie
 //     in LDS: no conversions, addresses without tables (1024 tokens of 128 heads over 16384 rows: 3.78 ms = 1200 TFLOP/s, of
-//     which the images take 0.01; converted in the kernel 5.3). Bound by the power limit: the clock falls to 1.8 - 2.0
-//     GHz, and a form that runs the softmax beside the next tile's score products takes as long.
+//     which the images take 0.01; converted in the kernel 5.3). The clock falls to 1.8 - 2.0
+//     GHz with the power, and a form that runs the softmax beside the next tile's score products takes as long.
 // Splits leave normalized fp32 partials and their lse in a workspace; a second kernel joins them.
 #include "spmla_common.h"
 #include "spmla_quant.h"

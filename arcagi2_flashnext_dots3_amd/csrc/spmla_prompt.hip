@@ -17,8 +17,8 @@
 //     their place, and the queries that see such a value get it at the end.
 //
 // Two waves a SIMD (three with heads of 64, one with heads of 256): the matrix products of one run beside the softmax of the
-// other. Heads of 128 and 192: 950 - 1140 TFLOP/s on long prompts, the matrix cores busy for half of the time at the clock
-// that the power limit leaves; of 64: 860, bound by the VALU (per 64 keys 32 exponentials of 16 clocks and 120 instructions of 4
+// other. Heads of 128 and 192: 950 - 1140 TFLOP/s on long prompts, the matrix cores busy for half of the time at 2.0 GHz (every
+// tile waits for its copies, one tile ahead, and at a barrier); of 64: 860, bound by the VALU (per 64 keys 32 exponentials of 16 clocks and 120 instructions of 4
 // against 512 clocks of products); of 256: 775 (one wave a SIMD, O in accumulation registers). Short prompts: the
 // launch, the search for the tile, two dependent loads and cold code, 11 us.
 #include "spmla_common.h"

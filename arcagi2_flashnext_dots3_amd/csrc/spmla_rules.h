@@ -1,4 +1,4 @@
-// Rules of sizes by which the launchers choose a kernel (plain host code).
+// Rules of sizes by which the launchers choose a kernel, and limits and LDS places that both sides share (plain host code).
 #pragma once
 
 namespace spmla {

@@ -1101,9 +1101,8 @@ def page_step(pool, new, n=None, start=None, req=None, positions=None, slots=Non
     none) -> (start [requests + 1] int32 sums of the new tokens; req [n] int32, positions [n] int64 and slots [n] int64 of
     each token). Pages the tokens need come from the pool's free stack and are entered in its table; where the stack is
     empty the rest go without (slot -1; pool.state[1] counts the missing pages; a later step enters pages for them, but their
-    rows were not written: such a request is to be computed again). n: places
-    for tokens (None: that of req); those behind the last token hold the last request, position 0 and slot -1, tokens
-    beyond n have none."""
+    rows were not written: such a request is to be computed again). n: places for tokens (None: that of req); those behind
+    the last token hold the last request, position 0 and slot -1, tokens beyond n have none."""
     dev = pool.table.device
     if n is None:
         _need(req is not None, "page_step: n, or req [n]")

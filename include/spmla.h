@@ -542,8 +542,9 @@ int spmla_attn_prompt(const void* q, long long q_st, long long q_sh, const void*
  * (row stride t_st, W columns) is not negative: cache row page * stride_rows + x % block_size (stride_rows: rows from a block
  * to the next; rows beyond `rows` are not read). row_bytes 656 or 576; s = sm_scale * kv_scale * (q . row), out [T][H][512]
  * bf16 = kv_scale * sum p latent, lse [T][H] optional, as spmla_attn_splitk over all of these rows; a token without one gets
- * 0 and -inf, tokens of no request nothing; of a step cut to T places (start[B] > T) the tokens that have one. Codes are taken exactly, scores, sums and statistics in fp32; weights (Row656:
- * times the row's scale) are rounded to fp16.
+ * 0 and -inf, tokens of no request nothing. Of a step cut to T places (start[B] > T) the tokens that have one get what they
+ * would in the whole step. Codes are taken exactly, scores, sums and statistics in fp32; weights (Row656: times the row's scale
+ * of each group) are rounded to fp16, once (Row656: small products to 2^-29 of the largest scale of the group that the token sees).
  * items: workgroups that the requests' positions are shared out to on the device, by their lengths (0, B > 256, or no more
  * than the tiles of query rows: one a tile; ELIMIT beyond 511 more), partial results joined by a second kernel through a
  * workspace of spmla_attn_chunk_ws_bytes. spmla_attn_chunk_items: a good number of them.
